@@ -16,6 +16,9 @@ reference package `vggt_omega` for the merged global-attention path:
   replay of the TTT planner's trace records (sparse_convex.py:77-80, 1907-1976)
 * `use_tuned_gemms`                      recorded hipBLASLt selections for the
   block's torch GEMMs (TunableOp)
+* `masked_attention`, `relative_position_bias` -- attention under score caps, position
+  biases and document, prefix and length masks, with gradients, and the learned bias by
+  buckets as a dense tensor (no counterpart in the reference)
 * `ops` -- the torch.library operators `torch.ops.vgo.*` (mass_bias_attention,
   top4_project, compaction, QKV epilogue, residual rows) with fake
   implementations for tracing
@@ -28,6 +31,7 @@ from __future__ import annotations
 from . import _lib, ops, plan_io
 from .gemm_tuning import use_tuned_gemms
 from .layers import LinearKMaskedBias, SelfAttention, SelfAttentionBlock
+from .masked_attention import masked_attention, relative_position_bias
 from .mass_bias_attention import dense_attention, mass_bias_attention
 from .projection import top4_project
 from .sparse_convex import build_sparse_convex_plan, convex_fit, start_sparse_convex_plan
@@ -50,9 +54,11 @@ __all__ = [
     "convex_fit",
     "dense_attention",
     "deterministic_weighted_normalizer",
+    "masked_attention",
     "mass_bias_attention",
     "ops",
     "plan_io",
+    "relative_position_bias",
     "start_sparse_convex_plan",
     "streaming_top4",
     "top4_project",

@@ -45,6 +45,35 @@ class AttnProblem(ctypes.Structure):
     ]
 
 
+class MaskedAttn(ctypes.Structure):
+    """`vgo_masked_attn` of include/vgo.h."""
+
+    _fields_ = [
+        ("q", _c_p), ("k", _c_p), ("v", _c_p),
+        ("batch", _c_i64), ("heads", _c_i64), ("kv_heads", _c_i64), ("n_query", _c_i64), ("n_key", _c_i64),
+        ("head_dim", _c_i64), ("q_stride", _i64x3), ("k_stride", _i64x3), ("v_stride", _i64x3),
+        ("scale", _c_f32), ("score_cap", _c_f32),
+        ("log_mass", _c_p), ("slopes", _c_p), ("bucket_table", _c_p), ("bucket_starts", ctypes.POINTER(ctypes.c_int32)),
+        ("n_buckets", ctypes.c_int32), ("n_starts", ctypes.c_int32), ("bidirectional", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("prefix_lengths", _c_p), ("query_documents", _c_p), ("key_documents", _c_p), ("key_lengths", _c_p),
+        ("query_starts", _c_p),
+    ]
+
+
+class MaskedAttnGrads(ctypes.Structure):
+    """`vgo_masked_attn_grads` of include/vgo.h."""
+
+    _fields_ = [
+        ("out", _c_p), ("grad_out", _c_p), ("lse", _c_p), ("out_stride", _i64x3), ("grad_out_stride", _i64x3),
+        ("dq", _c_p), ("dk", _c_p), ("dv", _c_p),
+        ("dq_stride", _i64x3), ("dk_stride", _i64x3), ("dv_stride", _i64x3),
+        ("d_log_mass", _c_p), ("d_slopes", _c_p), ("d_table", _c_p),
+    ]
+
+
+_starts = [ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.c_int32]  # starts, how many, bidirectional
+
 # name -> (restype, argtypes); every symbol declared in include/vgo.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vgo_last_error": (ctypes.c_char_p, []),
@@ -154,6 +183,21 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vgo_residual_layer_norm": (_c_int, [
         _c_p, _c_i64, _c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_f32, _c_i64, _c_i64, _c_p, _c_i64,
         _c_p, _c_i64, _c_int, _c_p, _c_i64, _c_p, _c_i64, _c_f32, _c_p,
+    ]),
+    "vgo_masked_attn_workspace": (_c_int, [ctypes.POINTER(MaskedAttn), _c_int, ctypes.POINTER(_c_size)]),
+    "vgo_masked_attn_fwd": (_c_int, [
+        ctypes.POINTER(MaskedAttn), _c_p, _i64x3, _c_p, _c_int, _c_p, _c_size, _c_p,
+    ]),
+    "vgo_masked_attn_grad_workspace": (_c_int, [
+        ctypes.POINTER(MaskedAttn), ctypes.POINTER(MaskedAttnGrads), _c_int, ctypes.POINTER(_c_size),
+    ]),
+    "vgo_masked_attn_grad": (_c_int, [
+        ctypes.POINTER(MaskedAttn), ctypes.POINTER(MaskedAttnGrads), _c_int, _c_p, _c_size, _c_p,
+    ]),
+    "vgo_position_bias": (_c_int, [_c_p, _c_i64, _c_i64, *_starts, _c_i64, _c_i64, _c_i64, _c_p, _c_int, _c_p]),
+    "vgo_position_bias_grad_workspace": (_c_int, [_c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_size)]),
+    "vgo_position_bias_grad": (_c_int, [
+        _c_p, _c_i64, _c_i64, *_starts, _c_i64, _c_i64, _c_i64, _c_p, _c_int, _c_p, _c_size, _c_p,
     ]),
     "vgo_restore_residual_layer_norm": (_c_int, [
         _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_f32, _c_i64,

@@ -1,0 +1,365 @@
+// What the masked-attention kernels share (forward: masked_attention.hip, gradients:
+// masked_attention_grad.hip): the problem as the kernels see it, which pairs attend, the scores'
+// rules, LDS tiles and their MFMA operands.
+//
+//   position of query i: p_i = query_start[b] + i;  distance r = j - p_i
+//   z_ij = cap tanh(scale q_i.k_j / cap) + mass_j - slope_h |r| + table[bucket(r), h]
+//   pair (i, j) attends if j < key_length[b], the documents are equal and >= 0, and, when causal,
+//   r <= 0 or j < prefix[b].  P = softmax over those; a row without any gives zeros.
+//
+// Scores are computed transposed where a wave holds queries (S^T = K Q^T: a lane owns one query,
+// its registers run over keys) and straight where it holds keys (S = Q K^T), so the accumulator of
+// v_mfma_f32_32x32x16 -- register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32 --
+// is the next product's B operand as it stands: its k slots take rows in the order that the
+// registers have them, and the A operand is read from LDS in that order (cols_op).
+#pragma once
+
+#include <algorithm>
+#include <climits>
+#include <string>
+
+#include "vgo_common.h"
+
+namespace vgo {
+namespace masked {
+
+constexpr int kTile = 64;  // keys (or queries) per LDS tile
+constexpr int kMaxStarts = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_inff();
+
+typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8;
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+typedef __attribute__((__vector_size__(8 * sizeof(short)))) short s16x8;
+
+// Operands of one 16-deep product step: eight k slots per lane.  fp32 has no 16-deep instruction:
+// eight 32x32x2 steps, step e with slot e of both halves, so both types share every layout.
+template <typename T>
+struct Op;
+template <>
+struct Op<bf16_t> {
+  typedef bf16x8 op8;
+  static __device__ __forceinline__ f32x16 mma(op8 a, op8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Op<f16_t> {
+  typedef f16x8 op8;
+  static __device__ __forceinline__ f32x16 mma(op8 a, op8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Op<float> {
+  typedef f32x8 op8;
+  static __device__ __forceinline__ f32x16 mma(op8 a, op8 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Accumulator registers 8 c .. 8 c + 7 as an operand of T (bf16 / f16: rounded, as both products of
+// a 16-bit attention take their probabilities).
+template <typename T>
+__device__ __forceinline__ typename Op<T>::op8 as_op(const f32x16& s, int c) {
+  typename Op<T>::op8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = from_f32<T>(s[8 * c + e]);
+  return r;
+}
+
+// ------------------------------------------------------------- LDS tiles ----
+// kTile rows of D elements without padding; the 16-byte chunks of a row are permuted by XOR with a
+// function of row % 16 that keeps apart, in the banks, both the 16 rows that a row-operand read
+// takes at one chunk and the 4 (fp32: 2) rows x 64 (128) bytes that a column-operand read takes.
+template <typename T, int D>
+struct Tile {
+  static constexpr int kRowBytes = D * static_cast<int>(sizeof(T));
+  static constexpr int kChunks = kRowBytes / 16;  // per row: 8, 16 or 32
+  static constexpr int kBytes = kTile * kRowBytes;
+  static constexpr int kSteps = D / 16;  // 16-deep steps over the channels
+  static constexpr int kCols = D / 32;   // 32-channel blocks
+  typedef typename Op<T>::op8 op8;
+
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (sizeof(T) == 4) return (row & 3) | ((row >> 1) & 4) | ((row << 1) & 8);
+    if constexpr (kChunks == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+    return ((row & 3) << 2) | ((row >> 2) & 3);
+  }
+
+  // A operand with rows row0 + l % 32 (row0 a multiple of 16), channels 16 t + 8 (l / 32) ..
+  static __device__ __forceinline__ op8 rows_op(const char* tile, int row0, int t) {
+    const int lane = lane_id(), row = row0 + (lane & 31), h = lane >> 5;
+    const char* base = tile + row * kRowBytes;
+    const int f = swz(lane & 15);
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const op8*>(base + (((2 * t + h) ^ f) << 4));
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(base + (((4 * t + 2 * h) ^ f) << 4));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(base + (((4 * t + 2 * h + 1) ^ f) << 4));
+      return op8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+
+  // A operand of the transposed tile: row l % 32 of channels 32 dt .., k slot e = tile row
+  // 16 c + 4 (l / 32) + e % 4 + 8 (e / 4).  16-bit types: two transposing reads, in each of which
+  // 16 lanes take a 4 x 16 block (lane i: 4 channels of row i / 4) and keep column i of it.
+  static __device__ __forceinline__ op8 cols_op(const char* tile, int dt, int c) {
+    const int lane = lane_id(), h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, gg = (lane >> 4) & 1;
+      s16x8 r;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = 4 * h + (i >> 2) + 8 * half;  // of 16
+        const int chunk = (4 * dt + 2 * gg + ((i >> 1) & 1)) ^ swz(row);
+        const char* p = tile + (16 * c + row) * kRowBytes + (chunk << 4) + ((i & 1) << 3);
+        typedef __attribute__((address_space(3))) s16x4* lds_p;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[4 * half + e] = x[e];
+      }
+      return __builtin_bit_cast(op8, r);
+    } else {
+      op8 r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int row = 4 * h + (e & 3) + 8 * (e >> 2);
+        const int d = 32 * dt + (lane & 31);
+        r[e] = *reinterpret_cast<const float*>(tile + (16 * c + row) * kRowBytes + (((d >> 2) ^ swz(row)) << 4) +
+                                               ((d & 3) << 2));
+      }
+      return r;
+    }
+  }
+};
+
+// 16 bytes that stand for every row a tile must not take: those past the end, and those that the
+// masks keep from every row whatever they hold.
+static __device__ __attribute__((aligned(16))) const char zero_chunk[16] = {};
+
+// Rows row0 .. row0 + kTile of a [*, D] operand into an LDS tile by LDS DMA, wave w of `kWaves`
+// taking its share of 1 KB pieces.  `whole`: every row is taken; else row r is taken if
+// row0 + r < limit and live(row0 + r).
+template <typename T, int D, int kWaves, typename Live>
+__device__ __forceinline__ void stage(const T* base, int64_t row_stride, int row0, int limit, bool whole,
+                                      uint32_t lds, Live live) {
+  typedef Tile<T, D> TL;
+  constexpr int kPieces = TL::kBytes / 1024 / kWaves;
+  const int lane = lane_id();
+  const int wave = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const char* first = reinterpret_cast<const char*>(base + row0 * row_stride);
+  const uint32_t row_bytes = static_cast<uint32_t>(row_stride * static_cast<int64_t>(sizeof(T)));
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int piece = wave * kPieces + i, c = piece * 64 + lane;
+    const int row = c / TL::kChunks;
+    const uint32_t offset = row * row_bytes + (((c % TL::kChunks) ^ TL::swz(row & 15)) << 4);
+    const uint32_t to = lds + piece * 1024;
+    if (whole) {
+      lds_dma16(first, offset, to);
+    } else {
+      const bool taken = row0 + row < limit && live(row0 + row);
+      lds_dma16_addr(taken ? first + offset : zero_chunk, to);
+    }
+  }
+}
+
+// Buckets of distances: that of r is the number of starts <= |r|, plus half of them for r > 0
+// (bidirectional), or the number <= max(-r, 0).  Distances from `reach` on share one a side.
+struct Buckets {
+  int count, bidirectional, n_starts, reach;
+  int starts[kMaxStarts];
+
+  __device__ __forceinline__ int of(int r) const {
+    const int n = bidirectional ? abs(r) : max(-r, 0);
+    int bucket = 0;
+    for (int t = 0; t < n_starts; ++t) bucket += starts[t] <= n;
+    return bucket + (bidirectional && r > 0 ? count / 2 : 0);
+  }
+  // The sum of at(r) over the distances -reach .. reach of bucket t.
+  template <typename At>
+  __device__ __forceinline__ float sum(int t, At at) const {
+    const int side = bidirectional ? count / 2 : count, index = t % side;
+    float s = 0.0f;
+    if (index > n_starts) return s;
+    const int from = index == 0 ? 0 : starts[index - 1], to = index < n_starts ? starts[index] : reach + 1;
+    if (t >= side) {
+      for (int n = max(1, from); n < to; ++n) s += at(n);
+      return s;
+    }
+    for (int n = from; n < to; ++n) s += at(-n);
+    if (!bidirectional && index == 0)
+      for (int n = 1; n <= reach; ++n) s += at(n);
+    return s;
+  }
+};
+
+inline Buckets make_buckets(int count, const int32_t* starts, int n_starts, int bidirectional) {
+  Buckets b{};
+  b.count = count, b.bidirectional = bidirectional != 0, b.n_starts = n_starts;
+  for (int t = 0; t < n_starts; ++t) b.starts[t] = starts[t];
+  b.reach = n_starts > 0 ? starts[n_starts - 1] : 1;
+  return b;
+}
+// VGO_OK, or the status of buckets that the kernels do not take.
+int check_buckets(int64_t count, const int32_t* starts, int n_starts, int bidirectional);
+
+// ---------------------------------------------------------- the problem ----
+// Strides in elements.  Documents: query_doc [batch, n_query], key_doc [batch, n_key] or null; the
+// tile_info of either: per kTile rows {smallest, largest} valid document, the smallest one's bits
+// inverted where a row of the tile is none's (negative, or past the end).
+template <typename T>
+struct Args {
+  const T *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3], os[3];
+  int batch, heads, kv_heads, n_query, n_key;
+  float scale, inv_cap, cap2;     // scale; scale / cap and cap log2(e) (0: no cap)
+  const float* mass;              // [n_key] or null
+  const float* slopes;            // [heads] or null
+  const float* table;             // [n_buckets, heads] or null
+  Buckets buckets;                // of the table
+  int causal, query_start;
+  const int *prefix, *key_lengths, *query_starts;  // [batch] or null
+  const int *query_doc, *key_doc;
+  const int2 *query_info, *key_info;  // [batch, tiles]
+};
+
+template <typename T>
+__device__ __forceinline__ int key_limit(const Args<T>& a, int b) {
+  return a.key_lengths ? max(0, min(a.n_key, a.key_lengths[b])) : a.n_key;
+}
+template <typename T>
+__device__ __forceinline__ int first_position(const Args<T>& a, int b) {
+  constexpr int kMost = 1 << 29;  // keeps every distance in 32 bits
+  return a.query_starts ? max(-kMost, min(kMost, a.query_starts[b])) : a.query_start;
+}
+template <typename T>
+__device__ __forceinline__ int prefix_of(const Args<T>& a, int b) {
+  return a.prefix ? a.prefix[b] : 0;
+}
+
+// Rows of one side as the other side's tiles are judged by: positions (queries) or indices (keys)
+// lo .. hi, the documents' smallest and largest, and whether every row is a document's.
+struct Range {
+  int lo, hi, doc_lo, doc_hi;
+  bool docs_whole;
+};
+
+__device__ __forceinline__ Range info_range(int2 info) {
+  Range r;
+  r.docs_whole = info.x >= 0;
+  r.doc_lo = r.docs_whole ? info.x : ~info.x;
+  r.doc_hi = info.y;
+  return r;
+}
+
+// Whether any pair of the two ranges attends, and whether all do.  Keys past the limit are the
+// caller's to leave out of `any` and to count against `all`.
+template <typename T>
+__device__ __forceinline__ void judge(const Args<T>& a, const Range& q, const Range& k, int prefix, bool& any,
+                                      bool& all) {
+  any = all = true;
+  if (a.causal) {
+    any = k.lo <= q.hi || k.lo < prefix;
+    all = k.hi <= q.lo || k.hi < prefix;
+  }
+  if (a.key_doc) {
+    any = any && q.doc_lo <= k.doc_hi && k.doc_lo <= q.doc_hi;
+    all = all && q.docs_whole && k.docs_whole && q.doc_lo == q.doc_hi && k.doc_lo == k.doc_hi &&
+          q.doc_lo == k.doc_lo;
+  }
+}
+
+// table[bucket(r), head] log2(e) for r = -reach .. reach into LDS, by the whole work-group.
+template <typename T>
+__device__ __forceinline__ void fill_distances(const Args<T>& a, float* to, int head, int threads) {
+  for (int i = threadIdx.x; i <= 2 * a.buckets.reach; i += threads)
+    to[i] = a.table[static_cast<int64_t>(a.buckets.of(i - a.buckets.reach)) * a.heads + head] * kLog2e;
+}
+
+// out[i] = sum over parts of part[p][i], in a fixed order: 64 outputs a work-group, four runs of parts each.
+template <typename T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t parts, int64_t n, T* out) {
+  __shared__ float s[4][64];
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
+  const int run = threadIdx.x >> 6;
+  float x = 0.0f;
+  if (i < n)
+    for (int64_t p = run; p < parts; p += 4) x += part[p * n + i];
+  s[run][threadIdx.x & 63] = x;
+  __syncthreads();
+  if (run == 0 && i < n)
+    out[i] = from_f32<T>(((s[0][threadIdx.x] + s[1][threadIdx.x]) + s[2][threadIdx.x]) + s[3][threadIdx.x]);
+}
+template <typename T>
+int sum_parts(const float* part, int64_t parts, int64_t n, T* out, hipStream_t stream) {
+  if (n == 0) return VGO_OK;
+  hipLaunchKernelGGL(sum_parts_kernel<T>, dim3(static_cast<unsigned>((n + 63) / 64)), dim3(256), 0, stream, part,
+                     parts, n, out);
+  return check_launch("sum of parts");
+}
+
+// tanh of the capped scores.  1 - 2 / (1 + e^2y) loses what 1 takes from a small y: about 1e-7
+// absolute, i.e. 5e-6 in a score capped at 50, below the rounding of 16-bit inputs; fp32 takes the
+// odd series below 0.3 (its next term is 1e-9).
+template <typename T>
+__device__ __forceinline__ float cap_tanh(float y) {
+  const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
+  float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+  if constexpr (sizeof(T) == 4) {
+    const float y2 = y * y;
+    float s = fmaf(y2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    s = fmaf(s, -y2, 17.0f / 315.0f);
+    s = fmaf(s, -y2, 2.0f / 15.0f);
+    s = fmaf(s, -y2, 1.0f / 3.0f);
+    t = fabsf(y) < 0.3f ? fmaf(-y * y2, s, y) : t;
+  }
+  return t;
+}
+
+inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+
+// Document ranges of the tiles of one side (tile_info above).
+void launch_doc_info(const int* docs, const int* lengths, int n, int batch, int tiles, int2* info,
+                     hipStream_t stream);
+
+// VGO_OK, or the status of a problem the kernels do not take, with its message.
+int check_problem(const vgo_masked_attn* p, int dtype);
+bool strides_fit(const int64_t stride[3], int64_t head_dim, int dtype);
+
+template <typename T>
+Args<T> make_args(const vgo_masked_attn* p) {
+  Args<T> a{};
+  a.q = static_cast<const T*>(p->q), a.k = static_cast<const T*>(p->k), a.v = static_cast<const T*>(p->v);
+  for (int i = 0; i < 3; ++i) a.qs[i] = p->q_stride[i], a.ks[i] = p->k_stride[i], a.vs[i] = p->v_stride[i];
+  a.batch = static_cast<int>(p->batch), a.heads = static_cast<int>(p->heads);
+  a.kv_heads = static_cast<int>(p->kv_heads);
+  a.n_query = static_cast<int>(p->n_query), a.n_key = static_cast<int>(p->n_key);
+  a.scale = p->scale;
+  if (p->score_cap > 0.0f) a.inv_cap = p->scale / p->score_cap, a.cap2 = p->score_cap * kLog2e;
+  a.mass = p->log_mass, a.slopes = p->slopes, a.table = p->bucket_table;
+  if (a.table) a.buckets = make_buckets(p->n_buckets, p->bucket_starts, p->n_starts, p->bidirectional);
+  a.causal = p->causal != 0, a.query_start = a.n_key - a.n_query;
+  a.prefix = p->prefix_lengths, a.key_lengths = p->key_lengths, a.query_starts = p->query_starts;
+  a.query_doc = p->query_documents, a.key_doc = p->key_documents;
+  return a;
+}
+
+// Document ranges of both sides' tiles: their bytes, and their launch into `ws`.
+size_t info_bytes(const vgo_masked_attn* p);
+template <typename T>
+void launch_info(Args<T>& a, char* ws, hipStream_t stream) {
+  if (!a.key_doc) return;
+  const int kt = static_cast<int>(tiles_of(a.n_key)), qt = static_cast<int>(tiles_of(a.n_query));
+  int2* key = reinterpret_cast<int2*>(ws);
+  int2* query = key + static_cast<int64_t>(a.batch) * kt;
+  launch_doc_info(a.key_doc, a.key_lengths, a.n_key, a.batch, kt, key, stream);
+  launch_doc_info(a.query_doc, nullptr, a.n_query, a.batch, qt, query, stream);
+  a.key_info = key, a.query_info = query;
+}
+
+}  // namespace masked
+}  // namespace vgo

@@ -11,12 +11,14 @@
 // tensors' device, which is the current device meanwhile (`on_device`); none
 // synchronises.  Autograd: outputs of a path operator whose inputs
 // require grad have a backward that raises (the path is inference only), those
-// of a planner's operator do not require grad, and tangents are dropped.
+// of a planner's operator do not require grad, and tangents are dropped; the masked
+// attention and the position bias have gradients.
 // No operator has a batching rule (see register_batched).
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -27,6 +29,7 @@
 #include <memory>
 #include <optional>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "../../include/vgo.h"
@@ -176,6 +179,198 @@ void attention_pair_into(const Tensor& q, const Tensor& k, const Tensor& v, cons
   check(vgo_mass_bias_attn_pair_workspace(problems, 2, dtype, &need));
   const Tensor ws = need > 0 ? scratch(need, q) : Tensor();
   check(vgo_mass_bias_attn_pair_fwd_ws(problems, 2, dtype, ptr(ws), need, stream_of(q)));
+}
+
+// --------------------------------------------------------- masked attention ----
+// An operand as the kernels address it: unit channel stride, the others whole 16 bytes; else a copy.
+Tensor operand(const Tensor& t) {
+  const int64_t size = t.element_size();
+  bool fits = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) fits &= t.size(i) <= 1 || (t.stride(i) >= 0 && t.stride(i) * size % 16 == 0);
+  fits &= t.stride(2) < (int64_t{1} << 31) / 64 / size;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+void set_strides(int64_t (&to)[3], const Tensor& t) {
+  for (int i = 0; i < 3; ++i) to[i] = t.size(i) <= 1 ? 0 : t.stride(i);
+}
+// A new [batch, heads, tokens, channels] tensor, token-major where `like` is.
+Tensor in_layout_of(const Tensor& like) {
+  if (like.size(1) > 1 && like.stride(2) > like.stride(1))
+    return at::empty({like.size(0), like.size(2), like.size(1), like.size(3)}, like.options()).transpose(1, 2);
+  return at::empty(like.sizes(), like.options());
+}
+
+// The rules of a masked attention beside q, k and v.
+struct Rules {
+  OptTensor log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts;
+  double scale, score_cap;
+  std::vector<int64_t> bucket_starts;
+  bool bidirectional, causal;
+};
+
+struct MaskedProblem {
+  vgo_masked_attn p{};
+  Tensor q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts;
+  std::vector<int32_t> starts;
+
+  MaskedProblem(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Rules& rules) {
+    require_gpu({&q0, &k0, &v0});
+    TORCH_CHECK_VALUE(q0.dim() == 4 && k0.dim() == 4 && v0.dim() == 4,
+                      "q, k and v must be [batch, heads, tokens, channels]");
+    TORCH_CHECK_VALUE(q0.scalar_type() == k0.scalar_type() && k0.scalar_type() == v0.scalar_type(),
+                      "q, k and v must share one dtype");
+    TORCH_CHECK_VALUE(k0.sizes() == v0.sizes() && q0.size(0) == k0.size(0) && q0.size(3) == k0.size(3),
+                      "incompatible q/k/v shapes");
+    const int64_t batch = q0.size(0), n_query = q0.size(2), n_key = k0.size(2), heads = q0.size(1);
+    TORCH_CHECK_VALUE(heads > 0 && k0.size(1) > 0 && heads % k0.size(1) == 0,
+                      "masked_attention: heads must be a multiple of the key heads");
+    const auto same_device = [&](const Tensor& t) {
+      TORCH_CHECK(t.device() == q0.device(), "masked_attention: every tensor must be on the device of q");
+    };
+    same_device(k0), same_device(v0);
+    q = operand(q0), k = operand(k0), v = operand(v0);
+    const auto number = [&](const OptTensor& t, at::IntArrayRef shape, const char* what) {
+      if (opt(t) == nullptr) return Tensor();
+      same_device(*t);
+      TORCH_CHECK_VALUE(t->is_floating_point() && t->sizes() == shape, what);
+      return t->to(at::kFloat).contiguous();
+    };
+    const auto whole = [&](const OptTensor& t, at::IntArrayRef shape, const char* what) {
+      if (opt(t) == nullptr) return Tensor();
+      same_device(*t);
+      TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->sizes() == shape, what);
+      return t->contiguous();
+    };
+    log_mass = number(rules.log_mass, {n_key}, "masked_attention: log_key_mass must be floating [n_key]");
+    slopes = number(rules.slopes, {heads}, "masked_attention: slopes must be floating [heads]");
+    if (opt(rules.table) != nullptr)
+      table = number(rules.table, {rules.table->dim() == 2 ? rules.table->size(0) : -1, heads},
+                     "masked_attention: bucket_table must be floating [buckets, heads]");
+    prefix = whole(rules.prefix, {batch}, "masked_attention: prefix_lengths must be int32 [batch]");
+    query_documents = whole(rules.query_documents, {batch, n_query},
+                            "masked_attention: documents must be int32 [batch, n_query]");
+    key_documents = whole(rules.key_documents, {batch, n_key},
+                          "masked_attention: key_documents must be int32 [batch, n_key]");
+    key_lengths = whole(rules.key_lengths, {batch}, "masked_attention: key_lengths must be int32 [batch]");
+    query_starts = whole(rules.query_starts, {batch}, "masked_attention: query_starts must be int32 [batch]");
+    p.q = ptr(q), p.k = ptr(k), p.v = ptr(v);
+    p.batch = batch, p.heads = heads, p.kv_heads = k.size(1), p.n_query = n_query, p.n_key = n_key;
+    p.head_dim = q.size(3);
+    set_strides(p.q_stride, q), set_strides(p.k_stride, k), set_strides(p.v_stride, v);
+    p.scale = static_cast<float>(rules.scale), p.score_cap = static_cast<float>(rules.score_cap);
+    p.log_mass = ptr<float>(log_mass), p.slopes = ptr<float>(slopes), p.bucket_table = ptr<float>(table);
+    starts.assign(rules.bucket_starts.begin(), rules.bucket_starts.end());
+    p.bucket_starts = starts.data(), p.n_starts = static_cast<int32_t>(starts.size());
+    p.n_buckets = table.defined() ? static_cast<int32_t>(table.size(0)) : 0;
+    p.bidirectional = rules.bidirectional, p.causal = rules.causal;
+    p.prefix_lengths = ptr<int32_t>(prefix), p.query_documents = ptr<int32_t>(query_documents);
+    p.key_documents = ptr<int32_t>(key_documents), p.key_lengths = ptr<int32_t>(key_lengths);
+    p.query_starts = ptr<int32_t>(query_starts);
+  }
+};
+
+// [out, lse]; lse (fp32 [batch, heads, n_query], what the gradients need of the forward) is empty
+// unless wanted.
+std::tuple<Tensor, Tensor> masked_attention(
+    const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass, const OptTensor& slopes,
+    const OptTensor& table, const OptTensor& prefix, const OptTensor& query_documents, const OptTensor& key_documents,
+    const OptTensor& key_lengths, const OptTensor& query_starts, double scale, double score_cap,
+    at::IntArrayRef bucket_starts, bool bidirectional, bool causal, bool want_lse) {
+  const MaskedProblem m(q, k, v, {log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths,
+                                  query_starts, scale, score_cap, bucket_starts.vec(), bidirectional, causal});
+  const int dtype = dtype_code(q.scalar_type());
+  const Tensor out = in_layout_of(q);
+  const Tensor lse = at::empty({want_lse ? q.size(0) : 0, q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  size_t need = 0;
+  check(vgo_masked_attn_workspace(&m.p, dtype, &need));
+  const Tensor ws = need > 0 ? scratch(need, q) : Tensor();
+  int64_t stride[3];
+  set_strides(stride, out);
+  check(vgo_masked_attn_fwd(&m.p, ptr(out), stride, want_lse ? ptr<float>(lse) : nullptr, dtype, ptr(ws), need,
+                            stream_of(q)));
+  return {out, lse};
+}
+
+// Gradients of q, k, v, log_mass, slopes and table (fp32 the last three); those not wanted are empty
+// (k and v come together).
+std::vector<Tensor> masked_attention_grad(
+    const Tensor& grad0, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass,
+    const OptTensor& slopes, const OptTensor& table, const OptTensor& prefix, const OptTensor& query_documents,
+    const OptTensor& key_documents, const OptTensor& key_lengths, const OptTensor& query_starts, const Tensor& out0,
+    const Tensor& lse, double scale, double score_cap, at::IntArrayRef bucket_starts, bool bidirectional, bool causal,
+    c10::List<bool> want) {
+  const MaskedProblem m(q, k, v, {log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths,
+                                  query_starts, scale, score_cap, bucket_starts.vec(), bidirectional, causal});
+  require_gpu({&grad0, &out0, &lse});
+  TORCH_CHECK_VALUE(want.size() == 6, "masked_attention_grad: want names six gradients");
+  TORCH_CHECK_VALUE(grad0.sizes() == q.sizes() && grad0.scalar_type() == q.scalar_type() &&
+                        out0.sizes() == q.sizes() && out0.scalar_type() == q.scalar_type(),
+                    "masked_attention_grad: out and its gradient must be like q");
+  TORCH_CHECK_VALUE(lse.dim() == 3 && lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat &&
+                        lse.is_contiguous(),
+                    "masked_attention_grad: lse must be contiguous float32 [batch, heads, n_query]");
+  TORCH_CHECK(grad0.device() == q.device() && out0.device() == q.device() && lse.device() == q.device(),
+              "masked_attention_grad: every tensor must be on the device of q");
+  const Tensor grad = operand(grad0), out = operand(out0);
+  vgo_masked_attn_grads g{};
+  g.out = ptr(out), g.grad_out = ptr(grad), g.lse = ptr<float>(lse);
+  set_strides(g.out_stride, out), set_strides(g.grad_out_stride, grad);
+  const bool keys = want.get(1) || want.get(2);
+  const Tensor none = at::empty({0}, q.options());
+  const Tensor dq = want.get(0) ? in_layout_of(q) : none, dk = keys ? in_layout_of(k) : none;
+  const Tensor dv = keys ? in_layout_of(v) : none;
+  const auto fill = [&](void*& p, int64_t (&stride)[3], const Tensor& t, bool wanted) {
+    if (!wanted || t.numel() == 0) return;
+    p = ptr(t);
+    set_strides(stride, t);
+  };
+  fill(g.dq, g.dq_stride, dq, want.get(0)), fill(g.dk, g.dk_stride, dk, keys), fill(g.dv, g.dv_stride, dv, keys);
+  const auto make = [&](bool wanted, const Tensor& of, float*& p) {
+    const Tensor t = wanted && of.defined() ? at::empty(of.sizes(), of.options()) : none;
+    if (wanted && of.defined()) p = ptr<float>(t);
+    return t;
+  };
+  const Tensor d_mass = make(want.get(3), m.log_mass, g.d_log_mass);
+  const Tensor d_slopes = make(want.get(4), m.slopes, g.d_slopes), d_table = make(want.get(5), m.table, g.d_table);
+  const int dtype = dtype_code(q.scalar_type());
+  size_t need = 0;
+  check(vgo_masked_attn_grad_workspace(&m.p, &g, dtype, &need));
+  const Tensor ws = need > 0 ? scratch(need, q) : Tensor();
+  check(vgo_masked_attn_grad(&m.p, &g, dtype, ptr(ws), need, stream_of(q)));
+  return {dq, dk, dv, d_mass, d_slopes, d_table};
+}
+
+// ------------------------------------------------------------ position bias ----
+Tensor position_bias(const Tensor& table0, int64_t n_query, int64_t n_key, int64_t query_start,
+                     at::IntArrayRef bucket_starts, bool bidirectional) {
+  require_gpu({&table0});
+  TORCH_CHECK_VALUE(table0.dim() == 2 && table0.size(1) > 0, "position_bias: the table must be [buckets, heads]");
+  TORCH_CHECK_VALUE(n_query >= 0 && n_key >= 0, "position_bias: negative size");
+  const Tensor table = table0.contiguous();
+  const std::vector<int32_t> starts(bucket_starts.begin(), bucket_starts.end());
+  const int dtype = dtype_code(table.scalar_type());
+  Tensor out = at::empty({table.size(1), n_query, n_key}, table.options());
+  check(vgo_position_bias(ptr(table), table.size(0), table.size(1), starts.data(),
+                          static_cast<int32_t>(starts.size()), bidirectional, query_start, n_query, n_key, ptr(out),
+                          dtype, stream_of(table)));
+  return out;
+}
+
+Tensor position_bias_grad(const Tensor& grad0, int64_t n_buckets, int64_t query_start, at::IntArrayRef bucket_starts,
+                          bool bidirectional) {
+  require_gpu({&grad0});
+  TORCH_CHECK_VALUE(grad0.dim() == 3 && grad0.size(0) > 0, "position_bias_grad: grad must be [heads, n_query, n_key]");
+  const Tensor grad = grad0.contiguous();
+  const std::vector<int32_t> starts(bucket_starts.begin(), bucket_starts.end());
+  const int dtype = dtype_code(grad.scalar_type());
+  Tensor out = at::empty({n_buckets, grad.size(0)}, grad.options());
+  size_t need = 0;
+  check(vgo_position_bias_grad_workspace(n_buckets, grad.size(0), grad.size(1), grad.size(2), &need));
+  const Tensor ws = need > 0 ? scratch(need, grad) : Tensor();
+  check(vgo_position_bias_grad(ptr(grad), n_buckets, grad.size(0), starts.data(), static_cast<int32_t>(starts.size()),
+                               bidirectional, query_start, grad.size(1), grad.size(2), ptr(out), dtype, ptr(ws), need,
+                               stream_of(grad)));
+  return out;
 }
 
 // --------------------------------------------------------------- projection ----
@@ -692,6 +887,9 @@ constexpr const char* kPlan[] = {"normalize_rows", "csr_build", "corner_csr", "s
                                  "fastvggt_match", "fastvggt_plan"};
 constexpr const char* kPlanInto[] = {"similarity_topk", "rope_table"};
 
+// Operators with a derivative, and those of their derivatives (path operators: no second one).
+constexpr const char* kGradients[] = {"masked_attention_grad", "position_bias_grad"};
+
 template <typename Visit>
 void each_tensor(const c10::IValue& value, Visit visit) {
   if (value.isTensor()) {
@@ -730,6 +928,107 @@ void autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::ji
     each_tensor(value, [&](const Tensor& t) {
       if (torch::autograd::isDifferentiableType(t.scalar_type())) torch::autograd::set_history(t, node);
     });
+}
+
+// A floating tensor that takes part in a recorded graph.  A tangent on one is refused: there is no
+// forward-mode derivative (tangents of tensors that require no grad end here, as at the path's operators).
+bool records(std::initializer_list<const Tensor*> tensors, const char* name) {
+  if (!at::GradMode::is_enabled()) return false;
+  bool any = false, tangent = false;
+  for (const Tensor* t : tensors)
+    if (t != nullptr && t->defined()) any |= t->requires_grad(), tangent |= t->_fw_grad(/*level=*/0).defined();
+  TORCH_CHECK_NOT_IMPLEMENTED(!any || !tangent, name, ": no forward-mode derivative");
+  return any;
+}
+template <typename Signature>
+auto typed_operator(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+// As c10::IValue: an optional tensor of a saved list, undefined for none.
+Tensor or_undefined(const OptTensor& t) { return opt(t) == nullptr ? Tensor() : *t; }
+OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct MaskedAttentionFunction : torch::autograd::Function<MaskedAttentionFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        const OptTensor& log_mass, const OptTensor& slopes, const OptTensor& table,
+                        const OptTensor& prefix, const OptTensor& query_documents, const OptTensor& key_documents,
+                        const OptTensor& key_lengths, const OptTensor& query_starts, double scale, double score_cap,
+                        at::IntArrayRef bucket_starts, bool bidirectional, bool causal) {
+    static const auto op = typed_operator<decltype(masked_attention)>("vgo::masked_attention");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, lse] = op.call(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths,
+                              query_starts, scale, score_cap, bucket_starts, bidirectional, causal, true);
+    ctx->save_for_backward({q, k, v, or_undefined(log_mass), or_undefined(slopes), or_undefined(table),
+                            or_undefined(prefix), or_undefined(query_documents), or_undefined(key_documents),
+                            or_undefined(key_lengths), or_undefined(query_starts), out, lse});
+    ctx->saved_data["scale"] = scale, ctx->saved_data["score_cap"] = score_cap;
+    ctx->saved_data["starts"] = bucket_starts.vec();
+    ctx->saved_data["bidirectional"] = bidirectional, ctx->saved_data["causal"] = causal;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = typed_operator<decltype(masked_attention_grad)>("vgo::masked_attention_grad");
+    const variable_list s = ctx->get_saved_variables();
+    c10::List<bool> want;
+    size_t edge = 0;  // of the inputs that are there
+    for (size_t i = 0; i < 6; ++i) want.push_back(s[i].defined() && ctx->needs_input_grad(edge++));
+    const std::vector<Tensor> d =
+        op.call(grads[0], s[0], s[1], s[2], or_none(s[3]), or_none(s[4]), or_none(s[5]), or_none(s[6]), or_none(s[7]),
+                or_none(s[8]), or_none(s[9]), or_none(s[10]), s[11], s[12], ctx->saved_data["scale"].toDouble(),
+                ctx->saved_data["score_cap"].toDouble(), ctx->saved_data["starts"].toIntVector(),
+                ctx->saved_data["bidirectional"].toBool(), ctx->saved_data["causal"].toBool(), want);
+    variable_list result(16);
+    for (size_t i = 0; i < 6; ++i)
+      if (want.get(i)) result[i] = i < 3 ? d[i] : d[i].to(s[i].scalar_type());
+    return result;
+  }
+};
+
+std::tuple<Tensor, Tensor> masked_attention_autograd(
+    const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass, const OptTensor& slopes,
+    const OptTensor& table, const OptTensor& prefix, const OptTensor& query_documents, const OptTensor& key_documents,
+    const OptTensor& key_lengths, const OptTensor& query_starts, double scale, double score_cap,
+    at::IntArrayRef bucket_starts, bool bidirectional, bool causal, bool want_lse) {
+  if (records({&q, &k, &v, opt(log_mass), opt(slopes), opt(table)}, "masked_attention")) {
+    const Tensor out = MaskedAttentionFunction::apply(q, k, v, log_mass, slopes, table, prefix, query_documents,
+                                                      key_documents, key_lengths, query_starts, scale, score_cap,
+                                                      bucket_starts, bidirectional, causal);
+    return {out, at::empty({0, q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
+  }
+  static const auto op = typed_operator<decltype(masked_attention)>("vgo::masked_attention");
+  const at::AutoDispatchBelowAutograd below;
+  return op.call(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts,
+                 scale, score_cap, bucket_starts, bidirectional, causal, want_lse);
+}
+
+struct PositionBiasFunction : torch::autograd::Function<PositionBiasFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, int64_t n_query, int64_t n_key, int64_t query_start,
+                        at::IntArrayRef bucket_starts, bool bidirectional) {
+    static const auto op = typed_operator<decltype(position_bias)>("vgo::position_bias");
+    ctx->saved_data["buckets"] = table.size(0), ctx->saved_data["start"] = query_start;
+    ctx->saved_data["starts"] = bucket_starts.vec(), ctx->saved_data["bidirectional"] = bidirectional;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(table, n_query, n_key, query_start, bucket_starts, bidirectional);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = typed_operator<decltype(position_bias_grad)>("vgo::position_bias_grad");
+    variable_list result(6);
+    result[0] = op.call(grads[0], ctx->saved_data["buckets"].toInt(), ctx->saved_data["start"].toInt(),
+                        ctx->saved_data["starts"].toIntVector(), ctx->saved_data["bidirectional"].toBool());
+    return result;
+  }
+};
+
+Tensor position_bias_autograd(const Tensor& table, int64_t n_query, int64_t n_key, int64_t query_start,
+                              at::IntArrayRef bucket_starts, bool bidirectional) {
+  if (records({&table}, "position_bias"))
+    return PositionBiasFunction::apply(table, n_query, n_key, query_start, bucket_starts, bidirectional);
+  static const auto op = typed_operator<decltype(position_bias)>("vgo::position_bias");
+  const at::AutoDispatchBelowAutograd below;
+  return op.call(table, n_query, n_key, query_start, bucket_starts, bidirectional);
 }
 
 // ADInplaceOrView key of operators that write arguments: their versions count the write.
@@ -794,6 +1093,10 @@ void register_cuda(torch::Library& m) {
   m.impl("fastvggt_plan", on_device<fastvggt_plan>);
   m.impl("similarity_topk", on_device<similarity_topk>);
   m.impl("merged_block", on_device<merged_block>);
+  m.impl("masked_attention", on_device<masked_attention>);
+  m.impl("masked_attention_grad", on_device<masked_attention_grad>);
+  m.impl("position_bias", on_device<position_bias>);
+  m.impl("position_bias_grad", on_device<position_bias_grad>);
 }
 
 void register_autograd(torch::Library& m) {
@@ -802,6 +1105,9 @@ void register_autograd(torch::Library& m) {
   for (const char* name : kBlocks) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
   for (const char* name : kPlan) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<false>>());
   for (const char* name : kPlanInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<false>>());
+  for (const char* name : kGradients) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
+  m.impl("masked_attention", masked_attention_autograd);
+  m.impl("position_bias", position_bias_autograd);
 }
 
 void register_inplace(torch::Library& m) {

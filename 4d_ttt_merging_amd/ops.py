@@ -27,6 +27,10 @@ dispatcher, `torch.compile` and fake-tensor tracing see them as single ops:
   `fastvggt_assemble`, `fastvggt_plan`, `csr_build`, `corner_csr`,
   `segment_mass`).
 
+* `vgo::masked_attention` (with `masked_attention_grad`) and `vgo::position_bias` (with
+  `position_bias_grad`) -- attention under score caps, position biases and masks, and the dense
+  bias by buckets; both have gradients.
+
 The CUDA (HIP) implementations are native (csrc/torch_ops.cpp, built into
 `libvgo_ops.so`) and call `libvgo.so` through its C ABI.  The operators a
 traced graph can hold have fake implementations that only describe their
@@ -99,6 +103,20 @@ _SCHEMAS = (
     "int removed) -> (Tensor, Tensor, Tensor)",
     "fastvggt_plan(Tensor best, Tensor target, Tensor sources, Tensor destinations, int total, "
     "int removed) -> Tensor[]",
+    # [out, lse] of vgo_masked_attn_fwd; lse (fp32 [B, H, Nq]) is empty unless wanted.
+    "masked_attention(Tensor q, Tensor k, Tensor v, Tensor? log_mass, Tensor? slopes, Tensor? table, "
+    "Tensor? prefix, Tensor? query_documents, Tensor? key_documents, Tensor? key_lengths, Tensor? query_starts, "
+    "float scale, float score_cap, int[] bucket_starts, bool bidirectional, bool causal, bool want_lse) "
+    "-> (Tensor, Tensor)",
+    # Gradients of q, k, v, log_mass, slopes, table; unwanted ones are empty.
+    "masked_attention_grad(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor? log_mass, Tensor? slopes, "
+    "Tensor? table, Tensor? prefix, Tensor? query_documents, Tensor? key_documents, Tensor? key_lengths, "
+    "Tensor? query_starts, Tensor out, Tensor lse, float scale, float score_cap, int[] bucket_starts, "
+    "bool bidirectional, bool causal, bool[] want) -> Tensor[]",
+    "position_bias(Tensor table, int n_query, int n_key, int query_start, int[] bucket_starts, "
+    "bool bidirectional) -> Tensor",
+    "position_bias_grad(Tensor grad, int n_buckets, int query_start, int[] bucket_starts, bool bidirectional) "
+    "-> Tensor",
 )
 
 _library = torch.library.Library("vgo", "DEF")
@@ -226,3 +244,37 @@ def _(best, target, sources, destinations, total, removed):
             sources.new_empty((1, n_src), dtype=torch.uint8), sources.new_empty((total,), **i32),
             sources.new_empty((total,), **i32), sources.new_empty((kept + 1,), **i32),
             sources.new_empty((kept,), **f32), sources.new_empty((kept,), **f32)]
+
+
+def _in_layout_of(t):
+    """As the kernels lay out a result: token-major where `t` is."""
+    b, h, n, d = t.shape
+    if h > 1 and t.stride(2) > t.stride(1):
+        return t.new_empty((b, n, h, d)).transpose(1, 2)
+    return t.new_empty((b, h, n, d))
+
+
+@_fake("masked_attention")
+def _(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts, scale,
+      score_cap, bucket_starts, bidirectional, causal, want_lse):
+    return _in_layout_of(q), q.new_empty((q.shape[0] if want_lse else 0, q.shape[1], q.shape[2]), dtype=torch.float32)
+
+
+@_fake("masked_attention_grad")
+def _(grad, q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts, out,
+      lse, scale, score_cap, bucket_starts, bidirectional, causal, want):
+    keys = want[1] or want[2]
+    none = q.new_empty((0,))
+    result = [_in_layout_of(t) if w else none for t, w in ((q, want[0]), (k, keys), (v, keys))]
+    return result + [t.new_empty(t.shape, dtype=torch.float32) if w and t is not None else none
+                     for t, w in zip((log_mass, slopes, table), want[3:])]
+
+
+@_fake("position_bias")
+def _(table, n_query, n_key, query_start, bucket_starts, bidirectional):
+    return table.new_empty((table.shape[1], n_query, n_key))
+
+
+@_fake("position_bias_grad")
+def _(grad, n_buckets, query_start, bucket_starts, bidirectional):
+    return grad.new_empty((n_buckets, grad.shape[0]))

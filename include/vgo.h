@@ -553,6 +553,98 @@ int vgo_restore_residual_layer_norm(const float* x, int64_t x_row_stride, const 
                                     int64_t x_out_row_stride, void* norm_out,
                                     int64_t norm_row_stride, int norm_dtype, void* stream);
 
+/*
+ * Masked attention with position biases, its gradients and its single-token form.  No counterpart in
+ * the reference, whose attention is unmasked and inference only (models/mass_bias_attention.py:85-129).
+ *
+ *   z_ij = cap * tanh(scale * q_i.k_j / cap) + log_mass[j] - slopes[h] * |r| + bucket_table[bucket(r), h]
+ *   r = j - (query_starts[b] + i)
+ *   out_i = sum_j softmax_j(z_ij) v_j over the pairs that attend: j < key_lengths[b]; the documents of
+ *   i and j are equal and not negative; and, if causal, r <= 0 or j < prefix_lengths[b].
+ * A query without such a key gives zeros (and an lse of +inf).
+ *
+ * q [batch, heads, n_query, head_dim], k / v [batch, kv_heads, n_key, head_dim], head_dim 64 or 128,
+ * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)); strides in elements for
+ * (batch, head, token), multiples of 16 bytes, with a unit channel stride; pointers 16-byte aligned.
+ * Types as in vgo_mass_bias_attn_fwd; everything beside q, k, v is fp32 or int32.
+ *   score_cap > 0: scores capped by a tanh (0: not).
+ *   log_mass [n_key] (taken in fp32, not rounded), slopes [heads], bucket_table [n_buckets, heads].
+ *   bucket(r) = the number of bucket_starts (host, ascending, > 0, at most 128, the last one at most
+ *     1024) that are <= |r|, plus n_buckets / 2 for r > 0 if bidirectional; else of max(-r, 0).
+ *   key_documents [batch, n_key] with query_documents [batch, n_query] (contiguous): both or neither.
+ *   prefix_lengths, key_lengths (values above n_key mean n_key), query_starts [batch]: device arrays or
+ *     NULL (no prefix, n_key, n_key - n_query).
+ * Keys past key_lengths and keys of negative documents are not read: they may hold anything.  Values of
+ * other pairs that do not attend may be anything finite.
+ */
+typedef struct vgo_masked_attn {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t batch, heads, kv_heads, n_query, n_key, head_dim;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  float scale, score_cap;
+  const float* log_mass;
+  const float* slopes;
+  const float* bucket_table;
+  const int32_t* bucket_starts;
+  int32_t n_buckets, n_starts, bidirectional, causal;
+  const int32_t* prefix_lengths;
+  const int32_t* query_documents;
+  const int32_t* key_documents;
+  const int32_t* key_lengths;
+  const int32_t* query_starts;
+} vgo_masked_attn;
+
+/*
+ * The forward: out (of the inputs' type, strides as theirs) and, where not NULL, lse [batch, heads,
+ * n_query] fp32: log2 of the row's sum of e^z, for vgo_masked_attn_grad.  Workspace (16-byte aligned, any contents):
+ * document ranges of the key tiles and the partial states of work split over the keys; its size is
+ * for the device that is current.
+ */
+int vgo_masked_attn_workspace(const vgo_masked_attn* problem, int dtype, size_t* bytes);
+int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, const int64_t out_stride[3], float* lse,
+                        int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of the forward for grad_out, from its out and lse.  dq / dk / dv have the inputs' type;
+ * dk / dv sum over the heads that share them; d_log_mass [n_key], d_slopes [heads] and d_table
+ * [n_buckets, heads] are fp32.  Outputs that are NULL are not computed (dk and dv: both or neither).
+ * Sums are in a fixed order: the same inputs give the same bits.
+ */
+typedef struct vgo_masked_attn_grads {
+  const void* out;
+  const void* grad_out;
+  const float* lse;
+  int64_t out_stride[3], grad_out_stride[3];
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+  float* d_log_mass;
+  float* d_slopes;
+  float* d_table;
+} vgo_masked_attn_grads;
+int vgo_masked_attn_grad_workspace(const vgo_masked_attn* problem, const vgo_masked_attn_grads* grads, int dtype,
+                                   size_t* bytes);
+int vgo_masked_attn_grad(const vgo_masked_attn* problem, const vgo_masked_attn_grads* grads, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Relative position bias by buckets, dense: out[h, i, j] = table[bucket(j - query_start - i), h] with
+ * bucket() as above, table [n_buckets, heads] and out [heads, n_query, n_key] contiguous of `dtype`; and its gradient d_table[t, h] = the sum of grad[h, i, j] over the pairs of bucket t, added up
+ * in fp32 in a fixed order.  No counterpart in the reference.
+ */
+int vgo_position_bias(const void* table, int64_t n_buckets, int64_t heads, const int32_t* bucket_starts,
+                      int32_t n_starts, int32_t bidirectional, int64_t query_start, int64_t n_query,
+                      int64_t n_key, void* out, int dtype, void* stream);
+int vgo_position_bias_grad_workspace(int64_t n_buckets, int64_t heads, int64_t n_query, int64_t n_key,
+                                     size_t* bytes);
+int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64_t heads, const int32_t* bucket_starts,
+                           int32_t n_starts, int32_t bidirectional, int64_t query_start, int64_t n_query,
+                           int64_t n_key, void* d_table, int dtype, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif
