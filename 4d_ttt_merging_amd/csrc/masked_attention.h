@@ -63,7 +63,7 @@ struct Op<float> {
 // Accumulator registers 8 c .. 8 c + 7 as an operand of T (bf16 / f16: rounded, as both products of
 // a 16-bit attention take their probabilities).
 template <typename T>
-__device__ __forceinline__ typename Op<T>::op8 as_op(const f32x16& s, int c) {
+__device__ __forceinline__ typename Op<T>::op8 as_op(const float (&s)[16], int c) {
   typename Op<T>::op8 r;
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = from_f32<T>(s[8 * c + e]);
@@ -89,14 +89,19 @@ struct Tile {
     return ((row & 3) << 2) | ((row >> 2) & 3);
   }
 
+  // Where the lane's 16 bytes of rows_op() of a 16-bit type lie in the tile.
+  static __device__ __forceinline__ int rows_at(int row0, int t) {
+    const int lane = lane_id();
+    return (row0 + (lane & 31)) * kRowBytes + (((2 * t + (lane >> 5)) ^ swz(lane & 15)) << 4);
+  }
   // A operand with rows row0 + l % 32 (row0 a multiple of 16), channels 16 t + 8 (l / 32) ..
   static __device__ __forceinline__ op8 rows_op(const char* tile, int row0, int t) {
-    const int lane = lane_id(), row = row0 + (lane & 31), h = lane >> 5;
-    const char* base = tile + row * kRowBytes;
-    const int f = swz(lane & 15);
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const op8*>(base + (((2 * t + h) ^ f) << 4));
+      return *reinterpret_cast<const op8*>(tile + rows_at(row0, t));
     } else {
+      const int lane = lane_id(), row = row0 + (lane & 31), h = lane >> 5;
+      const char* base = tile + row * kRowBytes;
+      const int f = swz(lane & 15);
       const f32x4 a = *reinterpret_cast<const f32x4*>(base + (((4 * t + 2 * h) ^ f) << 4));
       const f32x4 b = *reinterpret_cast<const f32x4*>(base + (((4 * t + 2 * h + 1) ^ f) << 4));
       return op8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -217,6 +222,7 @@ struct Args {
   int64_t qs[3], ks[3], vs[3], os[3];
   int batch, heads, kv_heads, n_query, n_key;
   float scale, inv_cap, cap2;     // scale; scale / cap and cap log2(e) (0: no cap)
+  float cap_reach, cap_series[5]; // kCapReach and kCapSeries for products before the scale (reach 0: not used)
   const float* mass;              // [n_key] or null
   const float* slopes;            // [heads] or null
   const float* table;             // [n_buckets, heads] or null
@@ -302,9 +308,22 @@ int sum_parts(const float* part, int64_t parts, int64_t n, T* out, hipStream_t s
   return check_launch("sum of parts");
 }
 
-// tanh of the capped scores.  1 - 2 / (1 + e^2y) loses what 1 takes from a small y: about 1e-7
-// absolute, i.e. 5e-6 in a score capped at 50, below the rounding of 16-bit inputs; fp32 takes the
-// odd series below 0.3 (its next term is 1e-9).
+// tanh of the capped scores.  For 16-bit inputs, where |y| stays below kCapReach, an odd polynomial (weighted least
+// squares at Chebyshev points towards the least largest error: 2e-7), six full-rate instructions in
+// place of two quarter-rate ones and three more; past it, and for fp32, 1 - 2 / (1 + e^2y), whose
+// 1 costs a small y about 1e-7 -- 5e-6 in a score capped at 50, below the rounding of 16-bit
+// inputs -- so that fp32 takes the odd series below 0.3 (its next term is 1e-9).
+constexpr float kCapReach = 0.75f;
+// tanh(y) / y in powers of y^2.
+constexpr float kCapSeries[5] = {0.999997228f, -0.333230765f, 0.132260916f, -0.0492804483f, 0.0123188331f};
+template <typename T>
+__device__ __forceinline__ float cap_short(const Args<T>& a, float s) {  // of the raw product s
+  const float u = s * s;
+  float x = fmaf(u, a.cap_series[4], a.cap_series[3]);
+  x = fmaf(x, u, a.cap_series[2]);
+  x = fmaf(x, u, a.cap_series[1]);
+  return s * fmaf(x, u, a.cap_series[0]);
+}
 template <typename T>
 __device__ __forceinline__ float cap_tanh(float y) {
   const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
@@ -318,6 +337,19 @@ __device__ __forceinline__ float cap_tanh(float y) {
     t = fabsf(y) < 0.3f ? fmaf(-y * y2, s, y) : t;
   }
   return t;
+}
+
+// Row sums of probabilities as the products take them: of bf16 the rounded values, two per instruction,
+// so that their rounding cancels where one key has most of a row (f16 and fp32: what is not
+// worth a second look, the sum of the unrounded ones; the two-value form would drop f16's subnormals).
+template <typename T>
+__device__ __forceinline__ float add_pair(float sum, float a, float b, T, T) {
+  return sum + a + b;
+}
+template <>
+__device__ __forceinline__ float add_pair<bf16_t>(float sum, float, float, bf16_t a, bf16_t b) {
+  const bf16x2 pair = {a, b}, one = {static_cast<bf16_t>(1.0f), static_cast<bf16_t>(1.0f)};
+  return __builtin_amdgcn_fdot2_f32_bf16(pair, one, sum, false);
 }
 
 inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
@@ -339,7 +371,15 @@ Args<T> make_args(const vgo_masked_attn* p) {
   a.kv_heads = static_cast<int>(p->kv_heads);
   a.n_query = static_cast<int>(p->n_query), a.n_key = static_cast<int>(p->n_key);
   a.scale = p->scale;
-  if (p->score_cap > 0.0f) a.inv_cap = p->scale / p->score_cap, a.cap2 = p->score_cap * kLog2e;
+  if (p->score_cap > 0.0f) {
+    a.inv_cap = p->scale / p->score_cap, a.cap2 = p->score_cap * kLog2e;
+    if (sizeof(T) == 2 && a.inv_cap > 1e-3f && a.inv_cap < 1e3f) {  // (its ninth power is a normal number)
+      a.cap_reach = kCapReach / a.inv_cap;
+      double power = a.inv_cap;
+      for (int i = 0; i < 5; ++i, power *= static_cast<double>(a.inv_cap) * a.inv_cap)
+        a.cap_series[i] = static_cast<float>(kCapSeries[i] * power);
+    }
+  }
   a.mass = p->log_mass, a.slopes = p->slopes, a.table = p->bucket_table;
   if (a.table) a.buckets = make_buckets(p->n_buckets, p->bucket_starts, p->n_starts, p->bidirectional);
   a.causal = p->causal != 0, a.query_start = a.n_key - a.n_query;

@@ -1,0 +1,11 @@
+// Masked attention, forward, of bf16.
+#include "masked_attention_fwd.h"
+
+namespace vgo {
+namespace masked {
+
+template int run_forward<bf16_t>(const vgo_masked_attn*, const ForwardPlan&, void*, const int64_t[3], float*, char*,
+                                 hipStream_t);
+
+}  // namespace masked
+}  // namespace vgo

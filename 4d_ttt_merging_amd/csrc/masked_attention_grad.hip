@@ -32,7 +32,7 @@ struct Grad {
   int key_blocks, row_blocks, key_tasks, row_tasks;
 };
 
-constexpr int kWaves = 4, kBlock = 32 * kWaves;
+constexpr int kWaves = 4, kBlock = 32 * kWaves;  // of the queries' side
 
 // delta and empty: four lanes a row, a work-group per tile of one head.
 template <typename T, int D>
@@ -62,18 +62,45 @@ __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
   if (threadIdx.x == 0) f.empty[blockIdx.x] = any;
 }
 
+// Raw products of one 32 x 32 block to what the factor returned makes exponents of 2; with a cap, to
+// their tanh, and cap' in `bend`.
+template <typename T, bool kCap>
+__device__ __forceinline__ float rescore(const Args<T>& a, float (&x)[16], float (&bend)[16]) {
+  if constexpr (!kCap) {
+    return a.scale * kLog2e;
+  } else {
+    float most = fabsf(x[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) most = fmaxf(most, fabsf(x[r]));
+    if (__any(!(most <= a.cap_reach))) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = cap_tanh<T>(x[r] * a.inv_cap);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = cap_short(a, x[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bend[r] = fmaf(-x[r], x[r], 1.0f);
+    return a.cap2;
+  }
+}
+
 // ------------------------------------------------------------ keys' side ----
 // LDS: Q and dO tiles (two buffers), lse, delta and documents of their rows, distance biases.
 template <typename T, int D>
 struct KeyLds {
-  static constexpr int kLse = 4 * Tile<T, D>::kBytes, kDelta = kLse + 2 * kTile * 4, kDocs = kDelta + 2 * kTile * 4;
+  static constexpr bool kValues = sizeof(T) == 2;  // V of the wave's keys in LDS, not in registers
+  static constexpr int kWaves = sizeof(T) == 2 && D == 128 ? 8 : 4, kBlock = 32 * kWaves;
+  static constexpr int kV = 4 * Tile<T, D>::kBytes, kLse = kV + (kValues ? kWaves * Tile<T, D>::kBytes / 2 : 0);
+  static constexpr int kDelta = kLse + 2 * kTile * 4, kDocs = kDelta + 2 * kTile * 4;
   static constexpr int kDistances = kDocs + 2 * kTile * 4;
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) void key_kernel(const Grad<T> f) {
+template <typename T, int D, bool kCap, bool kBias>
+__global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D == 64 ? 3 : 2) void key_kernel(const Grad<T> f) {
   typedef Tile<T, D> TL;
   typedef KeyLds<T, D> LO;
+  constexpr int kWaves = LO::kWaves, kBlock = LO::kBlock;
   typedef typename Op<T>::op8 op8;
   extern __shared__ __align__(16) char lds[];
   const Args<T>& a = f.a;
@@ -93,14 +120,19 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) voi
   const bool taken = key < limit && doc >= 0;
   const float mass2 = a.mass && key < a.n_key ? a.mass[key] * kLog2e : 0.0f;
 
-  op8 k[TL::kSteps], v[TL::kSteps];
+  op8 k[TL::kSteps], v[LO::kValues ? 1 : TL::kSteps];
+  const char* vl = lds + LO::kV + wave * (TL::kBytes / 2);
   {
     const T* kp = a.k + b * a.ks[0] + kvh * a.ks[1] + static_cast<int64_t>(min(key, a.n_key - 1)) * a.ks[2] + 8 * h;
     const T* vp = a.v + b * a.vs[0] + kvh * a.vs[1] + static_cast<int64_t>(min(key, a.n_key - 1)) * a.vs[2] + 8 * h;
 #pragma unroll
     for (int t = 0; t < TL::kSteps; ++t) {
       k[t] = taken ? *reinterpret_cast<const op8*>(kp + 16 * t) : op8{};
-      v[t] = taken ? *reinterpret_cast<const op8*>(vp + 16 * t) : op8{};
+      const op8 x = taken ? *reinterpret_cast<const op8*>(vp + 16 * t) : op8{};
+      if constexpr (LO::kValues)
+        *reinterpret_cast<op8*>(lds + LO::kV + wave * (TL::kBytes / 2) + TL::rows_at(0, t)) = x;
+      else
+        v[t] = x;
     }
   }
   // Ranges of the work-group's and the wave's keys; rows that are none's narrow only the documents.
@@ -113,9 +145,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) voi
     for (int off = 16; off >= 1; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
     rw.doc_lo = __builtin_amdgcn_readfirstlane(lo), rw.doc_hi = __builtin_amdgcn_readfirstlane(hi);
     rw.docs_whole = __all(taken);
-    const int tiles = (a.n_key + kTile - 1) / kTile, t0 = 2 * block;
+    constexpr int kSpan = kBlock / kTile;
+    const int tiles = (a.n_key + kTile - 1) / kTile, t0 = kSpan * block;
     rg.doc_lo = INT_MAX, rg.doc_hi = -1, rg.docs_whole = false;
-    for (int t = t0; t < min(t0 + 2, tiles); ++t) {
+    for (int t = t0; t < min(t0 + kSpan, tiles); ++t) {
       const Range r = info_range(a.key_info[static_cast<int64_t>(b) * tiles + t]);
       rg.doc_lo = min(rg.doc_lo, r.doc_lo), rg.doc_hi = max(rg.doc_hi, r.doc_hi);
     }
@@ -179,6 +212,116 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) voi
       lds_dma4(a.query_doc + static_cast<int64_t>(b) * a.n_query, i, lds0 + LO::kDocs + buf * kTile * 4);
   };
 
+  const auto compute = [&](bool partial, int q0, int head, int buf) {
+    const char* qt = lds + 2 * buf * TL::kBytes;
+    const char* gt = qt + TL::kBytes;
+    const float* lse = reinterpret_cast<const float*>(lds + LO::kLse) + buf * kTile;
+    const float* delta = reinterpret_cast<const float*>(lds + LO::kDelta) + buf * kTile;
+    const int* tags = reinterpret_cast<const int*>(lds + LO::kDocs) + buf * kTile;
+    const int p0 = start + q0;  // position of the tile's first row
+    // One 32-row half at a time, and the scheduling barriers, keep what is live within the registers
+    // that two waves (64 channels: three) a SIMD leave: without them the compiler reads operands ahead and
+    // spills.
+#pragma unroll 1
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 s{};
+#pragma unroll
+      for (int t = 0; t < TL::kSteps; ++t) s = Op<T>::mma(TL::rows_op(qt, 32 * sub, t), k[t], s);
+      const int i0 = 32 * sub + 4 * h;  // row of register r: q0 + i0 + 8 (r / 4) + r % 4
+      __builtin_amdgcn_sched_barrier(0);
+      float x[16], bend[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = s[r];
+      const float c = rescore<T, kCap>(a, x, bend);
+      if constexpr (kBias) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], c, mass2);
+        if (a.slopes) {
+          const float slope2 = a.slopes[head] * kLog2e, d0 = static_cast<float>(key - p0 - i0);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            x[r] = fmaf(-slope2, fabsf(d0 - static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
+        }
+        if (a.table) {
+          const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances);
+          const int reach = a.buckets.reach;
+          if (rw.lo + 31 - p0 <= -reach || rw.lo - (p0 + kTile - 1) >= reach) {
+            const float far = distance[rw.lo > p0 ? 2 * reach : 0];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] += far;
+          } else {
+            const int d0 = key - p0 - i0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              x[r] += distance[max(-reach, min(reach, d0 - (8 * (r / 4) + r % 4))) + reach];
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + i0 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          x[r] = __builtin_amdgcn_exp2f(kBias ? x[r] - l4[e] : fmaf(x[r], c, -l4[e]));
+        }
+      }
+      if (partial) {
+        const int i_first = q0 + i0 - first_row;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          x[r] = static_cast<unsigned>(i_first + 8 * (r / 4) + r % 4) < row_count ? x[r] : 0.0f;
+        if (a.key_doc) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const i32x4 tag = *reinterpret_cast<const i32x4*>(tags + i0 + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = tag[e] == doc ? x[4 * g + e] : 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const op8 pb = as_op<T>(x, half);
+#pragma unroll
+        for (int dt = 0; dt < TL::kCols; ++dt) dv[dt] = Op<T>::mma(TL::cols_op(gt, dt, 2 * sub + half), pb, dv[dt]);
+      }
+      if constexpr (kCap && !kBias) {  // nothing else needs P alone
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= bend[r];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 dp{};
+#pragma unroll
+      for (int t = 0; t < TL::kSteps; ++t)
+        dp = Op<T>::mma(TL::rows_op(gt, 32 * sub, t), LO::kValues ? TL::rows_op(vl, 0, t) : v[LO::kValues ? 0 : t], dp);
+      __builtin_amdgcn_sched_barrier(0);
+      float dz[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + i0 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dz[4 * g + e] = x[4 * g + e] * (dp[4 * g + e] - d4[e]);
+      }
+      if constexpr (kBias) {
+        if (f.part_mass) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mass_sum += dz[r];
+        }
+        if constexpr (kCap) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dz[r] *= bend[r];
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const op8 zb = as_op<T>(dz, half);
+#pragma unroll
+        for (int dt = 0; dt < TL::kCols; ++dt) dk[dt] = Op<T>::mma(TL::cols_op(qt, dt, 2 * sub + half), zb, dk[dt]);
+      }
+    }
+  };
+
   bool more = next();
   int buf = 0, table_head = -1;
   if (more) load(0);
@@ -194,106 +337,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) voi
     wait_vmem<0>();
     __syncthreads();
     if (more) load(buf ^ 1);
-    if (run) {
-      const char* qt = lds + 2 * buf * TL::kBytes;
-      const char* gt = qt + TL::kBytes;
-      const float* lse = reinterpret_cast<const float*>(lds + LO::kLse) + buf * kTile;
-      const float* delta = reinterpret_cast<const float*>(lds + LO::kDelta) + buf * kTile;
-      const int* tags = reinterpret_cast<const int*>(lds + LO::kDocs) + buf * kTile;
-      const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances);
-      const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
-      const int p0 = start + q0;  // position of the tile's first row
-      const bool behind = rw.lo + 31 - p0 <= -a.buckets.reach, ahead = rw.lo - (p0 + kTile - 1) >= a.buckets.reach;
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        f32x16 s{}, dp{};
-#pragma unroll
-        for (int t = 0; t < TL::kSteps; ++t) s = Op<T>::mma(TL::rows_op(qt, 32 * sub, t), k[t], s);
-#pragma unroll
-        for (int t = 0; t < TL::kSteps; ++t) dp = Op<T>::mma(TL::rows_op(gt, 32 * sub, t), v[t], dp);
-        const int i0 = 32 * sub + 4 * h;  // row of register r: q0 + i0 + 8 (r / 4) + r % 4
-        f32x16 bend{};                    // cap'
-        if (a.cap2) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float t = cap_tanh<T>(s[r] * a.inv_cap);
-            bend[r] = fmaf(-t, t, 1.0f);
-            s[r] = t * a.cap2;
-          }
-        } else {
-          const float c = a.scale * kLog2e;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= c;
-        }
-        if (a.mass) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] += mass2;
-        }
-        if (a.slopes) {
-          const float d0 = static_cast<float>(key - p0 - i0);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[r] = fmaf(-slope2, fabsf(d0 - static_cast<float>(8 * (r / 4) + r % 4)), s[r]);
-        }
-        if (a.table) {
-          if (behind || ahead) {
-            const float far = distance[ahead ? 2 * a.buckets.reach : 0];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] += far;
-          } else {
-            const int d0 = key - p0 - i0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[r] += distance[max(-a.buckets.reach, min(a.buckets.reach, d0 - (8 * (r / 4) + r % 4))) + a.buckets.reach];
-          }
-        }
-        f32x16 dz;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + i0 + 8 * g);
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + i0 + 8 * g);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e;
-            s[r] = __builtin_amdgcn_exp2f(s[r] - l4[e]);
-            dz[r] = dp[r] - d4[e];
-          }
-        }
-        if (!all) {
-          const int i_first = q0 + i0 - first_row;
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[r] = static_cast<unsigned>(i_first + 8 * (r / 4) + r % 4) < row_count ? s[r] : 0.0f;
-          if (a.key_doc) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const i32x4 tag = *reinterpret_cast<const i32x4*>(tags + i0 + 8 * g);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * g + e] = tag[e] == doc ? s[4 * g + e] : 0.0f;
-            }
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dz[r] *= s[r];
-        if (f.part_mass) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mass_sum += dz[r];
-        }
-        if (a.cap2) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dz[r] *= bend[r];
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const op8 pb = as_op<T>(s, c), zb = as_op<T>(dz, c);
-#pragma unroll
-          for (int dt = 0; dt < TL::kCols; ++dt) {
-            dv[dt] = Op<T>::mma(TL::cols_op(gt, dt, 2 * sub + c), pb, dv[dt]);
-            dk[dt] = Op<T>::mma(TL::cols_op(qt, dt, 2 * sub + c), zb, dk[dt]);
-          }
-        }
-      }
-    }
+    if (run) compute(!all, q0, head, buf);
     buf ^= 1;
   }
 
@@ -368,8 +412,8 @@ struct RowLds {
 };
 constexpr int kDiagonal = 32 * 33 * 4;
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) void row_kernel(const Grad<T> f) {
+template <typename T, int D, bool kCap, bool kBias>
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 2 ? 2 : 1) void row_kernel(const Grad<T> f) {
   typedef Tile<T, D> TL;
   typedef RowLds<T, D> LO;
   typedef typename Op<T>::op8 op8;
@@ -481,90 +525,77 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) voi
     }
   };
 
-  bool more = next();
-  int buf = 0;
-  if (more) load(0);
-  while (more) {
-    const int k0 = tile * kTile;
-    const bool run = in_mine, all = in_full;
-    more = next();
-    wait_vmem<0>();
-    __syncthreads();
-    if (LO::kBuffers == 2 && more) load(buf ^ 1);
-    if (run) {
-      const char* kt = lds + 2 * (LO::kBuffers == 2 ? buf : 0) * TL::kBytes;
-      const char* vt = kt + TL::kBytes;
-      const float* mass = reinterpret_cast<const float*>(lds + LO::kMass) + buf * kTile;
-      const int* tags = reinterpret_cast<const int*>(lds + LO::kDocs) + buf * kTile;
-      const bool behind = k0 + kTile - 1 - rw.lo <= -a.buckets.reach, ahead = k0 - (rw.lo + 31) >= a.buckets.reach;
+  const auto compute = [&](bool partial, int k0, int buf) {
+    const char* kt = lds + 2 * (LO::kBuffers == 2 ? buf : 0) * TL::kBytes;
+    const char* vt = kt + TL::kBytes;
+    const float* mass = reinterpret_cast<const float*>(lds + LO::kMass) + buf * kTile;
+    const int* tags = reinterpret_cast<const int*>(lds + LO::kDocs) + buf * kTile;
+    const int reach = a.buckets.reach;
+    const bool behind = k0 + kTile - 1 - rw.lo <= -reach, ahead = k0 - (rw.lo + 31) >= reach;
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        f32x16 s{}, dp{};
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 s{}, dp{};
 #pragma unroll
-        for (int t = 0; t < TL::kSteps; ++t) s = Op<T>::mma(TL::rows_op(kt, 32 * sub, t), q[t], s);
+      for (int t = 0; t < TL::kSteps; ++t) s = Op<T>::mma(TL::rows_op(kt, 32 * sub, t), q[t], s);
 #pragma unroll
-        for (int t = 0; t < TL::kSteps; ++t) dp = Op<T>::mma(TL::rows_op(vt, 32 * sub, t), go[t], dp);
-        const int j0 = 32 * sub + 4 * h;
-        f32x16 bend{};
-        if (a.cap2) {
+      for (int t = 0; t < TL::kSteps; ++t) dp = Op<T>::mma(TL::rows_op(vt, 32 * sub, t), go[t], dp);
+      const int j0 = 32 * sub + 4 * h;
+      float x[16], bend[16], dz[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float t = cap_tanh<T>(s[r] * a.inv_cap);
-            bend[r] = fmaf(-t, t, 1.0f);
-            s[r] = t * a.cap2;
-          }
-        } else {
-          const float c = a.scale * kLog2e;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= c;
-        }
+      for (int r = 0; r < 16; ++r) x[r] = s[r], dz[r] = dp[r];
+      const float c = rescore<T, kCap>(a, x, bend);
+      const float d0f = static_cast<float>(k0 + j0 - pos);
+      if constexpr (kBias) {
         if (a.mass) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const f32x4 m = *reinterpret_cast<const f32x4*>(mass + j0 + 8 * g);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(m[e], kLog2e, s[4 * g + e]);
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = fmaf(x[4 * g + e], c, m[e] * kLog2e);
           }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] *= c;
         }
-        const float d0f = static_cast<float>(k0 + j0 - pos);
         if (a.slopes) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            s[r] = fmaf(-slope2, fabsf(d0f + static_cast<float>(8 * (r / 4) + r % 4)), s[r]);
+            x[r] = fmaf(-slope2, fabsf(d0f + static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
         }
         if (a.table) {
           if (behind || ahead) {
-            const float far = distance[ahead ? 2 * a.buckets.reach : 0];
+            const float far = distance[ahead ? 2 * reach : 0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] += far;
+            for (int r = 0; r < 16; ++r) x[r] += far;
           } else {
             const int d0 = k0 + j0 - pos;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              s[r] += distance[max(-a.buckets.reach, min(a.buckets.reach, d0 + 8 * (r / 4) + r % 4)) + a.buckets.reach];
+              x[r] += distance[max(-reach, min(reach, d0 + 8 * (r / 4) + r % 4)) + reach];
           }
         }
-        f32x16 dz;
+      }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = __builtin_amdgcn_exp2f(s[r] - lse);
-          dz[r] = dp[r] - delta;
-        }
-        if (!all) {
-          const int last_r = last - k0 - j0;
+      for (int r = 0; r < 16; ++r) {
+        x[r] = __builtin_amdgcn_exp2f(kBias ? x[r] - lse : fmaf(x[r], c, -lse));
+        dz[r] -= delta;
+      }
+      if (partial) {
+        const int last_r = last - k0 - j0;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = 8 * (r / 4) + r % 4 <= last_r ? s[r] : 0.0f;
-          if (kdocs) {
+        for (int r = 0; r < 16; ++r) x[r] = 8 * (r / 4) + r % 4 <= last_r ? x[r] : 0.0f;
+        if (kdocs) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const i32x4 tag = *reinterpret_cast<const i32x4*>(tags + j0 + 8 * g);
+          for (int g = 0; g < 4; ++g) {
+            const i32x4 tag = *reinterpret_cast<const i32x4*>(tags + j0 + 8 * g);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * g + e] = tag[e] == doc ? s[4 * g + e] : 0.0f;
-            }
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = tag[e] == doc ? x[4 * g + e] : 0.0f;
           }
         }
+      }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dz[r] *= s[r];
+      for (int r = 0; r < 16; ++r) dz[r] *= x[r];
+      if constexpr (kBias) {
         if (f.part_slopes) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -585,30 +616,43 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && sizeof(T) == 2 ? 2 : 1) voi
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int j = i + d;
-              const float x = diagonal[max(0, min(31, j)) * 33 + i];
-              sum += j >= 0 && j < 32 ? x : 0.0f;
+              const float y = diagonal[max(0, min(31, j)) * 33 + i];
+              sum += j >= 0 && j < 32 ? y : 0.0f;
             }
             const int r = k0 + 32 * sub - rw.lo + d;
-            if (r <= -a.buckets.reach)
+            if (r <= -reach)
               far_behind += sum;
-            else if (r >= a.buckets.reach)
+            else if (r >= reach)
               far_ahead += sum;
             else if (lane < 63)
-              sums[r + a.buckets.reach] += sum;
+              sums[r + reach] += sum;
           }
         }
-        if (a.cap2) {
+      }
+      if constexpr (kCap) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dz[r] *= bend[r];
-        }
+        for (int r = 0; r < 16; ++r) dz[r] *= bend[r];
+      }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const op8 zb = as_op<T>(dz, c);
+      for (int half = 0; half < 2; ++half) {
+        const op8 zb = as_op<T>(dz, half);
 #pragma unroll
-          for (int dt = 0; dt < TL::kCols; ++dt) dq[dt] = Op<T>::mma(TL::cols_op(kt, dt, 2 * sub + c), zb, dq[dt]);
-        }
+        for (int dt = 0; dt < TL::kCols; ++dt) dq[dt] = Op<T>::mma(TL::cols_op(kt, dt, 2 * sub + half), zb, dq[dt]);
       }
     }
+  };
+
+  bool more = next();
+  int buf = 0;
+  if (more) load(0);
+  while (more) {
+    const int k0 = tile * kTile;
+    const bool run = in_mine, all = in_full;
+    more = next();
+    wait_vmem<0>();
+    __syncthreads();
+    if (LO::kBuffers == 2 && more) load(buf ^ 1);
+    if (run) compute(!all, k0, buf);
     if (LO::kBuffers == 1 && more) {
       __syncthreads();
       load(buf ^ 1);
@@ -660,10 +704,11 @@ struct Plan {
   int key_blocks, row_blocks, splits, query_tiles, key_tiles;
   int64_t key_tasks, row_tasks;
 };
-Plan plan_of(const vgo_masked_attn* p) {
+Plan plan_of(const vgo_masked_attn* p, int dtype) {
   Plan r{};
   r.query_tiles = static_cast<int>(tiles_of(p->n_query)), r.key_tiles = static_cast<int>(tiles_of(p->n_key));
-  r.key_blocks = static_cast<int>((p->n_key + kBlock - 1) / kBlock);
+  const int64_t keys = dtype != VGO_F32 && p->head_dim == 128 ? KeyLds<bf16_t, 128>::kBlock : KeyLds<bf16_t, 64>::kBlock;
+  r.key_blocks = static_cast<int>((p->n_key + keys - 1) / keys);
   r.row_blocks = static_cast<int>((p->n_query + kBlock - 1) / kBlock);
   r.row_tasks = p->batch * p->heads * r.row_blocks;
   const int64_t tasks = p->batch * p->kv_heads * r.key_blocks, want = 2 * device_cus();
@@ -747,12 +792,15 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const Plan& pl
     status = check_launch("masked_attn_grad delta");
     if (status != VGO_OK) return status;
   }
+  const bool cap = f.a.cap2 != 0.0f, bias = f.a.mass || f.a.slopes || f.a.table;
   const size_t distances = f.a.table ? static_cast<size_t>(2 * f.a.buckets.reach + 1) * 4 : 0;
   if ((f.dk || f.part_mass) && plan.key_tasks > 0) {
     const size_t bytes = KeyLds<T, D>::kDistances + distances;
-    status = allow_lds(key_kernel<T, D>, bytes);
+    const auto kernel = cap ? (bias ? key_kernel<T, D, true, true> : key_kernel<T, D, true, false>)
+                            : (bias ? key_kernel<T, D, false, true> : key_kernel<T, D, false, false>);
+    status = allow_lds(kernel, bytes);
     if (status != VGO_OK) return status;
-    hipLaunchKernelGGL((key_kernel<T, D>), dim3(static_cast<unsigned>(plan.key_tasks)), dim3(64 * kWaves), bytes,
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.key_tasks)), dim3(64 * KeyLds<T, D>::kWaves), bytes,
                        stream, f);
     status = check_launch("masked_attn_grad keys");
     if (status != VGO_OK) return status;
@@ -767,9 +815,11 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const Plan& pl
   if ((f.dq || f.part_slopes || f.part_table) && plan.row_tasks > 0) {
     const size_t bytes = RowLds<T, D>::kDistances + distances +
                          (f.part_table ? static_cast<size_t>(kWaves) * (kDiagonal + distances) : 0);
-    status = allow_lds(row_kernel<T, D>, bytes);
+    const auto kernel = cap ? (bias ? row_kernel<T, D, true, true> : row_kernel<T, D, true, false>)
+                            : (bias ? row_kernel<T, D, false, true> : row_kernel<T, D, false, false>);
+    status = allow_lds(kernel, bytes);
     if (status != VGO_OK) return status;
-    hipLaunchKernelGGL((row_kernel<T, D>), dim3(static_cast<unsigned>(plan.row_tasks)), dim3(64 * kWaves), bytes,
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.row_tasks)), dim3(64 * kWaves), bytes,
                        stream, f);
     status = check_launch("masked_attn_grad rows");
     if (status != VGO_OK) return status;
@@ -799,7 +849,7 @@ extern "C" int vgo_masked_attn_grad_workspace(const vgo_masked_attn* problem, co
   const int status = check_grads(problem, grads, dtype);
   if (status != VGO_OK) return status;
   VGO_REQUIRE(bytes, "masked_attn_grad: null pointer");
-  *bytes = pieces_of(problem, grads, plan_of(problem)).bytes;
+  *bytes = pieces_of(problem, grads, plan_of(problem, dtype)).bytes;
   return VGO_OK;
 }
 
@@ -821,7 +871,7 @@ extern "C" int vgo_masked_attn_grad(const vgo_masked_attn* problem, const vgo_ma
                               strides_fit(g->dk_stride, p->head_dim, dtype) &&
                               strides_fit(g->dv_stride, p->head_dim, dtype))),
               "masked_attn_grad: dq, dk and dv must be 16-byte aligned, with strides of whole 16 bytes");
-  const Plan plan = plan_of(p);
+  const Plan plan = plan_of(p, dtype);
   const size_t need = pieces_of(p, g, plan).bytes;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(VGO_EWORKSPACE, "masked_attn_grad: workspace of " + std::to_string(need) + " bytes needed");
