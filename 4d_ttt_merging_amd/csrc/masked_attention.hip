@@ -2,6 +2,8 @@
 // masked_attention_fwd.h), and the document ranges of tiles.
 #include "masked_attention_fwd.h"
 
+#include <cmath>
+
 namespace vgo {
 namespace masked {
 namespace {
@@ -23,6 +25,33 @@ __global__ __launch_bounds__(256) void doc_info_kernel(const int* docs, const in
 
 }  // namespace
 
+// Time of a launch by splits s, in us.  `tile_us`: a CU's time per tile and work-group where several keep it busy
+// (measured: 0.62 for 128 rows of 64 channels in 16 bits, 1.0 of 128, 4.3 and 8.6 in fp32).  Work-groups beside
+// each other hide each other's waits (`hides`): one alone takes twice that, two 2.6 times it, from three on it is
+// theirs each (from the first where the products take long, fp32, or a work-group has waves enough), and
+// what does not fill the last round costs as much as those few alone.  Joining
+// takes a launch and the partial states' way out and back (`join_us` per split).  16 heads of
+// 8,232 x 8,232 x 64: 397 us unsplit (1,040 tasks, 4.06 a CU), 370 in three; 2,058 in fp32: 287 and 188 (six).
+int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, bool hides, double tile_us, double join_us) {
+  // A causal mask leaves the tasks half of the tiles where all keys are the queries' own, documents fewer: their
+  // ends spread, so that only the whole work counts.
+  const bool all = !p->causal && !p->key_documents && !p->key_lengths;
+  const double share =
+      p->causal ? 1.0 - 0.5 * std::min<double>(p->n_query, p->n_key) / std::max<int64_t>(1, p->n_key) : 1.0;
+  const double cus = device_cus(), alone[3] = {0.0, 2.0, 2.6};
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= std::min(tiles, 512); s += s < 8 ? 1 : s < 32 ? 4 : 32) {
+    const double run = (tiles + s - 1) / s, per_cu = tasks * s / cus;
+    const int most = static_cast<int>(std::ceil(per_cu));
+    double beside = all ? most : std::max(1.0 / share, per_cu);
+    if (hides) beside = all ? most / 3 * 3 + alone[most % 3] : std::max(2.0 / share, per_cu);
+    const double us = run * share * beside * std::max(0.6, tile_us) + (s > 1 ? 6.0 + s * join_us : 0.0);
+    if (us < least * 0.98) least = us, best = s;
+  }
+  return best;
+}
+
 ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
   ForwardPlan r{};
   const int group = static_cast<int>(p->heads / p->kv_heads);
@@ -32,17 +61,12 @@ ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
   r.rows = static_cast<int>(r.pack * p->n_query);
   r.tiles = static_cast<int>(tiles_of(p->n_key));
   const int64_t vheads = p->batch * (p->heads / r.pack);
-  const int64_t cus = device_cus();
-  const auto count = [&](int rows) { return vheads * ((r.rows + rows - 1) / rows); };
-  r.waves = 4, r.blocks = 1;
-  if (dtype == VGO_F32 || p->head_dim == 128 || count(256) < cus) r.blocks = 1;
-  if (r.blocks == 1 && count(128) < cus) r.waves = 1;
-  const int rows = 32 * r.blocks * r.waves;
-  r.row_blocks = (r.rows + rows - 1) / rows;
+  constexpr int kRows = 128;  // a task's
+  r.row_blocks = (r.rows + kRows - 1) / kRows;
   const int64_t tasks = vheads * r.row_blocks;
-  r.splits = 1;
-  if (r.waves == 1 && tasks < 4 * cus)
-    r.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((4 * cus + tasks - 1) / tasks, r.tiles)));
+  const double tile_us = (dtype == VGO_F32 ? 4.3 : p->head_dim == 128 ? 0.5 : 0.62) * p->head_dim / 64;
+  const double bytes = 8.0 * vheads * r.rows * p->head_dim;
+  r.splits = splits_of(p, tasks, r.tiles, dtype != VGO_F32, tile_us, bytes / 8e6);
   r.tasks = tasks * r.splits;
   return r;
 }

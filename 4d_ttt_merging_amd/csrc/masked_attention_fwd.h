@@ -1,6 +1,6 @@
 // Masked attention, forward (rules and layouts: masked_attention.h).
 //
-// A task is kWaves x 32 QB rows of one (batch, head), or, where a head has few queries and shares
+// A task is kWaves x 32 rows of one (batch, head), or, where a head has few queries and shares
 // its keys, of all heads of one key head (rows r = head g, query i: r = g n_query + i); it runs over
 // the key tiles in which any pair of its rows attends, found 64 tiles at a time by one ballot, in
 // which each lane judges one tile.  K and V tiles come into LDS by DMA, row-major, double-buffered,
@@ -20,7 +20,7 @@ namespace masked {
 
 // How a problem is cut into tasks.
 struct ForwardPlan {
-  int pack, rows, row_blocks, splits, tiles, waves, blocks;  // blocks: QB
+  int pack, rows, row_blocks, splits, tiles;
   int64_t tasks;
 };
 
@@ -51,7 +51,7 @@ struct Forward {
   float* part_ml; // and [.., rows, 3] their reference maxima (log2) and row sums (rounded, unrounded)
   int pack;       // heads per task (1, or heads / kv_heads)
   int rows;       // pack * n_query
-  int row_blocks, splits, tiles, tasks;
+  int row_blocks, splits, tiles, tasks, joiners;
 };
 
 // The key tiles of one task that its work-group (`wg`) and this wave (`w`) take part in.
@@ -62,10 +62,12 @@ struct Walk {
   int b, limit, prefix, end, base, tile;
   uint64_t todo, mine, full, whole;  // of tiles base .. base + 63
   bool in_mine, in_full, in_whole;   // of `tile`
+  const bool rows_here;              // the wave has rows
 
-  __device__ __forceinline__ Walk(const Args<T>& args, const Range& group, const Range& wave, int batch, int begin,
-                                  int last)
-      : a(args), wg(group), w(wave), b(batch), end(last), base(begin - 64), tile(0), todo(0) {
+  __device__ __forceinline__ Walk(const Args<T>& args, const Range& group, const Range& wave, bool rows, int batch,
+                                  int begin, int last)
+      : a(args), wg(group), w(wave), b(batch), end(last), base(begin - 64), tile(0), todo(0),
+        rows_here(rows) {
     limit = key_limit(a, b);
     prefix = prefix_of(a, b);
     end = min(end, (limit + kTile - 1) / kTile);
@@ -84,6 +86,7 @@ struct Walk {
         judge(a, wg, k, prefix, any, all);
         judge(a, w, k, prefix, any_w, all_w);
         const bool inside = k.lo + kTile <= limit;
+      any_w = any_w && rows_here;
         all_w = all_w && inside;
         whole_t = inside && (!a.key_doc || k.docs_whole);
       }
@@ -97,9 +100,10 @@ struct Walk {
   }
 };
 
-template <typename T, int D, int QB, int kWaves>
+constexpr int kWaves = 4, kRowsPerWave = 32, kRows = kRowsPerWave * kWaves;  // of a work-group
+
+template <typename T, int D>
 struct Layout {
-  static constexpr int kRowsPerWave = 32 * QB, kRows = kRowsPerWave * kWaves;
   static constexpr int kTiles = 4 * Tile<T, D>::kBytes;  // K and V, two buffers
   static constexpr int kMass = kTiles, kDocs = kMass + 2 * kTile * 4, kRange = kDocs + 2 * kTile * 4;
   static constexpr int kDistances = kRange + kWaves * 16;
@@ -109,15 +113,16 @@ struct Layout {
 // stay below 2^8, far from f16's largest number.
 constexpr float kSlack = 8.0f;
 
-template <typename T, int D, int QB, int kWaves, bool kCap, bool kBias, bool kLse>
-__global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1 : 2) void forward_kernel(const Forward<T> f) {
+template <typename T, int D, bool kCap, bool kBias, bool kLse>
+__global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forward_kernel(
+    const Forward<T> f) {
   typedef Tile<T, D> TL;
-  typedef Layout<T, D, QB, kWaves> LO;
+  typedef Layout<T, D> LO;
   typedef typename Op<T>::op8 op8;
   extern __shared__ __align__(16) char lds[];
   const Args<T>& a = f.a;
   const int lane = lane_id(), l31 = lane & 31, h = lane >> 5;
-  const int wave = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   // Heads, then key splits, then row blocks from the last on (the longest first under a causal mask).
   int task = xcd_remap(blockIdx.x, f.tasks);
@@ -127,30 +132,21 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
   task /= f.splits;
   const int vheads = a.heads / f.pack, vh = task % vheads, b = task / vheads;
   const int kvh = vh * f.pack / (a.heads / a.kv_heads);
-  const int row0 = block * LO::kRows + wave * LO::kRowsPerWave;
+  const int row0 = block * kRows + wave * kRowsPerWave;
   const int start = first_position(a, b);
 
   // The wave's rows: operands, positions, documents.
-  op8 q[QB][TL::kSteps];
-  int pos[QB], doc[QB], head[QB], index[QB];
-  bool stored[QB];
-  const float* distance[QB];
-  float slope2[QB];
+  const int row = row0 + l31, rc = min(row, f.rows - 1);
+  const bool stored = row < f.rows;
+  const int of_group = f.pack == 1 ? 0 : rc / a.n_query;
+  const int index = rc - of_group * a.n_query, head = vh * f.pack + of_group, pos = start + index;
+  const int doc = a.query_doc ? a.query_doc[static_cast<int64_t>(b) * a.n_query + index] : 0;
+  const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+  const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances) + of_group * (2 * a.buckets.reach + 1);
+  op8 q[TL::kSteps];
+  const T* src = a.q + b * a.qs[0] + head * a.qs[1] + index * a.qs[2] + 8 * h;
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int r = row0 + 32 * qb + l31, rc = min(r, f.rows - 1);
-    const int g = f.pack == 1 ? 0 : rc / a.n_query;
-    index[qb] = rc - g * a.n_query;
-    head[qb] = vh * f.pack + g;
-    stored[qb] = r < f.rows;
-    pos[qb] = start + index[qb];
-    doc[qb] = a.query_doc ? a.query_doc[static_cast<int64_t>(b) * a.n_query + index[qb]] : 0;
-    slope2[qb] = a.slopes ? a.slopes[head[qb]] * kLog2e : 0.0f;
-    distance[qb] = reinterpret_cast<const float*>(lds + LO::kDistances) + (f.pack == 1 ? 0 : g * (2 * a.buckets.reach + 1));
-    const T* src = a.q + b * a.qs[0] + head[qb] * a.qs[1] + index[qb] * a.qs[2] + 8 * h;
-#pragma unroll
-    for (int t = 0; t < TL::kSteps; ++t) q[qb][t] = *reinterpret_cast<const op8*>(src + 16 * t);
-  }
+  for (int t = 0; t < TL::kSteps; ++t) q[t] = *reinterpret_cast<const op8*>(src + 16 * t);
   // Positions of rows first .. first + n: contiguous within a head, everything across heads.
   const auto positions = [&](int first, int n, Range& r) {
     const int last = min(first + n, f.rows) - 1;
@@ -160,35 +156,23 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
     r.hi = start + (one ? last % a.n_query : a.n_query - 1);
   };
   Range rw{}, rg{};
-  positions(row0, LO::kRowsPerWave, rw);
-  positions(block * LO::kRows, LO::kRows, rg);
+  positions(row0, kRowsPerWave, rw);
+  positions(block * kRows, kRows, rg);
   if (a.query_doc) {
-    int lo = INT_MAX, hi = -1, bad = 0;
+    const bool of = stored && doc >= 0;
+    int lo = of ? doc : INT_MAX, hi = of ? doc : -1;
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-      if (stored[qb]) {
-        if (doc[qb] >= 0) lo = min(lo, doc[qb]), hi = max(hi, doc[qb]);
-        bad |= doc[qb] < 0;
-      }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-      lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
-      bad |= __shfl_xor(bad, off);
-    }
+    for (int off = 16; off >= 1; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
     rw.doc_lo = __builtin_amdgcn_readfirstlane(lo), rw.doc_hi = __builtin_amdgcn_readfirstlane(hi);
-    rw.docs_whole = __builtin_amdgcn_readfirstlane(bad) == 0;
-    if constexpr (kWaves > 1) {
-      int* slot = reinterpret_cast<int*>(lds + LO::kRange);
-      if (lane == 0) slot[4 * wave] = lo, slot[4 * wave + 1] = hi;
-      __syncthreads();
-      rg.doc_lo = INT_MAX, rg.doc_hi = -1;
+    rw.docs_whole = __all(!stored || doc >= 0);
+    int* slot = reinterpret_cast<int*>(lds + LO::kRange);
+    if (lane == 0) slot[4 * wave] = lo, slot[4 * wave + 1] = hi;
+    __syncthreads();
+    rg.doc_lo = INT_MAX, rg.doc_hi = -1, rg.docs_whole = false;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i)
-        rg.doc_lo = min(rg.doc_lo, __builtin_amdgcn_readfirstlane(slot[4 * i])),
-        rg.doc_hi = max(rg.doc_hi, __builtin_amdgcn_readfirstlane(slot[4 * i + 1]));
-      rg.docs_whole = false;
-    } else {
-      rg = rw;
+    for (int i = 0; i < kWaves; ++i) {
+      rg.doc_lo = min(rg.doc_lo, __builtin_amdgcn_readfirstlane(slot[4 * i]));
+      rg.doc_hi = max(rg.doc_hi, __builtin_amdgcn_readfirstlane(slot[4 * i + 1]));
     }
   }
   if (a.table)
@@ -197,26 +181,20 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
                      64 * kWaves);
 
   // Reference maxima (exponents of 2; -inf until something attends) and row sums.
-  float mref[QB], lsum[QB], lsum32[QB];
-  f32x16 o[QB][TL::kCols];
+  float mref = -kInf, lsum = 0.0f, lsum32 = 0.0f;
+  f32x16 o[TL::kCols];
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    mref[qb] = -kInf, lsum[qb] = lsum32[qb] = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < TL::kCols; ++dt) o[qb][dt] = f32x16{};
-  }
+  for (int dt = 0; dt < TL::kCols; ++dt) o[dt] = f32x16{};
 
   const T* kbase = a.k + b * a.ks[0] + kvh * a.ks[1];
   const T* vbase = a.v + b * a.vs[0] + kvh * a.vs[1];
   const int* kdocs = a.key_doc ? a.key_doc + static_cast<int64_t>(b) * a.n_key : nullptr;
   const uint32_t lds0 = lds_offset(lds);
   const int per_split = (f.tiles + f.splits - 1) / f.splits;
-  Walk<T> walk(a, rg, rw, b, split * per_split, min(f.tiles, (split + 1) * per_split));
+  Walk<T> walk(a, rg, rw, row0 < f.rows, b, split * per_split, min(f.tiles, (split + 1) * per_split));
   const int limit = walk.limit;
-  int last[QB];  // of the keys that lengths and the causal mask leave a row
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb)
-    last[qb] = min(limit, a.causal ? max(pos[qb] + 1, walk.prefix) : INT_MAX) - 1;
+  // Last of the keys that lengths and the causal mask leave the row.
+  const int last = min(limit, a.causal ? max(pos + 1, walk.prefix) : INT_MAX) - 1;
 
   const auto load = [&](int buf) {
     const int k0 = walk.tile * kTile;
@@ -234,23 +212,21 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
   const auto compute = [&](bool partial, int k0, int buf) {
     const char* kt = lds + 2 * buf * TL::kBytes;
     const char* vt = kt + TL::kBytes;
-    f32x16 s[QB][2];
+    f32x16 s[2];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) s[qb][sub] = f32x16{};
+      s[sub] = f32x16{};
 #pragma unroll
       for (int t = 0; t < TL::kSteps; ++t) {
         const op8 ka = TL::rows_op(kt, 32 * sub, t);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) s[qb][sub] = Op<T>::mma(ka, q[qb][t], s[qb][sub]);
+        s[sub] = Op<T>::mma(ka, q[t], s[sub]);
       }
     }
-    // x = the scores of row block qb, sub-tile sub, before the factor c, -inf where a pair does not attend.
-    const auto scores = [&](int qb, int sub, bool in_full, float (&x)[16]) {
+    // x = the scores of sub-tile sub, before the factor c, -inf where a pair does not attend.
+    const auto scores = [&](int sub, bool in_full, float (&x)[16]) {
       const int j0 = 32 * sub + 4 * h;  // key of register r: k0 + j0 + 8 (r / 4) + r % 4
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = s[qb][sub][r];
+      for (int r = 0; r < 16; ++r) x[r] = s[sub][r];
       if constexpr (kCap) {
         if (in_full) {
 #pragma unroll
@@ -275,27 +251,27 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
           for (int r = 0; r < 16; ++r) x[r] *= to2;
         }
         if (a.slopes) {
-          const float d0 = static_cast<float>(k0 + j0 - pos[qb]);
+          const float d0 = static_cast<float>(k0 + j0 - pos);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            x[r] = fmaf(-slope2[qb], fabsf(d0 + static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
+            x[r] = fmaf(-slope2, fabsf(d0 + static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
         }
         if (a.table) {
           const int reach = a.buckets.reach;
           if (k0 + kTile - 1 - rw.lo <= -reach || k0 - rw.hi >= reach) {  // beyond the buckets' reach, all of it
-            const float far = distance[qb][k0 > rw.lo ? 2 * reach : 0];
+            const float far = distance[k0 > rw.lo ? 2 * reach : 0];
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] += far;
           } else {
-            const int d0 = k0 + j0 - pos[qb];
+            const int d0 = k0 + j0 - pos;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              x[r] += distance[qb][max(-reach, min(reach, d0 + 8 * (r / 4) + r % 4)) + reach];
+              x[r] += distance[max(-reach, min(reach, d0 + 8 * (r / 4) + r % 4)) + reach];
           }
         }
       }
       if (partial) {
-        const int last_r = last[qb] - k0 - j0;  // keys past it do not attend
+        const int last_r = last - k0 - j0;  // keys past it do not attend
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = 8 * (r / 4) + r % 4 <= last_r ? x[r] : -kInf;
         if (kdocs) {
@@ -304,58 +280,54 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
           for (int g = 0; g < 4; ++g) {
             const i32x4 tag = *reinterpret_cast<const i32x4*>(tags + 8 * g);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * g + e] = tag[e] == doc[qb] ? x[4 * g + e] : -kInf;
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = tag[e] == doc ? x[4 * g + e] : -kInf;
           }
         }
       }
     };
-    op8 p[QB][4];  // probabilities as operands
+    op8 p[4];  // probabilities as operands
+    bool exact = false;
+    if constexpr (kCap) {
+      float most = fabsf(s[0][0]);
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      bool exact = false;
-      if constexpr (kCap) {
-        float most = fabsf(s[qb][0][0]);
-#pragma unroll
-        for (int r = 1; r < 32; ++r) most = fmaxf(most, fabsf(s[qb][r / 16][r % 16]));
-        exact = __any(!(most <= a.cap_reach));
-      }
-      float x[2][16];
-      scores(qb, 0, exact, x[0]);
-      scores(qb, 1, exact, x[1]);
-      float top = fmaxf(x[0][0], x[1][0]);
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, x[0][r]), x[1][r]);
-      top = half_max(top) * c;
-      if (__any(top > mref[qb] + kSlack)) {
-        const float m = fmaxf(mref[qb], top);
-        const float alpha = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref[qb] - m);
-        mref[qb] = m;
-        lsum[qb] *= alpha, lsum32[qb] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < TL::kCols; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[qb][dt][r] *= alpha;
-      }
-      const float off = mref[qb] == -kInf ? 0.0f : -mref[qb];
-      float sum = 0.0f, sum32 = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 32; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16], c, off));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16 + 1], c, off));
-        op8& to = p[qb][r / 8];
-        to[r % 8] = from_f32<T>(p0), to[r % 8 + 1] = from_f32<T>(p1);
-        sum = add_pair<T>(sum, p0, p1, to[r % 8], to[r % 8 + 1]);
-        if constexpr (kLse && sizeof(T) == 2) sum32 += p0 + p1;
-      }
-      lsum[qb] += sum, lsum32[qb] += sum32;
+      for (int r = 1; r < 32; ++r) most = fmaxf(most, fabsf(s[r / 16][r % 16]));
+      exact = __any(!(most <= a.cap_reach));
     }
+    float x[2][16];
+    scores(0, exact, x[0]);
+    scores(1, exact, x[1]);
+    float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, x[0][r]), x[1][r]);
+    top = half_max(top) * c;
+    if (__any(top > mref + kSlack)) {
+      const float m = fmaxf(mref, top);
+      const float alpha = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - m);
+      mref = m;
+      lsum *= alpha, lsum32 *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < TL::kCols; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+    }
+    const float off = mref == -kInf ? 0.0f : -mref;
+    float sum = 0.0f, sum32 = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 32; r += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16], c, off));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16 + 1], c, off));
+      op8& to = p[r / 8];
+      to[r % 8] = from_f32<T>(p0), to[r % 8 + 1] = from_f32<T>(p1);
+      sum = add_pair<T>(sum, p0, p1, to[r % 8], to[r % 8 + 1]);
+      if constexpr (kLse && sizeof(T) == 2) sum32 += p0 + p1;
+    }
+    lsum += sum, lsum32 += sum32;
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc)
 #pragma unroll
       for (int dt = 0; dt < TL::kCols; ++dt) {
         const op8 va = TL::cols_op(vt, dt, kc);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) o[qb][dt] = Op<T>::mma(va, p[qb][kc], o[qb][dt]);
+        o[dt] = Op<T>::mma(va, p[kc], o[dt]);
       }
   };
 
@@ -373,70 +345,85 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 || D * sizeof(T) > 256 ? 1
     buf ^= 1;
   }
 
-#pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    if (!stored[qb]) continue;
-    const bool dead = a.query_doc && doc[qb] < 0;
-    float l = half_sum(lsum[qb]);
-    // The gradients divide by the sum of the unrounded probabilities, which they compute again.
-    float l32 = kLse && sizeof(T) == 2 ? half_sum(lsum32[qb]) : l;
-    if (dead) l = l32 = 0.0f;
-    if (f.splits > 1) {
-      const int64_t row = (static_cast<int64_t>(split) * a.batch * vheads + b * vheads + vh) * f.rows + row0 +
-                          32 * qb + l31;
-      float* dst = f.part_o + row * D;
-#pragma unroll
-      for (int dt = 0; dt < TL::kCols; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g + 4 * h) =
-              f32x4{o[qb][dt][4 * g], o[qb][dt][4 * g + 1], o[qb][dt][4 * g + 2], o[qb][dt][4 * g + 3]};
-      if (h == 0) {
-        f.part_ml[3 * row] = l == 0.0f ? -kInf : mref[qb];
-        f.part_ml[3 * row + 1] = l, f.part_ml[3 * row + 2] = l32;
-      }
-      continue;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* dst = f.out + b * a.os[0] + head[qb] * a.os[1] + index[qb] * a.os[2];
+  if (!stored) return;
+  const bool dead = a.query_doc && doc < 0;
+  float l = half_sum(lsum);
+  // The gradients divide by the sum of the unrounded probabilities, which they compute again.
+  float l32 = kLse && sizeof(T) == 2 ? half_sum(lsum32) : l;
+  if (dead) l = l32 = 0.0f;
+  if (f.splits > 1) {
+    const int64_t row = (static_cast<int64_t>(split) * a.batch * vheads + b * vheads + vh) * f.rows + row0 +
+                        l31;
+    float* dst = f.part_o + row * D;
 #pragma unroll
     for (int dt = 0; dt < TL::kCols; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0.0f : o[qb][dt][4 * g + e] * inv;
-        store4(dst + 32 * dt + 8 * g + 4 * h, y);
-      }
-    if (f.lse && h == 0)
-      f.lse[(static_cast<int64_t>(b) * a.heads + head[qb]) * a.n_query + index[qb]] =
-          l32 == 0.0f ? kInf : mref[qb] + __builtin_amdgcn_logf(l32);
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g + 4 * h) =
+            f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+    if (h == 0) {
+      f.part_ml[3 * row] = l == 0.0f ? -kInf : mref;
+      f.part_ml[3 * row + 1] = l, f.part_ml[3 * row + 2] = l32;
+    }
+    return;
   }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* dst = f.out + b * a.os[0] + head * a.os[1] + index * a.os[2];
+#pragma unroll
+  for (int dt = 0; dt < TL::kCols; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0.0f : o[dt][4 * g + e] * inv;
+      store4(dst + 32 * dt + 8 * g + 4 * h, y);
+    }
+  if (f.lse && h == 0)
+    f.lse[(static_cast<int64_t>(b) * a.heads + head) * a.n_query + index] =
+        l32 == 0.0f ? kInf : mref + __builtin_amdgcn_logf(l32);
 }
 
-// Joins the splits' states of each row: D / 4 lanes a row.
+// Joins the splits' states of each row: D / 4 lanes a row, `f.joiners` of them that take every
+// f.joiners-th split (many splits are few rows, where one lane would wait for each in turn).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
   const Args<T>& a = f.a;
   constexpr int kLanes = D / 4;
-  const int vheads = a.heads / f.pack;
+  __shared__ f32x4 sums[256];
+  __shared__ f32x4 states[256];  // reference, row sums (rounded, unrounded)
+  const int vheads = a.heads / f.pack, each = kLanes * f.joiners;
   const int64_t n = static_cast<int64_t>(a.batch) * vheads * f.rows;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int d = static_cast<int>(threadIdx.x) % kLanes * 4;
-  if (row >= n) return;
-  float m = -kInf;
-  for (int s = 0; s < f.splits; ++s) m = fmaxf(m, f.part_ml[3 * (s * n + row)]);
-  float l = 0.0f, l32 = 0.0f;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / each) + static_cast<int>(threadIdx.x) / each;
+  const int joiner = static_cast<int>(threadIdx.x) % each / kLanes, d = static_cast<int>(threadIdx.x) % kLanes * 4;
+  float m = -kInf, l = 0.0f, l32 = 0.0f;
   f32x4 y{};
-  for (int s = 0; s < f.splits; ++s) {
-    const float *ml = f.part_ml + 3 * (s * n + row), ms = ml[0], ls = ml[1];
-    if (ls == 0.0f) continue;  // nothing attended there
-    const float w = ms == m ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
-    l = fmaf(w, ls, l), l32 = fmaf(w, ml[2], l32);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(f.part_o + (s * n + row) * D + d);
+  const auto add = [&](float ms, float ls, float ls32, const f32x4& x) {
+    if (ls == 0.0f) return;  // nothing attended there
+    const float to = fmaxf(m, ms);
+    const float was = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to), now = ms == to ? 1.0f : __builtin_amdgcn_exp2f(ms - to);
+    m = to;
+    l = fmaf(was, l, now * ls), l32 = fmaf(was, l32, now * ls32);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = fmaf(w, x[e], y[e]);
+    for (int e = 0; e < 4; ++e) y[e] = fmaf(was, y[e], now * x[e]);
+  };
+  if (row < n) {
+#pragma unroll 4
+    for (int s = joiner; s < f.splits; s += f.joiners) {
+      const float* ml = f.part_ml + 3 * (s * n + row);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(f.part_o + (s * n + row) * D + d);
+      add(ml[0], ml[1], ml[2], x);
+    }
   }
+  if (f.joiners > 1) {
+    sums[threadIdx.x] = y, states[threadIdx.x] = f32x4{m, l, l32, 0.0f};
+    __syncthreads();
+    if (joiner > 0) return;
+    for (int j = 1; j < f.joiners; ++j) {
+      const f32x4 s = states[threadIdx.x + j * kLanes];
+      add(s[0], s[1], s[2], sums[threadIdx.x + j * kLanes]);
+    }
+  }
+  if (row >= n) return;
   const int vh = static_cast<int>(row / f.rows), r = static_cast<int>(row % f.rows);
   const int b = vh / vheads, head = vh % vheads * f.pack + r / a.n_query, i = r % a.n_query;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -448,11 +435,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
         l32 == 0.0f ? kInf : m + __builtin_amdgcn_logf(l32);
 }
 
-template <typename T, int D, int QB, int kWaves, bool kCap, bool kBias, bool kLse>
+template <typename T, int D, bool kCap, bool kBias, bool kLse>
 int launch(const Forward<T>& f, hipStream_t stream) {
-  typedef Layout<T, D, QB, kWaves> LO;
+  typedef Layout<T, D> LO;
   const size_t bytes = LO::kDistances + (f.a.table ? static_cast<size_t>(f.pack) * (2 * f.a.buckets.reach + 1) * 4 : 0);
-  const auto kernel = forward_kernel<T, D, QB, kWaves, kCap, kBias, kLse>;
+  const auto kernel = forward_kernel<T, D, kCap, kBias, kLse>;
   if (bytes > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
@@ -463,13 +450,13 @@ int launch(const Forward<T>& f, hipStream_t stream) {
 }
 
 // The kernel without the rules that the problem does not have.
-template <typename T, int D, int QB, int kWaves>
+template <typename T, int D>
 int choose(const Forward<T>& f, hipStream_t stream) {
   const bool cap = f.a.cap2 != 0.0f, bias = f.a.mass || f.a.slopes || f.a.table;
   const auto with = [&](auto lse) {
     constexpr bool kLse = decltype(lse)::value;
-    if (cap) return bias ? launch<T, D, QB, kWaves, true, true, kLse>(f, stream) : launch<T, D, QB, kWaves, true, false, kLse>(f, stream);
-    return bias ? launch<T, D, QB, kWaves, false, true, kLse>(f, stream) : launch<T, D, QB, kWaves, false, false, kLse>(f, stream);
+    if (cap) return bias ? launch<T, D, true, true, kLse>(f, stream) : launch<T, D, true, false, kLse>(f, stream);
+    return bias ? launch<T, D, false, true, kLse>(f, stream) : launch<T, D, false, false, kLse>(f, stream);
   };
   if constexpr (std::is_same<T, bf16_t>::value)
     if (f.lse) return with(std::true_type{});
@@ -491,16 +478,13 @@ int run(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int6
     f.part_o = reinterpret_cast<float*>(ws + info_bytes(p));
     f.part_ml = reinterpret_cast<float*>(ws + info_bytes(p) + align16(plan.splits * rows * p->head_dim * 4));
   }
-  int status;
-  if (plan.waves == 1)
-    status = choose<T, D, 1, 1>(f, stream);
-  else if constexpr (sizeof(T) == 2 && D == 64)
-    status = plan.blocks == 2 ? choose<T, D, 2, 4>(f, stream) : choose<T, D, 1, 4>(f, stream);
-  else
-    status = choose<T, D, 1, 4>(f, stream);
+  const int status = choose<T, D>(f, stream);
   if (status != VGO_OK || plan.splits == 1) return status;
-  const unsigned groups = static_cast<unsigned>((rows * (D / 4) + 255) / 256);
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3(groups), dim3(256), 0, stream, f);
+  f.joiners = 1;
+  while (f.joiners < 256 / (D / 4) && 2 * f.joiners < plan.splits && rows * (D / 4) * f.joiners < 256LL * 2 * device_cus())
+    f.joiners *= 2;
+  const int64_t each = 256 / (D / 4 * f.joiners);  // rows per work-group
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3(static_cast<unsigned>((rows + each - 1) / each)), dim3(256), 0, stream, f);
   return check_launch("masked_attn join");
 }
 

@@ -25,10 +25,11 @@ struct Grad {
   T *dq, *dk, *dv;       // dq null: not wanted; likewise dk and dv
   int64_t dqs[3], dks[3], dvs[3];
   float* part_kv;      // splits > 1: [splits, batch * kv_heads, n_key, 2 D]
+  float* part_q;       // row_splits > 1: [row_splits, batch * heads, n_query, D]
   float* part_mass;    // [splits * batch * kv_heads, n_key] or null
-  float* part_slopes;  // [batch * row_blocks, heads] or null
-  float* part_table;   // [batch * row_blocks, n_buckets, heads] or null
-  int query_tiles, key_tiles, splits;
+  float* part_slopes;  // [row_splits * batch * row_blocks, heads] or null
+  float* part_table;   // [row_splits * batch * row_blocks, n_buckets, heads] or null
+  int query_tiles, key_tiles, splits, row_splits;
   int key_blocks, row_blocks, key_tasks, row_tasks;
 };
 
@@ -425,6 +426,8 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 2 ? 2 : 1) void row_kerne
   int task = xcd_remap(blockIdx.x, f.row_tasks);
   const int block = f.row_blocks - 1 - task % f.row_blocks;
   task /= f.row_blocks;
+  const int split = task % f.row_splits;
+  task /= f.row_splits;
   const int head = task % a.heads, b = task / a.heads, kvh = head / (a.heads / a.kv_heads);
   const int start = first_position(a, b), limit = key_limit(a, b), prefix = prefix_of(a, b);
   const int row0 = block * kBlock + 32 * wave, row = row0 + l32, rc = min(row, a.n_query - 1);
@@ -483,8 +486,9 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 2 ? 2 : 1) void row_kerne
   const int* kdocs = a.key_doc ? a.key_doc + static_cast<int64_t>(b) * a.n_key : nullptr;
   const uint32_t lds0 = lds_offset(lds);
 
-  const int end = (limit + kTile - 1) / kTile;
-  int base = -64, tile = 0;
+  const int per_split = (f.key_tiles + f.row_splits - 1) / f.row_splits;
+  const int end = min((limit + kTile - 1) / kTile, (split + 1) * per_split);
+  int base = split * per_split - 64, tile = 0;
   uint64_t todo = 0, mine = 0, full = 0, whole = 0;
   bool in_mine = false, in_full = false, in_whole = false;
   const auto next = [&]() {
@@ -660,7 +664,19 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 2 ? 2 : 1) void row_kerne
     buf ^= 1;
   }
 
-  if (f.dq && stored) {
+  if (f.part_q && stored) {
+    const int64_t bh = static_cast<int64_t>(b) * a.heads + head;
+    float* dst = f.part_q + ((static_cast<int64_t>(split) * a.batch * a.heads + bh) * a.n_query + row) * D;
+#pragma unroll
+    for (int dt = 0; dt < TL::kCols; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = dq[dt][4 * g + e] * a.scale;
+        *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g + 4 * h) = y;
+      }
+  } else if (f.dq && stored) {
     T* dst = f.dq + b * f.dqs[0] + head * f.dqs[1] + row * f.dqs[2];
 #pragma unroll
     for (int dt = 0; dt < TL::kCols; ++dt)
@@ -672,7 +688,7 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 2 ? 2 : 1) void row_kerne
         store4(dst + 32 * dt + 8 * g + 4 * h, y);
       }
   }
-  const int64_t part = static_cast<int64_t>(b) * f.row_blocks + block;
+  const int64_t part = (static_cast<int64_t>(split) * a.batch + b) * f.row_blocks + block;
   if (!f.part_slopes && !f.part_table) return;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
@@ -700,8 +716,28 @@ __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 2 ? 2 : 1) void row_kerne
     f.part_table[(part * a.buckets.count + t) * a.heads + head] = a.buckets.sum(t, of_distance);
 }
 
+// dQ of split work, likewise.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_rows_kernel(const Grad<T> f) {
+  const Args<T>& a = f.a;
+  constexpr int kLanes = D / 4;
+  const int64_t n = static_cast<int64_t>(a.batch) * a.heads * a.n_query;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  if (row >= n) return;
+  const int d = static_cast<int>(threadIdx.x) % kLanes * 4;
+  f32x4 y{};
+#pragma unroll 4
+  for (int s = 0; s < f.row_splits; ++s) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(f.part_q + (s * n + row) * D + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] += x[e];
+  }
+  const int i = static_cast<int>(row % a.n_query), bh = static_cast<int>(row / a.n_query);
+  store4(f.dq + bh / a.heads * f.dqs[0] + bh % a.heads * f.dqs[1] + i * f.dqs[2] + d, y);
+}
+
 struct Plan {
-  int key_blocks, row_blocks, splits, query_tiles, key_tiles;
+  int key_blocks, row_blocks, splits, row_splits, query_tiles, key_tiles;
   int64_t key_tasks, row_tasks;
 };
 Plan plan_of(const vgo_masked_attn* p, int dtype) {
@@ -710,18 +746,24 @@ Plan plan_of(const vgo_masked_attn* p, int dtype) {
   const int64_t keys = dtype != VGO_F32 && p->head_dim == 128 ? KeyLds<bf16_t, 128>::kBlock : KeyLds<bf16_t, 64>::kBlock;
   r.key_blocks = static_cast<int>((p->n_key + keys - 1) / keys);
   r.row_blocks = static_cast<int>((p->n_query + kBlock - 1) / kBlock);
-  r.row_tasks = p->batch * p->heads * r.row_blocks;
-  const int64_t tasks = p->batch * p->kv_heads * r.key_blocks, want = 2 * device_cus();
-  const int64_t units = p->heads / p->kv_heads * std::max(1, r.query_tiles);
-  r.splits = tasks == 0 || tasks >= want ? 1
-                                         : static_cast<int>(std::min<int64_t>({(want + tasks - 1) / tasks, units, 16}));
-  r.key_tasks = tasks * r.splits;
+  // Times of a tile as splits_of() counts them, measured at 16 heads of 8,232 x 8,232: dK and dV 790 us (64 channels),
+  // 1,539 (128), dQ 494 and 909.
+  const double d = p->head_dim / 64.0;
+  const double key_us = dtype == VGO_F32 ? 8.7 * d : p->head_dim == 128 ? 4.0 : 1.2;
+  const double row_us = dtype == VGO_F32 ? 6.4 * d : 0.75 * d;
+  const int64_t tasks = p->batch * p->kv_heads * r.key_blocks, rows = p->batch * p->heads * r.row_blocks;
+  const int units = static_cast<int>(std::min<int64_t>(p->heads / p->kv_heads * std::max(1, r.query_tiles), 1 << 20));
+  const double key_bytes = 16.0 * p->batch * p->kv_heads * p->n_key * p->head_dim;
+  const double row_bytes = 8.0 * p->batch * p->heads * p->n_query * p->head_dim;
+  r.splits = tasks == 0 ? 1 : std::min(32, splits_of(p, tasks, units, dtype != VGO_F32 && p->head_dim == 64, key_us, key_bytes / 8e6));
+  r.row_splits = rows == 0 || r.key_tiles == 0 ? 1 : std::min(32, splits_of(p, rows, r.key_tiles, dtype != VGO_F32, row_us, row_bytes / 8e6));
+  r.key_tasks = tasks * r.splits, r.row_tasks = rows * r.row_splits;
   return r;
 }
 
 // Workspace pieces in order; each a multiple of 16 bytes.
 struct Pieces {
-  size_t delta, empty, kv, mass, slopes, table, bytes;
+  size_t delta, empty, kv, q, mass, slopes, table, bytes;
 };
 Pieces pieces_of(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const Plan& plan) {
   Pieces r{};
@@ -736,8 +778,9 @@ Pieces pieces_of(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const
   r.empty = take(rows * plan.query_tiles);
   const size_t keys = static_cast<size_t>(plan.splits) * p->batch * p->kv_heads * p->n_key;
   r.kv = take(plan.splits > 1 && g->dk ? keys * 2 * p->head_dim * 4 : 0);
+  r.q = take(plan.row_splits > 1 && g->dq ? plan.row_splits * rows * p->n_query * p->head_dim * 4 : 0);
   r.mass = take(g->d_log_mass ? keys * 4 : 0);
-  const size_t parts = static_cast<size_t>(p->batch) * plan.row_blocks * p->heads;
+  const size_t parts = static_cast<size_t>(plan.row_splits) * p->batch * plan.row_blocks * p->heads;
   r.slopes = take(g->d_slopes ? parts * 4 : 0);
   r.table = take(g->d_table ? parts * p->n_buckets * 4 : 0);
   r.bytes = at;
@@ -774,12 +817,13 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const Plan& pl
   }
   f.o = static_cast<const T*>(g->out), f.go = static_cast<const T*>(g->grad_out), f.lse = g->lse;
   f.dq = static_cast<T*>(g->dq), f.dk = static_cast<T*>(g->dk), f.dv = static_cast<T*>(g->dv);
-  f.query_tiles = plan.query_tiles, f.key_tiles = plan.key_tiles, f.splits = plan.splits;
+  f.query_tiles = plan.query_tiles, f.key_tiles = plan.key_tiles, f.splits = plan.splits, f.row_splits = plan.row_splits;
   f.key_blocks = plan.key_blocks, f.row_blocks = plan.row_blocks;
   f.key_tasks = static_cast<int>(plan.key_tasks), f.row_tasks = static_cast<int>(plan.row_tasks);
   const auto piece = [&](size_t offset) { return reinterpret_cast<float*>(ws + offset); };
   f.delta = piece(at.delta), f.empty = reinterpret_cast<unsigned char*>(ws + at.empty);
   if (plan.splits > 1 && f.dk) f.part_kv = piece(at.kv);
+  if (plan.row_splits > 1 && f.dq) f.part_q = piece(at.q);
   if (g->d_log_mass) f.part_mass = piece(at.mass);
   if (g->d_slopes) f.part_slopes = piece(at.slopes);
   if (g->d_table) f.part_table = piece(at.table);
@@ -823,13 +867,20 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const Plan& pl
                        stream, f);
     status = check_launch("masked_attn_grad rows");
     if (status != VGO_OK) return status;
+    if (f.part_q) {
+      const int64_t rows = p->batch * p->heads * p->n_query;
+      hipLaunchKernelGGL((join_rows_kernel<T, D>), dim3(static_cast<unsigned>((rows * (D / 4) + 255) / 256)), dim3(256),
+                         0, stream, f);
+      status = check_launch("masked_attn_grad join");
+      if (status != VGO_OK) return status;
+    }
   }
   if (g->d_log_mass) {
     status = sum_parts(f.part_mass, plan.key_tasks > 0 ? plan.splits * p->batch * p->kv_heads : 0, p->n_key,
                        g->d_log_mass, stream);
     if (status != VGO_OK) return status;
   }
-  const int64_t parts = p->batch * plan.row_blocks;
+  const int64_t parts = plan.row_splits * p->batch * plan.row_blocks;
   if (g->d_slopes) {
     status = sum_parts(f.part_slopes, parts, p->heads, g->d_slopes, stream);
     if (status != VGO_OK) return status;
