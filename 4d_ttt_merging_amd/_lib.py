@@ -55,7 +55,8 @@ class MaskedAttn(ctypes.Structure):
         ("scale", _c_f32), ("score_cap", _c_f32),
         ("log_mass", _c_p), ("slopes", _c_p), ("bucket_table", _c_p), ("bucket_starts", ctypes.POINTER(ctypes.c_int32)),
         ("n_buckets", ctypes.c_int32), ("n_starts", ctypes.c_int32), ("bidirectional", ctypes.c_int32),
-        ("causal", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("log_mass_dtype", ctypes.c_int32), ("slopes_dtype", ctypes.c_int32),
+        ("table_dtype", ctypes.c_int32),
         ("prefix_lengths", _c_p), ("query_documents", _c_p), ("key_documents", _c_p), ("key_lengths", _c_p),
         ("query_starts", _c_p),
     ]

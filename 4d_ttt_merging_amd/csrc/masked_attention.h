@@ -223,15 +223,36 @@ struct Args {
   int batch, heads, kv_heads, n_query, n_key;
   float scale, inv_cap, cap2;     // scale; scale / cap and cap log2(e) (0: no cap)
   float cap_reach, cap_series[5]; // kCapReach and kCapSeries for products before the scale (reach 0: not used)
-  const float* mass;              // [n_key] or null
-  const float* slopes;            // [heads] or null
-  const float* table;             // [n_buckets, heads] or null
+  const void* mass;               // [n_key] or null
+  const void* slopes;             // [heads] or null
+  const void* table;              // [n_buckets, heads] or null
+  int mass_type, slopes_type, table_type;
   Buckets buckets;                // of the table
   int causal, query_start;
   const int *prefix, *key_lengths, *query_starts;  // [batch] or null
   const int *query_doc, *key_doc;
   const int2 *query_info, *key_info;  // [batch, tiles]
 };
+
+// Element i of a parameter of any type, in units of log2.
+__device__ __forceinline__ float parameter2(const void* p, int type, int64_t i) {
+  const float x = type == VGO_F32    ? static_cast<const float*>(p)[i]
+                  : type == VGO_BF16 ? to_f32(static_cast<const bf16_t*>(p)[i])
+                                     : to_f32(static_cast<const f16_t*>(p)[i]);
+  return x * kLog2e;
+}
+template <typename T>
+__device__ __forceinline__ float mass2(const Args<T>& a, int key) { return parameter2(a.mass, a.mass_type, key); }
+template <typename T>
+__device__ __forceinline__ float slope2(const Args<T>& a, int head) {
+  return a.slopes ? parameter2(a.slopes, a.slopes_type, head) : 0.0f;
+}
+
+// A causal mask makes one end of a head's blocks the longest: every second list of blocks runs the other
+// way, so that work-groups that share a CU are long and short ones, and the last list ends with the short.
+__device__ __forceinline__ int zigzag(int index, int blocks, int list, int lists) {
+  return (lists - 1 - list) & 1 ? blocks - 1 - index : index;
+}
 
 template <typename T>
 __device__ __forceinline__ int key_limit(const Args<T>& a, int b) {
@@ -283,7 +304,7 @@ __device__ __forceinline__ void judge(const Args<T>& a, const Range& q, const Ra
 template <typename T>
 __device__ __forceinline__ void fill_distances(const Args<T>& a, float* to, int head, int threads) {
   for (int i = threadIdx.x; i <= 2 * a.buckets.reach; i += threads)
-    to[i] = a.table[static_cast<int64_t>(a.buckets.of(i - a.buckets.reach)) * a.heads + head] * kLog2e;
+    to[i] = parameter2(a.table, a.table_type, static_cast<int64_t>(a.buckets.of(i - a.buckets.reach)) * a.heads + head);
 }
 
 // out[i] = sum over parts of part[p][i], in a fixed order: 64 outputs a work-group, four runs of parts each.
@@ -300,11 +321,15 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64
   if (run == 0 && i < n)
     out[i] = from_f32<T>(((s[0][threadIdx.x] + s[1][threadIdx.x]) + s[2][threadIdx.x]) + s[3][threadIdx.x]);
 }
-template <typename T>
-int sum_parts(const float* part, int64_t parts, int64_t n, T* out, hipStream_t stream) {
+inline int sum_parts(const float* part, int64_t parts, int64_t n, void* out, int type, hipStream_t stream) {
   if (n == 0) return VGO_OK;
-  hipLaunchKernelGGL(sum_parts_kernel<T>, dim3(static_cast<unsigned>((n + 63) / 64)), dim3(256), 0, stream, part,
-                     parts, n, out);
+  const dim3 groups(static_cast<unsigned>((n + 63) / 64));
+  if (type == VGO_F32)
+    hipLaunchKernelGGL(sum_parts_kernel<float>, groups, dim3(256), 0, stream, part, parts, n, static_cast<float*>(out));
+  else if (type == VGO_BF16)
+    hipLaunchKernelGGL(sum_parts_kernel<bf16_t>, groups, dim3(256), 0, stream, part, parts, n, static_cast<bf16_t*>(out));
+  else
+    hipLaunchKernelGGL(sum_parts_kernel<f16_t>, groups, dim3(256), 0, stream, part, parts, n, static_cast<f16_t*>(out));
   return check_launch("sum of parts");
 }
 
@@ -354,9 +379,8 @@ __device__ __forceinline__ float add_pair<bf16_t>(float sum, float, float, bf16_
 
 inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
-// Document ranges of the tiles of one side (tile_info above).
-void launch_doc_info(const int* docs, const int* lengths, int n, int batch, int tiles, int2* info,
-                     hipStream_t stream);
+// Document ranges of the tiles of both sides (tile_info above): key_info [batch, key tiles], query_info behind it.
+void launch_doc_info(const vgo_masked_attn* p, int2* info, hipStream_t stream);
 
 // How many ways to split the `tiles` tiles of each of `tasks` work-groups (the rule stands at its definition).
 int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, bool hides, double tile_us, double join_us);
@@ -383,6 +407,7 @@ Args<T> make_args(const vgo_masked_attn* p) {
     }
   }
   a.mass = p->log_mass, a.slopes = p->slopes, a.table = p->bucket_table;
+  a.mass_type = p->log_mass_dtype, a.slopes_type = p->slopes_dtype, a.table_type = p->table_dtype;
   if (a.table) a.buckets = make_buckets(p->n_buckets, p->bucket_starts, p->n_starts, p->bidirectional);
   a.causal = p->causal != 0, a.query_start = a.n_key - a.n_query;
   a.prefix = p->prefix_lengths, a.key_lengths = p->key_lengths, a.query_starts = p->query_starts;
@@ -393,13 +418,11 @@ Args<T> make_args(const vgo_masked_attn* p) {
 // Document ranges of both sides' tiles: their bytes, and their launch into `ws`.
 size_t info_bytes(const vgo_masked_attn* p);
 template <typename T>
-void launch_info(Args<T>& a, char* ws, hipStream_t stream) {
+void launch_info(const vgo_masked_attn* p, Args<T>& a, char* ws, hipStream_t stream) {
   if (!a.key_doc) return;
-  const int kt = static_cast<int>(tiles_of(a.n_key)), qt = static_cast<int>(tiles_of(a.n_query));
   int2* key = reinterpret_cast<int2*>(ws);
-  int2* query = key + static_cast<int64_t>(a.batch) * kt;
-  launch_doc_info(a.key_doc, a.key_lengths, a.n_key, a.batch, kt, key, stream);
-  launch_doc_info(a.query_doc, nullptr, a.n_query, a.batch, qt, query, stream);
+  int2* query = key + static_cast<int64_t>(a.batch) * tiles_of(a.n_key);
+  launch_doc_info(p, key, stream);
   a.key_info = key, a.query_info = query;
 }
 

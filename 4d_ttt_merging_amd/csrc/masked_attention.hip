@@ -8,14 +8,17 @@ namespace vgo {
 namespace masked {
 namespace {
 
-// One wave per tile.
-__global__ __launch_bounds__(256) void doc_info_kernel(const int* docs, const int* lengths, int n, int batch,
-                                                       int tiles, int2* info) {
+// One wave per tile, the keys' tiles first.
+__global__ __launch_bounds__(256) void doc_info_kernel(const int* key_docs, const int* query_docs, const int* lengths,
+                                                       int n_key, int n_query, int batch, int key_tiles,
+                                                       int query_tiles, int2* info) {
   const int id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = lane_id();
-  if (id >= batch * tiles) return;
-  const int b = id / tiles, j = id % tiles * kTile + lane;
-  const int limit = lengths ? max(0, min(n, lengths[b])) : n;
-  const int doc = j < limit ? docs[static_cast<int64_t>(b) * n + j] : -1;
+  if (id >= batch * (key_tiles + query_tiles)) return;
+  const bool key = id < batch * key_tiles;
+  const int at = key ? id : id - batch * key_tiles, tiles = key ? key_tiles : query_tiles, n = key ? n_key : n_query;
+  const int b = at / tiles, j = at % tiles * kTile + lane;
+  const int limit = key && lengths ? max(0, min(n, lengths[b])) : n;
+  const int doc = j < limit ? (key ? key_docs : query_docs)[static_cast<int64_t>(b) * n + j] : -1;
   int lo = doc < 0 ? INT_MAX : doc, hi = doc < 0 ? -1 : doc;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
@@ -66,7 +69,12 @@ ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
   const int64_t tasks = vheads * r.row_blocks;
   const double tile_us = (dtype == VGO_F32 ? 4.3 : p->head_dim == 128 ? 0.5 : 0.62) * p->head_dim / 64;
   const double bytes = 8.0 * vheads * r.rows * p->head_dim;
-  r.splits = splits_of(p, tasks, r.tiles, dtype != VGO_F32, tile_us, bytes / 8e6);
+  // Few rows a task only wait for their keys: eight work-groups a CU keep the loads coming, and ragged lengths
+  // even out (32 sequences of up to 32,928 keys, 4 key heads: 208 us at 2 a CU, SEE at 8).
+  if (r.rows <= 32)
+    r.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((8 * device_cus() + tasks - 1) / std::max<int64_t>(1, tasks), r.tiles)));
+  else
+    r.splits = splits_of(p, tasks, r.tiles, dtype != VGO_F32, tile_us, bytes / 8e6);
   r.tasks = tasks * r.splits;
   return r;
 }
@@ -80,10 +88,13 @@ size_t forward_bytes(const vgo_masked_attn* p, const ForwardPlan& plan) {
   return n;
 }
 
-void launch_doc_info(const int* docs, const int* lengths, int n, int batch, int tiles, int2* info,
-                     hipStream_t stream) {
-  hipLaunchKernelGGL(doc_info_kernel, dim3((batch * tiles + 3) / 4), dim3(256), 0, stream, docs, lengths, n, batch,
-                     tiles, info);
+void launch_doc_info(const vgo_masked_attn* p, int2* info, hipStream_t stream) {
+  const int key_tiles = static_cast<int>(tiles_of(p->n_key)), query_tiles = static_cast<int>(tiles_of(p->n_query));
+  const int64_t waves = p->batch * (static_cast<int64_t>(key_tiles) + query_tiles);
+  if (waves == 0) return;
+  hipLaunchKernelGGL(doc_info_kernel, dim3(static_cast<unsigned>((waves + 3) / 4)), dim3(256), 0, stream,
+                     p->key_documents, p->query_documents, p->key_lengths, static_cast<int>(p->n_key),
+                     static_cast<int>(p->n_query), static_cast<int>(p->batch), key_tiles, query_tiles, info);
 }
 
 size_t info_bytes(const vgo_masked_attn* p) {
@@ -126,6 +137,11 @@ int check_problem(const vgo_masked_attn* p, int dtype) {
   VGO_REQUIRE(p->score_cap >= 0.0f && p->score_cap < kInf, "masked_attn: the score cap must be finite and not negative");
   VGO_REQUIRE(!p->prefix_lengths || p->causal, "masked_attn: a prefix goes with a causal mask");
   VGO_REQUIRE(!p->query_documents == !p->key_documents, "masked_attn: documents of queries and keys go together");
+  const auto number = [](int type) { return type == VGO_F32 || type == VGO_BF16 || type == VGO_F16; };
+  VGO_REQUIRE((!p->log_mass || number(p->log_mass_dtype)) && (!p->slopes || number(p->slopes_dtype)) &&
+                  (!p->bucket_table || number(p->table_dtype)),
+              "masked_attn: unsupported dtype of a parameter");
+  VGO_REQUIRE(p->batch * (tiles_of(p->n_key) + tiles_of(p->n_query)) < most, "masked_attn: too many rows");
   if (p->bucket_table) {
     const int status = check_buckets(p->n_buckets, p->bucket_starts, p->n_starts, p->bidirectional);
     if (status != VGO_OK) return status;

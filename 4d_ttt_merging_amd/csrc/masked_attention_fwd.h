@@ -113,7 +113,7 @@ struct Layout {
 // stay below 2^8, far from f16's largest number.
 constexpr float kSlack = 8.0f;
 
-template <typename T, int D, bool kCap, bool kBias, bool kLse>
+template <typename T, int D, bool kCap, int kBias, bool kLse>
 __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forward_kernel(
     const Forward<T> f) {
   typedef Tile<T, D> TL;
@@ -124,9 +124,9 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   const int lane = lane_id(), l31 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // Heads, then key splits, then row blocks from the last on (the longest first under a causal mask).
+  // Heads, then key splits, then row blocks.
   int task = xcd_remap(blockIdx.x, f.tasks);
-  const int block = f.row_blocks - 1 - task % f.row_blocks;
+  const int block = f.row_blocks - 1 - zigzag(task % f.row_blocks, f.row_blocks, task / f.row_blocks, f.tasks / f.row_blocks);
   task /= f.row_blocks;
   const int split = task % f.splits;
   task /= f.splits;
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   const int of_group = f.pack == 1 ? 0 : rc / a.n_query;
   const int index = rc - of_group * a.n_query, head = vh * f.pack + of_group, pos = start + index;
   const int doc = a.query_doc ? a.query_doc[static_cast<int64_t>(b) * a.n_query + index] : 0;
-  const float slope2 = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+  const float slope = slope2(a, head);
   const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances) + of_group * (2 * a.buckets.reach + 1);
   op8 q[TL::kSteps];
   const T* src = a.q + b * a.qs[0] + head * a.qs[1] + index * a.qs[2] + 8 * h;
@@ -196,15 +196,16 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   // Last of the keys that lengths and the causal mask leave the row.
   const int last = min(limit, a.causal ? max(pos + 1, walk.prefix) : INT_MAX) - 1;
 
+  float next_mass = 0.0f;  // of wave 0: the loaded tile's, one key a lane
   const auto load = [&](int buf) {
     const int k0 = walk.tile * kTile;
     const auto live = [&](int j) { return kdocs == nullptr || kdocs[j] >= 0; };
     stage<T, D, kWaves>(kbase, a.ks[2], k0, limit, walk.in_whole, lds0 + (2 * buf) * TL::kBytes, live);
     stage<T, D, kWaves>(vbase, a.vs[2], k0, limit, walk.in_whole, lds0 + (2 * buf + 1) * TL::kBytes, live);
     if (wave == 0) {
-      const uint32_t j = min(k0 + lane, a.n_key - 1) * 4u;
-      if (a.mass) lds_dma4(a.mass, j, lds0 + LO::kMass + buf * kTile * 4);
-      if (kdocs) lds_dma4(kdocs, j, lds0 + LO::kDocs + buf * kTile * 4);
+      const int j = min(k0 + lane, a.n_key - 1);
+      if (kdocs) lds_dma4(kdocs, j * 4u, lds0 + LO::kDocs + buf * kTile * 4);
+      if (kBias && a.mass) next_mass = mass2(a, j);
     }
   };
 
@@ -244,17 +245,19 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
           for (int g = 0; g < 4; ++g) {
             const f32x4 m = *reinterpret_cast<const f32x4*>(mass + 8 * g);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * g + e] = fmaf(x[4 * g + e], to2, m[e] * kLog2e);
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = fmaf(x[4 * g + e], to2, m[e]);
           }
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] *= to2;
         }
+      }
+      if constexpr (kBias == 2) {
         if (a.slopes) {
           const float d0 = static_cast<float>(k0 + j0 - pos);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            x[r] = fmaf(-slope2, fabsf(d0 + static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
+            x[r] = fmaf(-slope, fabsf(d0 + static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
         }
         if (a.table) {
           const int reach = a.buckets.reach;
@@ -339,6 +342,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
     const bool mine = walk.in_mine, full = walk.in_full;
     more = walk.next();
     wait_vmem<0>();
+    if (kBias && a.mass && wave == 0) reinterpret_cast<float*>(lds + LO::kMass)[buf * kTile + lane] = next_mass;
     __syncthreads();
     if (more) load(buf ^ 1);
     if (mine) compute(!full, k0, buf);
@@ -435,7 +439,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
         l32 == 0.0f ? kInf : m + __builtin_amdgcn_logf(l32);
 }
 
-template <typename T, int D, bool kCap, bool kBias, bool kLse>
+template <typename T, int D, bool kCap, int kBias, bool kLse>
 int launch(const Forward<T>& f, hipStream_t stream) {
   typedef Layout<T, D> LO;
   const size_t bytes = LO::kDistances + (f.a.table ? static_cast<size_t>(f.pack) * (2 * f.a.buckets.reach + 1) * 4 : 0);
@@ -449,18 +453,22 @@ int launch(const Forward<T>& f, hipStream_t stream) {
   return check_launch("masked_attn");
 }
 
-// The kernel without the rules that the problem does not have.
+// The kernel without the rules that the problem does not have: kBias 1 has masses alone, 2 slopes or a table too.
 template <typename T, int D>
 int choose(const Forward<T>& f, hipStream_t stream) {
-  const bool cap = f.a.cap2 != 0.0f, bias = f.a.mass || f.a.slopes || f.a.table;
-  const auto with = [&](auto lse) {
-    constexpr bool kLse = decltype(lse)::value;
-    if (cap) return bias ? launch<T, D, true, true, kLse>(f, stream) : launch<T, D, true, false, kLse>(f, stream);
-    return bias ? launch<T, D, false, true, kLse>(f, stream) : launch<T, D, false, false, kLse>(f, stream);
+  const int bias = f.a.slopes || f.a.table ? 2 : f.a.mass ? 1 : 0;
+  const auto with = [&](auto cap, auto lse) {
+    constexpr bool kCap = decltype(cap)::value, kLse = decltype(lse)::value;
+    return bias == 0   ? launch<T, D, kCap, 0, kLse>(f, stream)
+           : bias == 1 ? launch<T, D, kCap, 1, kLse>(f, stream)
+                       : launch<T, D, kCap, 2, kLse>(f, stream);
   };
+  const std::true_type yes{};
+  const std::false_type no{};
+  const bool cap = f.a.cap2 != 0.0f;
   if constexpr (std::is_same<T, bf16_t>::value)
-    if (f.lse) return with(std::true_type{});
-  return with(std::false_type{});
+    if (f.lse) return cap ? with(yes, yes) : with(no, yes);
+  return cap ? with(yes, no) : with(no, no);
 }
 
 template <typename T, int D>
@@ -472,7 +480,7 @@ int run(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int6
   f.out = static_cast<T*>(out), f.lse = lse;
   f.pack = plan.pack, f.rows = plan.rows, f.row_blocks = plan.row_blocks, f.splits = plan.splits;
   f.tiles = plan.tiles, f.tasks = static_cast<int>(plan.tasks);
-  launch_info(f.a, ws, stream);
+  launch_info(p, f.a, ws, stream);
   const int64_t rows = p->batch * (p->heads / plan.pack) * plan.rows;
   if (plan.splits > 1) {
     f.part_o = reinterpret_cast<float*>(ws + info_bytes(p));

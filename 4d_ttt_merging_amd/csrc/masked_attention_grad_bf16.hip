@@ -1,0 +1,10 @@
+// Gradients of the masked attention of bf16.
+#include "masked_attention_bwd.h"
+
+namespace vgo {
+namespace masked {
+
+template int run_grad<bf16_t>(const vgo_masked_attn*, const vgo_masked_attn_grads*, const GradPlan&, char*, hipStream_t);
+
+}  // namespace masked
+}  // namespace vgo

@@ -156,7 +156,7 @@ int run(BiasArgs<T> a, const void* table, void* out, hipStream_t stream) {
 }
 
 template <typename T>
-int run_grad(BiasGradArgs<T> a, const void* grad, void* d_table, float* part, hipStream_t stream) {
+int run_grad(BiasGradArgs<T> a, const void* grad, void* d_table, float* part, int dtype, hipStream_t stream) {
   a.grad = static_cast<const T*>(grad), a.part = part;
   if (a.row_blocks > 0) {
     hipLaunchKernelGGL(bias_grad_kernel<T>, dim3(static_cast<unsigned>(a.row_blocks) * a.heads), dim3(kThreads),
@@ -164,7 +164,7 @@ int run_grad(BiasGradArgs<T> a, const void* grad, void* d_table, float* part, hi
     const int status = check_launch("position_bias_grad");
     if (status != VGO_OK) return status;
   }
-  return sum_parts(part, a.row_blocks, static_cast<int64_t>(a.buckets.count) * a.heads, static_cast<T*>(d_table),
+  return sum_parts(part, a.row_blocks, static_cast<int64_t>(a.buckets.count) * a.heads, d_table, dtype,
                    stream);
 }
 
@@ -235,7 +235,7 @@ extern "C" int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64
   };
   float* part = static_cast<float*>(workspace);
   const hipStream_t s = as_stream(stream);
-  if (dtype == VGO_BF16) return run_grad(fill(BiasGradArgs<bf16_t>{}), grad, d_table, part, s);
-  if (dtype == VGO_F16) return run_grad(fill(BiasGradArgs<f16_t>{}), grad, d_table, part, s);
-  return run_grad(fill(BiasGradArgs<float>{}), grad, d_table, part, s);
+  if (dtype == VGO_BF16) return run_grad(fill(BiasGradArgs<bf16_t>{}), grad, d_table, part, dtype, s);
+  if (dtype == VGO_F16) return run_grad(fill(BiasGradArgs<f16_t>{}), grad, d_table, part, dtype, s);
+  return run_grad(fill(BiasGradArgs<float>{}), grad, d_table, part, dtype, s);
 }

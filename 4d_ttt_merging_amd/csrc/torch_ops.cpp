@@ -233,7 +233,7 @@ struct MaskedProblem {
       if (opt(t) == nullptr) return Tensor();
       same_device(*t);
       TORCH_CHECK_VALUE(t->is_floating_point() && t->sizes() == shape, what);
-      return t->to(at::kFloat).contiguous();
+      return t->contiguous();
     };
     const auto whole = [&](const OptTensor& t, at::IntArrayRef shape, const char* what) {
       if (opt(t) == nullptr) return Tensor();
@@ -258,7 +258,10 @@ struct MaskedProblem {
     p.head_dim = q.size(3);
     set_strides(p.q_stride, q), set_strides(p.k_stride, k), set_strides(p.v_stride, v);
     p.scale = static_cast<float>(rules.scale), p.score_cap = static_cast<float>(rules.score_cap);
-    p.log_mass = ptr<float>(log_mass), p.slopes = ptr<float>(slopes), p.bucket_table = ptr<float>(table);
+    p.log_mass = ptr(log_mass), p.slopes = ptr(slopes), p.bucket_table = ptr(table);
+    if (log_mass.defined()) p.log_mass_dtype = dtype_code(log_mass.scalar_type());
+    if (slopes.defined()) p.slopes_dtype = dtype_code(slopes.scalar_type());
+    if (table.defined()) p.table_dtype = dtype_code(table.scalar_type());
     starts.assign(rules.bucket_starts.begin(), rules.bucket_starts.end());
     p.bucket_starts = starts.data(), p.n_starts = static_cast<int32_t>(starts.size());
     p.n_buckets = table.defined() ? static_cast<int32_t>(table.size(0)) : 0;
@@ -291,7 +294,7 @@ std::tuple<Tensor, Tensor> masked_attention(
   return {out, lse};
 }
 
-// Gradients of q, k, v, log_mass, slopes and table (fp32 the last three); those not wanted are empty
+// Gradients of q, k, v, log_mass, slopes and table, each of its type; those not wanted are empty
 // (k and v come together).
 std::vector<Tensor> masked_attention_grad(
     const Tensor& grad0, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass,
@@ -325,9 +328,9 @@ std::vector<Tensor> masked_attention_grad(
     set_strides(stride, t);
   };
   fill(g.dq, g.dq_stride, dq, want.get(0)), fill(g.dk, g.dk_stride, dk, keys), fill(g.dv, g.dv_stride, dv, keys);
-  const auto make = [&](bool wanted, const Tensor& of, float*& p) {
+  const auto make = [&](bool wanted, const Tensor& of, void*& p) {
     const Tensor t = wanted && of.defined() ? at::empty(of.sizes(), of.options()) : none;
-    if (wanted && of.defined()) p = ptr<float>(t);
+    if (wanted && of.defined()) p = ptr(t);
     return t;
   };
   const Tensor d_mass = make(want.get(3), m.log_mass, g.d_log_mass);
@@ -982,7 +985,7 @@ struct MaskedAttentionFunction : torch::autograd::Function<MaskedAttentionFuncti
                 ctx->saved_data["bidirectional"].toBool(), ctx->saved_data["causal"].toBool(), want);
     variable_list result(16);
     for (size_t i = 0; i < 6; ++i)
-      if (want.get(i)) result[i] = i < 3 ? d[i] : d[i].to(s[i].scalar_type());
+      if (want.get(i)) result[i] = d[i];
     return result;
   }
 };

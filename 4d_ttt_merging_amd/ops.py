@@ -266,7 +266,7 @@ def _(grad, q, k, v, log_mass, slopes, table, prefix, query_documents, key_docum
     keys = want[1] or want[2]
     none = q.new_empty((0,))
     result = [_in_layout_of(t) if w else none for t, w in ((q, want[0]), (k, keys), (v, keys))]
-    return result + [t.new_empty(t.shape, dtype=torch.float32) if w and t is not None else none
+    return result + [t.new_empty(t.shape) if w and t is not None else none
                      for t, w in zip((log_mass, slopes, table), want[3:])]
 
 

@@ -566,9 +566,9 @@ int vgo_restore_residual_layer_norm(const float* x, int64_t x_row_stride, const 
  * q [batch, heads, n_query, head_dim], k / v [batch, kv_heads, n_key, head_dim], head_dim 64 or 128,
  * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)); strides in elements for
  * (batch, head, token), multiples of 16 bytes, with a unit channel stride; pointers 16-byte aligned.
- * Types as in vgo_mass_bias_attn_fwd; everything beside q, k, v is fp32 or int32.
+ * Types as in vgo_mass_bias_attn_fwd; log_mass, slopes and bucket_table each of its own such type.
  *   score_cap > 0: scores capped by a tanh (0: not).
- *   log_mass [n_key] (taken in fp32, not rounded), slopes [heads], bucket_table [n_buckets, heads].
+ *   log_mass [n_key] (not rounded to the inputs' type), slopes [heads], bucket_table [n_buckets, heads].
  *   bucket(r) = the number of bucket_starts (host, ascending, > 0, at most 128, the last one at most
  *     1024) that are <= |r|, plus n_buckets / 2 for r > 0 if bidirectional; else of max(-r, 0).
  *   key_documents [batch, n_key] with query_documents [batch, n_query] (contiguous): both or neither.
@@ -584,11 +584,12 @@ typedef struct vgo_masked_attn {
   int64_t batch, heads, kv_heads, n_query, n_key, head_dim;
   int64_t q_stride[3], k_stride[3], v_stride[3];
   float scale, score_cap;
-  const float* log_mass;
-  const float* slopes;
-  const float* bucket_table;
+  const void* log_mass;
+  const void* slopes;
+  const void* bucket_table;
   const int32_t* bucket_starts;
   int32_t n_buckets, n_starts, bidirectional, causal;
+  int32_t log_mass_dtype, slopes_dtype, table_dtype;
   const int32_t* prefix_lengths;
   const int32_t* query_documents;
   const int32_t* key_documents;
@@ -609,7 +610,7 @@ int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, const int64_t
 /*
  * Gradients of the forward for grad_out, from its out and lse.  dq / dk / dv have the inputs' type;
  * dk / dv sum over the heads that share them; d_log_mass [n_key], d_slopes [heads] and d_table
- * [n_buckets, heads] are fp32.  Outputs that are NULL are not computed (dk and dv: both or neither).
+ * [n_buckets, heads] have their parameter's type.  Outputs that are NULL are not computed (dk and dv: both or neither).
  * Sums are in a fixed order: the same inputs give the same bits.
  */
 typedef struct vgo_masked_attn_grads {
@@ -621,9 +622,9 @@ typedef struct vgo_masked_attn_grads {
   void* dk;
   void* dv;
   int64_t dq_stride[3], dk_stride[3], dv_stride[3];
-  float* d_log_mass;
-  float* d_slopes;
-  float* d_table;
+  void* d_log_mass;
+  void* d_slopes;
+  void* d_table;
 } vgo_masked_attn_grads;
 int vgo_masked_attn_grad_workspace(const vgo_masked_attn* problem, const vgo_masked_attn_grads* grads, int dtype,
                                    size_t* bytes);
