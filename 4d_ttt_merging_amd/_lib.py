@@ -66,7 +66,7 @@ class MaskedAttnGrads(ctypes.Structure):
     """`vgo_masked_attn_grads` of include/vgo.h."""
 
     _fields_ = [
-        ("out", _c_p), ("grad_out", _c_p), ("lse", _c_p), ("out_stride", _i64x3), ("grad_out_stride", _i64x3),
+        ("out", _c_p), ("grad_out", _c_p), ("lse", _c_p), ("out_rest", _c_p), ("out_stride", _i64x3), ("grad_out_stride", _i64x3),
         ("dq", _c_p), ("dk", _c_p), ("dv", _c_p),
         ("dq_stride", _i64x3), ("dk_stride", _i64x3), ("dv_stride", _i64x3),
         ("d_log_mass", _c_p), ("d_slopes", _c_p), ("d_table", _c_p),
@@ -187,7 +187,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ]),
     "vgo_masked_attn_workspace": (_c_int, [ctypes.POINTER(MaskedAttn), _c_int, ctypes.POINTER(_c_size)]),
     "vgo_masked_attn_fwd": (_c_int, [
-        ctypes.POINTER(MaskedAttn), _c_p, _i64x3, _c_p, _c_int, _c_p, _c_size, _c_p,
+        ctypes.POINTER(MaskedAttn), _c_p, _i64x3, _c_p, _c_p, _c_int, _c_p, _c_size, _c_p,
     ]),
     "vgo_masked_attn_grad_workspace": (_c_int, [
         ctypes.POINTER(MaskedAttn), ctypes.POINTER(MaskedAttnGrads), _c_int, ctypes.POINTER(_c_size),

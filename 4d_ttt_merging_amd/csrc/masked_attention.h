@@ -184,21 +184,36 @@ struct Buckets {
     for (int t = 0; t < n_starts; ++t) bucket += starts[t] <= n;
     return bucket + (bidirectional && r > 0 ? count / 2 : 0);
   }
-  // The sum of at(r) over the distances -reach .. reach of bucket t.
-  template <typename At>
-  __device__ __forceinline__ float sum(int t, At at) const {
-    const int side = bidirectional ? count / 2 : count, index = t % side;
-    float s = 0.0f;
-    if (index > n_starts) return s;
-    const int from = index == 0 ? 0 : starts[index - 1], to = index < n_starts ? starts[index] : reach + 1;
-    if (t >= side) {
-      for (int n = max(1, from); n < to; ++n) s += at(n);
-      return s;
+  // Sums by distance (by[r + reach], r = -reach .. reach, in LDS) to the sums of the buckets: put(t, sum), by
+  // the whole work-group, `kLanes` lanes a bucket.
+  template <int kThreads, typename Put>
+  __device__ __forceinline__ void gather(const float* by, Put put) const {
+    constexpr int kLanes = 8;
+    const int j = threadIdx.x % kLanes, side = bidirectional ? count / 2 : count;
+    for (int t0 = 0; t0 < count; t0 += kThreads / kLanes) {
+      const int t = t0 + threadIdx.x / kLanes, index = t % side;
+      float s = 0.0f;
+      if (t < count && index <= n_starts) {
+        const int from = index == 0 ? 0 : starts[index - 1], to = index < n_starts ? starts[index] : reach + 1;
+        const bool ahead = t >= side;
+        for (int n = (ahead ? max(1, from) : from) + j; n < to; n += kLanes) s += by[reach + (ahead ? n : -n)];
+        if (!bidirectional && index == 0)
+          for (int n = 1 + j; n <= reach; n += kLanes) s += by[reach + n];
+      }
+#pragma unroll
+      for (int off = kLanes / 2; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+      if (t < count && j == 0) put(t, s);
     }
-    for (int n = from; n < to; ++n) s += at(-n);
-    if (!bidirectional && index == 0)
-      for (int n = 1; n <= reach; ++n) s += at(n);
-    return s;
+  }
+};
+
+// A long sum in fp32 with what each addition lost.
+struct LongSum {
+  float sum = 0.0f, lost = 0.0f;
+  __device__ __forceinline__ void add(float x) {
+    const float y = x - lost, to = sum + y;
+    lost = (to - sum) - y;
+    sum = to;
   }
 };
 
@@ -314,8 +329,10 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
   const int run = threadIdx.x >> 6;
   float x = 0.0f;
-  if (i < n)
+  if (i < n) {
+#pragma unroll 8
     for (int64_t p = run; p < parts; p += 4) x += part[p * n + i];
+  }
   s[run][threadIdx.x & 63] = x;
   __syncthreads();
   if (run == 0 && i < n)

@@ -170,7 +170,7 @@ extern "C" int vgo_masked_attn_workspace(const vgo_masked_attn* problem, int dty
 }
 
 extern "C" int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, const int64_t out_stride[3], float* lse,
-                                   int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+                                   void* rest, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace vgo;
   using namespace vgo::masked;
   const int status = check_problem(problem, dtype);
@@ -178,13 +178,14 @@ extern "C" int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, co
   if (problem->batch == 0 || problem->n_query == 0) return VGO_OK;
   VGO_REQUIRE(out && out_stride && aligned(out, 16) && strides_fit(out_stride, problem->head_dim, dtype),
               "masked_attn: out must be 16-byte aligned, with strides of whole 16 bytes");
+  VGO_REQUIRE(aligned(rest, 16) && (!rest || dtype != VGO_F32), "masked_attn: rest must be 16-byte aligned, and of a 16-bit type");
   const ForwardPlan plan = forward_plan(problem, dtype);
   const size_t need = forward_bytes(problem, plan);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(VGO_EWORKSPACE, "masked_attn: workspace of " + std::to_string(need) + " bytes needed");
   char* ws = static_cast<char*>(workspace);
   const hipStream_t s = as_stream(stream);
-  if (dtype == VGO_BF16) return run_forward<bf16_t>(problem, plan, out, out_stride, lse, ws, s);
-  if (dtype == VGO_F16) return run_forward<f16_t>(problem, plan, out, out_stride, lse, ws, s);
-  return run_forward<float>(problem, plan, out, out_stride, lse, ws, s);
+  if (dtype == VGO_BF16) return run_forward<bf16_t>(problem, plan, out, out_stride, lse, rest, ws, s);
+  if (dtype == VGO_F16) return run_forward<f16_t>(problem, plan, out, out_stride, lse, rest, ws, s);
+  return run_forward<float>(problem, plan, out, out_stride, lse, rest, ws, s);
 }

@@ -56,7 +56,7 @@ namespace {
 template <typename T>
 struct Grad {
   Args<T> a;
-  const T *o, *go;
+  const T *o, *go, *rest;
   int64_t gos[3];
   const float* lse;
   float* delta;          // [batch, heads, n_query]; 0 for rows that attend to nothing
@@ -73,7 +73,8 @@ struct Grad {
 };
 
 
-// delta and empty: four lanes a row, a work-group per tile of one head.
+// delta and empty (delta from the unrounded outputs where their rest is there: what it is off by is off in every
+// score of the row): four lanes a row, a work-group per tile of one head.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
   const Args<T>& a = f.a;
@@ -89,7 +90,9 @@ __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      const f32x4 x = load4(o + 16 * c + 4 * part), y = load4(go + 16 * c + 4 * part);
+      f32x4 x = load4(o + 16 * c + 4 * part);
+      const f32x4 y = load4(go + 16 * c + 4 * part);
+      if (f.rest) x += load4(f.rest + row * D + 16 * c + 4 * part);
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum = fmaf(x[e], y[e], sum);
     }
@@ -190,7 +193,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
   f32x16 dk[TL::kCols], dv[TL::kCols];
 #pragma unroll
   for (int dt = 0; dt < TL::kCols; ++dt) dk[dt] = dv[dt] = f32x16{};
-  float mass_sum = 0.0f;
+  LongSum mass_sums;
 
   // (head of the group, query tile) units of this split, 64 judged at a time.
   const int units = group * f.query_tiles, per_split = (units + f.splits - 1) / f.splits;
@@ -336,8 +339,10 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       }
       if constexpr (kBias) {
         if (f.part_mass) {
+          float sum = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mass_sum += dz[r];
+          for (int r = 0; r < 16; ++r) sum += dz[r];
+          mass_sums.add(sum);
         }
         if constexpr (kCap) {
 #pragma unroll
@@ -374,7 +379,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
 
   const int64_t bk = static_cast<int64_t>(b) * a.kv_heads + kvh;
   if (f.part_mass) {
-    mass_sum = half_sum(mass_sum);
+    const float mass_sum = half_sum(mass_sums.sum);
     if (h == 0 && key < a.n_key)
       f.part_mass[(static_cast<int64_t>(split) * a.batch * a.kv_heads + bk) * a.n_key + key] = mass_sum;
   }
@@ -438,7 +443,7 @@ template <typename T, int D>
 struct RowLds {
   static constexpr int kBuffers = sizeof(T) == 4 && D == 128 ? 1 : 2;
   static constexpr int kMass = 2 * kBuffers * Tile<T, D>::kBytes, kDocs = kMass + 2 * kTile * 4;
-  static constexpr int kSums = kDocs + 2 * kTile * 4;  // [kRowWaves] slope sums, then far sums
+  static constexpr int kSums = kDocs + 2 * kTile * 4;  // the waves' slope sums
   static constexpr int kDistances = kSums + kRowWaves * 16;
 };
 constexpr int kDiagonal = 32 * 33 * 4;
@@ -509,7 +514,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
   f32x16 dq[TL::kCols];
 #pragma unroll
   for (int dt = 0; dt < TL::kCols; ++dt) dq[dt] = f32x16{};
-  float slope_sum = 0.0f, far_behind = 0.0f, far_ahead = 0.0f;
+  LongSum slope_sum, far_behind, far_ahead;
 
   const T* kbase = a.k + b * a.ks[0] + kvh * a.ks[1];
   const T* vbase = a.v + b * a.vs[0] + kvh * a.vs[1];
@@ -634,16 +639,17 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
       for (int r = 0; r < 16; ++r) dz[r] *= x[r];
       if constexpr (kBias == 2) {
         if (f.part_slopes) {
+          float sum = 0.0f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            slope_sum = fmaf(-fabsf(d0f + static_cast<float>(8 * (r / 4) + r % 4)), dz[r], slope_sum);
+          for (int r = 0; r < 16; ++r) sum = fmaf(-fabsf(d0f + static_cast<float>(8 * (r / 4) + r % 4)), dz[r], sum);
+          slope_sum.add(sum);
         }
         if (f.part_table) {
           if (behind || ahead) {
             float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) sum += dz[r];
-            (ahead ? far_ahead : far_behind) += sum;
+            (ahead ? far_ahead : far_behind).add(sum);
           } else {
             // dZ [32 keys][32 rows], then one lane a diagonal (key - row = lane - 31): 63 distances.
 #pragma unroll
@@ -658,9 +664,9 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
             }
             const int r = k0 + 32 * sub - rw.lo + d;
             if (r <= -reach)
-              far_behind += sum;
+              far_behind.add(sum);
             else if (r >= reach)
-              far_ahead += sum;
+              far_ahead.add(sum);
             else if (lane < 63)
               sums[r + reach] += sum;
           }
@@ -724,30 +730,24 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
   }
   const int64_t part = (static_cast<int64_t>(split) * a.batch + b) * f.row_blocks + block;
   if (kBias != 2 || (!f.part_slopes && !f.part_table)) return;
+  float slopes = slope_sum.sum, behind = far_behind.sum, ahead = far_ahead.sum;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
-    slope_sum += __shfl_xor(slope_sum, off);
-    far_behind += __shfl_xor(far_behind, off);
-    far_ahead += __shfl_xor(far_ahead, off);
+    slopes += __shfl_xor(slopes, off), behind += __shfl_xor(behind, off), ahead += __shfl_xor(ahead, off);
   }
   float* totals = reinterpret_cast<float*>(lds + LO::kSums);
-  if (lane == 0) {
-    totals[wave] = slope_sum, totals[kRowWaves + wave] = far_behind, totals[2 * kRowWaves + wave] = far_ahead;
-  }
+  if (lane == 0) totals[wave] = slopes;
+  if (f.part_table && lane == 0) sums[0] = behind, sums[2 * a.buckets.reach] = ahead;
   __syncthreads();
   if (f.part_slopes && threadIdx.x == 0)
     f.part_slopes[part * a.heads + head] = ((totals[0] + totals[1]) + totals[2]) + totals[3];
   if (!f.part_table) return;
-  const float* all_sums = distance + distances + kRowWaves * (kDiagonal / 4);
-  const auto of_distance = [&](int r) {
-    float s = 0.0f;
-    for (int w = 0; w < kRowWaves; ++w)
-      s += r <= -a.buckets.reach ? totals[kRowWaves + w] : r >= a.buckets.reach ? totals[2 * kRowWaves + w]
-                                                             : all_sums[w * distances + r + a.buckets.reach];
-    return s;
-  };
-  for (int t = threadIdx.x; t < a.buckets.count; t += 64 * kRowWaves)
-    f.part_table[(part * a.buckets.count + t) * a.heads + head] = a.buckets.sum(t, of_distance);
+  float* by = distance + distances + kRowWaves * (kDiagonal / 4);  // the waves' sums, into the first one's
+  for (int i = threadIdx.x; i < distances; i += 64 * kRowWaves)
+    by[i] = ((by[i] + by[distances + i]) + by[2 * distances + i]) + by[3 * distances + i];
+  __syncthreads();
+  a.buckets.template gather<64 * kRowWaves>(
+      by, [&](int t, float s) { f.part_table[(part * a.buckets.count + t) * a.heads + head] = s; });
 }
 
 // dQ of split work, likewise.
@@ -788,6 +788,7 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
     f.dqs[i] = g->dq_stride[i], f.dks[i] = g->dk_stride[i], f.dvs[i] = g->dv_stride[i];
   }
   f.o = static_cast<const T*>(g->out), f.go = static_cast<const T*>(g->grad_out), f.lse = g->lse;
+  f.rest = static_cast<const T*>(g->out_rest);
   f.dq = static_cast<T*>(g->dq), f.dk = static_cast<T*>(g->dk), f.dv = static_cast<T*>(g->dv);
   f.query_tiles = plan.query_tiles, f.key_tiles = plan.key_tiles, f.splits = plan.splits, f.row_splits = plan.row_splits;
   f.key_blocks = plan.key_blocks, f.row_blocks = plan.row_blocks;

@@ -4,8 +4,8 @@
 namespace vgo {
 namespace masked {
 
-template int run_forward<float>(const vgo_masked_attn*, const ForwardPlan&, void*, const int64_t[3], float*, char*,
-                                 hipStream_t);
+template int run_forward<float>(const vgo_masked_attn*, const ForwardPlan&, void*, const int64_t[3], float*, void*,
+                                 char*, hipStream_t);
 
 }  // namespace masked
 }  // namespace vgo

@@ -31,15 +31,23 @@ inline size_t align16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 // The launches of one type (instantiated in masked_attention_bf16.hip and its like).
 template <typename T>
 int run_forward(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int64_t out_stride[3], float* lse,
-                char* ws, hipStream_t stream);
+                void* rest, char* ws, hipStream_t stream);
 extern template int run_forward<bf16_t>(const vgo_masked_attn*, const ForwardPlan&, void*, const int64_t[3], float*,
-                                        char*, hipStream_t);
+                                        void*, char*, hipStream_t);
 extern template int run_forward<f16_t>(const vgo_masked_attn*, const ForwardPlan&, void*, const int64_t[3], float*,
-                                       char*, hipStream_t);
+                                       void*, char*, hipStream_t);
 extern template int run_forward<float>(const vgo_masked_attn*, const ForwardPlan&, void*, const int64_t[3], float*,
-                                       char*, hipStream_t);
+                                       void*, char*, hipStream_t);
 
 namespace {
+
+// What rounding to T takes from x.
+template <typename T>
+__device__ __forceinline__ f32x4 rounding(f32x4 x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] -= to_f32(from_f32<T>(x[e]));
+  return x;
+}
 
 // What a launch adds to the problem.
 template <typename T>
@@ -47,6 +55,7 @@ struct Forward {
   Args<T> a;
   T* out;
   float* lse;     // or null
+  T* rest;        // or null: what rounding took from out, [batch, heads, n_query, D]
   float* part_o;  // splits > 1: [splits, batch * virtual heads, rows, D] unnormalised sums
   float* part_ml; // and [.., rows, 3] their reference maxima (log2) and row sums (rounded, unrounded)
   int pack;       // heads per task (1, or heads / kv_heads)
@@ -381,6 +390,10 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0.0f : o[dt][4 * g + e] * inv;
       store4(dst + 32 * dt + 8 * g + 4 * h, y);
+      if (f.rest) {
+        const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.n_query + index;
+        store4(f.rest + at * D + 32 * dt + 8 * g + 4 * h, rounding<T>(y));
+      }
     }
   if (f.lse && h == 0)
     f.lse[(static_cast<int64_t>(b) * a.heads + head) * a.n_query + index] =
@@ -434,6 +447,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] *= inv;
   store4(f.out + b * a.os[0] + head * a.os[1] + i * a.os[2] + d, y);
+  if (f.rest)
+    store4(f.rest + ((static_cast<int64_t>(b) * a.heads + head) * a.n_query + i) * D + d, rounding<T>(y));
   if (f.lse && d == 0)
     f.lse[(static_cast<int64_t>(b) * a.heads + head) * a.n_query + i] =
         l32 == 0.0f ? kInf : m + __builtin_amdgcn_logf(l32);
@@ -472,12 +487,12 @@ int choose(const Forward<T>& f, hipStream_t stream) {
 }
 
 template <typename T, int D>
-int run(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int64_t out_stride[3], float* lse, char* ws,
-        hipStream_t stream) {
+int run(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int64_t out_stride[3], float* lse, void* rest,
+        char* ws, hipStream_t stream) {
   Forward<T> f{};
   f.a = make_args<T>(p);
   for (int i = 0; i < 3; ++i) f.a.os[i] = out_stride[i];
-  f.out = static_cast<T*>(out), f.lse = lse;
+  f.out = static_cast<T*>(out), f.lse = lse, f.rest = static_cast<T*>(rest);
   f.pack = plan.pack, f.rows = plan.rows, f.row_blocks = plan.row_blocks, f.splits = plan.splits;
   f.tiles = plan.tiles, f.tasks = static_cast<int>(plan.tasks);
   launch_info(p, f.a, ws, stream);
@@ -500,9 +515,9 @@ int run(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int6
 
 template <typename T>
 int run_forward(const vgo_masked_attn* p, const ForwardPlan& plan, void* out, const int64_t out_stride[3], float* lse,
-                char* ws, hipStream_t stream) {
-  return p->head_dim == 128 ? run<T, 128>(p, plan, out, out_stride, lse, ws, stream)
-                            : run<T, 64>(p, plan, out, out_stride, lse, ws, stream);
+                void* rest, char* ws, hipStream_t stream) {
+  return p->head_dim == 128 ? run<T, 128>(p, plan, out, out_stride, lse, rest, ws, stream)
+                            : run<T, 64>(p, plan, out, out_stride, lse, rest, ws, stream);
 }
 
 }  // namespace masked

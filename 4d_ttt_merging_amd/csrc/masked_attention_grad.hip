@@ -89,6 +89,8 @@ extern "C" int vgo_masked_attn_grad(const vgo_masked_attn* problem, const vgo_ma
                     strides_fit(g->out_stride, p->head_dim, dtype) &&
                     strides_fit(g->grad_out_stride, p->head_dim, dtype),
                 "masked_attn_grad: out and grad_out must be 16-byte aligned, with strides of whole 16 bytes");
+  VGO_REQUIRE(aligned(g->out_rest, 16) && (!g->out_rest || dtype != VGO_F32),
+              "masked_attn_grad: out_rest must be 16-byte aligned, and of a 16-bit type");
   VGO_REQUIRE((!g->dq || (aligned(g->dq, 16) && strides_fit(g->dq_stride, p->head_dim, dtype))) &&
                   (!g->dk || (aligned(g->dk, 16) && aligned(g->dv, 16) &&
                               strides_fit(g->dk_stride, p->head_dim, dtype) &&

@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kSegment = 2048;  // elements of a row per forward unit
-constexpr int kRows = 4;        // rows per wave of the gradient
+constexpr int kMostRows = 8;    // rows per wave of the gradient
 
 // LDS words of the table by distance: one of padding in 64, so that lanes 8 apart, 64 words on, do
 // not share a bank.
@@ -77,7 +77,7 @@ template <typename T>
 struct BiasGradArgs {
   const T* grad;
   float* part;  // [row blocks, buckets, heads]
-  int heads, n_query, n_key, start, row_blocks;
+  int heads, n_query, n_key, start, rows, row_blocks;  // rows: a wave's
   Buckets buckets;
 };
 
@@ -90,45 +90,57 @@ __global__ __launch_bounds__(kThreads) void bias_grad_kernel(const BiasGradArgs<
   float* sums = lds + wave * words;  // by distance + reach; the two ends take everything beyond
   for (int i = lane; i < words; i += 64) sums[i] = 0.0f;
   float behind = 0.0f, ahead = 0.0f;
-  for (int k = 0; k < kRows; ++k) {
-    const int i = (block * kRows + k) * kWaves + wave;
+  for (int k = 0; k < a.rows; ++k) {
+    const int i = (block * a.rows + k) * kWaves + wave;
     if (i >= a.n_query) break;
     const T* row = a.grad + (static_cast<int64_t>(head) * a.n_query + i) * a.n_key;
     const int pos = a.start + i;
-    // Keys 0 .. near0 lie behind the reach, near1 .. n_key ahead of it.
-    const int near0 = max(0, min(a.n_key, pos - reach + 1)), near1 = max(near0, min(a.n_key, pos + reach));
-    const auto run = [&](int j0, int j1) {
-      const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(row + j0) % 16 / sizeof(T));
-      const int lead = min(j1 - j0, skew == 0 ? 0 : kN - skew);
-      float s = lane < lead ? to_f32(row[j0 + lane]) : 0.0f;
-      const int body = j0 + lead, pieces = (j1 - body) / kN;
+    const auto single = [&](int j) {
+      const float x = to_f32(row[j]);
+      const int r = j - pos;
+      if (r <= -reach)
+        behind += x;
+      else if (r >= reach)
+        ahead += x;
+      else
+        sums[r + reach] += x;  // (every lane its own distance)
+    };
+    const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+    const int lead = min(a.n_key, skew == 0 ? 0 : kN - skew), pieces = (a.n_key - lead) / kN;
+    if (lane < lead) single(lane);
 #pragma unroll 4
-      for (int p = lane; p < pieces; p += 64) {
-        const Piece<T> x = *reinterpret_cast<const Piece<T>*>(row + body + p * kN);
+    for (int p = lane; p < pieces; p += 64) {
+      const int j = lead + p * kN, r = j - pos;
+      const Piece<T> x = *reinterpret_cast<const Piece<T>*>(row + j);
+      if (r + kN - 1 <= -reach || r >= reach) {
         float t = 0.0f;
 #pragma unroll
         for (int e = 0; e < kN; ++e) t += to_f32(x.x[e]);
-        s += t;
+        (r > 0 ? ahead : behind) += t;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          if (r + e <= -reach)
+            behind += to_f32(x.x[e]);
+          else if (r + e >= reach)
+            ahead += to_f32(x.x[e]);
+          else
+            sums[r + e + reach] += to_f32(x.x[e]);
+        }
       }
-      const int tail = body + pieces * kN;
-      return s + (tail + lane < j1 ? to_f32(row[tail + lane]) : 0.0f);
-    };
-    if (near0 > 0) behind += run(0, near0);
-    if (near1 < a.n_key) ahead += run(near1, a.n_key);
-#pragma unroll 4
-    for (int j = near0 + lane; j < near1; j += 64) sums[j - pos + reach] += to_f32(row[j]);
+    }
+    const int tail = lead + pieces * kN + lane;
+    if (tail < a.n_key) single(tail);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) behind += __shfl_xor(behind, off), ahead += __shfl_xor(ahead, off);
   if (lane == 0) sums[0] = behind, sums[2 * reach] = ahead;
   __syncthreads();
-  const auto at = [&](int r) {
-    float s = 0.0f;
-    for (int w = 0; w < kWaves; ++w) s += lds[w * words + r + reach];
-    return s;
-  };
-  for (int t = threadIdx.x; t < a.buckets.count; t += kThreads)
-    a.part[(static_cast<int64_t>(block) * a.buckets.count + t) * a.heads + head] = a.buckets.sum(t, at);
+  for (int i = threadIdx.x; i < words; i += kThreads)
+    lds[i] = ((lds[i] + lds[words + i]) + lds[2 * words + i]) + lds[3 * words + i];
+  __syncthreads();
+  a.buckets.template gather<kThreads>(
+      lds, [&](int t, float s) { a.part[(static_cast<int64_t>(block) * a.buckets.count + t) * a.heads + head] = s; });
 }
 
 int check(int64_t n_buckets, int64_t heads, const int32_t* starts, int n_starts, int bidirectional, int64_t query_start,
@@ -138,7 +150,7 @@ int check(int64_t n_buckets, int64_t heads, const int32_t* starts, int n_starts,
   VGO_REQUIRE(heads >= 1 && heads < most && n_query >= 0 && n_key >= 0 && n_query < most && n_key < most,
               "position_bias: sizes are below 2^28");
   VGO_REQUIRE(query_start > -most && query_start < most, "position_bias: the first position is below 2^28");
-  VGO_REQUIRE(heads * (n_query / (kRows * kWaves) + 1) < (int64_t{1} << 31) &&
+  VGO_REQUIRE(heads * (n_query / kWaves + 1) < (int64_t{1} << 31) &&
                   n_query * ((n_key + kSegment - 1) / kSegment) < (int64_t{1} << 31),
               "position_bias: too many rows");
   return check_buckets(n_buckets, starts, n_starts, bidirectional);
@@ -168,7 +180,15 @@ int run_grad(BiasGradArgs<T> a, const void* grad, void* d_table, float* part, in
                    stream);
 }
 
-int64_t row_blocks_of(int64_t n_query) { return (n_query + kRows * kWaves - 1) / (kRows * kWaves); }
+// Rows of a wave: one until the chip has 16 waves a CU, then up to eight (fewer partial sums).
+int rows_of(int64_t heads, int64_t n_query) {
+  const int64_t waves = 16LL * device_cus();
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMostRows, (heads * n_query + waves - 1) / waves)));
+}
+int64_t row_blocks_of(int64_t heads, int64_t n_query) {
+  const int64_t rows = static_cast<int64_t>(rows_of(heads, n_query)) * kWaves;
+  return (n_query + rows - 1) / rows;
+}
 
 }  // namespace
 }  // namespace masked
@@ -207,7 +227,7 @@ extern "C" int vgo_position_bias_grad_workspace(int64_t n_buckets, int64_t heads
   VGO_REQUIRE(bytes && n_buckets >= 0 && n_buckets <= 4096 && heads >= 1 && heads < (1 << 28) && n_query >= 0 &&
                   n_query < (1 << 28) && n_key >= 0,
               "position_bias_grad: sizes");
-  *bytes = n_key == 0 ? 0 : static_cast<size_t>(row_blocks_of(n_query)) * n_buckets * heads * 4;
+  *bytes = n_key == 0 ? 0 : static_cast<size_t>(row_blocks_of(heads, n_query)) * n_buckets * heads * 4;
   return VGO_OK;
 }
 
@@ -223,13 +243,14 @@ extern "C" int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64
   VGO_REQUIRE(d_table && (grad || n_query == 0 || n_key == 0), "position_bias_grad: null pointer");
   VGO_REQUIRE(aligned(grad, dtype == VGO_F32 ? 4 : 2) && aligned(d_table, dtype == VGO_F32 ? 4 : 2),
               "position_bias_grad: misaligned pointer");
-  const int64_t blocks = n_key == 0 ? 0 : row_blocks_of(n_query);
+  const int64_t blocks = n_key == 0 ? 0 : row_blocks_of(heads, n_query);
   const size_t need = static_cast<size_t>(blocks) * n_buckets * heads * 4;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
     return fail(VGO_EWORKSPACE, "position_bias_grad: workspace of " + std::to_string(need) + " bytes needed");
   const auto fill = [&](auto a) {
     a.heads = static_cast<int>(heads), a.n_query = static_cast<int>(n_query), a.n_key = static_cast<int>(n_key);
     a.start = static_cast<int>(query_start), a.row_blocks = static_cast<int>(blocks);
+    a.rows = rows_of(heads, n_query);
     a.buckets = make_buckets(static_cast<int>(n_buckets), bucket_starts, n_starts, bidirectional);
     return a;
   };

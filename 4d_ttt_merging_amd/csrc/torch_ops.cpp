@@ -272,9 +272,9 @@ struct MaskedProblem {
   }
 };
 
-// [out, lse]; lse (fp32 [batch, heads, n_query], what the gradients need of the forward) is empty
-// unless wanted.
-std::tuple<Tensor, Tensor> masked_attention(
+// [out, lse, rest]; what the gradients need of the forward -- lse (fp32 [batch, heads, n_query]) and, of
+// 16-bit types, rest (out's own rounding, like out) -- is empty unless wanted.
+std::tuple<Tensor, Tensor, Tensor> masked_attention(
     const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass, const OptTensor& slopes,
     const OptTensor& table, const OptTensor& prefix, const OptTensor& query_documents, const OptTensor& key_documents,
     const OptTensor& key_lengths, const OptTensor& query_starts, double scale, double score_cap,
@@ -284,14 +284,17 @@ std::tuple<Tensor, Tensor> masked_attention(
   const int dtype = dtype_code(q.scalar_type());
   const Tensor out = in_layout_of(q);
   const Tensor lse = at::empty({want_lse ? q.size(0) : 0, q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  const bool want_rest = want_lse && dtype != VGO_F32;
+  const Tensor rest = at::empty({want_rest ? q.size(0) : 0, q.size(1), q.size(2), q.size(3)}, q.options());
   size_t need = 0;
   check(vgo_masked_attn_workspace(&m.p, dtype, &need));
   const Tensor ws = need > 0 ? scratch(need, q) : Tensor();
   int64_t stride[3];
   set_strides(stride, out);
-  check(vgo_masked_attn_fwd(&m.p, ptr(out), stride, want_lse ? ptr<float>(lse) : nullptr, dtype, ptr(ws), need,
+  check(vgo_masked_attn_fwd(&m.p, ptr(out), stride, want_lse ? ptr<float>(lse) : nullptr,
+                            want_rest ? ptr(rest) : nullptr, dtype, ptr(ws), need,
                             stream_of(q)));
-  return {out, lse};
+  return {out, lse, rest};
 }
 
 // Gradients of q, k, v, log_mass, slopes and table, each of its type; those not wanted are empty
@@ -300,11 +303,11 @@ std::vector<Tensor> masked_attention_grad(
     const Tensor& grad0, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass,
     const OptTensor& slopes, const OptTensor& table, const OptTensor& prefix, const OptTensor& query_documents,
     const OptTensor& key_documents, const OptTensor& key_lengths, const OptTensor& query_starts, const Tensor& out0,
-    const Tensor& lse, double scale, double score_cap, at::IntArrayRef bucket_starts, bool bidirectional, bool causal,
-    c10::List<bool> want) {
+    const Tensor& lse, const Tensor& rest, double scale, double score_cap, at::IntArrayRef bucket_starts,
+    bool bidirectional, bool causal, c10::List<bool> want) {
   const MaskedProblem m(q, k, v, {log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths,
                                   query_starts, scale, score_cap, bucket_starts.vec(), bidirectional, causal});
-  require_gpu({&grad0, &out0, &lse});
+  require_gpu({&grad0, &out0, &lse, &rest});
   TORCH_CHECK_VALUE(want.size() == 6, "masked_attention_grad: want names six gradients");
   TORCH_CHECK_VALUE(grad0.sizes() == q.sizes() && grad0.scalar_type() == q.scalar_type() &&
                         out0.sizes() == q.sizes() && out0.scalar_type() == q.scalar_type(),
@@ -312,11 +315,16 @@ std::vector<Tensor> masked_attention_grad(
   TORCH_CHECK_VALUE(lse.dim() == 3 && lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat &&
                         lse.is_contiguous(),
                     "masked_attention_grad: lse must be contiguous float32 [batch, heads, n_query]");
-  TORCH_CHECK(grad0.device() == q.device() && out0.device() == q.device() && lse.device() == q.device(),
+  TORCH_CHECK_VALUE(rest.numel() == 0 || (rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() &&
+                                          rest.is_contiguous() && q.scalar_type() != at::kFloat),
+                    "masked_attention_grad: rest must be empty or contiguous and like q");
+  TORCH_CHECK(grad0.device() == q.device() && out0.device() == q.device() && lse.device() == q.device() &&
+                  rest.device() == q.device(),
               "masked_attention_grad: every tensor must be on the device of q");
   const Tensor grad = operand(grad0), out = operand(out0);
   vgo_masked_attn_grads g{};
   g.out = ptr(out), g.grad_out = ptr(grad), g.lse = ptr<float>(lse);
+  g.out_rest = rest.numel() > 0 ? ptr(rest) : nullptr;
   set_strides(g.out_stride, out), set_strides(g.grad_out_stride, grad);
   const bool keys = want.get(1) || want.get(2);
   const Tensor none = at::empty({0}, q.options());
@@ -962,11 +970,11 @@ struct MaskedAttentionFunction : torch::autograd::Function<MaskedAttentionFuncti
                         at::IntArrayRef bucket_starts, bool bidirectional, bool causal) {
     static const auto op = typed_operator<decltype(masked_attention)>("vgo::masked_attention");
     const at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, lse] = op.call(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths,
+    auto [out, lse, rest] = op.call(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths,
                               query_starts, scale, score_cap, bucket_starts, bidirectional, causal, true);
     ctx->save_for_backward({q, k, v, or_undefined(log_mass), or_undefined(slopes), or_undefined(table),
                             or_undefined(prefix), or_undefined(query_documents), or_undefined(key_documents),
-                            or_undefined(key_lengths), or_undefined(query_starts), out, lse});
+                            or_undefined(key_lengths), or_undefined(query_starts), out, lse, rest});
     ctx->saved_data["scale"] = scale, ctx->saved_data["score_cap"] = score_cap;
     ctx->saved_data["starts"] = bucket_starts.vec();
     ctx->saved_data["bidirectional"] = bidirectional, ctx->saved_data["causal"] = causal;
@@ -980,7 +988,7 @@ struct MaskedAttentionFunction : torch::autograd::Function<MaskedAttentionFuncti
     for (size_t i = 0; i < 6; ++i) want.push_back(s[i].defined() && ctx->needs_input_grad(edge++));
     const std::vector<Tensor> d =
         op.call(grads[0], s[0], s[1], s[2], or_none(s[3]), or_none(s[4]), or_none(s[5]), or_none(s[6]), or_none(s[7]),
-                or_none(s[8]), or_none(s[9]), or_none(s[10]), s[11], s[12], ctx->saved_data["scale"].toDouble(),
+                or_none(s[8]), or_none(s[9]), or_none(s[10]), s[11], s[12], s[13], ctx->saved_data["scale"].toDouble(),
                 ctx->saved_data["score_cap"].toDouble(), ctx->saved_data["starts"].toIntVector(),
                 ctx->saved_data["bidirectional"].toBool(), ctx->saved_data["causal"].toBool(), want);
     variable_list result(16);
@@ -990,7 +998,7 @@ struct MaskedAttentionFunction : torch::autograd::Function<MaskedAttentionFuncti
   }
 };
 
-std::tuple<Tensor, Tensor> masked_attention_autograd(
+std::tuple<Tensor, Tensor, Tensor> masked_attention_autograd(
     const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass, const OptTensor& slopes,
     const OptTensor& table, const OptTensor& prefix, const OptTensor& query_documents, const OptTensor& key_documents,
     const OptTensor& key_lengths, const OptTensor& query_starts, double scale, double score_cap,
@@ -999,7 +1007,8 @@ std::tuple<Tensor, Tensor> masked_attention_autograd(
     const Tensor out = MaskedAttentionFunction::apply(q, k, v, log_mass, slopes, table, prefix, query_documents,
                                                       key_documents, key_lengths, query_starts, scale, score_cap,
                                                       bucket_starts, bidirectional, causal);
-    return {out, at::empty({0, q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
+    const Tensor none = at::empty({0, q.size(1), q.size(2), q.size(3)}, q.options());
+    return {out, none.select(3, 0).to(at::kFloat), none};
   }
   static const auto op = typed_operator<decltype(masked_attention)>("vgo::masked_attention");
   const at::AutoDispatchBelowAutograd below;

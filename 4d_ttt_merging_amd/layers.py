@@ -20,7 +20,9 @@ library:
 
 Frame and register blocks (no plan) in bf16/f16 run the same attention kernel
 behind vgo_qkv_epilogue (LayerNorm64 + RoPE); other dtypes and layouts take
-the reference's torch op sequence.
+the reference's torch op sequence.  With `attn_bias` (keyword arguments of
+`masked_attention`) an unmerged block attends under masks and position biases, in
+inference and in training.
 The reference's experimental hooks that import the absent module
 `sampled_update_operator` (attention.py:267-299) and the source-query
 correction branch (attention.py:304-312, 376-385) are not part of this path
@@ -36,6 +38,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import _kernels, profiling
+from .masked_attention import masked_attention
 from .mass_bias_attention import _attention_into, _attention_pair_into
 from .token_merging import TokenPlan
 
@@ -199,6 +202,8 @@ class SelfAttention(nn.Module):
         if token_plan is not None and self.training:
             raise RuntimeError("token compaction is inference-only")
         self._check_hooks()
+        if attn_bias is not None and token_plan is not None:
+            raise ValueError("attn_bias does not go with a token plan")
         if token_plan is None:
             qkv = self.qkv(x)
             return self.proj_drop(self.proj(self.compute_attention(qkv=qkv, attn_bias=attn_bias,
@@ -243,16 +248,18 @@ class SelfAttention(nn.Module):
                 and (not self.use_qk_norm or (self.q_norm.eps == self.k_norm.eps)))
 
     def compute_attention(self, qkv: Tensor, attn_bias=None, rope=None, token_plan=None) -> Tensor:
-        assert attn_bias is None
+        """`attn_bias`: keyword arguments of `masked_attention` (masks, score cap, position biases)."""
         B, N, _ = qkv.shape
         C = self.qkv.in_features
         H = self.num_heads
         D = C // H
-        if self._fusable(qkv, C, H):
+        # The QKV epilogue has no derivative: a masked attention that is trained takes torch's operators
+        # in front of it.
+        if self._fusable(qkv, C, H) and (attn_bias is None or not torch.is_grad_enabled()):
             if token_plan is not None and rope is None:
                 return self._merged_fused(qkv, token_plan, B, N, C, H)
             if token_plan is None and self._attention_dtype(qkv) in (torch.bfloat16, torch.float16):
-                return self._dense_fused(qkv, rope, B, N, C, H)
+                return self._dense_fused(qkv, rope, B, N, C, H, attn_bias)
         # General path: the reference's op sequence (torch LayerNorm / RoPE / SDPA).
         q, k, v = torch.unbind(qkv.reshape(B, N, 3, H, D), 2)
         q, k, v = [t.transpose(1, 2) for t in (q, k, v)]
@@ -263,11 +270,14 @@ class SelfAttention(nn.Module):
             if rope is not None:
                 q, k = self.apply_rope(q, k, rope)
         if token_plan is None:
-            x = F.scaled_dot_product_attention(q, k, v)
+            if attn_bias is not None:
+                x = masked_attention(q, k.to(q.dtype), v.to(q.dtype), **attn_bias)
+            else:
+                x = F.scaled_dot_product_attention(q, k, v)
             return x.transpose(1, 2).reshape(B, N, C)
         return self._merged_attention(q, k, v, token_plan, B, N, C, H, D)
 
-    def _dense_fused(self, qkv: Tensor, rope, B: int, N: int, C: int, H: int) -> Tensor:
+    def _dense_fused(self, qkv: Tensor, rope, B: int, N: int, C: int, H: int, attn_bias=None) -> Tensor:
         """Frame/register attention: fused LayerNorm+RoPE epilogue, then the HIP kernel."""
         dtype = self._attention_dtype(qkv)
         qn, kn = self._norm_params()
@@ -282,6 +292,8 @@ class SelfAttention(nn.Module):
             k_norm=None if kn is None else kn[:2], eps=qn[2] if qn is not None else 1e-5,
             rope=rope, rope_prefix=rope_prefix, want=(True, True, values is None), out_dtype=dtype)
         v = v if values is None else values
+        if attn_bias is not None:
+            return masked_attention(q, k, v, **attn_bias).transpose(1, 2).reshape(B, N, C)
         out = torch.empty((B, N, H, 64), device=qkv.device, dtype=dtype)
         _attention_into(q, k, v, None, out.permute(0, 2, 1, 3))
         return out.view(B, N, C)
@@ -465,14 +477,17 @@ class SelfAttentionBlock(nn.Module):
         self.ls2 = LayerScale(dim, init_values=init_values, device=device) if init_values else nn.Identity()
         self.sample_drop_ratio = drop_path
 
-    def forward(self, x: Tensor, rope=None) -> Tensor:
-        """Inference forward of block.py:89-129 (no stochastic depth)."""
+    def forward(self, x: Tensor, rope=None, attn_bias=None) -> Tensor:
+        """Forward of block.py:89-129 (no stochastic depth).  `attn_bias`: keyword arguments of
+        `masked_attention` for the block's attention (not in the reference); trainable with it, under
+        autocast too."""
+        masked = {} if attn_bias is None else {"attn_bias": attn_bias}
         if self._fused_rows(x):
-            arguments = self._native_dense(x, rope)
+            arguments = self._native_dense(x, rope) if attn_bias is None else None
             if arguments is not None:
                 return torch.ops.vgo.dense_block(x, *arguments)
-            return self._fused_tail(x, self.attn(self._norm1_input(x), rope=rope))
-        x_attn = x + self.ls1(self.attn(self.norm1(x), rope=rope))
+            return self._fused_tail(x, self.attn(self._norm1_input(x), rope=rope, **masked))
+        x_attn = x + self.ls1(self.attn(self.norm1(x), rope=rope, **masked))
         return x_attn + self.ls2(self.mlp(self.norm2(x_attn)))
 
     def forward_compacted(self, x: Tensor, token_plan, *, normalized: Tensor = None) -> Tensor:

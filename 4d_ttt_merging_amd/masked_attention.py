@@ -68,8 +68,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
 
     q [B, H, Nq, D], k and v [B, Hk, Nk, D] of one type (bf16, f16 or fp32), D 64 or 128, H a multiple of
     Hk (head h reads key head h // (H // Hk)); any strides, those of a packed projection without a copy.
-    Returns [B, H, Nq, D], token-major in memory where q is.  Under bf16 autocast fp32 operands are cast
-    first, as in `mass_bias_attention`.
+    Returns [B, H, Nq, D], token-major in memory where q is.  Under bf16 or f16 autocast fp32 operands are
+    cast first.
 
     Position of query i: query_starts[b] + i (int32 [B]; default Nk - Nq, the queries at the keys' end).
     Scores:
@@ -101,9 +101,10 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
         raise ValueError("q, k and v must be [batch, heads, tokens, channels]")
     if q.shape[-1] not in (64, 128):
         raise ValueError("masked_attention takes 64 or 128 channels a head")
-    if (q.dtype == torch.float32 and torch.is_autocast_enabled("cuda")
-            and torch.get_autocast_dtype("cuda") == torch.bfloat16):
-        q, k, v = q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16)
+    if q.dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        if dtype in (torch.bfloat16, torch.float16):
+            q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
     if q.dtype not in _lib.DTYPE_CODE:
         raise ValueError(f"unsupported dtype {q.dtype}")
     if prefix_lengths is not None and not causal:

@@ -103,15 +103,16 @@ _SCHEMAS = (
     "int removed) -> (Tensor, Tensor, Tensor)",
     "fastvggt_plan(Tensor best, Tensor target, Tensor sources, Tensor destinations, int total, "
     "int removed) -> Tensor[]",
-    # [out, lse] of vgo_masked_attn_fwd; lse (fp32 [B, H, Nq]) is empty unless wanted.
+    # [out, lse, rest] of vgo_masked_attn_fwd; lse (fp32 [B, H, Nq]) and, of 16-bit types, rest are empty
+    # unless wanted.
     "masked_attention(Tensor q, Tensor k, Tensor v, Tensor? log_mass, Tensor? slopes, Tensor? table, "
     "Tensor? prefix, Tensor? query_documents, Tensor? key_documents, Tensor? key_lengths, Tensor? query_starts, "
     "float scale, float score_cap, int[] bucket_starts, bool bidirectional, bool causal, bool want_lse) "
-    "-> (Tensor, Tensor)",
+    "-> (Tensor, Tensor, Tensor)",
     # Gradients of q, k, v, log_mass, slopes, table; unwanted ones are empty.
     "masked_attention_grad(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor? log_mass, Tensor? slopes, "
     "Tensor? table, Tensor? prefix, Tensor? query_documents, Tensor? key_documents, Tensor? key_lengths, "
-    "Tensor? query_starts, Tensor out, Tensor lse, float scale, float score_cap, int[] bucket_starts, "
+    "Tensor? query_starts, Tensor out, Tensor lse, Tensor rest, float scale, float score_cap, int[] bucket_starts, "
     "bool bidirectional, bool causal, bool[] want) -> Tensor[]",
     "position_bias(Tensor table, int n_query, int n_key, int query_start, int[] bucket_starts, "
     "bool bidirectional) -> Tensor",
@@ -257,12 +258,14 @@ def _in_layout_of(t):
 @_fake("masked_attention")
 def _(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts, scale,
       score_cap, bucket_starts, bidirectional, causal, want_lse):
-    return _in_layout_of(q), q.new_empty((q.shape[0] if want_lse else 0, q.shape[1], q.shape[2]), dtype=torch.float32)
+    b = q.shape[0] if want_lse else 0
+    return (_in_layout_of(q), q.new_empty((b, *q.shape[1:3]), dtype=torch.float32),
+            q.new_empty((0 if q.dtype == torch.float32 else b, *q.shape[1:])))
 
 
 @_fake("masked_attention_grad")
 def _(grad, q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts, out,
-      lse, scale, score_cap, bucket_starts, bidirectional, causal, want):
+      lse, rest, scale, score_cap, bucket_starts, bidirectional, causal, want):
     keys = want[1] or want[2]
     none = q.new_empty((0,))
     result = [_in_layout_of(t) if w else none for t, w in ((q, want[0]), (k, keys), (v, keys))]

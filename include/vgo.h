@@ -599,16 +599,17 @@ typedef struct vgo_masked_attn {
 
 /*
  * The forward: out (of the inputs' type, strides as theirs) and, where not NULL, lse [batch, heads,
- * n_query] fp32: log2 of the row's sum of e^z, for vgo_masked_attn_grad.  Workspace (16-byte aligned, any contents):
+ * n_query] fp32: log2 of the row's sum of e^z, and (16-bit types) rest [batch, heads, n_query, head_dim]
+ * contiguous: out's own rounding, out + rest being the result to twice the bits; both for vgo_masked_attn_grad.  Workspace (16-byte aligned, any contents):
  * document ranges of the key tiles and the partial states of work split over the keys; its size is
  * for the device that is current.
  */
 int vgo_masked_attn_workspace(const vgo_masked_attn* problem, int dtype, size_t* bytes);
 int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, const int64_t out_stride[3], float* lse,
-                        int dtype, void* workspace, size_t workspace_bytes, void* stream);
+                        void* rest, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * Gradients of the forward for grad_out, from its out and lse.  dq / dk / dv have the inputs' type;
+ * Gradients of the forward for grad_out, from its out, lse and rest (out_rest; NULL: out alone).  dq / dk / dv have the inputs' type;
  * dk / dv sum over the heads that share them; d_log_mass [n_key], d_slopes [heads] and d_table
  * [n_buckets, heads] have their parameter's type.  Outputs that are NULL are not computed (dk and dv: both or neither).
  * Sums are in a fixed order: the same inputs give the same bits.
@@ -617,6 +618,7 @@ typedef struct vgo_masked_attn_grads {
   const void* out;
   const void* grad_out;
   const float* lse;
+  const void* out_rest;
   int64_t out_stride[3], grad_out_stride[3];
   void* dq;
   void* dk;
