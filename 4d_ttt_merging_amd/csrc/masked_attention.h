@@ -400,7 +400,7 @@ inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 void launch_doc_info(const vgo_masked_attn* p, int2* info, hipStream_t stream);
 
 // How many ways to split the `tiles` tiles of each of `tasks` work-groups (the rule stands at its definition).
-int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, bool hides, double tile_us, double join_us);
+int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, int resident, double tile_us, double join_us);
 // VGO_OK, or the status of a problem the kernels do not take, with its message.
 int check_problem(const vgo_masked_attn* p, int dtype);
 bool strides_fit(const int64_t stride[3], int64_t head_dim, int dtype);

@@ -28,28 +28,29 @@ __global__ __launch_bounds__(256) void doc_info_kernel(const int* key_docs, cons
 
 }  // namespace
 
-// Time of a launch by splits s, in us.  `tile_us`: a CU's time per tile and work-group where several keep it busy
-// (measured: 0.62 for 128 rows of 64 channels in 16 bits, 1.0 of 128, 4.3 and 8.6 in fp32).  Work-groups beside
-// each other hide each other's waits (`hides`): one alone takes twice that, two 2.6 times it, from three on it is
-// theirs each (from the first where the products take long, fp32, or a work-group has waves enough), and
-// what does not fill the last round costs as much as those few alone.  Joining
-// takes a launch and the partial states' way out and back (`join_us` per split).  16 heads of
-// 8,232 x 8,232 x 64: 397 us unsplit (1,040 tasks, 4.06 a CU), 370 in three; 2,058 in fp32: 287 and 188 (six).
-int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, bool hides, double tile_us, double join_us) {
-  // A causal mask leaves the tasks half of the tiles where all keys are the queries' own, documents fewer: their
-  // ends spread, so that only the whole work counts.
+// Time of a launch by splits s, in us.  `tile_us`: a CU's time per tile and work-group where `resident` of them,
+// as many as fit it, keep it busy (measured for 128 rows: 0.62 of 64 channels in 16 bits, 1.1 of 128, 4.3 and
+// 8.6 in fp32).  They hide each other's waits: of three, one alone takes 1.5 times its share and two 2.3 times
+// it, of two one 1.3 times it, and what does not fill the last round costs as much as those few alone.
+// Joining takes a launch and the partial states' way out and back (`join_us` per split).  16 heads of
+// 8,232 x 8,232 x 64: 412 us unsplit (1,040 tasks, 4.06 a CU), 388 in three; 2,058 x 128: 74 and 82 (in two);
+// 2,058 x 64 in fp32: 286 and 187 (in six).
+int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, int resident, double tile_us, double join_us) {
+  // A causal mask leaves the tasks half of the tiles where all keys are the queries' own, documents fewer: where
+  // more follow, their ends spread and the whole work counts; where all start at once, the longest does (2 x 16
+  // heads of 2,058 x 2,058, causal and capped: dQ 91 us unsplit, 79 in two).
   const bool all = !p->causal && !p->key_documents && !p->key_lengths;
   const double share =
       p->causal ? 1.0 - 0.5 * std::min<double>(p->n_query, p->n_key) / std::max<int64_t>(1, p->n_key) : 1.0;
-  const double cus = device_cus(), alone[3] = {0.0, 2.0, 2.6};
+  const double alone[4][3] = {{}, {0.0}, {0.0, 1.3}, {0.0, 1.5, 2.3}}, one = resident == 1 ? 1.0 : alone[resident][1];
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= std::min(tiles, 512); s += s < 8 ? 1 : s < 32 ? 4 : 32) {
-    const double run = (tiles + s - 1) / s, per_cu = tasks * s / cus;
+    const double run = (tiles + s - 1) / s, per_cu = tasks * s / static_cast<double>(device_cus());
     const int most = static_cast<int>(std::ceil(per_cu));
-    double beside = all ? most : std::max(1.0 / share, per_cu);
-    if (hides) beside = all ? most / 3 * 3 + alone[most % 3] : std::max(2.0 / share, per_cu);
-    const double us = run * share * beside * std::max(0.6, tile_us) + (s > 1 ? 6.0 + s * join_us : 0.0);
+    const double beside = all ? most / resident * resident + alone[resident][most % resident]
+                              : std::max(one / share, per_cu * (per_cu <= resident ? 2.0 : 1.15));
+    const double us = run * share * beside * tile_us * (p->score_cap > 0.0f ? 1.5 : 1.0) + (s > 1 ? 6.0 + s * join_us : 0.0);
     if (us < least * 0.98) least = us, best = s;
   }
   return best;
@@ -67,14 +68,19 @@ ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
   constexpr int kRows = 128;  // a task's
   r.row_blocks = (r.rows + kRows - 1) / kRows;
   const int64_t tasks = vheads * r.row_blocks;
-  const double tile_us = (dtype == VGO_F32 ? 4.3 : p->head_dim == 128 ? 0.5 : 0.62) * p->head_dim / 64;
-  const double bytes = 8.0 * vheads * r.rows * p->head_dim;
-  // Few rows a task only wait for their keys: eight work-groups a CU keep the loads coming, and ragged lengths
-  // even out (32 sequences of up to 32,928 keys, 4 key heads: 208 us at 2 a CU, SEE at 8).
-  if (r.rows <= 32)
-    r.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((8 * device_cus() + tasks - 1) / std::max<int64_t>(1, tasks), r.tiles)));
-  else
-    r.splits = splits_of(p, tasks, r.tiles, dtype != VGO_F32, tile_us, bytes / 8e6);
+  // Few rows a task only wait for their keys: two work-groups a CU at least, up to eight where each keeps four
+  // tiles (lengths even out), and no more than the join takes in its stride (32 sequences of 32,928 keys, 4 key
+  // heads: 554 us unsplit, 201 in 16; one of them: 541, and 22 in 64).
+  if (r.rows <= 32) {
+    const int64_t cus = device_cus(), n = std::max<int64_t>(1, tasks), tiles = std::max(1, r.tiles);
+    const int64_t want = std::max((2 * cus + n - 1) / n, std::min((8 * cus + n - 1) / n, tiles / 4));
+    r.splits = static_cast<int>(std::min<int64_t>({tiles, want, static_cast<int64_t>(std::ceil(std::sqrt(20.0 * tiles)))}));
+  } else {
+    const bool wide = p->head_dim == 128;
+    const double tile_us = dtype == VGO_F32 ? (wide ? 8.6 : 4.3) : wide ? 1.1 : 0.62;
+    const double bytes = 8.0 * vheads * r.rows * p->head_dim;
+    r.splits = splits_of(p, tasks, r.tiles, dtype == VGO_F32 ? 1 : wide ? 2 : 3, tile_us, bytes / 7e6);
+  }
   r.tasks = tasks * r.splits;
   return r;
 }

@@ -586,7 +586,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
       const float c = rescore<T, kCap>(a, x, bend);
       const float d0f = static_cast<float>(k0 + j0 - pos);
       if constexpr (kBias) {
-        if (a.mass) {
+        if (kBias == 1 || a.mass) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const f32x4 m = *reinterpret_cast<const f32x4*>(mass + j0 + 8 * g);

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
       if constexpr (kBias) {
         const float* mass = reinterpret_cast<const float*>(lds + LO::kMass) + buf * kTile + j0;
         const float to2 = kCap ? a.cap2 : a.scale * kLog2e;
-        if (a.mass) {
+        if (kBias == 1 || a.mass) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const f32x4 m = *reinterpret_cast<const f32x4*>(mass + 8 * g);

@@ -11,17 +11,16 @@ GradPlan grad_plan(const vgo_masked_attn* p, int dtype) {
   const int64_t keys = dtype != VGO_F32 && p->head_dim == 128 ? KeyLds<bf16_t, 128>::kBlock : KeyLds<bf16_t, 64>::kBlock;
   r.key_blocks = static_cast<int>((p->n_key + keys - 1) / keys);
   r.row_blocks = static_cast<int>((p->n_query + kRowBlock - 1) / kRowBlock);
-  // Times of a tile as splits_of() counts them, measured at 16 heads of 8,232 x 8,232: dK and dV 790 us (64 channels),
-  // 1,539 (128), dQ 494 and 909.
-  const double d = p->head_dim / 64.0;
-  const double key_us = dtype == VGO_F32 ? 8.7 * d : p->head_dim == 128 ? 4.0 : 1.2;
-  const double row_us = dtype == VGO_F32 ? 6.4 * d : 0.75 * d;
+  // Times of a tile and work-groups a CU holds, as splits_of() counts them, from 16 heads of 8,232 x 8,232: dK and
+  // dV 790 us (64 channels), 1,539 (128), dQ 494 and 909; and 2,058 x 2,058 in fp32.
+  const bool wide = p->head_dim == 128, f32 = dtype == VGO_F32;
+  const double key_us = f32 ? (wide ? 17.4 : 8.7) : wide ? 4.0 : 1.1, row_us = f32 ? (wide ? 12.8 : 6.4) : wide ? 1.26 : 0.68;
   const int64_t tasks = p->batch * p->kv_heads * r.key_blocks, rows = p->batch * p->heads * r.row_blocks;
   const int units = static_cast<int>(std::min<int64_t>(p->heads / p->kv_heads * std::max(1, r.query_tiles), 1 << 20));
   const double key_bytes = 16.0 * p->batch * p->kv_heads * p->n_key * p->head_dim;
   const double row_bytes = 8.0 * p->batch * p->heads * p->n_query * p->head_dim;
-  r.splits = tasks == 0 ? 1 : std::min(32, splits_of(p, tasks, units, dtype != VGO_F32 && p->head_dim == 64, key_us, key_bytes / 8e6));
-  r.row_splits = rows == 0 || r.key_tiles == 0 ? 1 : std::min(32, splits_of(p, rows, r.key_tiles, dtype != VGO_F32, row_us, row_bytes / 8e6));
+  r.splits = tasks == 0 ? 1 : std::min(32, splits_of(p, tasks, units, f32 || wide ? 1 : 3, key_us, key_bytes / 7e6));
+  r.row_splits = rows == 0 || r.key_tiles == 0 ? 1 : std::min(32, splits_of(p, rows, r.key_tiles, f32 ? 1 : wide ? 2 : 3, row_us, row_bytes / 7e6));
   r.key_tasks = tasks * r.splits, r.row_tasks = rows * r.row_splits;
   return r;
 }
