@@ -315,11 +315,16 @@ __device__ __forceinline__ void judge(const Args<T>& a, const Range& q, const Ra
   }
 }
 
-// table[bucket(r), head] log2(e) for r = -reach .. reach into LDS, by the whole work-group.
+// table[bucket(r), head] log2(e) by distance in LDS, r = 0 at distance_zero(): as far as a 64 x 32 block that
+// touches the buckets' reach does, so that lookups need no bounds of their own.
+constexpr int kMargin = 96;
+__host__ __device__ inline int distance_zero(int reach) { return reach + kMargin; }
+__host__ __device__ inline int distance_words(int reach) { return (2 * distance_zero(reach) + 4) & ~3; }
 template <typename T>
 __device__ __forceinline__ void fill_distances(const Args<T>& a, float* to, int head, int threads) {
-  for (int i = threadIdx.x; i <= 2 * a.buckets.reach; i += threads)
-    to[i] = parameter2(a.table, a.table_type, static_cast<int64_t>(a.buckets.of(i - a.buckets.reach)) * a.heads + head);
+  const int zero = distance_zero(a.buckets.reach);
+  for (int i = threadIdx.x; i <= 2 * zero; i += threads)
+    to[i] = parameter2(a.table, a.table_type, static_cast<int64_t>(a.buckets.of(i - zero)) * a.heads + head);
 }
 
 // out[i] = sum over parts of part[p][i], in a fixed order: 64 outputs a work-group, four runs of parts each.

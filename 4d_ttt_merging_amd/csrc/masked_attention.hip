@@ -60,7 +60,7 @@ ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
   ForwardPlan r{};
   const int group = static_cast<int>(p->heads / p->kv_heads);
   const int reach = p->bucket_table && p->n_starts ? p->bucket_starts[p->n_starts - 1] : 1;
-  const bool table_fits = !p->bucket_table || static_cast<int64_t>(group) * (2 * reach + 1) * 4 <= 32768;
+  const bool table_fits = !p->bucket_table || static_cast<int64_t>(group) * distance_words(reach) * 4 <= 32768;
   r.pack = p->n_query < 32 && table_fits ? group : 1;
   r.rows = static_cast<int>(r.pack * p->n_query);
   r.tiles = static_cast<int>(tiles_of(p->n_key));

@@ -280,14 +280,13 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
           const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances);
           const int reach = a.buckets.reach;
           if (rw.lo + 31 - p0 <= -reach || rw.lo - (p0 + kTile - 1) >= reach) {
-            const float far = distance[rw.lo > p0 ? 2 * reach : 0];
+            const float far = distance[rw.lo > p0 ? 2 * distance_zero(reach) : 0];
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] += far;
           } else {
-            const int d0 = key - p0 - i0;
+            const float* near = distance + (key - p0 - i0 + distance_zero(reach));
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              x[r] += distance[max(-reach, min(reach, d0 - (8 * (r / 4) + r % 4))) + reach];
+            for (int r = 0; r < 16; ++r) x[r] += near[-(8 * (r / 4) + r % 4)];
           }
         }
       }
@@ -437,8 +436,8 @@ __global__ __launch_bounds__(256) void join_keys_kernel(const Grad<T> f) {
 
 // --------------------------------------------------------- queries' side ----
 // LDS: K and V tiles (two buffers; one where two leave no room for the rest), masses and documents of
-// their keys, distance biases; for the table's gradient, per wave a 32 x 32 block of dZ (33 columns:
-// diagonals spread over the banks) and the sums by distance.
+// their keys, distance biases; for the table's gradient, per wave a sheared 32 x 32 block of dZ (rows of
+// kShear words: 16-byte reads spread over the banks) and the sums by distance.
 template <typename T, int D>
 struct RowLds {
   static constexpr int kBuffers = sizeof(T) == 4 && D == 128 ? 1 : 2;
@@ -446,7 +445,8 @@ struct RowLds {
   static constexpr int kSums = kDocs + 2 * kTile * 4;  // the waves' slope sums
   static constexpr int kDistances = kSums + kRowWaves * 16;
 };
-constexpr int kDiagonal = 32 * 33 * 4;
+constexpr int kShear = 36, kDiagonal = 63 * kShear;  // words
+__host__ __device__ inline int sum_words(int reach) { return (2 * reach + 4) & ~3; }
 
 template <typename T, int D, bool kCap, int kBias>
 __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_kernel(const Grad<T> f) {
@@ -504,12 +504,14 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
     }
   }
   float* distance = reinterpret_cast<float*>(lds + LO::kDistances);
-  const int distances = 2 * a.buckets.reach + 1;
-  float* diagonal = distance + distances + wave * (kDiagonal / 4);
-  float* sums = distance + distances + kRowWaves * (kDiagonal / 4) + wave * distances;
+  const int words = sum_words(a.buckets.reach);
+  float* diagonal = distance + distance_words(a.buckets.reach) + wave * kDiagonal;
+  float* sums = distance + distance_words(a.buckets.reach) + kRowWaves * kDiagonal + wave * words;
   if (kBias == 2 && a.table) fill_distances(a, distance, head, 64 * kRowWaves);
-  if (f.part_table)
-    for (int i = lane; i < distances; i += 64) sums[i] = 0.0f;
+  if (kBias == 2 && f.part_table) {
+    for (int i = lane; i < words; i += 64) sums[i] = 0.0f;
+    for (int i = lane; i < kDiagonal; i += 64) diagonal[i] = 0.0f;
+  }
 
   f32x16 dq[TL::kCols];
 #pragma unroll
@@ -606,14 +608,13 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
         }
         if (a.table) {
           if (behind || ahead) {
-            const float far = distance[ahead ? 2 * reach : 0];
+            const float far = distance[ahead ? 2 * distance_zero(reach) : 0];
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] += far;
           } else {
-            const int d0 = k0 + j0 - pos;
+            const float* near = distance + (k0 + j0 - pos + distance_zero(reach));
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              x[r] += distance[max(-reach, min(reach, d0 + 8 * (r / 4) + r % 4)) + reach];
+            for (int r = 0; r < 16; ++r) x[r] += near[8 * (r / 4) + r % 4];
           }
         }
       }
@@ -651,24 +652,27 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
             for (int r = 0; r < 16; ++r) sum += dz[r];
             (ahead ? far_ahead : far_behind).add(sum);
           } else {
-            // dZ [32 keys][32 rows], then one lane a diagonal (key - row = lane - 31): 63 distances.
+            // dZ sheared: row key - row + 31, column row, so that a diagonal is a row, one lane's; what no
+            // pair has was cleared at the start and stays.
 #pragma unroll
-            for (int r = 0; r < 16; ++r) diagonal[(8 * (r / 4) + 4 * h + r % 4) * 33 + l32] = dz[r];
+            for (int r = 0; r < 16; ++r)
+              diagonal[(8 * (r / 4) + 4 * h + r % 4 - l32 + 31) * kShear + l32] = dz[r];
             const int d = lane - 31;
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int j = i + d;
-              const float y = diagonal[max(0, min(31, j)) * 33 + i];
-              sum += j >= 0 && j < 32 ? y : 0.0f;
+            for (int i = 0; i < 8; ++i) {
+              const f32x4 y = *reinterpret_cast<const f32x4*>(diagonal + min(lane, 62) * kShear + 4 * i);
+              sum += (y[0] + y[1]) + (y[2] + y[3]);
             }
             const int r = k0 + 32 * sub - rw.lo + d;
-            if (r <= -reach)
-              far_behind.add(sum);
-            else if (r >= reach)
-              far_ahead.add(sum);
-            else if (lane < 63)
-              sums[r + reach] += sum;
+            if (lane < 63) {
+              if (r <= -reach)
+                far_behind.add(sum);
+              else if (r >= reach)
+                far_ahead.add(sum);
+              else
+                sums[r + reach] += sum;
+            }
           }
         }
       }
@@ -742,9 +746,9 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
   if (f.part_slopes && threadIdx.x == 0)
     f.part_slopes[part * a.heads + head] = ((totals[0] + totals[1]) + totals[2]) + totals[3];
   if (!f.part_table) return;
-  float* by = distance + distances + kRowWaves * (kDiagonal / 4);  // the waves' sums, into the first one's
-  for (int i = threadIdx.x; i < distances; i += 64 * kRowWaves)
-    by[i] = ((by[i] + by[distances + i]) + by[2 * distances + i]) + by[3 * distances + i];
+  float* by = distance + distance_words(a.buckets.reach) + kRowWaves * kDiagonal;  // all waves', into the first one's
+  for (int i = threadIdx.x; i < words; i += 64 * kRowWaves)
+    by[i] = ((by[i] + by[words + i]) + by[2 * words + i]) + by[3 * words + i];
   __syncthreads();
   a.buckets.template gather<64 * kRowWaves>(
       by, [&](int t, float s) { f.part_table[(part * a.buckets.count + t) * a.heads + head] = s; });
@@ -811,7 +815,7 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
   }
   const bool cap = f.a.cap2 != 0.0f;
   const int bias = f.a.slopes || f.a.table ? 2 : f.a.mass ? 1 : 0;  // (kBias: masses alone, or distances too)
-  const size_t distances = f.a.table ? static_cast<size_t>(2 * f.a.buckets.reach + 1) * 4 : 0;
+  const size_t distances = f.a.table ? static_cast<size_t>(distance_words(f.a.buckets.reach)) * 4 : 0;
   if ((f.dk || f.part_mass) && plan.key_tasks > 0) {
     const size_t bytes = KeyLds<T, D>::kDistances + distances;
     const auto kernel = cap ? (bias == 0 ? key_kernel<T, D, true, 0> : bias == 1 ? key_kernel<T, D, true, 1> : key_kernel<T, D, true, 2>)
@@ -832,7 +836,7 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
   }
   if ((f.dq || f.part_slopes || f.part_table) && plan.row_tasks > 0) {
     const size_t bytes = RowLds<T, D>::kDistances + distances +
-                         (f.part_table ? static_cast<size_t>(kRowWaves) * (kDiagonal + distances) : 0);
+                         (f.part_table ? static_cast<size_t>(kRowWaves) * (kDiagonal + sum_words(f.a.buckets.reach)) * 4 : 0);
     const auto kernel = cap ? (bias == 0 ? row_kernel<T, D, true, 0> : bias == 1 ? row_kernel<T, D, true, 1> : row_kernel<T, D, true, 2>)
                             : (bias == 0 ? row_kernel<T, D, false, 0> : bias == 1 ? row_kernel<T, D, false, 1> : row_kernel<T, D, false, 2>);
     status = allow_lds(kernel, bytes);

@@ -151,7 +151,8 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   const int index = rc - of_group * a.n_query, head = vh * f.pack + of_group, pos = start + index;
   const int doc = a.query_doc ? a.query_doc[static_cast<int64_t>(b) * a.n_query + index] : 0;
   const float slope = slope2(a, head);
-  const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances) + of_group * (2 * a.buckets.reach + 1);
+  const float* distance = reinterpret_cast<const float*>(lds + LO::kDistances) +
+                          of_group * distance_words(a.buckets.reach);
   op8 q[TL::kSteps];
   const T* src = a.q + b * a.qs[0] + head * a.qs[1] + index * a.qs[2] + 8 * h;
 #pragma unroll
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   }
   if (a.table)
     for (int g = 0; g < f.pack; ++g)
-      fill_distances(a, reinterpret_cast<float*>(lds + LO::kDistances) + g * (2 * a.buckets.reach + 1), vh * f.pack + g,
+      fill_distances(a, reinterpret_cast<float*>(lds + LO::kDistances) + g * distance_words(a.buckets.reach), vh * f.pack + g,
                      64 * kWaves);
 
   // Reference maxima (exponents of 2; -inf until something attends) and row sums.
@@ -271,14 +272,13 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
         if (a.table) {
           const int reach = a.buckets.reach;
           if (k0 + kTile - 1 - rw.lo <= -reach || k0 - rw.hi >= reach) {  // beyond the buckets' reach, all of it
-            const float far = distance[k0 > rw.lo ? 2 * reach : 0];
+            const float far = distance[k0 > rw.lo ? 2 * distance_zero(reach) : 0];
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] += far;
           } else {
-            const int d0 = k0 + j0 - pos;
+            const float* near = distance + (k0 + j0 - pos + distance_zero(reach));
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              x[r] += distance[max(-reach, min(reach, d0 + 8 * (r / 4) + r % 4)) + reach];
+            for (int r = 0; r < 16; ++r) x[r] += near[8 * (r / 4) + r % 4];
           }
         }
       }
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
 template <typename T, int D, bool kCap, int kBias, bool kLse>
 int launch(const Forward<T>& f, hipStream_t stream) {
   typedef Layout<T, D> LO;
-  const size_t bytes = LO::kDistances + (f.a.table ? static_cast<size_t>(f.pack) * (2 * f.a.buckets.reach + 1) * 4 : 0);
+  const size_t bytes = LO::kDistances + (f.a.table ? static_cast<size_t>(f.pack) * distance_words(f.a.buckets.reach) * 4 : 0);
   const auto kernel = forward_kernel<T, D, kCap, kBias, kLse>;
   if (bytes > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
