@@ -74,31 +74,41 @@ struct Grad {
 
 
 // delta and empty (delta from the unrounded outputs where their rest is there: what it is off by is off in every
-// score of the row): four lanes a row, a work-group per tile of one head.
+// score of the row): a work-group per tile of one head, 16 bytes a lane, every load of a lane's rows in flight
+// together.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
   const Args<T>& a = f.a;
+  constexpr int kEach = 16 / sizeof(T), kLanes = D / kEach, kStep = 256 / kLanes, kTimes = kTile / kStep;
+  typedef T Part __attribute__((ext_vector_type(kEach)));
   const int tile = blockIdx.x % f.query_tiles, bh = blockIdx.x / f.query_tiles;
   const int b = bh / a.heads, head = bh % a.heads;
-  const int i = tile * kTile + (threadIdx.x >> 2), part = threadIdx.x & 3;
+  const int part = threadIdx.x % kLanes, i0 = tile * kTile + threadIdx.x / kLanes;
+  const T* o = f.o + b * a.os[0] + head * a.os[1] + part * kEach;
+  const T* go = f.go + b * f.gos[0] + head * f.gos[1] + part * kEach;
+  const int64_t row0 = static_cast<int64_t>(bh) * a.n_query;
+  Part x[kTimes], y[kTimes], z[kTimes];
+  float lse[kTimes];
+#pragma unroll
+  for (int t = 0; t < kTimes; ++t) {
+    const int i = min(i0 + t * kStep, a.n_query - 1);
+    x[t] = *reinterpret_cast<const Part*>(o + i * a.os[2]);
+    y[t] = *reinterpret_cast<const Part*>(go + i * f.gos[2]);
+    z[t] = f.rest ? *reinterpret_cast<const Part*>(f.rest + (row0 + i) * D + part * kEach) : Part{};
+    lse[t] = f.lse[row0 + i];
+  }
   bool none = false;
-  if (i < a.n_query) {
-    const int64_t row = static_cast<int64_t>(bh) * a.n_query + i;
-    none = f.lse[row] == kInf;
-    const T* o = f.o + b * a.os[0] + head * a.os[1] + i * a.os[2];
-    const T* go = f.go + b * f.gos[0] + head * f.gos[1] + i * f.gos[2];
+#pragma unroll
+  for (int t = 0; t < kTimes; ++t) {
     float sum = 0.0f;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      f32x4 x = load4(o + 16 * c + 4 * part);
-      const f32x4 y = load4(go + 16 * c + 4 * part);
-      if (f.rest) x += load4(f.rest + row * D + 16 * c + 4 * part);
+    for (int e = 0; e < kEach; ++e) sum = fmaf(to_f32(x[t][e]) + to_f32(z[t][e]), to_f32(y[t][e]), sum);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum = fmaf(x[e], y[e], sum);
-    }
-    sum += quad_xor<1>(sum);
-    sum += quad_xor<2>(sum);
-    if (part == 0) f.delta[row] = none ? 0.0f : sum;
+    for (int off = 1; off < kLanes; off <<= 1) sum += __shfl_xor(sum, off);
+    const int i = i0 + t * kStep;
+    const bool empty = lse[t] == kInf;
+    none = none || (empty && i < a.n_query);
+    if (part == 0 && i < a.n_query) f.delta[row0 + i] = empty ? 0.0f : sum;
   }
   const bool any = __syncthreads_or(none);
   if (threadIdx.x == 0) f.empty[blockIdx.x] = any;
@@ -195,17 +205,16 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
   for (int dt = 0; dt < TL::kCols; ++dt) dk[dt] = dv[dt] = f32x16{};
   LongSum mass_sums;
 
-  // (head of the group, query tile) units of this split, 64 judged at a time.
-  const int units = group * f.query_tiles, per_split = (units + f.splits - 1) / f.splits;
-  const int end = rg.lo < limit ? min(units, (split + 1) * per_split) : 0;
-  int base = split * per_split - 64, unit = 0, unit_head = 0, unit_tile = 0;
+  // (head of the group, query tile) units of this split, every f.splits-th, 64 judged at a time.
+  const int end = rg.lo < limit ? group * f.query_tiles : 0;
+  int base = -64, unit = 0, unit_head = 0, unit_tile = 0;
   uint64_t todo = 0, mine = 0, full = 0, whole = 0;
   bool in_mine = false, in_full = false, in_whole = false;
   const auto next = [&]() {
     while (todo == 0) {
       base += 64;
-      if (base >= end) return false;
-      const int u = base + lane, g = u / f.query_tiles, t = u % f.query_tiles;
+      if (split + f.splits * base >= end) return false;
+      const int u = split + f.splits * (base + lane), g = u / f.query_tiles, t = u % f.query_tiles;
       bool any = u < end, any_w = false, all_w = false, all = false, inside = false;
       if (any) {
         Range r{};
@@ -222,7 +231,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
     }
     const int bit = __builtin_ctzll(todo);
     todo &= todo - 1;
-    unit = base + bit;
+    unit = split + f.splits * (base + bit);
     unit_head = kvh * group + unit / f.query_tiles, unit_tile = unit % f.query_tiles;
     in_mine = mine >> bit & 1, in_full = full >> bit & 1, in_whole = whole >> bit & 1;
     return true;
@@ -523,16 +532,16 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
   const int* kdocs = a.key_doc ? a.key_doc + static_cast<int64_t>(b) * a.n_key : nullptr;
   const uint32_t lds0 = lds_offset(lds);
 
-  const int per_split = (f.key_tiles + f.row_splits - 1) / f.row_splits;
-  const int end = min((limit + kTile - 1) / kTile, (split + 1) * per_split);
-  int base = split * per_split - 64, tile = 0;
+  // Key tiles of this split, every f.row_splits-th.
+  const int end = min((limit + kTile - 1) / kTile, f.key_tiles);
+  int base = -64, tile = 0;
   uint64_t todo = 0, mine = 0, full = 0, whole = 0;
   bool in_mine = false, in_full = false, in_whole = false;
   const auto next = [&]() {
     while (todo == 0) {
       base += 64;
-      if (base >= end) return false;
-      const int t = base + lane;
+      if (split + f.row_splits * base >= end) return false;
+      const int t = split + f.row_splits * (base + lane);
       bool any = t < end, any_w = false, all_w = false, all = false, inside = false;
       if (any) {
         Range r{};
@@ -549,7 +558,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
     }
     const int bit = __builtin_ctzll(todo);
     todo &= todo - 1;
-    tile = base + bit;
+    tile = split + f.row_splits * (base + bit);
     in_mine = mine >> bit & 1, in_full = full >> bit & 1, in_whole = whole >> bit & 1;
     return true;
   };

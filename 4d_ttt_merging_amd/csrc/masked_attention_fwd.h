@@ -63,19 +63,20 @@ struct Forward {
   int row_blocks, splits, tiles, tasks, joiners;
 };
 
-// The key tiles of one task that its work-group (`wg`) and this wave (`w`) take part in.
+// The key tiles of one task that its work-group (`wg`) and this wave (`w`) take part in, of every `step`-th from
+// `first` on: splits take turns, so that each gets its share of what masks and lengths leave.
 template <typename T>
 struct Walk {
   const Args<T>& a;
   Range wg, w;
-  int b, limit, prefix, end, base, tile;
-  uint64_t todo, mine, full, whole;  // of tiles base .. base + 63
+  int b, limit, prefix, end, first, step, base, tile;
+  uint64_t todo, mine, full, whole;  // of the 64 tiles first + step * (base ..)
   bool in_mine, in_full, in_whole;   // of `tile`
   const bool rows_here;              // the wave has rows
 
   __device__ __forceinline__ Walk(const Args<T>& args, const Range& group, const Range& wave, bool rows, int batch,
-                                  int begin, int last)
-      : a(args), wg(group), w(wave), b(batch), end(last), base(begin - 64), tile(0), todo(0),
+                                  int split, int splits, int tiles)
+      : a(args), wg(group), w(wave), b(batch), end(tiles), first(split), step(splits), base(-64), tile(0), todo(0),
         rows_here(rows) {
     limit = key_limit(a, b);
     prefix = prefix_of(a, b);
@@ -84,8 +85,8 @@ struct Walk {
   __device__ __forceinline__ bool next() {
     while (todo == 0) {
       base += 64;
-      if (base >= end) return false;
-      const int t = base + lane_id();
+      if (first + step * base >= end) return false;
+      const int t = first + step * (base + lane_id());
       bool any = t < end, all_w = false, any_w = false, whole_t = false;
       if (any) {
         Range k{};
@@ -95,7 +96,7 @@ struct Walk {
         judge(a, wg, k, prefix, any, all);
         judge(a, w, k, prefix, any_w, all_w);
         const bool inside = k.lo + kTile <= limit;
-      any_w = any_w && rows_here;
+        any_w = any_w && rows_here;
         all_w = all_w && inside;
         whole_t = inside && (!a.key_doc || k.docs_whole);
       }
@@ -103,7 +104,7 @@ struct Walk {
     }
     const int bit = __builtin_ctzll(todo);
     todo &= todo - 1;
-    tile = base + bit;
+    tile = first + step * (base + bit);
     in_mine = mine >> bit & 1, in_full = full >> bit & 1, in_whole = whole >> bit & 1;
     return true;
   }
@@ -200,8 +201,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   const T* vbase = a.v + b * a.vs[0] + kvh * a.vs[1];
   const int* kdocs = a.key_doc ? a.key_doc + static_cast<int64_t>(b) * a.n_key : nullptr;
   const uint32_t lds0 = lds_offset(lds);
-  const int per_split = (f.tiles + f.splits - 1) / f.splits;
-  Walk<T> walk(a, rg, rw, row0 < f.rows, b, split * per_split, min(f.tiles, (split + 1) * per_split));
+  Walk<T> walk(a, rg, rw, row0 < f.rows, b, split, f.splits, f.tiles);
   const int limit = walk.limit;
   // Last of the keys that lengths and the causal mask leave the row.
   const int last = min(limit, a.causal ? max(pos + 1, walk.prefix) : INT_MAX) - 1;
