@@ -59,7 +59,7 @@ struct Grad {
   const T *o, *go, *rest;
   int64_t gos[3];
   const float* lse;
-  float* delta;          // [batch, heads, n_query]; 0 for rows that attend to nothing
+  float* delta;          // [batch, heads, n_query], -D; 0 for rows that attend to nothing
   unsigned char* empty;  // [batch, heads, query tiles]: a row of the tile attends to nothing
   T *dq, *dk, *dv;       // dq null: not wanted; likewise dk and dv
   int64_t dqs[3], dks[3], dvs[3];
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
     const int i = i0 + t * kStep;
     const bool empty = lse[t] == kInf;
     none = none || (empty && i < a.n_query);
-    if (part == 0 && i < a.n_query) f.delta[row0 + i] = empty ? 0.0f : sum;
+    if (part == 0 && i < a.n_query) f.delta[row0 + i] = empty ? 0.0f : -sum;
   }
   const bool any = __syncthreads_or(none);
   if (threadIdx.x == 0) f.empty[blockIdx.x] = any;
@@ -333,18 +333,20 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
         for (int r = 0; r < 16; ++r) x[r] *= bend[r];
       }
       __builtin_amdgcn_sched_barrier(0);
-      f32x16 dp{};
+      f32x16 dp;  // starts from -D
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + i0 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * g + e] = d4[e];
+      }
 #pragma unroll
       for (int t = 0; t < TL::kSteps; ++t)
         dp = Op<T>::mma(TL::rows_op(gt, 32 * sub, t), LO::kValues ? TL::rows_op(vl, 0, t) : v[LO::kValues ? 0 : t], dp);
       __builtin_amdgcn_sched_barrier(0);
       float dz[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + i0 + 8 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dz[4 * g + e] = x[4 * g + e] * (dp[4 * g + e] - d4[e]);
-      }
+      for (int r = 0; r < 16; ++r) dz[r] = x[r] * dp[r];
       if constexpr (kBias) {
         if (f.part_mass) {
           float sum = 0.0f;
@@ -630,7 +632,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         x[r] = __builtin_amdgcn_exp2f(kBias ? x[r] - lse : fmaf(x[r], c, -lse));
-        dz[r] -= delta;
+        dz[r] += delta;
       }
       if (partial) {
         const int last_r = last - k0 - j0;
