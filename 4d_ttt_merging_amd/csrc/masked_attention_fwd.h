@@ -123,7 +123,11 @@ struct Layout {
 // stay below 2^8, far from f16's largest number.
 constexpr float kSlack = 8.0f;
 
-template <typename T, int D, bool kCap, int kBias, bool kLse>
+// kTrain: 1 where gradients follow, whose probabilities are those of the unrounded row sum; 2 with slopes, too.
+// D = dO . O then has to be the mean of dP under the very probabilities that the gradients compute again: the
+// slopes' weigh what it is off by with the distances, and from rounded probabilities they were off by 0.2 to
+// 0.5% in bf16.  A second product takes what the rounding left out (1e-5).
+template <typename T, int D, bool kCap, int kBias, int kTrain>
 __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forward_kernel(
     const Forward<T> f) {
   typedef Tile<T, D> TL;
@@ -326,12 +330,12 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
     float sum = 0.0f, sum32 = 0.0f;
 #pragma unroll
     for (int r = 0; r < 32; r += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16], c, off));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16 + 1], c, off));
+      float& p0 = x[r / 16][r % 16] = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16], c, off));
+      float& p1 = x[r / 16][r % 16 + 1] = __builtin_amdgcn_exp2f(fmaf(x[r / 16][r % 16 + 1], c, off));
       op8& to = p[r / 8];
       to[r % 8] = from_f32<T>(p0), to[r % 8 + 1] = from_f32<T>(p1);
       sum = add_pair<T>(sum, p0, p1, to[r % 8], to[r % 8 + 1]);
-      if constexpr (kLse && sizeof(T) == 2) sum32 += p0 + p1;
+      if constexpr (kTrain) sum32 += p0 + p1;
     }
     lsum += sum, lsum32 += sum32;
 #pragma unroll
@@ -341,6 +345,15 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
         const op8 va = TL::cols_op(vt, dt, kc);
         o[dt] = Op<T>::mma(va, p[kc], o[dt]);
       }
+    if constexpr (kTrain == 2) {
+#pragma unroll
+      for (int r = 0; r < 32; ++r)
+        p[r / 8][r % 8] = from_f32<T>(x[r / 16][r % 16] - to_f32(static_cast<T>(p[r / 8][r % 8])));
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc)
+#pragma unroll
+        for (int dt = 0; dt < TL::kCols; ++dt) o[dt] = Op<T>::mma(TL::cols_op(vt, dt, kc), p[kc], o[dt]);
+    }
   };
 
   bool more = walk.next();
@@ -362,7 +375,8 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
   const bool dead = a.query_doc && doc < 0;
   float l = half_sum(lsum);
   // The gradients divide by the sum of the unrounded probabilities, which they compute again.
-  float l32 = kLse && sizeof(T) == 2 ? half_sum(lsum32) : l;
+  float l32 = kTrain ? half_sum(lsum32) : l;
+  if constexpr (kTrain == 2) l = l32;
   if (dead) l = l32 = 0.0f;
   if (f.splits > 1) {
     const int64_t row = (static_cast<int64_t>(split) * a.batch * vheads + b * vheads + vh) * f.rows + row0 +
@@ -454,11 +468,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
         l32 == 0.0f ? kInf : m + __builtin_amdgcn_logf(l32);
 }
 
-template <typename T, int D, bool kCap, int kBias, bool kLse>
+template <typename T, int D, bool kCap, int kBias, int kTrain>
 int launch(const Forward<T>& f, hipStream_t stream) {
   typedef Layout<T, D> LO;
   const size_t bytes = LO::kDistances + (f.a.table ? static_cast<size_t>(f.pack) * distance_words(f.a.buckets.reach) * 4 : 0);
-  const auto kernel = forward_kernel<T, D, kCap, kBias, kLse>;
+  const auto kernel = forward_kernel<T, D, kCap, kBias, kTrain>;
   if (bytes > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
@@ -472,18 +486,20 @@ int launch(const Forward<T>& f, hipStream_t stream) {
 template <typename T, int D>
 int choose(const Forward<T>& f, hipStream_t stream) {
   const int bias = f.a.slopes || f.a.table ? 2 : f.a.mass ? 1 : 0;
-  const auto with = [&](auto cap, auto lse) {
-    constexpr bool kCap = decltype(cap)::value, kLse = decltype(lse)::value;
-    return bias == 0   ? launch<T, D, kCap, 0, kLse>(f, stream)
-           : bias == 1 ? launch<T, D, kCap, 1, kLse>(f, stream)
-                       : launch<T, D, kCap, 2, kLse>(f, stream);
+  const auto with = [&](auto cap) {
+    constexpr bool kCap = decltype(cap)::value;
+    if constexpr (sizeof(T) == 2)
+      if (f.lse && f.a.slopes) return launch<T, D, kCap, 2, 2>(f, stream);
+    if constexpr (std::is_same<T, bf16_t>::value)
+      if (f.lse)
+        return bias == 0   ? launch<T, D, kCap, 0, 1>(f, stream)
+               : bias == 1 ? launch<T, D, kCap, 1, 1>(f, stream)
+                           : launch<T, D, kCap, 2, 1>(f, stream);
+    return bias == 0   ? launch<T, D, kCap, 0, 0>(f, stream)
+           : bias == 1 ? launch<T, D, kCap, 1, 0>(f, stream)
+                       : launch<T, D, kCap, 2, 0>(f, stream);
   };
-  const std::true_type yes{};
-  const std::false_type no{};
-  const bool cap = f.a.cap2 != 0.0f;
-  if constexpr (std::is_same<T, bf16_t>::value)
-    if (f.lse) return cap ? with(yes, yes) : with(no, yes);
-  return cap ? with(yes, no) : with(no, no);
+  return f.a.cap2 != 0.0f ? with(std::true_type{}) : with(std::false_type{});
 }
 
 template <typename T, int D>

@@ -460,3 +460,36 @@ def test_operators_together(vgo, device):
         token = vgo.masked_attention(q[:, :, t:t + 1], cache_k, cache_v, bucket_table=table.detach(), key_lengths=length,
                                      query_starts=length - 1, **rules)
         assert (token.double() - plain[:, :, t:t + 1]).abs().max() <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_slope_gradient_under_equal_rows(vgo, device, dtype, d):
+    """Rows that all round their probabilities alike, where what D = dO . O is off by adds up: q = 0, slopes of 0, and
+    keys told apart by their masses alone.
+
+    Each of P, O and the dP . P that D stands for is taken with a rounding of what a rounding left out, u^2 with
+    u = eps / 2, or in 32 bits; the distances weigh it.  So d slope is off by at most (2 u^2 + 2^-18) times
+    T = sum over pairs of P |r| (|dO| . |v| + |dO| . sum P |v|): 2^-18 for the exponentials (2^-21 on exponents
+    of at most 8), 128 products and the sums of at most 2^6 terms of 2^-24 each, T times.
+    """
+    n, heads = 64, 2
+    mass = torch.tensor([1.0, 1.7, 3.1, 0.9, 2.3, 1.1, 5.9], dtype=torch.float64).log().float()
+    nk = len(mass)
+    q = torch.zeros(1, heads, n, d)
+    k = torch.ones(1, heads, nk, d)
+    v = torch.tensor([1.0, -1.0, 0.5, 2.0, -0.25, 0.75, 0.125])[:, None].expand(1, heads, nk, d).contiguous()
+    grad = torch.zeros(1, heads, n, d)
+    grad[..., 0] = 1.0
+    slopes = torch.zeros(heads, device=device, requires_grad=True)
+    on = lambda t: t.to(device, dtype)
+    out = vgo.masked_attention(on(q), on(k), on(v), mass.to(device), slopes=slopes)
+    (got,) = torch.autograd.grad(out, slopes, on(grad))
+
+    p = torch.softmax(mass.double(), 0)
+    r = (torch.arange(nk) - (nk - n + torch.arange(n))[:, None]).abs().double()
+    value = v[0, 0, :, 0].double()
+    expected = -(r * (p * (value - p @ value))).sum()
+    terms = (r * (p * (value.abs() + p @ value.abs()))).sum()
+    bound = (2 * (torch.finfo(dtype).eps / 2) ** 2 + 2.0 ** -18) * terms
+    assert (got.double().cpu() - expected).abs().max() <= bound
