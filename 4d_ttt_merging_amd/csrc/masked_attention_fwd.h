@@ -128,7 +128,7 @@ constexpr float kSlack = 8.0f;
 // slopes' weigh what it is off by with the distances, and from rounded probabilities they were off by 0.2 to
 // 0.5% in bf16.  A second product takes what the rounding left out (1e-5).
 template <typename T, int D, bool kCap, int kBias, int kTrain>
-__global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forward_kernel(
+__global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T) > 128 ? 2 : 3) void forward_kernel(
     const Forward<T> f) {
   typedef Tile<T, D> TL;
   typedef Layout<T, D> LO;
@@ -339,20 +339,19 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : 2) void forw
     }
     lsum += sum, lsum32 += sum32;
 #pragma unroll
-    for (int kc = 0; kc < 4; ++kc)
+    for (int kc = 0; kc < 4; ++kc) {
+      op8 left;
+      if constexpr (kTrain == 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          left[e] = from_f32<T>(x[kc / 2][8 * (kc % 2) + e] - to_f32(static_cast<T>(p[kc][e])));
+      }
 #pragma unroll
       for (int dt = 0; dt < TL::kCols; ++dt) {
         const op8 va = TL::cols_op(vt, dt, kc);
         o[dt] = Op<T>::mma(va, p[kc], o[dt]);
+        if constexpr (kTrain == 2) o[dt] = Op<T>::mma(va, left, o[dt]);
       }
-    if constexpr (kTrain == 2) {
-#pragma unroll
-      for (int r = 0; r < 32; ++r)
-        p[r / 8][r % 8] = from_f32<T>(x[r / 16][r % 16] - to_f32(static_cast<T>(p[r / 8][r % 8])));
-#pragma unroll
-      for (int kc = 0; kc < 4; ++kc)
-#pragma unroll
-        for (int dt = 0; dt < TL::kCols; ++dt) o[dt] = Op<T>::mma(TL::cols_op(vt, dt, kc), p[kc], o[dt]);
     }
   };
 
