@@ -459,8 +459,10 @@ struct RowLds {
 constexpr int kShear = 36, kDiagonal = 63 * kShear;  // words
 __host__ __device__ inline int sum_words(int reach) { return (2 * reach + 4) & ~3; }
 
+// kBias 3: with the table's gradient, whose registers and LDS leave two work-groups a CU (64 channels; three without:
+// 2 x 16 heads of 4,116 with slopes 277 us against 352, with a table 306 against 385).
 template <typename T, int D, bool kCap, int kBias>
-__global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_kernel(const Grad<T> f) {
+__global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBias < 3 ? 3 : 2) void row_kernel(const Grad<T> f) {
   typedef Tile<T, D> TL;
   typedef RowLds<T, D> LO;
   typedef typename Op<T>::op8 op8;
@@ -518,8 +520,8 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
   const int words = sum_words(a.buckets.reach);
   float* diagonal = distance + distance_words(a.buckets.reach) + wave * kDiagonal;
   float* sums = distance + distance_words(a.buckets.reach) + kRowWaves * kDiagonal + wave * words;
-  if (kBias == 2 && a.table) fill_distances(a, distance, head, 64 * kRowWaves);
-  if (kBias == 2 && f.part_table) {
+  if (kBias >= 2 && a.table) fill_distances(a, distance, head, 64 * kRowWaves);
+  if (kBias == 3) {
     for (int i = lane; i < words; i += 64) sums[i] = 0.0f;
     for (int i = lane; i < kDiagonal; i += 64) diagonal[i] = 0.0f;
   }
@@ -611,7 +613,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
           for (int r = 0; r < 16; ++r) x[r] *= c;
         }
       }
-      if constexpr (kBias == 2) {
+      if constexpr (kBias >= 2) {
         if (a.slopes) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -649,14 +651,14 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dz[r] *= x[r];
-      if constexpr (kBias == 2) {
+      if constexpr (kBias >= 2) {
         if (f.part_slopes) {
           float sum = 0.0f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) sum = fmaf(-fabsf(d0f + static_cast<float>(8 * (r / 4) + r % 4)), dz[r], sum);
           slope_sum.add(sum);
         }
-        if (f.part_table) {
+        if constexpr (kBias == 3) {
           if (behind || ahead) {
             float sum = 0.0f;
 #pragma unroll
@@ -744,7 +746,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
       }
   }
   const int64_t part = (static_cast<int64_t>(split) * a.batch + b) * f.row_blocks + block;
-  if (kBias != 2 || (!f.part_slopes && !f.part_table)) return;
+  if (kBias < 2 || (kBias == 2 && !f.part_slopes)) return;
   float slopes = slope_sum.sum, behind = far_behind.sum, ahead = far_ahead.sum;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
@@ -752,11 +754,11 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 ? 2 : 1) void row_ke
   }
   float* totals = reinterpret_cast<float*>(lds + LO::kSums);
   if (lane == 0) totals[wave] = slopes;
-  if (f.part_table && lane == 0) sums[0] = behind, sums[2 * a.buckets.reach] = ahead;
+  if (kBias == 3 && lane == 0) sums[0] = behind, sums[2 * a.buckets.reach] = ahead;
   __syncthreads();
   if (f.part_slopes && threadIdx.x == 0)
     f.part_slopes[part * a.heads + head] = ((totals[0] + totals[1]) + totals[2]) + totals[3];
-  if (!f.part_table) return;
+  if (kBias < 3) return;
   float* by = distance + distance_words(a.buckets.reach) + kRowWaves * kDiagonal;  // all waves', into the first one's
   for (int i = threadIdx.x; i < words; i += 64 * kRowWaves)
     by[i] = ((by[i] + by[words + i]) + by[2 * words + i]) + by[3 * words + i];
@@ -848,8 +850,14 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
   if ((f.dq || f.part_slopes || f.part_table) && plan.row_tasks > 0) {
     const size_t bytes = RowLds<T, D>::kDistances + distances +
                          (f.part_table ? static_cast<size_t>(kRowWaves) * (kDiagonal + sum_words(f.a.buckets.reach)) * 4 : 0);
-    const auto kernel = cap ? (bias == 0 ? row_kernel<T, D, true, 0> : bias == 1 ? row_kernel<T, D, true, 1> : row_kernel<T, D, true, 2>)
-                            : (bias == 0 ? row_kernel<T, D, false, 0> : bias == 1 ? row_kernel<T, D, false, 1> : row_kernel<T, D, false, 2>);
+    const auto of_bias = [&](auto capped) {
+      constexpr bool kCap = decltype(capped)::value;
+      return f.part_table ? row_kernel<T, D, kCap, 3>
+             : bias == 2  ? row_kernel<T, D, kCap, 2>
+             : bias == 1  ? row_kernel<T, D, kCap, 1>
+                          : row_kernel<T, D, kCap, 0>;
+    };
+    const auto kernel = cap ? of_bias(std::true_type{}) : of_bias(std::false_type{});
     status = allow_lds(kernel, bytes);
     if (status != VGO_OK) return status;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.row_tasks)), dim3(64 * kRowWaves), bytes,
