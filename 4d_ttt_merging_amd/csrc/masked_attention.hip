@@ -8,7 +8,8 @@ namespace vgo {
 namespace masked {
 namespace {
 
-// One wave per tile, the keys' tiles first.
+// The documents' range of every tile, ~ of its first where a row is of none.  One wave per tile, the keys' tiles
+// first; bound by the launch (4 us).
 __global__ __launch_bounds__(256) void doc_info_kernel(const int* key_docs, const int* query_docs, const int* lengths,
                                                        int n_key, int n_query, int batch, int key_tiles,
                                                        int query_tiles, int2* info) {

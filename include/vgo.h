@@ -600,18 +600,20 @@ typedef struct vgo_masked_attn {
 /*
  * The forward: out (of the inputs' type, strides as theirs) and, where not NULL, lse [batch, heads,
  * n_query] fp32: log2 of the row's sum of e^z, and (16-bit types) rest [batch, heads, n_query, head_dim]
- * contiguous: out's own rounding, out + rest being the result to twice the bits; both for vgo_masked_attn_grad.  Workspace (16-byte aligned, any contents):
- * document ranges of the key tiles and the partial states of work split over the keys; its size is
- * for the device that is current.
+ * contiguous: out's own rounding, out + rest being the result to twice the bits; both for vgo_masked_attn_grad.
+ * With lse and slopes, P V of the 16-bit types takes P to twice the bits as well, which the slopes' gradient needs.
+ * Workspace (16-byte aligned, any contents): document ranges of the key tiles and the partial states of
+ * work split over the keys; its size is for the device that is current.
  */
 int vgo_masked_attn_workspace(const vgo_masked_attn* problem, int dtype, size_t* bytes);
 int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, const int64_t out_stride[3], float* lse,
                         void* rest, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * Gradients of the forward for grad_out, from its out, lse and rest (out_rest; NULL: out alone).  dq / dk / dv have the inputs' type;
- * dk / dv sum over the heads that share them; d_log_mass [n_key], d_slopes [heads] and d_table
- * [n_buckets, heads] have their parameter's type.  Outputs that are NULL are not computed (dk and dv: both or neither).
+ * Gradients of the forward for grad_out, from its out, lse and rest (out_rest; NULL: out alone).  dq / dk / dv
+ * have the inputs' type; dk / dv sum over the heads that share them; d_log_mass [n_key], d_slopes [heads] and
+ * d_table [n_buckets, heads] have their parameter's type.  Outputs that are NULL are not computed (dk and dv:
+ * both or neither).
  * Sums are in a fixed order: the same inputs give the same bits.
  */
 typedef struct vgo_masked_attn_grads {
@@ -635,8 +637,9 @@ int vgo_masked_attn_grad(const vgo_masked_attn* problem, const vgo_masked_attn_g
 
 /*
  * Relative position bias by buckets, dense: out[h, i, j] = table[bucket(j - query_start - i), h] with
- * bucket() as above, table [n_buckets, heads] and out [heads, n_query, n_key] contiguous of `dtype`; and its gradient d_table[t, h] = the sum of grad[h, i, j] over the pairs of bucket t, added up
- * in fp32 in a fixed order.  No counterpart in the reference.
+ * bucket() as above, table [n_buckets, heads] and out [heads, n_query, n_key] contiguous of `dtype`; and its
+ * gradient d_table[t, h] = the sum of grad[h, i, j] over the pairs of bucket t, added up in fp32 in a fixed
+ * order.  No counterpart in the reference.
  */
 int vgo_position_bias(const void* table, int64_t n_buckets, int64_t heads, const int32_t* bucket_starts,
                       int32_t n_starts, int32_t bidirectional, int64_t query_start, int64_t n_query,

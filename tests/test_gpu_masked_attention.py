@@ -493,3 +493,81 @@ def test_slope_gradient_under_equal_rows(vgo, device, dtype, d):
     terms = (r * (p * (value.abs() + p @ value.abs()))).sum()
     bound = (2 * (torch.finfo(dtype).eps / 2) ** 2 + 2.0 ** -18) * terms
     assert (got.double().cpu() - expected).abs().max() <= bound
+
+
+def test_offsets_past_32_bits(vgo, device):
+    """Rows of keys and values 2**23 elements apart, the last of them past 2**32, in and out of training."""
+    n, apart = 600, 2 ** 23
+    g = torch.Generator().manual_seed(5)
+    q, k, v, grad = (torch.randn(1, 2, n, 64, generator=g).bfloat16().to(device) for _ in range(4))
+    far = torch.empty(n * apart, dtype=BF16, device=device)
+    held = [far.as_strided((1, 2, n, 64), (apart, 64, apart, 1), at) for at in (0, 1024)]
+    for to, of in zip(held, (k, v)):
+        to.copy_(of)
+    results = []
+    for operands in ((k, v), held):
+        leaves = [t.detach().requires_grad_() for t in (q, *operands)]
+        out = vgo.masked_attention(*leaves, causal=True)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, grad)])
+        with torch.no_grad():
+            results[-1].append(vgo.masked_attention(q[:, :, -1:], *operands))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_lengths_and_positions_out_of_range(vgo, device):
+    """Lengths, prefixes and positions past the keys, or negative, are what they are clamped to."""
+    most, least = 2 ** 31 - 1, -2 ** 31
+    q, k, v, _, _ = make(device, BF16, b=2, nq=70, nk=130)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)
+    run = lambda **rules: vgo.masked_attention(q, k, v, **rules)
+    assert torch.equal(run(key_lengths=i32(most, least)), run(key_lengths=i32(130, 0)))
+    assert torch.equal(run(causal=True, prefix_lengths=i32(most, least)), run(causal=True, prefix_lengths=i32(130, 0)))
+    assert torch.equal(run(causal=True, query_starts=i32(most, least)), run(causal=True, query_starts=i32(130, -70)))
+    table = torch.randn(32, 2, device=device)
+    far = run(bucket_table=table, slopes=torch.zeros(2, device=device), query_starts=i32(most, least))
+    assert torch.equal(far, run(bucket_table=table, slopes=torch.zeros(2, device=device), query_starts=i32(10 ** 6, -10 ** 6)))
+
+
+def test_two_streams_at_once(vgo, device):
+    """Calls in flight together, each split over the keys with partial states of its own."""
+    q, k, v, rules, grad = make(device, BF16, b=1, h=4, nq=500, nk=2000, causal=True, slopes=True)
+
+    def step(scale):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = vgo.masked_attention(*leaves, **{**rules, "scale": scale})
+        return [out.detach(), *torch.autograd.grad(out, leaves, grad)]
+
+    expect = [step(0.125), step(0.25)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step((0.125, 0.25)[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, expect[i]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_padded_batch_in_training(vgo, device, dtype):
+    """Sequences of 0, 1, 64 and 100 of 100 keys: each alone, and what lies behind its keys without gradient."""
+    lengths = [0, 1, 64, 100]
+    q, k, v, _, grad = make(device, dtype, b=4, nq=100, nk=100, seed=3)
+    k, v = k.clone(), v.clone()
+    for b, n in enumerate(lengths):
+        k[b, :, n:], v[b, :, n:] = math.nan, math.nan
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = vgo.masked_attention(*leaves, key_lengths=torch.tensor(lengths, dtype=torch.int32, device=device))
+    grads = torch.autograd.grad(out, leaves, grad)
+    assert not out[0].any() and not any(g[0].any() for g in grads)
+    for b, n in enumerate(lengths[1:], 1):
+        assert not grads[1][b, :, n:].any() and not grads[2][b, :, n:].any()
+        start = torch.tensor([0], dtype=torch.int32, device=device)
+        res, bound = oracle.attention(q[b:b + 1], k[b:b + 1, :, :n], v[b:b + 1, :, :n], grad=grad[b:b + 1], query_starts=start)
+        for name, got in zip(("out", "q", "k", "v"), (out.detach(), *grads)):
+            got = got[b:b + 1] if name in ("out", "q") else got[b:b + 1, :, :n]
+            within(got, res[name], bound[name], f"{name} of {n} keys")
