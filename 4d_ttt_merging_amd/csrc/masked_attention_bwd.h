@@ -127,7 +127,10 @@ __device__ __forceinline__ float rescore(const Args<T>& a, float (&x)[16], float
     float most = fabsf(x[0]);
 #pragma unroll
     for (int r = 1; r < 16; ++r) most = fmaxf(most, fabsf(x[r]));
-    if (__any(!(most <= a.cap_reach))) {
+    if (!__any(!(most <= a.cap_low))) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = cap_low(a, x[r]);
+    } else if (__any(!(most <= a.cap_reach))) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = cap_tanh<T>(x[r] * a.inv_cap);
     } else {

@@ -15,7 +15,7 @@
 // on the same SIMD, which together fill it (counters: 16 x 16,464 x 64, causal); 32 rows a wave, so that three waves
 // (64 channels) overlap, where 64 rows at two were as fast on long rows and slower on short ones (8,232 causal: 294
 // us, 240).  16 heads of 8,232 x 8,232: 390 to 411 us with 64 channels (0.7 PFLOP/s; a library product 1.2), 680
-// with 128 (0.82), 16,464 causal 640 to 690 (0.8 to 0.87), capped 900; fp32 2,058 x 2,058 194 us (89 of 140 TFLOP/s).
+// with 128 (0.82), 16,464 causal 640 to 690 (0.8 to 0.87), capped 830; fp32 2,058 x 2,058 194 us (89 of 140 TFLOP/s).
 // Single tokens: HBM, 32 of 32,928 keys with 4 key heads 156 us capped and ragged (0.88 of a copy's rate).
 #pragma once
 
@@ -245,13 +245,24 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
         s[sub] = Op<T>::mma(ka, q[t], s[sub]);
       }
     }
+    // Whether any score of the wave's tile is past the series' reach, and whether none is past the short one's.
+    bool exact = false, low = false;
+    if constexpr (kCap) {
+      float most = fabsf(s[0][0]);
+#pragma unroll
+      for (int r = 1; r < 32; ++r) most = fmaxf(most, fabsf(s[r / 16][r % 16]));
+      exact = __any(!(most <= a.cap_reach)), low = !__any(!(most <= a.cap_low));
+    }
     // x = the scores of sub-tile sub, before the factor c, -inf where a pair does not attend.
-    const auto scores = [&](int sub, bool in_full, float (&x)[16]) {
+    const auto scores = [&](int sub, float (&x)[16]) {
       const int j0 = 32 * sub + 4 * h;  // key of register r: k0 + j0 + 8 (r / 4) + r % 4
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = s[sub][r];
       if constexpr (kCap) {
-        if (in_full) {
+        if (low) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = cap_low(a, x[r]);
+        } else if (exact) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = cap_tanh<T>(x[r] * a.inv_cap);
         } else {
@@ -310,16 +321,9 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
       }
     };
     op8 p[4];  // probabilities as operands
-    bool exact = false;
-    if constexpr (kCap) {
-      float most = fabsf(s[0][0]);
-#pragma unroll
-      for (int r = 1; r < 32; ++r) most = fmaxf(most, fabsf(s[r / 16][r % 16]));
-      exact = __any(!(most <= a.cap_reach));
-    }
     float x[2][16];
-    scores(0, exact, x[0]);
-    scores(1, exact, x[1]);
+    scores(0, x[0]);
+    scores(1, x[1]);
     float top = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, x[0][r]), x[1][r]);

@@ -571,3 +571,12 @@ def test_padded_batch_in_training(vgo, device, dtype):
         for name, got in zip(("out", "q", "k", "v"), (out.detach(), *grads)):
             got = got[b:b + 1] if name in ("out", "q") else got[b:b + 1, :, :n]
             within(got, res[name], bound[name], f"{name} of {n} keys")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("reach", [0.05, 0.27, 0.29, 0.74, 0.76, 3.0])
+def test_scores_around_the_caps_series(vgo, device, dtype, reach):
+    """Caps that put the largest score on either side of where the tanh is taken another way."""
+    q, k, v, rules, grad = make(device, dtype, nq=70, nk=130, causal=True)
+    largest = (q.double() @ k.double().transpose(-1, -2) / 8).abs().max().item()
+    check(vgo, q, k, v, {**rules, "score_cap": largest / reach}, grad)
