@@ -16,7 +16,7 @@
 // (64 channels) overlap, where 64 rows at two were as fast on long rows and slower on short ones (8,232 causal: 294
 // us, 240).  16 heads of 8,232 x 8,232: 390 to 411 us with 64 channels (0.7 PFLOP/s; a library product 1.2), 680
 // with 128 (0.82), 16,464 causal 640 to 690 (0.8 to 0.87), capped 830; fp32 2,058 x 2,058 194 us (89 of 140 TFLOP/s).
-// Single tokens: HBM, 32 of 32,928 keys with 4 key heads 156 us capped and ragged (0.88 of a copy's rate).
+// Single tokens: HBM, 32 of 32,928 keys with 4 key heads 152 us capped and ragged (0.90 of a copy's rate).
 #pragma once
 
 #include <type_traits>
