@@ -12,7 +12,8 @@
 // has most of a row its rounding then cancels (sums of the unrounded ones are as fast, within 1%).
 //
 // Bound: the issue of matrix instructions and of the softmax's (exponential, FMA, conversion, maximum per score)
-// on the same SIMD, which together fill it (counters: 16 x 16,464 x 64, causal); 32 rows a wave, so that three waves
+// on the same SIMD (counters: 0.35 and 0.62 of the time at 16 x 8,232 x 64 causal, 0.43 and 0.42 with 128 channels,
+// 0.31 and 0.88 at 16 x 16,464 x 64 capped); 32 rows a wave, so that three waves
 // (64 channels) overlap, where 64 rows at two were as fast on long rows and slower on short ones (8,232 causal: 294
 // us, 240).  16 heads of 8,232 x 8,232: 390 to 411 us with 64 channels (0.7 PFLOP/s; a library product 1.2), 680
 // with 128 (0.82), 16,464 causal 640 to 690 (0.8 to 0.87), capped 830; fp32 2,058 x 2,058 194 us (89 of 140 TFLOP/s).
