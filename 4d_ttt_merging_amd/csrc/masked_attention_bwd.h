@@ -1,6 +1,6 @@
 // Gradients of the masked attention (rules and layouts: masked_attention.h).
 //
-//   P = exp2(x - lse2) with the forward's row sums;  D_i = dO_i . O_i;  dZ = P (dO V^T - D)
+//   P = exp2(x - lse) exp2(-lse's rest) with the forward's row sums;  D_i = dO_i . O_i;  dZ = P (dO V^T - D)
 //   dV = P^T dO;  dK = scale (dZ cap')^T Q;  dQ = scale (dZ cap') K;  cap' = 1 - tanh^2
 //   d log_mass_j = sum dZ;  d slope = -sum dZ |r|;  d table[t] = sum of dZ over the pairs of bucket t
 //
@@ -40,7 +40,7 @@ GradPlan grad_plan(const vgo_masked_attn* p, int dtype);
 
 // Workspace pieces in order; each a multiple of 16 bytes.
 struct GradPieces {
-  size_t delta, empty, kv, q, mass, slopes, table, bytes;
+  size_t delta, marks, kv, q, mass, slopes, table, bytes;
 };
 GradPieces grad_pieces(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan& plan);
 
@@ -62,9 +62,9 @@ struct Grad {
   Args<T> a;
   const T *o, *go, *rest;
   int64_t gos[3];
-  const float* lse;
+  const float *lse, *lse_rest;  // the two planes
   float* delta;          // [batch, heads, n_query], -D; 0 for rows that attend to nothing
-  unsigned char* empty;  // [batch, heads, query tiles]: a row of the tile attends to nothing
+  unsigned char* marks;  // [batch, heads, query tiles]: kEmpty and kRests of the tile's rows
   T *dq, *dk, *dv;       // dq null: not wanted; likewise dk and dv
   int64_t dqs[3], dks[3], dvs[3];
   float* part_kv;      // splits > 1: [splits, batch * kv_heads, n_key, 2 D]
@@ -76,7 +76,13 @@ struct Grad {
   int key_blocks, row_blocks, key_tasks, row_tasks;
 };
 
-// delta and empty (delta from the unrounded outputs where their rest is there: what it is off by is off in every
+// A tile's marks: a row attends to nothing; a row's lse left a rest past the rounding of a score of 64.  Such tiles are
+// done as partly masked ones are, whose probabilities take the rest as a factor; the others are spared it (a subtraction
+// in all of them, or the rests beside lse in LDS, was 1 to 3% of the keys' kernel).
+constexpr unsigned char kEmpty = 1, kRests = 2;
+constexpr float kRestReach = 0x1p-18f;
+
+// delta and marks (delta from the unrounded outputs where their rest is there: what it is off by is off in every
 // score of the row): a work-group per tile of one head, 16 bytes a lane, every load of a lane's rows in flight
 // together.
 template <typename T, int D>
@@ -91,16 +97,16 @@ __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
   const T* go = f.go + b * f.gos[0] + head * f.gos[1] + part * kEach;
   const int64_t row0 = static_cast<int64_t>(bh) * a.n_query;
   Part x[kTimes], y[kTimes], z[kTimes];
-  float lse[kTimes];
+  float lse[kTimes], rest[kTimes];
 #pragma unroll
   for (int t = 0; t < kTimes; ++t) {
     const int i = min(i0 + t * kStep, a.n_query - 1);
     x[t] = *reinterpret_cast<const Part*>(o + i * a.os[2]);
     y[t] = *reinterpret_cast<const Part*>(go + i * f.gos[2]);
     z[t] = f.rest ? *reinterpret_cast<const Part*>(f.rest + (row0 + i) * D + part * kEach) : Part{};
-    lse[t] = f.lse[row0 + i];
+    lse[t] = f.lse[row0 + i], rest[t] = f.lse_rest[row0 + i];
   }
-  bool none = false;
+  bool none = false, rests = false;
 #pragma unroll
   for (int t = 0; t < kTimes; ++t) {
     float sum = 0.0f;
@@ -111,10 +117,11 @@ __global__ __launch_bounds__(256) void delta_kernel(const Grad<T> f) {
     const int i = i0 + t * kStep;
     const bool empty = lse[t] == kInf;
     none = none || (empty && i < a.n_query);
+    rests = rests || fabsf(rest[t]) > kRestReach;
     if (part == 0 && i < a.n_query) f.delta[row0 + i] = empty ? 0.0f : -sum;
   }
-  const bool any = __syncthreads_or(none);
-  if (threadIdx.x == 0) f.empty[blockIdx.x] = any;
+  const bool any = __syncthreads_or(none), any_rests = __syncthreads_or(rests);
+  if (threadIdx.x == 0) f.marks[blockIdx.x] = (any ? kEmpty : 0) | (any_rests ? kRests : 0);
 }
 
 // Raw products of one 32 x 32 block to what the factor returned makes exponents of 2; with a cap, to
@@ -231,7 +238,9 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
         inside = t * kTile + kTile <= a.n_query;
         all_w = all_w && inside && rw.hi == rw.lo + 31;
         any_w = any_w && rw.lo < limit;
-        inside = inside && !f.empty[(static_cast<int64_t>(b) * a.heads + kvh * group + g) * f.query_tiles + t];
+        const int marks = f.marks[(static_cast<int64_t>(b) * a.heads + kvh * group + g) * f.query_tiles + t];
+        inside = inside && !(marks & kEmpty);
+        all_w = all_w && !(marks & kRests);
       }
       todo = __ballot(any), mine = __ballot(any && any_w), full = __ballot(all_w), whole = __ballot(inside);
     }
@@ -316,6 +325,13 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
         }
       }
       if (partial) {
+        const int64_t bh = static_cast<int64_t>(b) * a.heads + head;
+        if (f.marks[bh * f.query_tiles + q0 / kTile] & kRests) {
+          const float* rest = f.lse_rest + bh * a.n_query;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            x[r] *= __builtin_amdgcn_exp2f(-rest[min(q0 + i0 + 8 * (r / 4) + r % 4, a.n_query - 1)]);
+        }
         const int i_first = q0 + i0 - first_row;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -491,7 +507,8 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
   const int pos = start + row;
   const int doc = a.query_doc ? a.query_doc[static_cast<int64_t>(b) * a.n_query + rc] : 0;
   const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.n_query + rc;
-  const float lse = stored ? f.lse[at] : kInf;
+  const float lse = stored ? f.lse[at] : kInf, lse_rest = f.lse_rest[at], unrest = __builtin_amdgcn_exp2f(-lse_rest);
+  const bool rests = __any(fabsf(lse_rest) > kRestReach);
   const bool live = lse != kInf;
   const float delta = live ? f.delta[at] : 0.0f;
   const float slope = slope2(a, head);
@@ -647,7 +664,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
       if (partial) {
         const int last_r = last - k0 - j0;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = 8 * (r / 4) + r % 4 <= last_r ? x[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) x[r] = 8 * (r / 4) + r % 4 <= last_r ? x[r] * unrest : 0.0f;
         if (kdocs) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -721,7 +738,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
     if (kBias && a.mass && wave == 0) reinterpret_cast<float*>(lds + LO::kMass)[buf * kTile + lane] = next_mass;
     __syncthreads();
     if (LO::kBuffers == 2 && more) load(buf ^ 1);
-    if (run) compute(!all, k0, buf);
+    if (run) compute(!all || rests, k0, buf);
     if (LO::kBuffers == 1 && more) {
       __syncthreads();
       load(buf ^ 1);
@@ -813,13 +830,14 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
     f.dqs[i] = g->dq_stride[i], f.dks[i] = g->dk_stride[i], f.dvs[i] = g->dv_stride[i];
   }
   f.o = static_cast<const T*>(g->out), f.go = static_cast<const T*>(g->grad_out), f.lse = g->lse;
+  f.lse_rest = g->lse + p->batch * p->heads * p->n_query;
   f.rest = static_cast<const T*>(g->out_rest);
   f.dq = static_cast<T*>(g->dq), f.dk = static_cast<T*>(g->dk), f.dv = static_cast<T*>(g->dv);
   f.query_tiles = plan.query_tiles, f.key_tiles = plan.key_tiles, f.splits = plan.splits, f.row_splits = plan.row_splits;
   f.key_blocks = plan.key_blocks, f.row_blocks = plan.row_blocks;
   f.key_tasks = static_cast<int>(plan.key_tasks), f.row_tasks = static_cast<int>(plan.row_tasks);
   const auto piece = [&](size_t offset) { return reinterpret_cast<float*>(ws + offset); };
-  f.delta = piece(at.delta), f.empty = reinterpret_cast<unsigned char*>(ws + at.empty);
+  f.delta = piece(at.delta), f.marks = reinterpret_cast<unsigned char*>(ws + at.marks);
   if (plan.splits > 1 && f.dk) f.part_kv = piece(at.kv);
   if (plan.row_splits > 1 && f.dq) f.part_q = piece(at.q);
   if (g->d_log_mass) f.part_mass = piece(at.mass);

@@ -58,12 +58,21 @@ __device__ __forceinline__ f32x4 rounding(f32x4 x) {
   return x;
 }
 
+// log2 of a row's sum of e^z, l 2^m, as two numbers: beside a large m, the same for all of a row's scores, log2(l)
+// would be rounded away, and with it what makes the gradients' probabilities add up to one (fp32 keys that share a
+// mass of -1e6: off by a sixteenth).
+__device__ __forceinline__ void store_lse(float* lse, int64_t rows, int64_t at, float m, float l) {
+  const float log = __builtin_amdgcn_logf(l), sum = m + log;
+  lse[at] = l == 0.0f ? kInf : sum;
+  lse[rows + at] = l == 0.0f ? 0.0f : log - (sum - m);
+}
+
 // What a launch adds to the problem.
 template <typename T>
 struct Forward {
   Args<T> a;
   T* out;
-  float* lse;     // or null
+  float* lse;     // or null: two planes [batch, heads, n_query], what the sum of the first rounds and that rest
   T* rest;        // or null: what rounding took from out, [batch, heads, n_query, D]
   float* part_o;  // splits > 1: [splits, batch * virtual heads, rows, D] unnormalised sums
   float* part_ml; // and [.., rows, 3] their reference maxima (log2) and row sums (rounded, unrounded)
@@ -422,8 +431,8 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
       }
     }
   if (f.lse && h == 0)
-    f.lse[(static_cast<int64_t>(b) * a.heads + head) * a.n_query + index] =
-        l32 == 0.0f ? kInf : mref + __builtin_amdgcn_logf(l32);
+    store_lse(f.lse, static_cast<int64_t>(a.batch) * a.heads * a.n_query,
+              (static_cast<int64_t>(b) * a.heads + head) * a.n_query + index, mref, l32);
 }
 
 // Joins the splits' states of each row: D / 4 lanes a row, `f.joiners` of them that take every
@@ -476,8 +485,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Forward<T> f) {
   if (f.rest)
     store4(f.rest + ((static_cast<int64_t>(b) * a.heads + head) * a.n_query + i) * D + d, rounding<T>(y));
   if (f.lse && d == 0)
-    f.lse[(static_cast<int64_t>(b) * a.heads + head) * a.n_query + i] =
-        l32 == 0.0f ? kInf : m + __builtin_amdgcn_logf(l32);
+    store_lse(f.lse, static_cast<int64_t>(a.batch) * a.heads * a.n_query,
+              (static_cast<int64_t>(b) * a.heads + head) * a.n_query + i, m, l32);
 }
 
 template <typename T, int D, bool kCap, int kBias, int kTrain>

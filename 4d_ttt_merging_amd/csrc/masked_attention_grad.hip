@@ -35,7 +35,7 @@ GradPieces grad_pieces(const vgo_masked_attn* p, const vgo_masked_attn_grads* g,
   };
   const size_t rows = static_cast<size_t>(p->batch) * p->heads;
   r.delta = take(rows * p->n_query * 4);
-  r.empty = take(rows * plan.query_tiles);
+  r.marks = take(rows * plan.query_tiles);
   const size_t keys = static_cast<size_t>(plan.splits) * p->batch * p->kv_heads * p->n_key;
   r.kv = take(plan.splits > 1 && g->dk ? keys * 2 * p->head_dim * 4 : 0);
   r.q = take(plan.row_splits > 1 && g->dq ? plan.row_splits * rows * p->n_query * p->head_dim * 4 : 0);

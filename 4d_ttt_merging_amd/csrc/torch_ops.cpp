@@ -272,7 +272,7 @@ struct MaskedProblem {
   }
 };
 
-// [out, lse, rest]; what the gradients need of the forward -- lse (fp32 [batch, heads, n_query]) and, of
+// [out, lse, rest]; what the gradients need of the forward -- lse (fp32 [2, batch, heads, n_query]) and, of
 // 16-bit types, rest (out's own rounding, like out) -- is empty unless wanted.
 std::tuple<Tensor, Tensor, Tensor> masked_attention(
     const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& log_mass, const OptTensor& slopes,
@@ -283,7 +283,7 @@ std::tuple<Tensor, Tensor, Tensor> masked_attention(
                                   query_starts, scale, score_cap, bucket_starts.vec(), bidirectional, causal});
   const int dtype = dtype_code(q.scalar_type());
   const Tensor out = in_layout_of(q);
-  const Tensor lse = at::empty({want_lse ? q.size(0) : 0, q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  const Tensor lse = at::empty({want_lse ? 2 : 0, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   const bool want_rest = want_lse && dtype != VGO_F32;
   const Tensor rest = at::empty({want_rest ? q.size(0) : 0, q.size(1), q.size(2), q.size(3)}, q.options());
   size_t need = 0;
@@ -312,9 +312,9 @@ std::vector<Tensor> masked_attention_grad(
   TORCH_CHECK_VALUE(grad0.sizes() == q.sizes() && grad0.scalar_type() == q.scalar_type() &&
                         out0.sizes() == q.sizes() && out0.scalar_type() == q.scalar_type(),
                     "masked_attention_grad: out and its gradient must be like q");
-  TORCH_CHECK_VALUE(lse.dim() == 3 && lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat &&
-                        lse.is_contiguous(),
-                    "masked_attention_grad: lse must be contiguous float32 [batch, heads, n_query]");
+  TORCH_CHECK_VALUE(lse.dim() == 4 && lse.size(0) == 2 && lse.sizes().slice(1) == q.sizes().slice(0, 3) &&
+                        lse.scalar_type() == at::kFloat && lse.is_contiguous(),
+                    "masked_attention_grad: lse must be contiguous float32 [2, batch, heads, n_query]");
   TORCH_CHECK_VALUE(rest.numel() == 0 || (rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() &&
                                           rest.is_contiguous() && q.scalar_type() != at::kFloat),
                     "masked_attention_grad: rest must be empty or contiguous and like q");
@@ -1007,8 +1007,8 @@ std::tuple<Tensor, Tensor, Tensor> masked_attention_autograd(
     const Tensor out = MaskedAttentionFunction::apply(q, k, v, log_mass, slopes, table, prefix, query_documents,
                                                       key_documents, key_lengths, query_starts, scale, score_cap,
                                                       bucket_starts, bidirectional, causal);
-    const Tensor none = at::empty({0, q.size(1), q.size(2), q.size(3)}, q.options());
-    return {out, none.select(3, 0).to(at::kFloat), none};
+    return {out, at::empty({0, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)),
+            at::empty({0, q.size(1), q.size(2), q.size(3)}, q.options())};
   }
   static const auto op = typed_operator<decltype(masked_attention)>("vgo::masked_attention");
   const at::AutoDispatchBelowAutograd below;

@@ -103,7 +103,7 @@ _SCHEMAS = (
     "int removed) -> (Tensor, Tensor, Tensor)",
     "fastvggt_plan(Tensor best, Tensor target, Tensor sources, Tensor destinations, int total, "
     "int removed) -> Tensor[]",
-    # [out, lse, rest] of vgo_masked_attn_fwd; lse (fp32 [B, H, Nq]) and, of 16-bit types, rest are empty
+    # [out, lse, rest] of vgo_masked_attn_fwd; lse (fp32 [2, B, H, Nq]) and, of 16-bit types, rest are empty
     # unless wanted.
     "masked_attention(Tensor q, Tensor k, Tensor v, Tensor? log_mass, Tensor? slopes, Tensor? table, "
     "Tensor? prefix, Tensor? query_documents, Tensor? key_documents, Tensor? key_lengths, Tensor? query_starts, "
@@ -259,7 +259,7 @@ def _in_layout_of(t):
 def _(q, k, v, log_mass, slopes, table, prefix, query_documents, key_documents, key_lengths, query_starts, scale,
       score_cap, bucket_starts, bidirectional, causal, want_lse):
     b = q.shape[0] if want_lse else 0
-    return (_in_layout_of(q), q.new_empty((b, *q.shape[1:3]), dtype=torch.float32),
+    return (_in_layout_of(q), q.new_empty((2 if want_lse else 0, *q.shape[:3]), dtype=torch.float32),
             q.new_empty((0 if q.dtype == torch.float32 else b, *q.shape[1:])))
 
 

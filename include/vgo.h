@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define VGO_ABI_VERSION 1
+#define VGO_ABI_VERSION 2
 
 #define VGO_OK 0
 #define VGO_EINVAL (-1)       /* bad shape, stride, dtype, size or null pointer */
@@ -598,8 +598,8 @@ typedef struct vgo_masked_attn {
 } vgo_masked_attn;
 
 /*
- * The forward: out (of the inputs' type, strides as theirs) and, where not NULL, lse [batch, heads,
- * n_query] fp32: log2 of the row's sum of e^z, and (16-bit types) rest [batch, heads, n_query, head_dim]
+ * The forward: out (of the inputs' type, strides as theirs) and, where not NULL, lse [2, batch, heads,
+ * n_query] fp32: log2 of the row's sum of e^z, then what rounding took from that, and (16-bit types) rest [batch, heads, n_query, head_dim]
  * contiguous: out's own rounding, out + rest being the result to twice the bits; both for vgo_masked_attn_grad.
  * With lse and slopes, P V of the 16-bit types takes P to twice the bits as well, which the slopes' gradient needs.
  * Workspace (16-byte aligned, any contents): document ranges of the key tiles and the partial states of

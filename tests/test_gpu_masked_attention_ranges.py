@@ -1,0 +1,63 @@
+"""Masked attention at the ends of its ranges: masses that keep keys out, caps, positions, lengths and sizes."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import masked_attention as oracle
+from tests.test_gpu_masked_attention import BF16, F16, F32, check, make, within
+
+pytestmark = pytest.mark.gpu
+
+
+def equal_keys(q, k, v, grad, seen):
+    """(results, bounds) of attention whose keys' scores are all equal: the mean over the keys that a row sees
+    ([nq, nk]), one key head a head, scale 1 / sqrt(d).
+
+    P is 1 / n up to the exponential, the logarithm and a division of the hardware's, 2^-22 each: 2^-20 with what
+    they multiply.  Sums of n, d and the rows' terms lose half a step of fp32 a term; P, score gradients and results
+    of 16 bits half a step of the type each."""
+    u, u32 = torch.finfo(q.dtype).eps / 2, 2.0 ** -24
+    rounded = 0.0 if q.dtype == F32 else u
+    q, k, v, grad = (t.detach().double().cpu() for t in (q, k, v, grad))
+    d, nq, nk = q.shape[-1], q.shape[2], k.shape[2]
+    p = seen.double() / seen.sum(1, keepdim=True).clamp(min=1)
+    kappa = 2.0 ** -20 + (nk + nq + 2 * d) * u32
+    out = p @ v
+    dp, delta = grad @ v.transpose(-1, -2), (grad * out).sum(-1, keepdim=True)
+    dz = p * (dp - delta)
+    res = dict(out=out, q=dz @ k * d ** -0.5, k=dz.transpose(-1, -2) @ q * d ** -0.5, v=p.T @ grad,
+               log_key_mass=dz.sum((0, 1, 2)))
+    a = p @ v.abs()
+    e_out = (rounded + kappa) * a + u * out.abs()
+    size = grad.abs() @ v.abs().transpose(-1, -2) + (grad.abs() * a).sum(-1, keepdim=True)
+    # D comes from the output as rounded (and, in 16 bits, from what that took, so this is more than it loses).
+    e_dz = p * ((grad.abs() * e_out).sum(-1, keepdim=True) + kappa * size)
+    e_ds = e_dz + (rounded + kappa) * dz.abs()
+    bound = dict(out=e_out, q=e_ds @ k.abs() * d ** -0.5 + u * res["q"].abs(),
+                 k=e_ds.transpose(-1, -2) @ q.abs() * d ** -0.5 + u * res["k"].abs(),
+                 v=(rounded + kappa) * (p.T @ grad.abs()) + u * res["v"].abs(),
+                 log_key_mass=(e_dz + kappa * dz.abs()).sum((0, 1, 2)))
+    return res, bound
+
+
+def check_equal_keys(vgo, q, k, v, grad, mass, causal):
+    nq, nk = q.shape[2], k.shape[2]
+    seen = torch.arange(nk) <= nk - nq + torch.arange(nq)[:, None] if causal else torch.ones(nq, nk, dtype=torch.bool)
+    res, bound = equal_keys(q, k, v, grad, seen)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, mass)]
+    out = vgo.masked_attention(*leaves, causal=causal)
+    within(out.detach(), res["out"], bound["out"], "out")
+    for name, got in zip(("q", "k", "v", "log_key_mass"), torch.autograd.grad(out, leaves, grad)):
+        within(got, res[name], bound[name] + torch.finfo(got.dtype).eps / 2 * res[name].abs(), f"gradient of {name}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("offset", [-1e5, -1e6, -1e9, 1e7])
+@pytest.mark.parametrize("nq, nk, causal", [(70, 140, False), (300, 300, True), (5, 1000, False)])
+def test_gradients_under_a_common_mass(vgo, device, dtype, offset, nq, nk, causal):
+    """Every key's mass the same large number: the row's statistics hold the logarithm of its few terms beside it."""
+    q, k, v, _, grad = make(device, dtype, nq=nq, nk=nk)
+    check_equal_keys(vgo, torch.zeros_like(q), k, v, grad, torch.full((nk,), offset, device=device), causal)
