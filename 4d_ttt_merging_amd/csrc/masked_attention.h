@@ -250,12 +250,16 @@ struct Args {
   const int2 *query_info, *key_info;  // [batch, tiles]
 };
 
-// Element i of a parameter of any type, in units of log2.
+// Element i of a parameter of any type, in units of log2.  A type's lowest value, which masks use to keep keys out,
+// is a finite number, and a row of nothing else a softmax over them: what is finite stays so, here and where a mass and
+// a table add up.
+constexpr float kMostParameter = 0x1p126f;
 __device__ __forceinline__ float parameter2(const void* p, int type, int64_t i) {
   const float x = type == VGO_F32    ? static_cast<const float*>(p)[i]
                   : type == VGO_BF16 ? to_f32(static_cast<const bf16_t*>(p)[i])
                                      : to_f32(static_cast<const f16_t*>(p)[i]);
-  return x * kLog2e;
+  const float y = x * kLog2e;
+  return fabsf(x) < kInf ? fmaxf(-kMostParameter, fminf(y, kMostParameter)) : y;
 }
 template <typename T>
 __device__ __forceinline__ float mass2(const Args<T>& a, int key) { return parameter2(a.mass, a.mass_type, key); }

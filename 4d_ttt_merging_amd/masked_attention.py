@@ -76,7 +76,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
       scale         default 1 / sqrt(D); positive
       score_cap     cap * tanh(score / cap); None or 0: none
       log_key_mass  floating [Nk], added to every score of that key (taken in fp32, not rounded to q's type
-                    as `mass_bias_attention` does); -inf keeps a key out
+                    as `mass_bias_attention` does); -inf keeps a key out, while a type's lowest value is a
+                    number: where a row's keys have nothing else it is a mean over them
       slopes        floating [H]: less slopes[h] * distance
       bucket_table  floating [buckets, H]: plus its row for the bucket of the distance, as in
                     `relative_position_bias` (`bidirectional`, `max_distance`)

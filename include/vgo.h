@@ -568,7 +568,8 @@ int vgo_restore_residual_layer_norm(const float* x, int64_t x_row_stride, const 
  * (batch, head, token), multiples of 16 bytes, with a unit channel stride; pointers 16-byte aligned.
  * Types as in vgo_mass_bias_attn_fwd; log_mass, slopes and bucket_table each of its own such type.
  *   score_cap > 0: scores capped by a tanh (0: not).
- *   log_mass [n_key] (not rounded to the inputs' type), slopes [heads], bucket_table [n_buckets, heads].
+ *   log_mass [n_key] (not rounded to the inputs' type), slopes [heads], bucket_table [n_buckets, heads].  Finite values
+ *     of theirs beyond 5.89e37 in size count as that: a type's lowest value is a number, -inf alone keeps a key out.
  *   bucket(r) = the number of bucket_starts (host, ascending, > 0, at most 128, the last one at most
  *     1024) that are <= |r|, plus n_buckets / 2 for r > 0 if bidirectional; else of max(-r, 0).
  *   key_documents [batch, n_key] with query_documents [batch, n_query] (contiguous): both or neither.

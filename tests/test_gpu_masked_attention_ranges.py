@@ -61,3 +61,34 @@ def test_gradients_under_a_common_mass(vgo, device, dtype, offset, nq, nk, causa
     """Every key's mass the same large number: the row's statistics hold the logarithm of its few terms beside it."""
     q, k, v, _, grad = make(device, dtype, nq=nq, nk=nk)
     check_equal_keys(vgo, torch.zeros_like(q), k, v, grad, torch.full((nk,), offset, device=device), causal)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_whose_masses_are_all_the_lowest_value(vgo, device, dtype, kind, causal):
+    """torch.finfo(t).min is a number: where every key of a row has it, scores vanish beside it and the row is a mean."""
+    q, k, v, _, grad = make(device, dtype, nq=70, nk=140)
+    check_equal_keys(vgo, q, k, v, grad, torch.full((140,), torch.finfo(kind).min, dtype=kind, device=device), causal)
+
+
+def test_lowest_masses_before_others(vgo, device):
+    """Left padding by the lowest value under a causal mask: rows of the padding take its mean, the others none of it."""
+    q, k, v, _, grad = make(device, F32, nq=140, nk=140)
+    mass = torch.zeros(140, device=device)
+    mass[:75] = torch.finfo(F32).min
+    out = vgo.masked_attention(q, k, v, mass, causal=True)
+    seen = torch.arange(75) <= torch.arange(75)[:, None]
+    res, bound = equal_keys(q[:, :, :75], k[:, :, :75], v[:, :, :75], grad[:, :, :75], seen)
+    within(out[:, :, :75], res["out"], bound["out"], "out of the padding")
+    res, bound = oracle.attention(q[:, :, 75:], k[:, :, 75:], v[:, :, 75:], causal=True)
+    within(out[:, :, 75:], res["out"], bound["out"], "out behind the padding")
+
+
+def test_lowest_values_of_a_table_and_masses(vgo, device):
+    """A table whose every bucket is the type's lowest value, alone and beside such masses: means too."""
+    q, k, v, _, grad = make(device, BF16, nq=70, nk=140)
+    res, bound = equal_keys(q, k, v, grad, torch.ones(70, 140, dtype=torch.bool))
+    table = torch.full((32, 2), torch.finfo(F32).min, device=device)
+    for mass in (None, torch.full((140,), torch.finfo(BF16).min, dtype=BF16, device=device)):
+        within(vgo.masked_attention(q, k, v, mass, bucket_table=table), res["out"], bound["out"], "out")
