@@ -239,6 +239,7 @@ struct Args {
   float scale, inv_cap, cap2;     // scale; scale / cap and cap log2(e) (0: no cap)
   float cap_reach, cap_series[5]; // kCapReach and kCapSeries for products before the scale (reach 0: not used)
   float cap_low, cap_low_series[3];  // likewise kCapLow and kCapLowSeries
+  int cap_large;                  // past kCapShort: kTanhReach, kTanhLow and kTanhSeries in their places
   const void* mass;               // [n_key] or null
   const void* slopes;             // [heads] or null
   const void* table;              // [n_buckets, heads] or null
@@ -363,8 +364,12 @@ inline int sum_parts(const float* part, int64_t parts, int64_t n, void* out, int
 // tanh of the capped scores.  For 16-bit inputs, where |y| stays below kCapReach, an odd polynomial (weighted least
 // squares at Chebyshev points towards the least largest error: 2e-7), six full-rate instructions in
 // place of two quarter-rate ones and three more; past it, and for fp32, 1 - 2 / (1 + e^2y), whose
-// 1 costs a small y about 1e-7 -- 5e-6 in a score capped at 50, below the rounding of 16-bit
-// inputs -- so that fp32 takes the odd series below 0.3 (its next term is 1e-9).
+// 1 costs a small y about 1e-7, so that fp32 takes the odd series below 0.3 (its next term is 1e-9).
+// Both errors are multiplied by the cap: past a cap of kCapShort, where 2e-7 of it is 2e-5 of a score, 16-bit inputs
+// take the odd series too, as far as its error is fp32's rounding: 0.3, and 0.1 of its first three terms.
+constexpr float kCapShort = 100.0f;
+constexpr double kTanhSeries[5] = {1.0, -1.0 / 3.0, 2.0 / 15.0, -17.0 / 315.0, 62.0 / 2835.0};
+constexpr float kTanhReach = 0.3f, kTanhLow = 0.1f;
 constexpr float kCapReach = 0.75f;
 // tanh(y) / y in powers of y^2.
 constexpr float kCapSeries[5] = {0.999997228f, -0.333230765f, 0.132260916f, -0.0492804483f, 0.0123188331f};
@@ -398,6 +403,20 @@ __device__ __forceinline__ float cap_tanh(float y) {
     t = fabsf(y) < 0.3f ? fmaf(-y * y2, s, y) : t;
   }
   return t;
+}
+// tanh of 16 raw products, some past the series' reach; of a large cap, the others by the series all the same.
+template <typename T>
+__device__ __forceinline__ void cap_all(const Args<T>& a, float (&x)[16]) {
+  if (sizeof(T) == 2 && a.cap_large) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float near = cap_short(a, x[r]), far = cap_tanh<T>(x[r] * a.inv_cap);
+      x[r] = fabsf(x[r]) <= a.cap_reach ? near : far;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = cap_tanh<T>(x[r] * a.inv_cap);
+  }
 }
 
 // Row sums of probabilities as the products take them: of bf16 the rounded values, two per instruction,
@@ -434,16 +453,19 @@ Args<T> make_args(const vgo_masked_attn* p) {
   a.n_query = static_cast<int>(p->n_query), a.n_key = static_cast<int>(p->n_key);
   a.scale = p->scale;
   if (p->score_cap > 0.0f) {
-    a.inv_cap = p->scale / p->score_cap, a.cap2 = p->score_cap * kLog2e;
-    if (sizeof(T) == 2 && a.inv_cap > 1e-3f && a.inv_cap < 1e3f) {  // (its ninth power is a normal number)
-      a.cap_reach = kCapReach / a.inv_cap;
-      a.cap_low = kCapLow / a.inv_cap;
+    // Caps beyond these leave scores up to 1e11 as they are, or next to nothing of any; within them the factors and the
+    // series' squares are finite.
+    const float cap = std::max(1e-20f, std::min(p->score_cap, 1e15f));
+    a.inv_cap = p->scale / cap, a.cap2 = cap * kLog2e;
+    a.cap_large = cap > kCapShort;
+    if (sizeof(T) == 2 && a.inv_cap < 1e3f) {  // (below, ninth powers grow out of range)
+      a.cap_reach = (a.cap_large ? kTanhReach : kCapReach) / a.inv_cap;
+      a.cap_low = (a.cap_large ? kTanhLow : kCapLow) / a.inv_cap;
       double power = a.inv_cap;
-      for (int i = 0; i < 3; ++i, power *= static_cast<double>(a.inv_cap) * a.inv_cap)
-        a.cap_low_series[i] = static_cast<float>(kCapLowSeries[i] * power);
-      power = a.inv_cap;
-      for (int i = 0; i < 5; ++i, power *= static_cast<double>(a.inv_cap) * a.inv_cap)
-        a.cap_series[i] = static_cast<float>(kCapSeries[i] * power);
+      for (int i = 0; i < 5; ++i, power *= static_cast<double>(a.inv_cap) * a.inv_cap) {
+        a.cap_series[i] = static_cast<float>((a.cap_large ? kTanhSeries[i] : kCapSeries[i]) * power);
+        if (i < 3) a.cap_low_series[i] = static_cast<float>((a.cap_large ? kTanhSeries[i] : kCapLowSeries[i]) * power);
+      }
     }
   }
   a.mass = p->log_mass, a.slopes = p->slopes, a.table = p->bucket_table;

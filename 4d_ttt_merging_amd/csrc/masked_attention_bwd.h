@@ -138,8 +138,7 @@ __device__ __forceinline__ float rescore(const Args<T>& a, float (&x)[16], float
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = cap_low(a, x[r]);
     } else if (__any(!(most <= a.cap_reach))) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = cap_tanh<T>(x[r] * a.inv_cap);
+      cap_all(a, x);
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = cap_short(a, x[r]);

@@ -273,8 +273,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = cap_low(a, x[r]);
         } else if (exact) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = cap_tanh<T>(x[r] * a.inv_cap);
+          cap_all(a, x);
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) x[r] = cap_short(a, x[r]);

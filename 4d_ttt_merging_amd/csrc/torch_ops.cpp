@@ -25,7 +25,9 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
+#include <limits>
 #include <memory>
 #include <optional>
 #include <string>
@@ -257,7 +259,9 @@ struct MaskedProblem {
     p.batch = batch, p.heads = heads, p.kv_heads = k.size(1), p.n_query = n_query, p.n_key = n_key;
     p.head_dim = q.size(3);
     set_strides(p.q_stride, q), set_strides(p.k_stride, k), set_strides(p.v_stride, v);
-    p.scale = static_cast<float>(rules.scale), p.score_cap = static_cast<float>(rules.score_cap);
+    p.scale = static_cast<float>(rules.scale);
+    p.score_cap = static_cast<float>(rules.score_cap);
+    if (rules.score_cap > 0.0) p.score_cap = std::max(p.score_cap, std::numeric_limits<float>::min());  // (0: no cap)
     p.log_mass = ptr(log_mass), p.slopes = ptr(slopes), p.bucket_table = ptr(table);
     if (log_mass.defined()) p.log_mass_dtype = dtype_code(log_mass.scalar_type());
     if (slopes.defined()) p.slopes_dtype = dtype_code(slopes.scalar_type());

@@ -7,9 +7,35 @@ import pytest
 import torch
 
 from oracle import masked_attention as oracle
-from tests.test_gpu_masked_attention import BF16, F16, F32, check, make, within
+from tests.test_gpu_masked_attention import BF16, F16, F32, make, within
 
 pytestmark = pytest.mark.gpu
+
+
+def check(vgo, q, k, v, rules, grad=None):
+    """Against the oracle, within its bounds.  They count a half step relative to a value: score gradients are held
+    in the operands' type for dQ and dK, and those of f16 below 2^-14 are off by up to 2^-25 each, whatever their size."""
+    leaves = {}
+    if grad is not None:
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        leaves, rules = dict(q=q, k=k, v=v), dict(rules)
+        for n in ("log_key_mass", "slopes", "bucket_table"):
+            if rules.get(n) is not None:
+                rules[n] = leaves[n] = rules[n].detach().requires_grad_()
+    out = vgo.masked_attention(q, k, v, **rules)
+    res, bound = oracle.attention(q, k, v, grad=grad, **rules)
+    within(out.detach(), res["out"], bound["out"], "out")
+    if grad is None:
+        return
+    if q.dtype == F16:
+        b, h, nq, d = q.shape
+        step = 2.0 ** -25 * (rules.get("scale") or d ** -0.5)
+        q64, k64 = (t.detach().double().cpu().abs() for t in (q, k))
+        group = h // k.shape[1]
+        bound["q"] = bound["q"] + step * k64.sum(2, keepdim=True).repeat_interleave(group, 1)
+        bound["k"] = bound["k"] + step * q64.view(b, k.shape[1], group * nq, d).sum(2, keepdim=True)
+    for name, got in zip(leaves, torch.autograd.grad(out, list(leaves.values()), grad)):
+        within(got, res[name], bound[name], f"gradient of {name}")
 
 
 def equal_keys(q, k, v, grad, seen):
@@ -92,3 +118,28 @@ def test_lowest_values_of_a_table_and_masses(vgo, device):
     table = torch.full((32, 2), torch.finfo(F32).min, device=device)
     for mass in (None, torch.full((140,), torch.finfo(BF16).min, dtype=BF16, device=device)):
         within(vgo.masked_attention(q, k, v, mass, bucket_table=table), res["out"], bound["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap", [120.0, 200.0, 1e4, 1e6, 1e8, 1e20, 1e30, 3e38])
+def test_caps_far_above_the_scores(vgo, device, dtype, d, cap):
+    """A cap that no score comes near leaves the scores as they are."""
+    q, k, v, rules, grad = make(device, dtype, nq=70, nk=130, d=d, causal=True, gain=3.0)
+    check(vgo, q, k, v, {**rules, "score_cap": cap}, grad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("gain", [30.0, 300.0])
+def test_large_scores_under_large_caps(vgo, device, dtype, gain):
+    """Scores of hundreds, some past 0.3 of a cap of 1,000."""
+    q, k, v, rules, grad = make(device, dtype, nq=70, nk=130, gain=gain)
+    check(vgo, q, k, v, {**rules, "score_cap": 1000.0}, grad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("cap", [1e-3, 1e-10, 1e-30, 1e-44, 1e-60])
+def test_caps_far_below_the_scores(vgo, device, dtype, cap):
+    """Scores cut to next to nothing: all keys alike, and no gradient through a tanh that is flat."""
+    q, k, v, rules, grad = make(device, dtype, nq=70, nk=130)
+    check(vgo, q, k, v, {**rules, "score_cap": cap}, grad)
