@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <climits>
 #include <string>
+#include <type_traits>
 
 #include "vgo_common.h"
 
@@ -60,15 +61,23 @@ struct Op<float> {
   }
 };
 
-// Accumulator registers 8 c .. 8 c + 7 as an operand of T (bf16 / f16: rounded, as both products of
+// Accumulator registers 8 c .. 8 c + 7, times 2^raise, as an operand of T (bf16 / f16: rounded, as both products of
 // a 16-bit attention take their probabilities).
-template <typename T>
+template <typename T, int raise = 0>
 __device__ __forceinline__ typename Op<T>::op8 as_op(const float (&s)[16], int c) {
   typename Op<T>::op8 r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = from_f32<T>(s[8 * c + e]);
+  for (int e = 0; e < 8; ++e) r[e] = from_f32<T>(raise ? s[8 * c + e] * static_cast<float>(1 << raise) : s[8 * c + e]);
   return r;
 }
+
+// Powers of 2 by which f16 probabilities are held larger than they are, within f16's largest number, so that those
+// of improbable keys keep their bits: its normal numbers end at 2^-14, all of them at 2^-25.  In the forward by a lower
+// reference, which probabilities pass by 2^8; in the gradients, where 1 is the most, by a factor.
+template <typename T>
+constexpr int kLowerReference = std::is_same<T, f16_t>::value ? 7 : 0;
+template <typename T>
+constexpr int kRaise = std::is_same<T, f16_t>::value ? 14 : 0;
 
 // ------------------------------------------------------------- LDS tiles ----
 // kTile rows of D elements without padding; the 16-byte chunks of a row are permuted by XOR with a

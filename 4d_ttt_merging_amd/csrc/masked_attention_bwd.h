@@ -346,7 +346,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const op8 pb = as_op<T>(x, half);
+        const op8 pb = as_op<T, kRaise<T>>(x, half);
 #pragma unroll
         for (int dt = 0; dt < TL::kCols; ++dt) dv[dt] = Op<T>::mma(TL::cols_op(gt, dt, 2 * sub + half), pb, dv[dt]);
       }
@@ -416,6 +416,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       f.part_mass[(static_cast<int64_t>(split) * a.batch * a.kv_heads + bk) * a.n_key + key] = mass_sum;
   }
   if (!f.dk || key >= a.n_key) return;
+  constexpr float lower = 1.0f / (1 << kRaise<T>);
   if (f.splits > 1) {
     float* dst = f.part_kv + ((static_cast<int64_t>(split) * a.batch * a.kv_heads + bk) * a.n_key + key) * (2 * D);
 #pragma unroll
@@ -424,7 +425,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       for (int g = 0; g < 4; ++g) {
         f32x4 x, y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = dk[dt][4 * g + e] * a.scale, y[e] = dv[dt][4 * g + e];
+        for (int e = 0; e < 4; ++e) x[e] = dk[dt][4 * g + e] * a.scale, y[e] = dv[dt][4 * g + e] * lower;
         *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g + 4 * h) = x;
         *reinterpret_cast<f32x4*>(dst + D + 32 * dt + 8 * g + 4 * h) = y;
       }
@@ -438,7 +439,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
     for (int g = 0; g < 4; ++g) {
       f32x4 x, y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dk[dt][4 * g + e] * a.scale, y[e] = dv[dt][4 * g + e];
+      for (int e = 0; e < 4; ++e) x[e] = dk[dt][4 * g + e] * a.scale, y[e] = dv[dt][4 * g + e] * lower;
       store4(kd + 32 * dt + 8 * g + 4 * h, x);
       store4(vd + 32 * dt + 8 * g + 4 * h, y);
     }

@@ -137,8 +137,8 @@ struct Layout {
   static constexpr int kDistances = kRange + kWaves * 16;
 };
 
-// A row's reference moves when a logit passes it by more than this many powers of 2: probabilities
-// stay below 2^8, far from f16's largest number.
+// A row's reference moves when a logit passes it by more than this many powers of 2 (f16: and those by which it is
+// lower): probabilities stay below 2^8, 2^15 of f16.
 constexpr float kSlack = 8.0f;
 
 // kTrain: 1 where gradients follow, whose probabilities are those of the unrounded row sum; 2 with slopes, too.
@@ -337,8 +337,8 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, x[0][r]), x[1][r]);
     top = half_max(top) * c;
-    if (__any(top > mref + kSlack)) {
-      const float m = fmaxf(mref, top);
+    if (__any(top > mref + kSlack + kLowerReference<T>)) {
+      const float m = fmaxf(mref, top - kLowerReference<T>);
       const float alpha = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - m);
       mref = m;
       lsum *= alpha, lsum32 *= alpha;

@@ -33,7 +33,7 @@ def check(vgo, q, k, v, rules, grad=None):
         q64, k64 = (t.detach().double().cpu().abs() for t in (q, k))
         group = h // k.shape[1]
         bound["q"] = bound["q"] + step * k64.sum(2, keepdim=True).repeat_interleave(group, 1)
-        bound["k"] = bound["k"] + step * q64.view(b, k.shape[1], group * nq, d).sum(2, keepdim=True)
+        bound["k"] = bound["k"] + step * q64.reshape(b, k.shape[1], group * nq, d).sum(2, keepdim=True)
     for name, got in zip(leaves, torch.autograd.grad(out, list(leaves.values()), grad)):
         within(got, res[name], bound[name], f"gradient of {name}")
 
@@ -143,3 +143,45 @@ def test_caps_far_below_the_scores(vgo, device, dtype, cap):
     """Scores cut to next to nothing: all keys alike, and no gradient through a tanh that is flat."""
     q, k, v, rules, grad = make(device, dtype, nq=70, nk=130)
     check(vgo, q, k, v, {**rules, "score_cap": cap}, grad)
+
+
+@pytest.mark.parametrize("n", [70, 5000, 70000])
+def test_many_improbable_keys_in_half_precision(vgo, device, n):
+    """One key with all but 22.5 * 2^-24 of the weight for each of the others, and a value of 0: the output is the
+    others' alone, whose weights have all their bits where the largest leaves them above f16's smallest normal number."""
+    q, k, v, _, _ = make(device, F16, h=1, hk=1, nq=40, nk=n)
+    v = v + 2.0
+    v[:, :, 0] = 0.0
+    mass = torch.full((n,), math.log(22.5) - 24.0 * math.log(2.0), device=device)
+    mass[0] = 0.0
+    q = torch.zeros_like(q)
+    out = vgo.masked_attention(q, k, v, mass)
+    res, bound = oracle.attention(q, k, v, mass)
+    # (Scaled, so that small outputs count beside within()'s 1e-7; half a step of f16's subnormals is 2^-25.)
+    within(out.double() * 2.0 ** 20, res["out"] * 2.0 ** 20, (bound["out"] + 2.0 ** -25) * 2.0 ** 20, "out")
+
+
+@pytest.mark.parametrize("gain", [30.0, 300.0])
+def test_large_scores_in_half_precision(vgo, device, gain):
+    q, k, v, rules, grad = make(device, F16, nq=70, nk=130, gain=gain)
+    check(vgo, q, k, v, {**rules, "score_cap": 1000.0}, grad)
+    check(vgo, q, k, v, rules, grad)
+
+
+RULES_F16 = ["causal", "causal_more_queries", "prefix", "documents", "documents_mixed", "causal_documents", "lengths",
+             "lengths_causal", "cap", "cap_small_scores", "mass", "slopes", "buckets", "buckets_far", "buckets_behind",
+             "buckets_starts", "everything"]
+
+
+@pytest.mark.parametrize("rule", RULES_F16)
+def test_rules_and_gradients_in_half_precision(vgo, device, rule):
+    from tests.test_gpu_masked_attention import RULES
+    check(vgo, *make(device, F16, **RULES[rule]))
+
+
+@pytest.mark.parametrize("b, h, hk, nq, nk, d, rules", [
+    (3, 8, 2, 1, 3000, 64, dict(lengths=[3000, 1, 1777], starts=[2999, 0, 1776], cap=6.0)),
+    (1, 8, 8, 1, 4096, 128, dict(slopes=True)), (2, 16, 1, 4, 700, 64, dict(causal=True, buckets=32)),
+    (2, 4, 2, 1, 500, 64, dict(docs="mixed", mass=True)), (2, 4, 2, 7, 90, 64, dict(lengths=[0, 90]))])
+def test_few_queries_in_half_precision(vgo, device, b, h, hk, nq, nk, d, rules):
+    check(vgo, *make(device, F16, b=b, h=h, hk=hk, nq=nq, nk=nk, d=d, **rules))
