@@ -441,6 +441,18 @@ __device__ __forceinline__ float add_pair<bf16_t>(float sum, float, float, bf16_
   return __builtin_amdgcn_fdot2_f32_bf16(pair, one, sum, false);
 }
 
+constexpr size_t kLdsBytes = 163840;  // a CU's
+// Lets a kernel have `bytes` of dynamic LDS.
+template <typename K>
+int allow_lds(K kernel, size_t bytes, const char* what) {
+  if (bytes <= 65536) return VGO_OK;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == hipSuccess) return VGO_OK;
+  (void)hipGetLastError();  // (or the next launch would report it)
+  return fail(VGO_ELAUNCH, std::string(what) + ": " + hipGetErrorString(e));
+}
+
 inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
 // Document ranges of the tiles of both sides (tile_info above): key_info [batch, key tiles], query_info behind it.

@@ -61,7 +61,13 @@ ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
   ForwardPlan r{};
   const int group = static_cast<int>(p->heads / p->kv_heads);
   const int reach = p->bucket_table && p->n_starts ? p->bucket_starts[p->n_starts - 1] : 1;
-  const bool table_fits = !p->bucket_table || static_cast<int64_t>(group) * distance_words(reach) * 4 <= 32768;
+  // The heads' tables beside the tiles, in 32 KB (two work-groups a CU of the 16-bit kernels) and in what LDS there is:
+  // fp32 tiles of 128 channels leave 31,680 bytes.
+  const bool wide = p->head_dim == 128;
+  const size_t tile_bytes = dtype == VGO_F32 ? (wide ? Layout<float, 128>::kDistances : Layout<float, 64>::kDistances)
+                                             : (wide ? Layout<bf16_t, 128>::kDistances : Layout<bf16_t, 64>::kDistances);
+  const size_t tables = static_cast<size_t>(group) * distance_words(reach) * 4;
+  const bool table_fits = !p->bucket_table || tables <= std::min<size_t>(32768, kLdsBytes - tile_bytes);
   r.pack = p->n_query < 32 && table_fits ? group : 1;
   r.rows = static_cast<int>(r.pack * p->n_query);
   r.tiles = static_cast<int>(tiles_of(p->n_key));
@@ -77,7 +83,6 @@ ForwardPlan forward_plan(const vgo_masked_attn* p, int dtype) {
     const int64_t want = std::max((2 * cus + n - 1) / n, std::min((8 * cus + n - 1) / n, tiles / 4));
     r.splits = static_cast<int>(std::min<int64_t>({tiles, want, static_cast<int64_t>(std::ceil(std::sqrt(20.0 * tiles)))}));
   } else {
-    const bool wide = p->head_dim == 128;
     const double tile_us = dtype == VGO_F32 ? (wide ? 8.6 : 4.3) : wide ? 1.1 : 0.62;
     const double bytes = 8.0 * vheads * r.rows * p->head_dim;
     r.splits = splits_of(p, tasks, r.tiles, dtype == VGO_F32 ? 1 : wide ? 2 : 3, tile_us, bytes / 7e6);

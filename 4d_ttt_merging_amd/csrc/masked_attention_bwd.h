@@ -812,14 +812,6 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Grad<T> f) {
   store4(f.dq + bh / a.heads * f.dqs[0] + bh % a.heads * f.dqs[1] + i * f.dqs[2] + d, y);
 }
 
-template <typename K>
-int allow_lds(K kernel, size_t bytes) {
-  if (bytes <= 65536) return VGO_OK;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  return e == hipSuccess ? VGO_OK : fail(VGO_ELAUNCH, std::string("masked_attn_grad: ") + hipGetErrorString(e));
-}
-
 template <typename T, int D>
 int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan& plan, char* ws, hipStream_t stream) {
   Grad<T> f{};
@@ -859,7 +851,7 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
     const size_t bytes = KeyLds<T, D>::kDistances + distances;
     const auto kernel = cap ? (bias == 0 ? key_kernel<T, D, true, 0> : bias == 1 ? key_kernel<T, D, true, 1> : key_kernel<T, D, true, 2>)
                             : (bias == 0 ? key_kernel<T, D, false, 0> : bias == 1 ? key_kernel<T, D, false, 1> : key_kernel<T, D, false, 2>);
-    status = allow_lds(kernel, bytes);
+    status = allow_lds(kernel, bytes, "masked_attn_grad");
     if (status != VGO_OK) return status;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.key_tasks)), dim3(64 * KeyLds<T, D>::kWaves), bytes,
                        stream, f);
@@ -884,7 +876,7 @@ int run(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, const GradPlan
                           : row_kernel<T, D, kCap, 0>;
     };
     const auto kernel = cap ? of_bias(std::true_type{}) : of_bias(std::false_type{});
-    status = allow_lds(kernel, bytes);
+    status = allow_lds(kernel, bytes, "masked_attn_grad");
     if (status != VGO_OK) return status;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.row_tasks)), dim3(64 * kRowWaves), bytes,
                        stream, f);

@@ -493,11 +493,8 @@ int launch(const Forward<T>& f, hipStream_t stream) {
   typedef Layout<T, D> LO;
   const size_t bytes = LO::kDistances + (f.a.table ? static_cast<size_t>(f.pack) * distance_words(f.a.buckets.reach) * 4 : 0);
   const auto kernel = forward_kernel<T, D, kCap, kBias, kTrain>;
-  if (bytes > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (e != hipSuccess) return fail(VGO_ELAUNCH, std::string("masked_attn: ") + hipGetErrorString(e));
-  }
+  const int status = allow_lds(kernel, bytes, "masked_attn");
+  if (status != VGO_OK) return status;
   hipLaunchKernelGGL(kernel, dim3(f.tasks), dim3(64 * kWaves), bytes, stream, f);
   return check_launch("masked_attn");
 }

@@ -185,3 +185,12 @@ def test_rules_and_gradients_in_half_precision(vgo, device, rule):
     (2, 4, 2, 1, 500, 64, dict(docs="mixed", mass=True)), (2, 4, 2, 7, 90, 64, dict(lengths=[0, 90]))])
 def test_few_queries_in_half_precision(vgo, device, b, h, hk, nq, nk, d, rules):
     check(vgo, *make(device, F16, b=b, h=h, hk=hk, nq=nq, nk=nk, d=d, **rules))
+
+
+@pytest.mark.parametrize("h, hk, buckets, both, distance", [
+    (8, 1, 64, True, 500), (8, 1, 32, False, 512), (16, 1, 16, True, 500), (4, 1, 64, False, 1000), (16, 1, 32, True, 128),
+    (18, 1, 32, True, 128), (32, 1, 8, True, 40)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_few_queries_with_tables_that_fill_the_lds(vgo, device, dtype, h, hk, buckets, both, distance):
+    """128 channels, where the heads of a group, packed into a task, would bring more tables than beside the tiles fit."""
+    check(vgo, *make(device, dtype, h=h, hk=hk, nq=1, nk=300, d=128, buckets=buckets, both=both, distance=distance))
