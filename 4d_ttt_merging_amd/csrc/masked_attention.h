@@ -458,6 +458,11 @@ inline int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 // Document ranges of the tiles of both sides (tile_info above): key_info [batch, key tiles], query_info behind it.
 void launch_doc_info(const vgo_masked_attn* p, int2* info, hipStream_t stream);
 
+// Whether documents keep pairs apart: there are any to keep apart (arrays of no element may be null).
+inline bool has_documents(const vgo_masked_attn* p) {
+  return p->n_query > 0 && p->n_key > 0 && p->query_documents && p->key_documents;
+}
+
 // How many ways to split the `tiles` tiles of each of `tasks` work-groups (the rule stands at its definition).
 int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, int resident, double tile_us, double join_us);
 // VGO_OK, or the status of a problem the kernels do not take, with its message.
@@ -494,7 +499,7 @@ Args<T> make_args(const vgo_masked_attn* p) {
   if (a.table) a.buckets = make_buckets(p->n_buckets, p->bucket_starts, p->n_starts, p->bidirectional);
   a.causal = p->causal != 0, a.query_start = a.n_key - a.n_query;
   a.prefix = p->prefix_lengths, a.key_lengths = p->key_lengths, a.query_starts = p->query_starts;
-  a.query_doc = p->query_documents, a.key_doc = p->key_documents;
+  if (has_documents(p)) a.query_doc = p->query_documents, a.key_doc = p->key_documents;
   return a;
 }
 

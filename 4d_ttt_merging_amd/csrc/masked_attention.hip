@@ -40,7 +40,7 @@ int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, int resident, 
   // A causal mask leaves the tasks half of the tiles where all keys are the queries' own, documents fewer: where
   // more follow, their ends spread and the whole work counts; where all start at once, the longest does (2 x 16
   // heads of 2,058 x 2,058, causal and capped: dQ 91 us unsplit, 79 in two).
-  const bool all = !p->causal && !p->key_documents && !p->key_lengths;
+  const bool all = !p->causal && !has_documents(p) && !p->key_lengths;
   const double share =
       p->causal ? 1.0 - 0.5 * std::min<double>(p->n_query, p->n_key) / std::max<int64_t>(1, p->n_key) : 1.0;
   const double alone[4][3] = {{}, {0.0}, {0.0, 1.3}, {0.0, 1.5, 2.3}}, one = resident == 1 ? 1.0 : alone[resident][1];
@@ -110,7 +110,7 @@ void launch_doc_info(const vgo_masked_attn* p, int2* info, hipStream_t stream) {
 }
 
 size_t info_bytes(const vgo_masked_attn* p) {
-  return p->key_documents ? align16(static_cast<size_t>(p->batch) * (tiles_of(p->n_key) + tiles_of(p->n_query)) * 8)
+  return has_documents(p) ? align16(static_cast<size_t>(p->batch) * (tiles_of(p->n_key) + tiles_of(p->n_query)) * 8)
                           : 0;
 }
 
@@ -148,7 +148,8 @@ int check_problem(const vgo_masked_attn* p, int dtype) {
   VGO_REQUIRE(p->scale > 0.0f && p->scale < kInf, "masked_attn: the scale must be positive and finite");
   VGO_REQUIRE(p->score_cap >= 0.0f && p->score_cap < kInf, "masked_attn: the score cap must be finite and not negative");
   VGO_REQUIRE(!p->prefix_lengths || p->causal, "masked_attn: a prefix goes with a causal mask");
-  VGO_REQUIRE(!p->query_documents == !p->key_documents, "masked_attn: documents of queries and keys go together");
+  VGO_REQUIRE(p->batch == 0 || p->n_query == 0 || p->n_key == 0 || !p->query_documents == !p->key_documents,
+              "masked_attn: documents of queries and keys go together");
   const auto number = [](int type) { return type == VGO_F32 || type == VGO_BF16 || type == VGO_F16; };
   VGO_REQUIRE((!p->log_mass || number(p->log_mass_dtype)) && (!p->slopes || number(p->slopes_dtype)) &&
                   (!p->bucket_table || number(p->table_dtype)),

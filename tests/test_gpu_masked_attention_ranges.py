@@ -194,3 +194,14 @@ def test_few_queries_in_half_precision(vgo, device, b, h, hk, nq, nk, d, rules):
 def test_few_queries_with_tables_that_fill_the_lds(vgo, device, dtype, h, hk, buckets, both, distance):
     """128 channels, where the heads of a group, packed into a task, would bring more tables than beside the tiles fit."""
     check(vgo, *make(device, dtype, h=h, hk=hk, nq=1, nk=300, d=128, buckets=buckets, both=both, distance=distance))
+
+
+def test_documents_of_no_token(vgo, device):
+    """Document masks beside no queries, no keys or no batch."""
+    for b, nq, nk in ((0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 0)):
+        q, k, v, rules, grad = make(device, BF16, b=b, nq=nq, nk=nk, docs="mixed", mass=True, slopes=True, buckets=8, distance=9)
+        leaves = [t.requires_grad_() for t in (q, k, v, rules["log_key_mass"], rules["slopes"], rules["bucket_table"])]
+        out = vgo.masked_attention(q, k, v, **rules)
+        assert out.shape == q.shape and not out.any()
+        for leaf, got in zip(leaves, torch.autograd.grad(out, leaves, grad)):
+            assert got.shape == leaf.shape and not got.any()
