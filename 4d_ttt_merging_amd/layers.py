@@ -248,7 +248,10 @@ class SelfAttention(nn.Module):
                 and (not self.use_qk_norm or (self.q_norm.eps == self.k_norm.eps)))
 
     def compute_attention(self, qkv: Tensor, attn_bias=None, rope=None, token_plan=None) -> Tensor:
-        """`attn_bias`: keyword arguments of `masked_attention` (masks, score cap, position biases)."""
+        """`attn_bias`: keyword arguments of `masked_attention` (masks, score cap, position biases); not with a
+        token plan, whose merged attention has none of them."""
+        if attn_bias is not None and token_plan is not None:
+            raise ValueError("attn_bias does not go with a token plan")
         B, N, _ = qkv.shape
         C = self.qkv.in_features
         H = self.num_heads

@@ -23,3 +23,15 @@ def test_documents_of_an_empty_side_may_be_null(sizes, side):
     lib_mod = import_package("_lib")
     assert workspace(**{side: 16}, **sizes)[0] == lib_mod.VGO_OK
     assert workspace(**{side: 16})[0] == lib_mod.VGO_EINVAL
+
+
+def test_rules_beside_a_token_plan_are_refused():
+    """In attention itself as in the module's forward, which hands them on."""
+    import torch
+    attention = import_package("layers").SelfAttention(128, 2).eval()
+    qkv = torch.zeros(1, 5, 384)
+    for call in (lambda: attention.compute_attention(qkv, attn_bias=dict(causal=True), token_plan=object()),
+                 lambda: attention._forward_merged(torch.zeros(1, 5, 128), dict(causal=True), None, object()),
+                 lambda: attention(torch.zeros(1, 5, 128), attn_bias=dict(causal=True), token_plan=object())):
+        with pytest.raises(ValueError, match="token plan"):
+            call()
