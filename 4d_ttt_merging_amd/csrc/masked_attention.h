@@ -293,6 +293,13 @@ __device__ __forceinline__ int first_position(const Args<T>& a, int b) {
   constexpr int kMost = 1 << 29;  // keeps every distance in 32 bits
   return a.query_starts ? max(-kMost, min(kMost, a.query_starts[b])) : a.query_start;
 }
+// What the slopes take off the positions of a tile of queries (whose first is `first`): nothing, or, where the tile lies
+// beyond all keys, what brings its nearer end to theirs.  A softmax leaves out what that takes off every distance of a
+// row, and so does the slopes' gradient (a row's dZ add up to nothing); left on, the difference of two keys' scores was
+// lost in fp32 (a position of 1e6 and a slope of 0.5: 0.03).  By tiles, so that a tile's positions stay in a row.
+__device__ __forceinline__ int slope_shift(int first, int limit) {
+  return max(0, first - (limit - 1)) + min(0, first + kTile - 1);
+}
 template <typename T>
 __device__ __forceinline__ int prefix_of(const Args<T>& a, int b) {
   return a.prefix ? a.prefix[b] : 0;

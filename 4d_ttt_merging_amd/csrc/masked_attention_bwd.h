@@ -267,6 +267,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       lds_dma4(a.query_doc + static_cast<int64_t>(b) * a.n_query, i, lds0 + LO::kDocs + buf * kTile * 4);
   };
 
+  float slope = 0.0f;
   const auto compute = [&](bool partial, int q0, int head, int buf) {
     const char* qt = lds + 2 * buf * TL::kBytes;
     const char* gt = qt + TL::kBytes;
@@ -295,7 +296,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       }
       if constexpr (kBias == 2) {
         if (a.slopes) {
-          const float slope = slope2(a, head), d0 = static_cast<float>(key - p0 - i0);
+          const float d0 = static_cast<float>(key - p0 + slope_shift(p0, limit) - i0);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             x[r] = fmaf(-slope, fabsf(d0 - static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
@@ -325,7 +326,7 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
       }
       if (partial) {
         const int64_t bh = static_cast<int64_t>(b) * a.heads + head;
-        if (f.marks[bh * f.query_tiles + q0 / kTile] & kRests) {
+        if (__builtin_expect(f.marks[bh * f.query_tiles + q0 / kTile] & kRests, 0)) {
           const float* rest = f.lse_rest + bh * a.n_query;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -391,15 +392,19 @@ __global__ __launch_bounds__((64 * KeyLds<T, D>::kWaves), sizeof(T) == 4 ? 1 : D
   };
 
   bool more = next();
-  int buf = 0, table_head = -1;
+  int buf = 0, distance_head = -1;
   if (more) load(0);
   while (more) {
     const int q0 = unit_tile * kTile, head = unit_head;
     const bool run = in_mine, all = in_full;
-    if (kBias == 2 && a.table && head != table_head) {  // (the last reads of the head before ended at this barrier)
-      __syncthreads();
-      fill_distances(a, reinterpret_cast<float*>(lds + LO::kDistances), head, 64 * kWaves);
-      table_head = head;
+    if (kBias == 2 && head != distance_head) {
+      if (a.table) {
+        __syncthreads();  // (where the last reads of the head before end)
+        fill_distances(a, reinterpret_cast<float*>(lds + LO::kDistances), head, 64 * kWaves);
+      }
+      // Here, where no DMA but the one about to be waited for is in flight: a load's wait is a wait for all of them.
+      slope = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slope2(a, head))));
+      distance_head = head;
     }
     more = next();
     wait_vmem<0>();
@@ -512,6 +517,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
   const bool live = lse != kInf;
   const float delta = live ? f.delta[at] : 0.0f;
   const float slope = slope2(a, head);
+  const int shift = kBias >= 2 ? slope_shift(start + row - row % kTile, limit) : 0;
 
   const int last = min(limit, a.causal ? max(pos + 1, prefix) : INT_MAX) - 1;  // key that may attend
 
@@ -624,7 +630,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = s[r], dz[r] = dp[r];
       const float c = rescore<T, kCap>(a, x, bend);
-      const float d0f = static_cast<float>(k0 + j0 - pos);
+      const float d0f = static_cast<float>(k0 + j0 - pos + shift);
       if constexpr (kBias) {
         if (kBias == 1 || a.mass) {
 #pragma unroll

@@ -225,6 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
   const uint32_t lds0 = lds_offset(lds);
   Walk<T> walk(a, rg, rw, row0 < f.rows, b, split, f.splits, f.tiles);
   const int limit = walk.limit;
+  const int shift = kBias == 2 ? slope_shift(pos - index % kTile, limit) : 0;
   // Last of the keys that lengths and the causal mask leave the row.
   const int last = min(limit, a.causal ? max(pos + 1, walk.prefix) : INT_MAX) - 1;
 
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(64 * kWaves, D * sizeof(T) > 256 ? 1 : D * sizeof(T
       }
       if constexpr (kBias == 2) {
         if (a.slopes) {
-          const float d0 = static_cast<float>(k0 + j0 - pos);
+          const float d0 = static_cast<float>(k0 + j0 - pos + shift);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             x[r] = fmaf(-slope, fabsf(d0 + static_cast<float>(8 * (r / 4) + r % 4)), x[r]);

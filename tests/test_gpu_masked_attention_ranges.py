@@ -205,3 +205,33 @@ def test_documents_of_no_token(vgo, device):
         assert out.shape == q.shape and not out.any()
         for leaf, got in zip(leaves, torch.autograd.grad(out, leaves, grad)):
             assert got.shape == leaf.shape and not got.any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq", [1, 40, 100])
+@pytest.mark.parametrize("start, at", [(10 ** 6, 129), (-10 ** 6, 0), (2 ** 31 - 1, 129), (-2 ** 31, 0)])
+def test_slopes_at_positions_far_from_the_keys(vgo, device, dtype, nq, start, at):
+    """A position beyond the keys differs from that of the nearest one by what a softmax leaves out: all of its rows
+    attend as from there, and the slopes' gradient, whose score gradients add up to nothing in a row, is the same."""
+    q, k, v, rules, grad = make(device, dtype, nq=nq, nk=130, slopes=True)
+    i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=device)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, rules["slopes"])]
+    out = vgo.masked_attention(*leaves[:3], slopes=leaves[3], query_starts=i32(start))
+    grads = torch.autograd.grad(out, leaves, grad)
+    total, bounds = {}, {}
+    for i in range(nq):
+        res, bound = oracle.attention(q[:, :, i:i + 1], k, v, slopes=rules["slopes"], query_starts=i32(at),
+                                      grad=grad[:, :, i:i + 1])
+        within(out.detach()[:, :, i:i + 1], res["out"], bound["out"], f"out of row {i}")
+        within(grads[0][:, :, i:i + 1], res["q"], bound["q"], f"gradient of q, row {i}")
+        for n in ("k", "v", "slopes"):
+            total[n], bounds[n] = total.get(n, 0.0) + res[n], bounds.get(n, 0.0) + bound[n]
+    for n, got in zip(("k", "v", "slopes"), grads[1:]):
+        within(got, total[n], bounds[n] + torch.finfo(got.dtype).eps / 2 * total[n].abs(), f"gradient of {n}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("start", [-40, -3, 60, 128, 200])
+def test_slopes_of_rows_on_both_sides_of_the_keys_ends(vgo, device, dtype, d, start):
+    check(vgo, *make(device, dtype, b=2, nq=100, nk=130, d=d, slopes=True, starts=[start, 10], lengths=[130, 70]))
