@@ -181,6 +181,14 @@ __device__ __forceinline__ void stage(const T* base, int64_t row_stride, int row
   }
 }
 
+// Where lanes of a wave read, or add to, LDS words that other lanes of it wrote.  The hardware keeps a wave's LDS
+// operations in order; this keeps the compiler, which sees one lane's addresses, from moving them past each other.  No
+// instruction.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Buckets of distances: that of r is the number of starts <= |r|, plus half of them for r > 0
 // (bidirectional), or the number <= max(-r, 0).  Distances from `reach` on share one a side.
 struct Buckets {

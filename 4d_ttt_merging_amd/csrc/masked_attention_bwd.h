@@ -555,6 +555,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
   if (kBias == 3) {
     for (int i = lane; i < words; i += 64) sums[i] = 0.0f;
     for (int i = lane; i < kDiagonal; i += 64) diagonal[i] = 0.0f;
+    wave_lds_order();
   }
 
   f32x16 dq[TL::kCols];
@@ -701,6 +702,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
 #pragma unroll
             for (int r = 0; r < 16; ++r)
               diagonal[(8 * (r / 4) + 4 * h + r % 4 - l32 + 31) * kShear + l32] = dz[r];
+            wave_lds_order();
             const int d = lane - 31;
             float sum = 0.0f;
 #pragma unroll
@@ -717,6 +719,7 @@ __global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 4 ? 1 : D == 64 && kBi
               else
                 sums[r + reach] += sum;
             }
+            wave_lds_order();  // (the next block's diagonals, and their words of `sums`, are other lanes')
           }
         }
       }

@@ -92,6 +92,7 @@ __global__ __launch_bounds__(kThreads) void bias_grad_kernel(const BiasGradArgs<
   const int block = blockIdx.x % a.row_blocks, head = blockIdx.x / a.row_blocks;
   float* sums = lds + wave * words;  // by distance + reach; the two ends take everything beyond
   for (int i = lane; i < words; i += 64) sums[i] = 0.0f;
+  wave_lds_order();
   float behind = 0.0f, ahead = 0.0f;
   for (int k = 0; k < a.rows; ++k) {
     const int i = (block * a.rows + k) * kWaves + wave;
@@ -134,6 +135,7 @@ __global__ __launch_bounds__(kThreads) void bias_grad_kernel(const BiasGradArgs<
     }
     const int tail = lead + pieces * kN + lane;
     if (tail < a.n_key) single(tail);
+    wave_lds_order();  // (the next row's distances are other lanes')
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) behind += __shfl_xor(behind, off), ahead += __shfl_xor(ahead, off);

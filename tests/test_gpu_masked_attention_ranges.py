@@ -235,3 +235,41 @@ def test_slopes_at_positions_far_from_the_keys(vgo, device, dtype, nq, start, at
 @pytest.mark.parametrize("start", [-40, -3, 60, 128, 200])
 def test_slopes_of_rows_on_both_sides_of_the_keys_ends(vgo, device, dtype, d, start):
     check(vgo, *make(device, dtype, b=2, nq=100, nk=130, d=d, slopes=True, starts=[start, 10], lengths=[130, 70]))
+
+
+def uniform_parameters(heads=2, n=256, d=64):
+    """q = 0 and no other rule: P = 1 / 256, values of whole numbers whose mean is one, gradients of whole numbers, so that
+    every dZ is a whole multiple of 2^-8 and their sums are exact in fp32."""
+    g = torch.Generator().manual_seed(11)
+    q = torch.zeros(1, heads, n, d)
+    k = torch.randn(1, heads, n, d, generator=g)
+    v = torch.randint(-4, 5, (1, heads, n // 2, d), generator=g).float()
+    v = torch.cat([v, 2.0 - v], 2)[:, :, torch.randperm(n, generator=g)]  # a mean of 1
+    grad = torch.randint(-2, 3, (1, heads, n, d), generator=g).float()
+    return q, k, v, grad
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_parameter_gradients_that_are_exact(vgo, device, dtype):
+    """Gradients of masses, slopes and table where every term is exact but for P's exponential, the same in all rows:
+    2^-20 of the result, and 2^-22 of the terms for what fp32 sums may lose.  A term is 2^-22 of all terms and more, many
+    times that on average: one left out or counted twice shows."""
+    q, k, v, grad = uniform_parameters()
+    n, heads, buckets = 256, 2, 32
+    on = lambda t: t.to(device, dtype)
+    mass, slopes, table = (torch.zeros(*s, device=device, requires_grad=True) for s in ((n,), (heads,), (buckets, heads)))
+    dp = (grad.double() @ v.double().transpose(-1, -2))[0]
+    dz = (dp - grad.double()[0].sum(-1, keepdim=True)) / n
+    gap = torch.arange(n) - torch.arange(n)[:, None]
+    which = oracle.bucket(gap, buckets, 128, True)
+    expected = [dz.sum((0, 1)), -(dz * gap.abs()).sum((1, 2)),
+                torch.stack([(dz * (which == t)).sum((1, 2)) for t in range(buckets)])]
+    terms = {"masses": dz.abs().sum((0, 1)), "masses alone": dz.abs().sum((0, 1)), "slopes": (dz * gap).abs().sum((1, 2)),
+             "table": torch.stack([(dz * (which == t)).abs().sum((1, 2)) for t in range(buckets)])}
+    # Slopes and tables together, and masses alone: other kernels.
+    out = vgo.masked_attention(on(q), on(k), on(v), mass, slopes=slopes, bucket_table=table)
+    got = torch.autograd.grad(out, (mass, slopes, table), on(grad))
+    alone = torch.autograd.grad(vgo.masked_attention(on(q), on(k), on(v), mass), mass, on(grad))
+    for name, a, b in zip(("masses", "slopes", "table", "masses alone"), (*got, *alone), (*expected, expected[0])):
+        off = (a.double().cpu() - b).abs()
+        assert (off <= 2.0 ** -20 * b.abs() + 2.0 ** -22 * terms[name]).all(), (name, off.max().item())
