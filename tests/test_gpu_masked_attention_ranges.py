@@ -273,3 +273,73 @@ def test_parameter_gradients_that_are_exact(vgo, device, dtype):
     for name, a, b in zip(("masses", "slopes", "table", "masses alone"), (*got, *alone), (*expected, expected[0])):
         off = (a.double().cpu() - b).abs()
         assert (off <= 2.0 ** -20 * b.abs() + 2.0 ** -22 * terms[name]).all(), (name, off.max().item())
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rules", [{}, dict(docs="sorted", mass=True), dict(causal=True, prefix=[4500], cap=8.0)])
+def test_more_than_64_tiles_a_task(vgo, device, dtype, rules):
+    """2,048 single rows over 4,500 keys that they share by strides: a task to a row and 71 tiles a task, unsplit."""
+    q, k, v, more, _ = make(device, dtype, h=1, nq=1, nk=4500, hk=1, **rules)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(1, 2048, 1, 64, generator=g).to(device, dtype)
+    out = vgo.masked_attention(q, k.expand(-1, 2048, -1, -1), v.expand(-1, 2048, -1, -1), **more)
+    some = torch.arange(0, 2048, 37)
+    res, bound = oracle.attention(q[:, some], k.expand(-1, len(some), -1, -1), v.expand(-1, len(some), -1, -1), **more)
+    within(out[:, some], res["out"], bound["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("h, nq, nk, rules", [(2100, 1, 70, dict(slopes=False)), (300, 30, 100, dict(docs="mixed")),
+                                              (64, 130, 4300, dict(causal=True)), (16, 40, 9000, dict(mass=True))])
+def test_gradients_of_one_key_head(vgo, device, dtype, h, nq, nk, rules):
+    """Many heads on one key head, few of them or long keys: units and tiles past 64 a split, and splits past a few."""
+    check(vgo, *make(device, dtype, h=h, hk=1, nq=nq, nk=nk, **rules))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_large_equal_scores(vgo, device, dtype, causal):
+    """Scores of 2^15, all the same, without a bias; and masses of 1e6 under slopes and a table of zeros."""
+    q, k, v, _, grad = make(device, dtype, nq=150, nk=150)
+    seen = torch.arange(150) <= torch.arange(150)[:, None] if causal else torch.ones(150, 150, dtype=torch.bool)
+    same = [torch.full_like(t, 64.0).requires_grad_() for t in (q, k)]
+    v = v.detach().requires_grad_()
+    res, bound = equal_keys(*same, v, grad, seen)
+    out = vgo.masked_attention(*same, v, causal=causal)
+    within(out.detach(), res["out"], bound["out"], "out")
+    for name, got in zip(("q", "k", "v"), torch.autograd.grad(out, (*same, v), grad)):
+        within(got, res[name], bound[name], f"gradient of {name}")
+    zeros = lambda *shape: torch.zeros(*shape, device=device, requires_grad=True)
+    leaves = [torch.zeros_like(q).requires_grad_(), k.requires_grad_(), v, torch.full((150,), 1e6, device=device).requires_grad_()]
+    res, bound = equal_keys(*leaves[:3], grad, seen)
+    for more in (dict(slopes=zeros(2)), dict(slopes=zeros(2), bucket_table=zeros(32, 2))):
+        out = vgo.masked_attention(*leaves[:3], leaves[3], causal=causal, **more)
+        within(out.detach(), res["out"], bound["out"], "out")
+        grads = torch.autograd.grad(out, [*leaves, *more.values()], grad)
+        for name, got in zip(("q", "k", "v", "log_key_mass"), grads):
+            within(got, res[name], bound[name] + torch.finfo(got.dtype).eps / 2 * res[name].abs(), f"gradient of {name}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rules", [{}, dict(causal=True, mass=True), dict(docs="mixed", cap=5.0), dict(nq=3, nk=300)])
+def test_buckets_that_keep_pairs_apart(vgo, device, dtype, rules):
+    """Entries of -inf in the table: a mask by distance, which leaves some rows nothing, without gradient for them."""
+    q, k, v, more, grad = make(device, dtype, **{**dict(nq=150, nk=150, buckets=16, distance=60), **rules})
+    more["bucket_table"][8:] = -math.inf   # the keys ahead,
+    more["bucket_table"][0] = -math.inf    # the query's own
+    more["bucket_table"][3:6, 1] = -math.inf  # and, of one head, some behind
+    check(vgo, q, k, v, more, grad)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_masses_of_keys_that_nothing_reads(vgo, device, dtype):
+    """NaN and infinities in the masses of padded keys."""
+    q, k, v, rules, grad = make(device, dtype, b=2, nq=100, nk=150, lengths=[150, 120], mass=True, docs="mixed")
+    rules["key_lengths"] = rules["key_lengths"].clamp(max=120)
+    mass = rules.pop("log_key_mass")
+    results = []
+    for fill in (0.0, math.nan, math.inf):
+        leaf = torch.cat([mass[:120], torch.full_like(mass[120:], fill)]).requires_grad_()
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)] + [leaf]
+        out = vgo.masked_attention(*leaves, **rules)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, grad)])
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
