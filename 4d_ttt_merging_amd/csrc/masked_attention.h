@@ -480,6 +480,9 @@ inline bool has_documents(const vgo_masked_attn* p) {
 
 // How many ways to split the `tiles` tiles of each of `tasks` work-groups (the rule stands at its definition).
 int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, int resident, double tile_us, double join_us);
+// Whether a launch of so many work-groups is one: threads of a grid are counted in 32 bits.
+inline bool fits_grid(int64_t groups, int threads) { return groups < (int64_t{1} << 32) / threads; }
+
 // VGO_OK, or the status of a problem the kernels do not take, with its message.
 int check_problem(const vgo_masked_attn* p, int dtype);
 bool strides_fit(const int64_t stride[3], int64_t head_dim, int dtype);

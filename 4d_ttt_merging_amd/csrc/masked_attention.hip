@@ -154,7 +154,8 @@ int check_problem(const vgo_masked_attn* p, int dtype) {
   VGO_REQUIRE((!p->log_mass || number(p->log_mass_dtype)) && (!p->slopes || number(p->slopes_dtype)) &&
                   (!p->bucket_table || number(p->table_dtype)),
               "masked_attn: unsupported dtype of a parameter");
-  VGO_REQUIRE(p->batch * (tiles_of(p->n_key) + tiles_of(p->n_query)) < most, "masked_attn: too many rows");
+  VGO_REQUIRE(p->batch * (tiles_of(p->n_key) + tiles_of(p->n_query)) < (has_documents(p) ? most / 4 : most),
+              "masked_attn: too many rows");  // (documents: a wave a tile)
   if (p->bucket_table) {
     const int status = check_buckets(p->n_buckets, p->bucket_starts, p->n_starts, p->bidirectional);
     if (status != VGO_OK) return status;
@@ -178,7 +179,11 @@ extern "C" int vgo_masked_attn_workspace(const vgo_masked_attn* problem, int dty
   const int status = check_problem(problem, dtype);
   if (status != VGO_OK) return status;
   VGO_REQUIRE(bytes, "masked_attn: null pointer");
-  *bytes = problem->batch == 0 || problem->n_query == 0 ? 0 : forward_bytes(problem, forward_plan(problem, dtype));
+  *bytes = 0;
+  if (problem->batch == 0 || problem->n_query == 0) return VGO_OK;
+  const ForwardPlan plan = forward_plan(problem, dtype);
+  VGO_REQUIRE(fits_grid(plan.tasks, 256), "masked_attn: too many rows");
+  *bytes = forward_bytes(problem, plan);
   return VGO_OK;
 }
 
@@ -193,6 +198,7 @@ extern "C" int vgo_masked_attn_fwd(const vgo_masked_attn* problem, void* out, co
               "masked_attn: out must be 16-byte aligned, with strides of whole 16 bytes");
   VGO_REQUIRE(aligned(rest, 16) && (!rest || dtype != VGO_F32), "masked_attn: rest must be 16-byte aligned, and of a 16-bit type");
   const ForwardPlan plan = forward_plan(problem, dtype);
+  VGO_REQUIRE(fits_grid(plan.tasks, 256), "masked_attn: too many rows");
   const size_t need = forward_bytes(problem, plan);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(VGO_EWORKSPACE, "masked_attn: workspace of " + std::to_string(need) + " bytes needed");

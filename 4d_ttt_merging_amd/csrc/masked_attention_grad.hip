@@ -57,6 +57,10 @@ int check_grads(const vgo_masked_attn* p, const vgo_masked_attn_grads* g, int dt
   VGO_REQUIRE(!g->d_log_mass || p->log_mass, "masked_attn_grad: no log_mass to take the gradient of");
   VGO_REQUIRE(!g->d_slopes || p->slopes, "masked_attn_grad: no slopes to take the gradient of");
   VGO_REQUIRE(!g->d_table || p->bucket_table, "masked_attn_grad: no table to take the gradient of");
+  const GradPlan plan = grad_plan(p, dtype);
+  VGO_REQUIRE(fits_grid(p->batch * p->heads * plan.query_tiles, 256) && fits_grid(plan.key_tasks, 512) &&
+                  fits_grid(plan.row_tasks, 256),
+              "masked_attn_grad: too many rows");
   return VGO_OK;
 }
 

@@ -158,6 +158,7 @@ int check(int64_t n_buckets, int64_t heads, const int32_t* starts, int n_starts,
   VGO_REQUIRE(heads * (n_query / kWaves + 1) < (int64_t{1} << 31) &&
                   n_query * ((n_key + kSegment - 1) / kSegment) < (int64_t{1} << 31),
               "position_bias: too many rows");
+  VGO_REQUIRE(fits_grid(heads, kThreads), "position_bias: too many heads");
   return check_buckets(n_buckets, starts, n_starts, bidirectional);
 }
 
@@ -249,6 +250,7 @@ extern "C" int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64
   VGO_REQUIRE(aligned(grad, dtype == VGO_F32 ? 4 : 2) && aligned(d_table, dtype == VGO_F32 ? 4 : 2),
               "position_bias_grad: misaligned pointer");
   const int64_t blocks = n_key == 0 ? 0 : row_blocks_of(heads, n_query);
+  VGO_REQUIRE(fits_grid(blocks * heads, kThreads), "position_bias_grad: too many rows");
   const size_t need = static_cast<size_t>(blocks) * n_buckets * heads * 4;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 4)))
     return fail(VGO_EWORKSPACE, "position_bias_grad: workspace of " + std::to_string(need) + " bytes needed");

@@ -35,3 +35,22 @@ def test_rules_beside_a_token_plan_are_refused():
                  lambda: attention(torch.zeros(1, 5, 128), attn_bias=dict(causal=True), token_plan=object())):
         with pytest.raises(ValueError, match="token plan"):
             call()
+
+
+def test_more_work_groups_than_a_grid_has_threads_for():
+    """Refused on the host, not left to the launch: a grid's threads are counted in 32 bits."""
+    lib_mod = import_package("_lib")
+    lib = lib_mod.load()
+    sizes = dict(heads=16, kv_heads=16, n_query=1, n_key=1)
+    assert workspace(batch=1 << 20, **sizes)[0] == lib_mod.VGO_EINVAL
+    assert workspace(batch=(1 << 20) - 1, **sizes)[0] == lib_mod.VGO_OK
+    grads = lib_mod.MaskedAttnGrads(out=16, grad_out=16, lse=16, dq=16)
+    size = ctypes.c_size_t()
+    for batch, status in ((1 << 20, lib_mod.VGO_EINVAL), (1 << 18, lib_mod.VGO_OK)):
+        problem = _problem(lib_mod, batch=batch, **sizes)
+        assert lib.vgo_masked_attn_grad_workspace(ctypes.byref(problem), ctypes.byref(grads), 1, ctypes.byref(size)) == status
+    starts = (ctypes.c_int32 * 1)(1)
+    many = lambda n_query: lib.vgo_position_bias_grad(16, 4, 16, starts, 1, 1, 0, n_query, 1, 16, 1, None, 0, None)
+    assert many(1 << 25) == lib_mod.VGO_EINVAL and "too many rows" in lib_mod.last_error()
+    assert many(1 << 20) == lib_mod.VGO_EWORKSPACE
+    assert lib.vgo_position_bias(16, 4, 1 << 24, starts, 1, 1, 0, 1, 1, 16, 1, None) == lib_mod.VGO_EINVAL
