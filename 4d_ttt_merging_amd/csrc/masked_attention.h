@@ -398,7 +398,8 @@ constexpr float kCapReach = 0.75f;
 // tanh(y) / y in powers of y^2.
 constexpr float kCapSeries[5] = {0.999997228f, -0.333230765f, 0.132260916f, -0.0492804483f, 0.0123188331f};
 // Below kCapLow, where a cap well past the scores leaves nearly all, two terms less do for half of that error: the
-// capped forward is bound by its vector instructions (16 x 16,464 x 64 causal: 902 us with the longer series, 828).
+// capped forward is bound by its vector instructions (16 x 16,464 x 64 causal: 902 us with the longer series, 842 now;
+// 990 with the exponential's form, where scores come near the cap or pass it).
 constexpr float kCapLow = 0.28f;
 constexpr float kCapLowSeries[3] = {0.9999973373f, -0.3330590180f, 0.1262284013f};
 template <typename T>

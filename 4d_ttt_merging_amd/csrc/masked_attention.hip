@@ -35,7 +35,8 @@ __global__ __launch_bounds__(256) void doc_info_kernel(const int* key_docs, cons
 // it, of two one 1.3 times it, and what does not fill the last round costs as much as those few alone.
 // Joining takes a launch and the partial states' way out and back (`join_us` per split).  16 heads of
 // 8,232 x 8,232 x 64: 412 us unsplit (1,040 tasks, 4.06 a CU), 388 in three; 2,058 x 128: 74 and 82 (in two);
-// 2,058 x 64 in fp32: 286 and 187 (in six).
+// 2,058 x 64 in fp32: 286 and 187 (in six).  All measured without biases: masses, slopes and tables have no factor here,
+// and documents count as if the longest ran over all keys.
 int splits_of(const vgo_masked_attn* p, int64_t tasks, int tiles, int resident, double tile_us, double join_us) {
   // A causal mask leaves the tasks half of the tiles where all keys are the queries' own, documents fewer: where
   // more follow, their ends spread and the whole work counts; where all start at once, the longest does (2 x 16

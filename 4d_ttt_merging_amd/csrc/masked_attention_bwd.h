@@ -9,10 +9,11 @@
 // queries a wave and runs over the key tiles (dQ, d slope, d table).  Both recompute the scores: seven
 // products in place of five.
 //
-// Bound: as the forward, matrix and vector instructions of the same SIMDs.  16 heads of 8,232 x 8,232 in bf16: dQ 475
-// to 490 us (0.86 PFLOP/s of its three products), dK and dV 715 to 765 (0.75 of four) with 64 channels, 876 and 1,397
-// (0.95 and 0.79) with 128; fp32 2,058 x 2,058: 269 and 373 (96 and 93 of 140 TFLOP/s).  D comes in a pass of its own,
-// bound by HBM: 17 us for 16 x 8,232 x 128.
+// Bound: as the forward's, no pipe full (matrix and vector busy 0.52 and 0.66 of the time in dQ, 0.42 and 0.50 in dK and
+// dV with 64 channels, 0.54 and 0.40, 0.42 and 0.30 with 128).  16 heads of 8,232 x 8,232 in bf16: dQ 479 us (0.87
+// PFLOP/s of its three products), dK and dV 714 (0.78 of four) with 64 channels, 883 and 1,413 (0.94 and 0.79) with
+// 128; f16 504 and 781, whose dV takes P raised; fp32 2,058 x 2,058: 270 and 377 (96 and 92 of 140 TFLOP/s, matrix
+// pipes busy 0.76 and 0.72).  D comes in a pass of its own, bound by HBM: 17 us for 16 x 8,232 x 128.
 #pragma once
 
 #include "masked_attention.h"

@@ -11,13 +11,15 @@
 // sums and outputs are kept in fp32.  In bf16 the row sums take the rounded P, two per instruction: where one key
 // has most of a row its rounding then cancels (sums of the unrounded ones are as fast, within 1%).
 //
-// Bound: the issue of matrix instructions and of the softmax's (exponential, FMA, conversion, maximum per score)
-// on the same SIMD (counters: 0.35 and 0.62 of the time at 16 x 8,232 x 64 causal, 0.43 and 0.42 with 128 channels,
-// 0.31 and 0.88 at 16 x 16,464 x 64 capped); 32 rows a wave, so that three waves
-// (64 channels) overlap, where 64 rows at two were as fast on long rows and slower on short ones (8,232 causal: 294
-// us, 240).  16 heads of 8,232 x 8,232: 390 to 411 us with 64 channels (0.7 PFLOP/s; a library product 1.2), 680
-// with 128 (0.82), 16,464 causal 640 to 690 (0.8 to 0.87), capped 830; fp32 2,058 x 2,058 194 us (89 of 140 TFLOP/s).
-// Single tokens: HBM, 32 of 32,928 keys with 4 key heads 152 us capped and ragged (0.90 of a copy's rate).
+// Bound: with a cap the issue of vector instructions (busy 0.87 of the time at 16 x 16,464 x 64 causal, 0.90 where
+// scores come near the cap; the matrix pipes 0.30 and 0.23).  Else neither pipe is full (matrix and vector, which may be
+// busy at once: 0.36 and 0.63 at 16 x 8,232 x 64 causal, 0.43 and 0.42 with 128 channels): a work-group's waves are in
+// products, or in the softmax (exponential, FMA, conversion, maximum per score), together, between barriers a tile.
+// 32 rows a wave, so that three waves (64 channels) overlap, where 64 rows at two were as fast on long rows and slower
+// on short ones (8,232 causal: 294 us, 240).  16 heads of 8,232 x 8,232: 390 us with 64 channels (0.71 PFLOP/s; a
+// library product 1.2), 687 with 128 (0.81), 16,464 causal 660 (0.84), capped 842, and 990 where scores come near
+// the cap; fp32 2,058 x 2,058 191 us (91 of 140 TFLOP/s; matrix pipes busy 0.72, then the join).
+// Single tokens: HBM, 32 of 32,928 keys with 4 key heads 140 to 152 us capped and ragged (0.9 of a copy's rate).
 #pragma once
 
 #include <type_traits>

@@ -74,7 +74,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     Position of query i: query_starts[b] + i (int32 [B]; default Nk - Nq, the queries at the keys' end).
     Scores:
       scale         default 1 / sqrt(D); positive
-      score_cap     cap * tanh(score / cap); None or 0: none
+      score_cap     cap * tanh(score / cap); None or 0: none.  Of any size: past 1e15 it leaves scores as they are
       log_key_mass  floating [Nk], added to every score of that key (taken in fp32, not rounded to q's type
                     as `mass_bias_attention` does); -inf keeps a key out, while a type's lowest value is a
                     number: where a row's keys have nothing else it is a mean over them
@@ -91,7 +91,14 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_key_
     negative documents are never read and may hold anything; other keys and values must be finite
     wherever some query of their 64 attends to them.  Few queries (a decoding step: Nq below 32) take the
     heads of one key head together and split the keys over the chip.  Results and gradients are the
-    same bits every time."""
+    same bits every time.
+
+    Products take probabilities and score gradients rounded to the operands' type; sums are fp32.  A call that
+    records a graph divides by the sum of the unrounded probabilities (bf16), and with slopes multiplies what
+    rounding took from them too, so its output is not bit for bit that of the same call without one.  For its
+    backward it keeps q, k, v, the output, two fp32 numbers a row and, of 16-bit types, as much again as the
+    output (what rounding took from it).  Score gradients in f16 lose bits below 2^-14 and are gone below
+    2^-25: scale the loss."""
     try:
         _lib.load()
     except _lib.ExtensionUnavailable as error:
