@@ -16,6 +16,7 @@
 // No operator has a batching rule (see register_batched).
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -945,14 +946,17 @@ void autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::ji
     });
 }
 
-// A floating tensor that takes part in a recorded graph.  A tangent on one is refused: there is no
-// forward-mode derivative (tangents of tensors that require no grad end here, as at the path's operators).
+// Whether a floating tensor takes part in a recorded graph.  A tangent on any is refused: operators with gradients have
+// no forward-mode derivative, and dropping it, as the path's operators do, would be a derivative of zero.
 bool records(std::initializer_list<const Tensor*> tensors, const char* name) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool reverse = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   bool any = false, tangent = false;
   for (const Tensor* t : tensors)
-    if (t != nullptr && t->defined()) any |= t->requires_grad(), tangent |= t->_fw_grad(/*level=*/0).defined();
-  TORCH_CHECK_NOT_IMPLEMENTED(!any || !tangent, name, ": no forward-mode derivative");
+    if (t != nullptr && t->defined()) {
+      any |= reverse && t->requires_grad();
+      tangent |= forward && t->_fw_grad(/*level=*/0).defined();
+    }
+  TORCH_CHECK_NOT_IMPLEMENTED(!tangent, name, ": no forward-mode derivative");
   return any;
 }
 template <typename Signature>
