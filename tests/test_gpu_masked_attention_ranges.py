@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -343,3 +344,35 @@ def test_masses_of_keys_that_nothing_reads(vgo, device, dtype):
         results.append([out.detach(), *torch.autograd.grad(out, leaves, grad)])
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def drawn(seed):
+    """Keyword arguments of make() with rules, sizes and positions drawn together."""
+    r = random.Random(seed)
+    size = lambda most: int(round(math.exp(r.uniform(0.0, math.log(most)))))
+    hk, b = r.choice([1, 2, 3]), r.choice([1, 1, 2, 3])
+    nq = r.choice([1, 2, size(31), size(400)])
+    nk = r.choice([size(700), nq])
+    case = dict(b=b, h=hk * r.choice([1, 1, 2, 4, 5]), hk=hk, nq=nq, nk=nk, d=r.choice([64, 128]), seed=seed,
+                gain=r.choice([0.5, 1.0, 2.0, 6.0]), causal=r.random() < 0.5, mass=r.random() < 0.4, slopes=r.random() < 0.4,
+                cap=r.choice([None, None, 0.5, 3.0, 50.0, 300.0]), scale=r.choice([None, None, 0.05, 0.3]))
+    if case["causal"] and r.random() < 0.4:
+        case["prefix"] = [r.randint(-3, nk + 5) for _ in range(b)]
+    if r.random() < 0.4:
+        case["docs"] = "mixed" if nq > 2 * nk else r.choice(["mixed", "sorted"])
+    if r.random() < 0.4:
+        case["lengths"] = [r.choice([0, nk, r.randint(0, nk + 3)]) for _ in range(b)]
+    if r.random() < 0.4:
+        case["starts"] = [r.randint(-nq - 5, nk + 5) for _ in range(b)]
+    if r.random() < 0.4:
+        both = r.random() < 0.6
+        buckets = r.choice([8, 16, 32, 64] if both else [2, 7, 16, 33, 64])
+        alone = buckets // 2 // 2 if both else buckets // 2
+        case.update(buckets=buckets, both=both, distance=r.choice([alone + r.randint(1, 20), alone + 128, 300]))
+    return case
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("seed", range(40))
+def test_drawn_rules(vgo, device, dtype, seed):
+    check(vgo, *make(device, dtype, **drawn(seed)))
