@@ -6,7 +6,7 @@ choice of codes; rounded once at the end), or the package's entry points `cache_
 `cached_attention`.  Heads, widths and lengths are those of the aggregator (16 heads of 64 channels, 1,029 tokens
 per frame of 512 x 512, 261 of a small one, 4 to 32 frames), with grouped key heads and 128 channels beside them.
 
-The cache: uint8 [pages, key heads, page_size / 32 * 34 * dim], blocks of 32 tokens, each
+The cache: uint8 [pages, key heads, page_size / 32, 34 * dim], blocks of 32 tokens, each
     keys' codes   [32 tokens][dim / 2]           byte c: channel 2c in its low half, 2c + 1 in its high half
     values' codes [4][dim / 2][8 tokens]         tokens 8g .. 8g + 7 of a channel pair side by side
     keys' scales  [32 tokens][dim / 32]          2^(byte - 127), one for 32 channels of a token; 255: NaN
@@ -164,7 +164,7 @@ def prepare(case: dict, seed: int):
     packed = randn(b, nq, h + 2 * hk, d, scale=c["gain"]).to(dtype).transpose(1, 2)
     state["q"], k, v = packed.split([h, hk, hk], 1)
     if c["kind"] == "append":
-        state.update(k=k, v=v, data=torch.zeros(pages, hk, page // 32 * 34 * d, dtype=torch.uint8, device="cuda"))
+        state.update(k=k, v=v, data=torch.zeros(pages, hk, page // 32, 34 * d, dtype=torch.uint8, device="cuda"))
         if c["table"]:
             angle = torch.outer(torch.arange(c["table"], device="cuda", dtype=torch.float64),
                                 100.0 ** (-torch.arange(d // 2, device="cuda", dtype=torch.float64) / (d // 2)))
@@ -179,7 +179,7 @@ def prepare(case: dict, seed: int):
     # A cache in use: every page filled by tokens of unit size.
     blocks = page // 32
     codes = [_quantised(randn(pages, hk, blocks, 32, d)) for _ in range(2)]
-    state["data"] = _packed(*codes[0], *codes[1]).flatten(2).contiguous()
+    state["data"] = _packed(*codes[0], *codes[1]).contiguous()
     if c["mass"]:
         state["page_mass"] = randint(1, 9, (pages, page)).float().log()
     return state
@@ -216,8 +216,8 @@ def _plain_append(s) -> dict:
     where = s["page_table"][seq, at // page].long()
     slot, base = at % 32, at % page // 32 * 34 * d
     flat = s["data"].view(-1)
-    heads = torch.arange(hk, device="cuda") * s["data"].shape[2]
-    row = (where * hk * s["data"].shape[2] + base)[:, None, None] + heads[:, None]
+    size = page // 32 * 34 * d  # of a page of one head
+    row = (where * hk * size + base)[:, None, None] + torch.arange(hk, device="cuda")[:, None] * size
     pair = lambda c: (c[..., 0::2] | c[..., 1::2] << 4).transpose(1, 2)[seq, token]
     byte, part = torch.arange(d // 2, device="cuda"), torch.arange(d // 32, device="cuda")
     slot = slot[:, None, None]
@@ -235,8 +235,7 @@ def _plain_append(s) -> dict:
 def _plain_attend(s) -> torch.Tensor:
     b, h, hk, d, nq, page = (s[n] for n in ("batch", "heads", "kv_heads", "dim", "nq", "page"))
     # Every sequence's pages in a row, [b, hk, tokens, d].
-    held = s["data"][s["page_table"].clamp(min=0)]
-    held = held.transpose(1, 2).unflatten(-1, (-1, 34 * d))  # [b, hk, pages, blocks, bytes]
+    held = s["data"][s["page_table"].clamp(min=0)].transpose(1, 2)  # [b, hk, pages, blocks, bytes]
     kc, ks, vc, vs = _unpacked(held, d)
     k, v = (_numbers(*t).flatten(2, 4) for t in ((kc, ks), (vc, vs)))
     n = k.shape[2]
