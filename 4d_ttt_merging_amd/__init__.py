@@ -19,6 +19,8 @@ reference package `vggt_omega` for the merged global-attention path:
 * `masked_attention`, `relative_position_bias` -- attention under score caps, position
   biases and document, prefix and length masks, with gradients, and the learned bias by
   buckets as a dense tensor (no counterpart in the reference)
+* `PagedCache`, `cache_append`, `cache_read`, `cached_attention` -- a cache of keys and values in 4 bits, in
+  pages: appending with the rotation, reading back, attention over it (no counterpart in the reference)
 * `ops` -- the torch.library operators `torch.ops.vgo.*` (mass_bias_attention,
   top4_project, compaction, QKV epilogue, residual rows) with fake
   implementations for tracing
@@ -32,6 +34,7 @@ from . import _lib, ops, plan_io
 from .gemm_tuning import use_tuned_gemms
 from .layers import LinearKMaskedBias, SelfAttention, SelfAttentionBlock
 from .masked_attention import masked_attention, relative_position_bias
+from .paged_cache import PagedCache, cache_append, cache_read, cached_attention
 from .mass_bias_attention import dense_attention, mass_bias_attention
 from .projection import top4_project
 from .sparse_convex import build_sparse_convex_plan, convex_fit, start_sparse_convex_plan
@@ -45,12 +48,16 @@ from .token_merging import (
 
 __all__ = [
     "LinearKMaskedBias",
+    "PagedCache",
     "SelfAttention",
     "SelfAttentionBlock",
     "TokenPlan",
     "WeightedBilinearTokenPlan",
     "build_fastvggt_plan",
     "build_sparse_convex_plan",
+    "cache_append",
+    "cache_read",
+    "cached_attention",
     "convex_fit",
     "dense_attention",
     "deterministic_weighted_normalizer",

@@ -73,6 +73,26 @@ class MaskedAttnGrads(ctypes.Structure):
     ]
 
 
+class PagedCacheStruct(ctypes.Structure):
+    """`vgo_paged_cache` of include/vgo.h."""
+
+    _fields_ = [
+        ("data", _c_p), ("log_mass", _c_p), ("page_table", _c_p), ("pages", _c_i64), ("page_size", _c_i64),
+        ("kv_heads", _c_i64), ("head_dim", _c_i64), ("batch", _c_i64), ("table_width", _c_i64),
+    ]
+
+
+class CacheTokens(ctypes.Structure):
+    """`vgo_cache_tokens` of include/vgo.h."""
+
+    _fields_ = [
+        ("k", _c_p), ("v", _c_p), ("q", _c_p), ("q_out", _c_p), ("heads", _c_i64), ("n_tokens", _c_i64),
+        ("k_stride", _i64x3), ("v_stride", _i64x3), ("q_stride", _i64x3), ("q_out_stride", _i64x3),
+        ("starts", _c_p), ("counts", _c_p), ("rope_sin", _c_p), ("rope_cos", _c_p), ("rope_rows", _c_i64),
+        ("positions", _c_p), ("log_mass", _c_p),
+    ]
+
+
 _starts = [ctypes.POINTER(ctypes.c_int32), ctypes.c_int32, ctypes.c_int32]  # starts, how many, bidirectional
 
 # name -> (restype, argtypes); every symbol declared in include/vgo.h.
@@ -199,6 +219,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vgo_position_bias_grad_workspace": (_c_int, [_c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_size)]),
     "vgo_position_bias_grad": (_c_int, [
         _c_p, _c_i64, _c_i64, *_starts, _c_i64, _c_i64, _c_i64, _c_p, _c_int, _c_p, _c_size, _c_p,
+    ]),
+    "vgo_cache_append": (_c_int, [ctypes.POINTER(PagedCacheStruct), ctypes.POINTER(CacheTokens), _c_int, _c_p]),
+    "vgo_cache_read": (_c_int, [
+        ctypes.POINTER(PagedCacheStruct), _c_p, _c_p, _c_i64, _c_p, _c_p, _c_int, _c_p,
+    ]),
+    "vgo_cached_attn_workspace": (_c_int, [
+        ctypes.POINTER(PagedCacheStruct), _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_size),
+    ]),
+    "vgo_cached_attn_fwd": (_c_int, [
+        ctypes.POINTER(PagedCacheStruct), _c_p, _i64x3, _c_i64, _c_i64, _c_p, _c_p, _c_int, _c_f32, _c_p, _i64x3,
+        _c_int, _c_p, _c_size, _c_p,
     ]),
     "vgo_restore_residual_layer_norm": (_c_int, [
         _c_p, _c_i64, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_f32, _c_i64,

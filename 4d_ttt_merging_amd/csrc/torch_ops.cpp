@@ -356,6 +356,128 @@ std::vector<Tensor> masked_attention_grad(
   return {dq, dk, dv, d_mass, d_slopes, d_table};
 }
 
+// ------------------------------------------------------------- paged cache ----
+struct CacheProblem {
+  vgo_paged_cache p{};
+  Tensor data, mass, table;
+
+  // `dim`: channels a head of the tensor beside it.
+  CacheProblem(const Tensor& data0, const OptTensor& mass0, const Tensor& table0, const Tensor& beside, const char* name) {
+    require_gpu({&data0, opt(mass0), &table0, &beside});
+    TORCH_CHECK(data0.device() == beside.device() && table0.device() == beside.device() &&
+                    (opt(mass0) == nullptr || mass0->device() == beside.device()),
+                name, ": every tensor must be on one device");
+    TORCH_CHECK_VALUE(data0.dim() == 4 && data0.scalar_type() == at::kByte && data0.is_contiguous() &&
+                          (data0.size(3) == 34 * 64 || data0.size(3) == 34 * 128),
+                      name, ": the cache's data must be contiguous uint8 [pages, kv_heads, page_size / 32, 34 * head_dim]");
+    TORCH_CHECK_VALUE(table0.dim() == 2 && table0.scalar_type() == at::kInt,
+                      name, ": the page table must be int32 [batch, pages of a sequence]");
+    data = data0, table = table0.contiguous();
+    p.pages = data.size(0), p.kv_heads = data.size(1), p.page_size = 32 * data.size(2), p.head_dim = data.size(3) / 34;
+    p.batch = table.size(0), p.table_width = table.size(1);
+    if (opt(mass0) != nullptr) {
+      TORCH_CHECK_VALUE(mass0->scalar_type() == at::kFloat && mass0->is_contiguous() && mass0->dim() == 2 &&
+                            mass0->size(0) == p.pages && mass0->size(1) == p.page_size,
+                        name, ": the cache's masses must be contiguous float32 [pages, page_size]");
+      mass = *mass0;
+    }
+    p.data = ptr(data), p.log_mass = ptr<float>(mass), p.page_table = ptr<int32_t>(table);
+  }
+};
+// A contiguous int32 tensor of this shape on the device of `beside` (undefined if absent).
+Tensor whole(const OptTensor& t, at::IntArrayRef shape, const Tensor& beside, const char* name, const char* what) {
+  if (opt(t) == nullptr) return Tensor();
+  require_gpu({&*t});
+  TORCH_CHECK(t->device() == beside.device(), name, ": every tensor must be on one device");
+  TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->sizes() == shape, name, ": ", what, " must be int32 ", shape);
+  return t->contiguous();
+}
+
+Tensor cache_append(const Tensor& k0, const Tensor& v0, const OptTensor& q0, const Tensor& data, const OptTensor& page_mass,
+                    const Tensor& page_table, const Tensor& starts0, const OptTensor& counts0, const OptTensor& sin0,
+                    const OptTensor& cos0, const OptTensor& positions0, const OptTensor& log_mass0) {
+  constexpr const char* name = "cache_append";
+  require_gpu({&k0, &v0, opt(q0), opt(sin0), opt(cos0), opt(log_mass0)});
+  for (const Tensor* t : {&v0, opt(q0), opt(sin0), opt(cos0), opt(log_mass0)})
+    TORCH_CHECK(t == nullptr || t->device() == k0.device(), name, ": every tensor must be on one device");
+  const CacheProblem c(data, page_mass, page_table, k0, name);
+  TORCH_CHECK_VALUE(k0.dim() == 4 && k0.sizes() == v0.sizes() && k0.size(0) == c.p.batch && k0.size(1) == c.p.kv_heads &&
+                        k0.size(3) == c.p.head_dim,
+                    name, ": k and v must be [batch, kv_heads, tokens, channels] of the cache's heads and channels");
+  TORCH_CHECK_VALUE(k0.scalar_type() == v0.scalar_type() && (opt(q0) == nullptr || q0->scalar_type() == k0.scalar_type()),
+                    name, ": q, k and v must share one dtype");
+  const int dtype = dtype_code(k0.scalar_type());
+  const int64_t batch = c.p.batch, n = k0.size(2);
+  const Tensor k = operand(k0), v = operand(v0);
+  const Tensor starts = whole(starts0, {batch}, k0, name, "starts"), counts = whole(counts0, {batch}, k0, name, "counts");
+  const Tensor positions = whole(positions0, {batch, n}, k0, name, "positions");
+  TORCH_CHECK_VALUE((opt(sin0) == nullptr) == (opt(cos0) == nullptr), name, ": the rotation's two tables go together");
+  vgo_cache_tokens t{};
+  Tensor sin, cos, mass, q, out;
+  if (opt(sin0) != nullptr) {
+    TORCH_CHECK_VALUE(sin0->dim() == 2 && sin0->size(1) == c.p.head_dim && sin0->sizes() == cos0->sizes() &&
+                          sin0->is_floating_point() && cos0->is_floating_point(),
+                      name, ": the rotation's tables must be floating [rows, channels]");
+    sin = f32(sin0), cos = f32(cos0);
+    t.rope_sin = ptr<float>(sin), t.rope_cos = ptr<float>(cos), t.rope_rows = sin.size(0);
+  }
+  if (opt(log_mass0) != nullptr) {
+    TORCH_CHECK_VALUE(log_mass0->is_floating_point() && log_mass0->dim() == 2 && log_mass0->size(0) == batch &&
+                          log_mass0->size(1) == n,
+                      name, ": log_mass must be floating [batch, tokens]");
+    TORCH_CHECK_VALUE(c.mass.defined(), name, ": this cache holds no masses");
+    mass = f32(log_mass0);
+    t.log_mass = ptr<float>(mass);
+  }
+  if (opt(q0) != nullptr) {
+    TORCH_CHECK_VALUE(q0->dim() == 4 && q0->size(0) == batch && q0->size(2) == n && q0->size(3) == c.p.head_dim,
+                      name, ": q must be [batch, heads, tokens, channels] beside k");
+    q = operand(*q0), out = in_layout_of(*q0);
+    t.q = ptr(q), t.q_out = ptr(out), t.heads = q.size(1);
+    set_strides(t.q_stride, q), set_strides(t.q_out_stride, out);
+  } else {
+    out = at::empty({0}, k0.options());
+  }
+  t.k = ptr(k), t.v = ptr(v), t.n_tokens = n;
+  set_strides(t.k_stride, k), set_strides(t.v_stride, v);
+  t.starts = ptr<int32_t>(starts), t.counts = ptr<int32_t>(counts), t.positions = ptr<int32_t>(positions);
+  check(vgo_cache_append(&c.p, &t, dtype, stream_of(k0)));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> cache_read(const Tensor& data, const Tensor& page_table, const Tensor& starts0,
+                                      const OptTensor& counts0, int64_t n, at::ScalarType type) {
+  constexpr const char* name = "cache_read";
+  const CacheProblem c(data, std::nullopt, page_table, data, name);
+  const int dtype = dtype_code(type);
+  TORCH_CHECK_VALUE(n >= 0, name, ": negative size");
+  const Tensor starts = whole(starts0, {c.p.batch}, data, name, "starts");
+  const Tensor counts = whole(counts0, {c.p.batch}, data, name, "counts");
+  const Tensor k = at::empty({c.p.batch, c.p.kv_heads, n, c.p.head_dim}, data.options().dtype(type)), v = at::empty_like(k);
+  check(vgo_cache_read(&c.p, ptr<int32_t>(starts), ptr<int32_t>(counts), n, ptr(k), ptr(v), dtype, stream_of(data)));
+  return {k, v};
+}
+
+Tensor cached_attention(const Tensor& q0, const Tensor& data, const OptTensor& page_mass, const Tensor& page_table,
+                        const Tensor& lengths0, const OptTensor& counts0, bool causal, double scale) {
+  constexpr const char* name = "cached_attention";
+  const CacheProblem c(data, page_mass, page_table, q0, name);
+  TORCH_CHECK_VALUE(q0.dim() == 4 && q0.size(0) == c.p.batch && q0.size(3) == c.p.head_dim,
+                    name, ": q must be [batch, heads, tokens, channels] of the cache's channels");
+  const int dtype = dtype_code(q0.scalar_type());
+  const Tensor q = operand(q0), out = in_layout_of(q0);
+  const Tensor lengths = whole(lengths0, {c.p.batch}, q0, name, "lengths");
+  const Tensor counts = whole(counts0, {c.p.batch}, q0, name, "counts");
+  size_t need = 0;
+  check(vgo_cached_attn_workspace(&c.p, q.size(1), q.size(2), dtype, &need));
+  const Tensor ws = need > 0 ? scratch(need, q) : Tensor();
+  int64_t q_stride[3], out_stride[3];
+  set_strides(q_stride, q), set_strides(out_stride, out);
+  check(vgo_cached_attn_fwd(&c.p, ptr(q), q_stride, q.size(1), q.size(2), ptr<int32_t>(lengths), ptr<int32_t>(counts), causal,
+                            static_cast<float>(scale), ptr(out), out_stride, dtype, ptr(ws), need, stream_of(q)));
+  return out;
+}
+
 // ------------------------------------------------------------ position bias ----
 Tensor position_bias(const Tensor& table0, int64_t n_query, int64_t n_key, int64_t query_start,
                      at::IntArrayRef bucket_starts, bool bidirectional) {
@@ -905,6 +1027,9 @@ constexpr const char* kPlanInto[] = {"similarity_topk", "rope_table"};
 
 // Operators with a derivative, and those of their derivatives (path operators: no second one).
 constexpr const char* kGradients[] = {"masked_attention_grad", "position_bias_grad"};
+// The paged cache: path operators, and the one that writes (path, with a written argument).
+constexpr const char* kCache[] = {"cache_read", "cached_attention"};
+constexpr const char* kCacheInto[] = {"cache_append"};
 
 template <typename Visit>
 void each_tensor(const c10::IValue& value, Visit visit) {
@@ -1117,6 +1242,9 @@ void register_cuda(torch::Library& m) {
   m.impl("masked_attention_grad", on_device<masked_attention_grad>);
   m.impl("position_bias", on_device<position_bias>);
   m.impl("position_bias_grad", on_device<position_bias_grad>);
+  m.impl("cache_append", on_device<cache_append>);
+  m.impl("cache_read", on_device<cache_read>);
+  m.impl("cached_attention", on_device<cached_attention>);
 }
 
 void register_autograd(torch::Library& m) {
@@ -1126,6 +1254,8 @@ void register_autograd(torch::Library& m) {
   for (const char* name : kPlan) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<false>>());
   for (const char* name : kPlanInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<false>>());
   for (const char* name : kGradients) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
+  for (const char* name : kCache) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
+  for (const char* name : kCacheInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
   m.impl("masked_attention", masked_attention_autograd);
   m.impl("position_bias", position_bias_autograd);
 }
@@ -1133,13 +1263,14 @@ void register_autograd(torch::Library& m) {
 void register_inplace(torch::Library& m) {
   for (const char* name : kPathInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&written>());
   for (const char* name : kPlanInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&written>());
+  for (const char* name : kCacheInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&written>());
 }
 
 void register_batched(torch::Library& m) {
   const auto refuse = [&](const auto& names) {
     for (const char* name : names) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&no_batching>());
   };
-  refuse(kBlocks), refuse(kPlan), refuse(kPlanInto);
+  refuse(kBlocks), refuse(kPlan), refuse(kPlanInto), refuse(kCache), refuse(kCacheInto);
 }
 
 }  // namespace

@@ -31,6 +31,9 @@ dispatcher, `torch.compile` and fake-tensor tracing see them as single ops:
   `position_bias_grad`) -- attention under score caps, position biases and masks, and the dense
   bias by buckets; both have gradients.
 
+* `vgo::cache_append`, `vgo::cache_read`, `vgo::cached_attention` -- the paged cache of keys and values in
+  4 bits (inference).
+
 The CUDA (HIP) implementations are native (csrc/torch_ops.cpp, built into
 `libvgo_ops.so`) and call `libvgo.so` through its C ABI.  The operators a
 traced graph can hold have fake implementations that only describe their
@@ -118,6 +121,14 @@ _SCHEMAS = (
     "bool bidirectional) -> Tensor",
     "position_bias_grad(Tensor grad, int n_buckets, int query_start, int[] bucket_starts, bool bidirectional) "
     "-> Tensor",
+    # The paged cache of keys and values in 4 bits, data uint8 [pages, kv_heads, page_size / 32, 34 * head_dim]: append
+    # (returns the rotated q, empty without one), read tokens back, attend.
+    "cache_append(Tensor k, Tensor v, Tensor? q, Tensor(a!) data, Tensor(b!)? page_mass, Tensor page_table, "
+    "Tensor starts, Tensor? counts, Tensor? rope_sin, Tensor? rope_cos, Tensor? positions, Tensor? log_mass) -> Tensor",
+    "cache_read(Tensor data, Tensor page_table, Tensor starts, Tensor? counts, SymInt n_tokens, ScalarType dtype) "
+    "-> (Tensor, Tensor)",
+    "cached_attention(Tensor q, Tensor data, Tensor? page_mass, Tensor page_table, Tensor lengths, Tensor? counts, "
+    "bool causal, float scale) -> Tensor",
 )
 
 _library = torch.library.Library("vgo", "DEF")
@@ -281,3 +292,19 @@ def _(table, n_query, n_key, query_start, bucket_starts, bidirectional):
 @_fake("position_bias_grad")
 def _(grad, n_buckets, query_start, bucket_starts, bidirectional):
     return grad.new_empty((n_buckets, grad.shape[0]))
+
+
+@_fake("cache_append")
+def _(k, v, q, data, page_mass, page_table, starts, counts, rope_sin, rope_cos, positions, log_mass):
+    return k.new_empty((0,)) if q is None else _in_layout_of(q)
+
+
+@_fake("cache_read")
+def _(data, page_table, starts, counts, n_tokens, dtype):
+    shape = (page_table.shape[0], data.shape[1], n_tokens, data.shape[3] // 34)
+    return data.new_empty(shape, dtype=dtype), data.new_empty(shape, dtype=dtype)
+
+
+@_fake("cached_attention")
+def _(q, data, page_mass, page_table, lengths, counts, causal, scale):
+    return _in_layout_of(q)

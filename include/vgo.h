@@ -652,6 +652,79 @@ int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64_t heads, c
                            int64_t n_key, void* d_table, int dtype, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/*
+ * A cache of keys and values in 4 bits, in pages; appending to it, reading it back and attention over it.  No
+ * counterpart in the reference, whose attention reads 16-bit keys of one call (models/mass_bias_attention.py:85-129).
+ *
+ * 32 channels of one token and head share a power of two 2^e, the smallest from 2^-125 to 2^125 of which 7 are at
+ * least their largest magnitude; each is the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times that (ties to the even
+ * one of the list, counted from 0; past 6: 6), so that none is off by more than 2^e.  The code is sign, then the place in that list
+ * (OCP E2M1), the scale's byte e + 127 (E8M0); 255 where one of the 32 is not finite: all of them then read as NaN.
+ *
+ * data: uint8 [pages, kv_heads, page_size / 32, 34 * head_dim], 16-byte aligned.  A block holds 32 tokens:
+ *   keys' codes [32][head_dim / 2] (byte c: channel 2c in its low half, 2c + 1 in its high half), values' codes
+ *   [4][head_dim / 2][8] (tokens 8g .. 8g + 7 of a channel pair side by side), keys' scales [32][head_dim / 32],
+ *   values' scales [4][head_dim / 32][8].
+ * log_mass: fp32 [pages, page_size], added to every score of a token; NULL: the cache holds none.
+ * page_size: a power of two, 32 to 1,024; head_dim 64 or 128.
+ * page_table: int32 [batch, table_width]; token t of sequence b lies in page page_table[b, t / page_size].  Tokens past
+ * the table, or whose page is not one of the cache's, are not there: appending leaves them out, reading gives zeros,
+ * no query attends to them.  A sequence has at most INT32_MAX tokens.
+ */
+typedef struct vgo_paged_cache {
+  void* data;
+  float* log_mass;
+  const int32_t* page_table;
+  int64_t pages, page_size, kv_heads, head_dim, batch, table_width;
+} vgo_paged_cache;
+
+/*
+ * New tokens of every sequence.  k / v [batch, kv_heads, n_tokens, head_dim] and, with heads > 0, q [batch, heads,
+ * n_tokens, head_dim] of one type, strides in elements for (batch, head, token), multiples of 16 bytes, unit channel
+ * stride, 16-byte aligned.  Token i of sequence b goes to place starts[b] + i; those from counts[b] on (NULL: none;
+ * clamped to 0 .. n_tokens) are padding and are not stored.
+ * rope_sin / rope_cos fp32 [rope_rows, head_dim] or NULL: k is stored, and q is written to q_out, as
+ *   x cos + (-x[D/2 ..], x[.. D/2]) sin   with row positions[b, i] (int32 [batch, n_tokens]; NULL: starts[b] + i) of
+ * the tables, taken in 64 bits and rounded once; tokens whose row the tables do not have are not rotated.  q_out's padding is zeros.
+ * log_mass fp32 [batch, n_tokens]; NULL: zeros, where the cache holds masses.
+ * Tokens of one call must not share a place (sequences that share a page may do so only for tokens that are there).
+ */
+typedef struct vgo_cache_tokens {
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  int64_t heads, n_tokens;
+  int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
+  const int32_t* starts;
+  const int32_t* counts;
+  const float* rope_sin;
+  const float* rope_cos;
+  int64_t rope_rows;
+  const int32_t* positions;
+  const float* log_mass;
+} vgo_cache_tokens;
+int vgo_cache_append(const vgo_paged_cache* cache, const vgo_cache_tokens* tokens, int dtype, void* stream);
+
+/* Tokens starts[b] .. starts[b] + n_tokens - 1 of every sequence as numbers: k, v [batch, kv_heads, n_tokens, head_dim]
+ * contiguous (exact in bf16 and fp32; f16 rounds what it does not hold); zeros from counts[b] on. */
+int vgo_cache_read(const vgo_paged_cache* cache, const int32_t* starts, const int32_t* counts, int64_t n_tokens,
+                   void* k, void* v, int dtype, void* stream);
+
+/*
+ * Attention over the cache: query i of sequence b stands at place lengths[b] - counts[b] + i (counts NULL: n_query) and
+ *   out_i = sum_j softmax_j(scale * q_i.k_j + log_mass[j]) v_j   over j < lengths[b], and, if causal, j <= its place.
+ * Queries from counts[b] on, and those that attend to nothing, give zeros.  q / out [batch, heads, n_query, head_dim],
+ * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)), strides as in vgo_cache_tokens.
+ * Tokens past a sequence's length are not read.  Workspace (16-byte aligned, any contents): the states of work split over the keys; its size
+ * is for the device that is current.
+ */
+int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int dtype, size_t* bytes);
+int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, const int64_t q_stride[3], int64_t heads,
+                        int64_t n_query, const int32_t* lengths, const int32_t* counts, int causal, float scale,
+                        void* out, const int64_t out_stride[3], int dtype, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

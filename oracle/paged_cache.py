@@ -1,0 +1,156 @@
+"""The paged cache of keys and values in 4 bits and attention over it, in 64 bits on the CPU, with error bounds.
+
+Written from the definition (4d_ttt_merging_amd/paged_cache.py states it): one token, one head, one query at a
+time where that is simplest.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+LEVELS = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+
+
+def scale_exponents(top: torch.Tensor) -> torch.Tensor:
+    """e of blocks whose largest magnitudes are `top` (float64): the first of -125, -124, ... that holds, at most 125."""
+    e = torch.full(top.shape, -125)
+    while ((short := (top > 7.0 * 2.0 ** e.double()) & (e < 125))).any():
+        e = e + short.long()
+    return e
+
+
+def encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scale bytes) of x [..., D], D a multiple of 32."""
+    blocks = x.double().reshape(-1, 32)
+    top = blocks.abs().amax(1)
+    fine = torch.isfinite(top)
+    blocks = torch.where(fine[:, None], blocks, 0.0)
+    e = scale_exponents(torch.where(fine, top, 0.0))
+    away = (blocks.abs()[..., None] / 2.0 ** e.double()[:, None, None] - LEVELS).abs()
+    # Of two that are as near, the even code; past 6 all round to 6.
+    order = torch.tensor([0, 2, 4, 6, 1, 3, 5, 7])
+    nearest = (away == away.amin(-1, keepdim=True))[..., order].to(torch.uint8).argmax(-1)
+    codes = order[nearest].to(torch.uint8) + 8 * (blocks < 0).to(torch.uint8)
+    scales = torch.where(fine, e + 127, 255).to(torch.uint8)
+    return codes.reshape(x.shape), scales.reshape(*x.shape[:-1], x.shape[-1] // 32)
+
+
+def decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """float64 numbers of codes [..., D] and scale bytes [..., D / 32]."""
+    value = LEVELS[(codes & 7).long()] * torch.where(codes >= 8, -1.0, 1.0).double()
+    factor = torch.where(scales == 255, math.nan, 2.0 ** (scales.double() - 127))
+    return value * factor.repeat_interleave(32, -1)
+
+
+def rotate(x: torch.Tensor, sin: torch.Tensor, cos: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    """x [H, N, D] rotated by the tables' rows [N]; tokens without a row as they are."""
+    x, out = x.double(), x.double().clone()
+    half = x.shape[-1] // 2
+    for i, row in enumerate(rows.tolist()):
+        if 0 <= row < sin.shape[0]:
+            s, c = sin[row].double(), cos[row].double()
+            out[:, i] = x[:, i] * c + torch.cat([-x[:, i, half:], x[:, i, :half]], -1) * s
+    return out
+
+
+class Pages:
+    """A cache's tokens as numbers: what is stored in each place of each page."""
+
+    def __init__(self, pages, kv_heads, page_size, dim):
+        self.k = torch.zeros(pages, kv_heads, page_size, dim, dtype=torch.float64)
+        self.v = torch.zeros_like(self.k)
+        self.mass = torch.zeros(pages, page_size, dtype=torch.float64)
+
+    def place(self, table, b, t):
+        """(page, slot) of token t of sequence b, or None."""
+        size = self.k.shape[2]
+        if t < 0 or t // size >= table.shape[1]:
+            return None
+        page = int(table[b, t // size])
+        return (page, t % size) if 0 <= page < self.k.shape[0] else None
+
+
+def append(pages: Pages, k, v, table, starts, counts=None, *, q=None, rope=None, positions=None, log_mass=None):
+    """Stores the tokens; returns q rotated (float64, padding as zeros) or None."""
+    b, _, n, _ = k.shape
+    out = None if q is None else torch.zeros(q.shape, dtype=torch.float64)
+    for i in range(b):
+        start = int(starts[i])
+        count = n if counts is None else min(max(int(counts[i]), 0), n)
+        if count == 0:
+            continue
+        rows = start + torch.arange(count) if positions is None else positions[i, :count]
+        turn = (lambda x: x.double()) if rope is None else (lambda x: rotate(x, rope[0], rope[1], rows))
+        if q is not None:
+            out[i, :, :count] = turn(q[i, :, :count])
+        keys, values = decode(*encode(turn(k[i, :, :count]))), decode(*encode(v[i, :, :count]))
+        for t in range(count):
+            place = pages.place(table, i, start + t)
+            if place is not None:
+                pages.k[place[0], :, place[1]] = keys[:, t]
+                pages.v[place[0], :, place[1]] = values[:, t]
+                pages.mass[place] = 0.0 if log_mass is None else float(log_mass[i, t])
+    return out
+
+
+def read(pages: Pages, table, starts, n, counts=None):
+    b, (hk, d) = table.shape[0], pages.k.shape[1::2]
+    k, v = torch.zeros(b, hk, n, d, dtype=torch.float64), torch.zeros(b, hk, n, d, dtype=torch.float64)
+    for i in range(b):
+        for t in range(n if counts is None else min(max(int(counts[i]), 0), n)):
+            place = pages.place(table, i, int(starts[i]) + t)
+            if place is not None:
+                k[i, :, t], v[i, :, t] = pages.k[place[0], :, place[1]], pages.v[place[0], :, place[1]]
+    return k, v
+
+
+def attention(q, pages: Pages, table, lengths, counts=None, *, causal=False, scale=None, masses=False, p_bits=None):
+    """(out, bound), float64 [B, H, N, D]; `p_bits`: how far a probability may be rounded, relative to it (default
+    half a step of q's type).
+
+    The bound, element by element: with u = 2^-24 and probabilities p, a score is off by at most
+    e_j = u (D + 4) scale sum_d |q_d k_jd| + 4 u (|z_j| + |largest z|), of which the last part are the change to base 2, the
+    mass and the distance from the running maximum; p_j by p_j (e_j + 8 u) (exp2 to 4 ulp) and its rounding; sums
+    over n keys by (32 + n / 16) u of their magnitudes (32 or fewer products at a time, then one addition per
+    32 keys and per part), in the numerator and in the denominator; and the result by half a step of its type."""
+    u, half = 2.0 ** -24, torch.finfo(q.dtype).eps / 2
+    p_bits = half if p_bits is None else p_bits
+    b, h, n, d = q.shape
+    hk, size = pages.k.shape[1], pages.k.shape[2]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    for i in range(b):
+        length, count = int(lengths[i]), n if counts is None else min(max(int(counts[i]), 0), n)
+        places = [pages.place(table, i, t) for t in range(min(length, table.shape[1] * size))]
+        seen = torch.tensor([t for t, place in enumerate(places) if place is not None], dtype=torch.long)
+        if count == 0 or seen.numel() == 0:
+            continue
+        at = [places[t] for t in seen.tolist()]
+        page, slot = torch.tensor([p for p, _ in at]), torch.tensor([s for _, s in at])
+        k, v = pages.k[page, :, slot].transpose(0, 1), pages.v[page, :, slot].transpose(0, 1)  # [hk, keys, d]
+        ok = torch.ones(count, seen.numel(), dtype=torch.bool)
+        if causal:
+            ok = seen[None] <= (length - count + torch.arange(count))[:, None]
+        for head in range(h):
+            x, key, value = q[i, head, :count].double(), k[head // (h // hk)], v[head // (h // hk)]
+            z = scale * (x @ key.T)
+            size_z = scale * (x.abs() @ key.abs().T)
+            if masses:
+                z = z + pages.mass[page, slot]
+            z = torch.where(ok, z, -math.inf)
+            top = z.amax(1, keepdim=True)
+            p = torch.exp(z - torch.where(top == -math.inf, 0.0, top))
+            total = p.sum(1, keepdim=True)
+            p = p / torch.where(total == 0, 1.0, total)
+            value = torch.where((p > 0).any(0)[:, None], value, 0.0)
+            off = u * (d + 4) * size_z + torch.where(p > 0, 4 * u * (z.abs() + top.abs()), 0.0) + 8 * u
+            off = torch.where(p > 0, off, 0.0)
+            sums = (32 + seen.numel() / 16) * u
+            o = p @ value
+            out[i, head, :count] = o
+            weight = (p * (off + p_bits + sums)) @ value.abs()
+            bound[i, head, :count] = weight + o.abs() * ((p * off).sum(1, keepdim=True) + sums + half) + 2.0 ** -126
+            if q.dtype == torch.float16:
+                bound[i, head, :count] += 2.0 ** -25
+    return out, bound

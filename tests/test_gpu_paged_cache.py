@@ -1,0 +1,275 @@
+"""The paged cache in 4 bits -- append, read, attention -- against the 64-bit oracle."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import paged_cache as oracle
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def int32(values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def tables(rows, dim):
+    angle = torch.outer(torch.arange(rows, dtype=torch.float64), 100.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2)))
+    angle = torch.cat([angle, angle], 1)
+    return angle.sin().float(), angle.cos().float()
+
+
+def layout(batch, tokens, page, seed, spare=2):
+    """(page table in no order, pages)."""
+    per = max(1, -(-tokens // page))
+    g = torch.Generator().manual_seed(seed)
+    return torch.randperm(batch * per + spare, generator=g)[:batch * per].view(batch, per).int(), batch * per + spare
+
+
+class Both:
+    """A cache on the GPU and the oracle's pages, written together."""
+
+    def __init__(self, vgo, device, pages, kv_heads, page, dim, masses=False):
+        self.vgo, self.device, self.masses = vgo, device, masses
+        self.cache = vgo.PagedCache.empty(pages, kv_heads, dim, page_size=page, masses=masses, device=device)
+        self.pages = oracle.Pages(pages, kv_heads, page, dim)
+
+    def to(self, t):
+        return t.to(self.device) if isinstance(t, torch.Tensor) else None if t is None else tuple(x.to(self.device) for x in t)
+
+    def append(self, k, v, table, starts, counts=None, q=None, rope=None, positions=None, log_mass=None):
+        got = self.vgo.cache_append(self.cache, self.to(k), self.to(v), self.to(table), self.to(starts), self.to(counts),
+                                    q=self.to(q), rope=self.to(rope), positions=self.to(positions), log_mass=self.to(log_mass))
+        want = oracle.append(self.pages, k, v, table, starts, counts, q=q, rope=rope, positions=positions, log_mass=log_mass)
+        if q is not None:
+            got = got.double().cpu()
+            # Rounded once from 64 bits; the smallest normal of the type for what rounds to less.
+            assert ((got - want).abs() <= torch.finfo(q.dtype).eps / 2 * want.abs() + torch.finfo(q.dtype).tiny).all()
+        return got
+
+    def check_everything(self):
+        """Every place of every page, and the masses."""
+        pages, page = self.cache.data.shape[0], self.cache.page_size
+        table = torch.arange(pages, dtype=torch.int32, device=self.device)[:, None]
+        k, v = self.vgo.cache_read(self.cache, table, torch.zeros(pages, dtype=torch.int32, device=self.device), page, dtype=F32)
+        assert torch.equal(torch.nan_to_num(k.double().cpu(), nan=1e300), torch.nan_to_num(self.pages.k, nan=1e300))
+        assert torch.equal(torch.nan_to_num(v.double().cpu(), nan=1e300), torch.nan_to_num(self.pages.v, nan=1e300))
+        if self.masses:
+            assert torch.equal(self.cache.log_mass.double().cpu(), self.pages.mass)
+
+    def fill(self, seed, gain=1.0):
+        """Random tokens in every page."""
+        pages, hk, page, d = self.pages.k.shape
+        g = torch.Generator().manual_seed(seed)
+        k, v = (torch.randn(pages, hk, page, d, generator=g) * gain for _ in range(2))
+        mass = torch.randint(1, 9, (pages, page), generator=g).float().log() if self.masses else None
+        self.append(k, v, torch.arange(pages, dtype=torch.int32)[:, None], torch.zeros(pages, dtype=torch.int32), log_mass=mass)
+
+    def attend(self, q, table, lengths, counts=None, causal=False, scale=None):
+        got = self.vgo.cached_attention(self.to(q), self.cache, self.to(table), self.to(lengths), self.to(counts), causal=causal,
+                                        scale=scale)
+        want, bound = oracle.attention(q, self.pages, table, lengths, counts, causal=causal, scale=scale, masses=self.masses)
+        assert got.shape == q.shape and got.dtype == q.dtype
+        off = (got.double().cpu() - want).abs()
+        assert torch.isfinite(off).all()
+        worst = (off - bound).max().item() if off.numel() else 0.0
+        assert worst <= 0, f"off by {worst:.3e} beyond its bound, {off.max():.3e} in all"
+        return got
+
+
+# ----------------------------------------------------------------- append, read ----
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("starts,counts,n", [([0], None, 1), ([7], None, 1), ([3, 31], [5, 2], 5), ([0, 30, 61], [70, 0, 33], 70),
+                                             ([5, 64], None, 129), ([8, 16], [24, 31], 32)])
+def test_append(vgo, device, dtype, dim, starts, counts, n):
+    b = len(starts)
+    both = Both(vgo, device, b * 7 + 2, 3, 32, dim)
+    both.fill(1)
+    table, _ = layout(b, 7 * 32, 32, 2)
+    g = torch.Generator().manual_seed(3)
+    k, v, q = (torch.randn(b, n, h, dim, generator=g).to(dtype).transpose(1, 2) for h in (3, 3, 6))
+    got = both.append(k, v, table, int32(starts), None if counts is None else int32(counts), q=q, rope=tables(90, dim))
+    assert got.stride(2) > got.stride(1)  # token-major, as q
+    both.check_everything()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("page", [32, 64, 256, 1024])
+def test_append_positions_masses_and_no_rotation(vgo, device, dtype, page):
+    b, n, dim = 2, 41, 64
+    both = Both(vgo, device, 9, 2, page, dim, masses=True)
+    both.fill(1)
+    table, _ = layout(b, 3 * page, page, 2)
+    g = torch.Generator().manual_seed(4)
+    k, v, q = (torch.randn(b, h, n, dim, generator=g).to(dtype) for h in (2, 2, 2))
+    positions = torch.randint(-2, 40, (b, n), generator=g).int()
+    mass = torch.randn(b, n, generator=g)
+    mass[0, 3] = -math.inf
+    both.append(k, v, table, int32([page - 11, 2 * page - 5]), int32([41, 30]), q=q, rope=tables(37, dim), positions=positions,
+                log_mass=mass)
+    both.append(v, k, table, int32([0, 5]), int32([2, 3]))  # masses of zero
+    both.check_everything()
+
+
+def test_append_values_next_to_a_border(vgo, device):
+    """Exact ties, their neighbours, zeros, blocks that are tiny, huge, infinite or NaN."""
+    dim = 64
+    both = Both(vgo, device, 2, 1, 64, dim)
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0], dtype=F32)
+    rows = [torch.cat([ties, torch.nextafter(ties, ties * 2), torch.nextafter(ties, ties * 0), -ties]).repeat(2) * s
+            for s in (1.0, 2.0 ** -20, 2.0 ** 100, 2.0 ** -126)]
+    rows += [torch.zeros(64), torch.full((64,), 3.4028234663852886e38), torch.full((64,), 1e-45), torch.full((64,), -3e38)]
+    bad = torch.ones(2, 64)
+    bad[0, 5], bad[1, 63] = math.nan, -math.inf
+    x = torch.cat([torch.stack(rows), bad])[None, None]
+    both.append(x, x.flip(2), int32([[0]]), int32([3]))
+    both.check_everything()
+    both.append(x, x.flip(2), int32([[1]]), int32([3]), rope=tables(1, dim), positions=torch.zeros(1, x.shape[2], dtype=torch.int32))
+    # (sin 0, cos 1: a rotation by nothing keeps ties ties; of the block with an infinity its partner's becomes NaN)
+    pages = both.pages
+    k, _ = vgo.cache_read(both.cache, both.to(int32([[1]])), both.to(int32([3])), x.shape[2], dtype=F32)
+    assert torch.equal(torch.nan_to_num(k[0, 0].double().cpu(), nan=1e300), torch.nan_to_num(pages.k[1, 0, 3:3 + x.shape[2]], nan=1e300))
+
+
+@pytest.mark.parametrize("case", ["no page", "past the table", "page of another cache", "before the first", "counts out of range"])
+def test_tokens_without_a_place_are_left_out(vgo, device, case):
+    both = Both(vgo, device, 4, 2, 32, 64, masses=True)
+    both.fill(5)
+    g = torch.Generator().manual_seed(6)
+    k, v = torch.randn(2, 2, 40, 64, generator=g), torch.randn(2, 2, 40, 64, generator=g)
+    table, starts, counts = int32([[0, 1], [2, 3]]), int32([10, 20]), None
+    if case == "no page":
+        table = int32([[0, -1], [-7, 3]])
+    elif case == "past the table":
+        starts = int32([50, 2000000000])
+    elif case == "page of another cache":
+        table = int32([[0, 4], [2147483647, 3]])
+    elif case == "before the first":
+        starts = int32([-13, -2147483648])
+    else:
+        counts = int32([-3, 1000])
+    both.append(k, v, table, starts, counts, q=k, rope=tables(64, 64))
+    both.check_everything()
+
+
+def test_read_ranges(vgo, device):
+    both = Both(vgo, device, 8, 2, 64, 128)
+    both.fill(7)
+    table = int32([[5, 1, -1], [0, 9, 3]])
+    for starts, n, counts in (([3, 62], 70, None), ([0, 127], 9, [4, 9]), ([100, -4], 100, [100, 50]), ([0, 0], 1, [0, 1])):
+        k, v = vgo.cache_read(both.cache, both.to(table), both.to(int32(starts)), n, None if counts is None else both.to(int32(counts)),
+                              dtype=F32)
+        want = oracle.read(both.pages, table, int32(starts), n, counts)
+        assert torch.equal(k.double().cpu(), want[0]) and torch.equal(v.double().cpu(), want[1])
+        half = vgo.cache_read(both.cache, both.to(table), both.to(int32(starts)), n, None if counts is None else both.to(int32(counts)))
+        assert half[0].dtype == BF16 and torch.equal(half[0].float(), k) and torch.equal(half[1].float(), v)
+
+
+# -------------------------------------------------------------------- attention ----
+SHAPES = [  # batch, heads, key heads, dim, queries, tokens, page
+    (1, 1, 1, 64, 1, 1, 32), (1, 4, 1, 64, 1, 33, 32), (2, 4, 4, 128, 1, 300, 64), (3, 16, 2, 64, 1, 517, 128),
+    (2, 8, 2, 64, 4, 259, 64), (1, 2, 2, 128, 17, 100, 32), (1, 2, 1, 64, 50, 261, 64), (2, 6, 2, 64, 130, 333, 256),
+    (1, 4, 2, 128, 150, 700, 64), (1, 1, 1, 64, 300, 300, 1024)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention(vgo, device, shape, causal, dtype):
+    b, h, hk, dim, n, tokens, page = shape
+    table, pages = layout(b, tokens, page, 8)
+    both = Both(vgo, device, pages, hk, page, dim, masses=n % 2 == 1)
+    both.fill(9)
+    g = torch.Generator().manual_seed(10)
+    q = (torch.randn(b, n, h, dim, generator=g) * 2).to(dtype).transpose(1, 2)
+    out = both.attend(q, table, torch.full((b,), tokens, dtype=torch.int32), causal=causal)
+    assert h == 1 or n == 1 or out.stride(2) > out.stride(1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [1, 3, 40, 140])
+@pytest.mark.parametrize("causal", [False, True])
+def test_ragged(vgo, device, dtype, n, causal):
+    """Lengths of nothing, one, within and past the table; counts of nothing and all; lengths below the counts."""
+    b, page = 7, 64
+    table, pages = layout(b, 5 * page, page, 11)
+    both = Both(vgo, device, pages, 2, page, 64, masses=True)
+    both.fill(12)
+    q = torch.randn(b, 4, n, 64, generator=torch.Generator().manual_seed(13)).to(dtype)
+    lengths = int32([0, 1, 64, 65, 320, 1000, 200])
+    counts = int32([n, n, 0, max(1, n // 2), n, n, n + 5])
+    both.attend(q, table, lengths, counts, causal)
+
+
+@pytest.mark.parametrize("n", [1, 40, 140])
+@pytest.mark.parametrize("causal", [False, True])
+def test_missing_pages_and_masses_that_leave_nothing(vgo, device, n, causal):
+    page = 32
+    table = int32([[0, -1, 2, 3, 99, 5], [-1, -1, -1, -1, -1, -1], [6, 7, 8, 9, 10, 11], [6, 0, 8, 2, 10, 11]])
+    both = Both(vgo, device, 12, 2, page, 64, masses=True)
+    both.fill(14)
+    for place in ((6, slice(None)), (8, slice(5, 9)), (10, 0), (3, slice(None))):  # (a mass of -inf keeps a token out)
+        both.pages.mass[place] = -math.inf
+        both.cache.log_mass[place] = -math.inf
+    both.pages.mass[11, 3] = both.cache.log_mass[11, 3] = torch.finfo(F32).min
+    q = torch.randn(4, 2, n, 64, generator=torch.Generator().manual_seed(15))
+    both.attend(q, table, int32([190, 192, 170, 32]), causal=causal)
+
+
+@pytest.mark.parametrize("n", [1, 40, 140])
+def test_masked_places_may_hold_anything(vgo, device, n):
+    """Tokens past the length: NaN blocks and masses, in the last tile and in pages beyond."""
+    table, pages = layout(2, 192, 64, 16)
+    both = Both(vgo, device, pages, 2, 64, 64, masses=True)
+    both.fill(17)
+    lengths = int32([75, 128])
+    for b in range(2):
+        for t in range(int(lengths[b]), 192):
+            page, slot = int(table[b, t // 64]), t % 64
+            bad = torch.full((1, 2, 1, 64), math.nan)
+            both.append(bad, bad, int32([[page]]), int32([slot]), log_mass=torch.full((1, 1), math.nan))
+            both.pages.k[page, :, slot] = both.pages.v[page, :, slot] = 0.0
+            both.pages.mass[page, slot] = 0.0
+    q = torch.randn(2, 4, n, 64, generator=torch.Generator().manual_seed(18))
+    both.attend(q, table, lengths)
+    if n > 1:
+        both.attend(q, table, lengths, causal=True)
+
+
+@pytest.mark.parametrize("n", [1, 140])
+def test_large_equal_scores_and_large_scales(vgo, device, n):
+    """Scores far from zero and far apart, one key's probability all of it."""
+    table, pages = layout(1, 260, 64, 19)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    both.fill(20, gain=8.0)
+    q = torch.randn(1, 2, n, 64, generator=torch.Generator().manual_seed(21)) * 8
+    both.attend(q, table, int32([260]))
+    both.attend(q, table, int32([260]), scale=1e-3)
+    both.attend(torch.zeros(1, 2, n, 64), table, int32([260]))
+
+
+def test_strides(vgo, device):
+    table, pages = layout(2, 200, 64, 22)
+    both = Both(vgo, device, pages, 2, 64, 64)
+    both.fill(23)
+    g = torch.Generator().manual_seed(24)
+    wide = torch.randn(2, 9, 4, 3, 64, generator=g)
+    for q in (wide[:, :, :, 1].transpose(1, 2), wide[:, ::2, :, 0].transpose(1, 2), wide[:1, :, :, 2].transpose(1, 2).expand(2, 4, 9, 64),
+              torch.randn(2, 4, 64, 9, generator=g).transpose(2, 3), torch.randn(2, 4, 9, 65, generator=g)[..., 1:]):
+        both.attend(q, table, int32([200, 123]))
+
+
+def test_results_are_the_same_bits(vgo, device):
+    table, pages = layout(2, 3000, 64, 25)
+    both = Both(vgo, device, pages, 2, 64, 64)
+    both.fill(26)
+    for n in (1, 70, 200):
+        q = torch.randn(2, 8, n, 64, generator=torch.Generator().manual_seed(27)).to(BF16).to(device)
+        call = lambda: vgo.cached_attention(q, both.cache, both.to(table), both.to(int32([3000, 1234])), causal=True)
+        first = call()
+        for _ in range(4):
+            assert torch.equal(first, call())
