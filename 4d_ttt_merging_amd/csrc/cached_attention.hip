@@ -1,90 +1,79 @@
 // Attention over the paged cache of keys and values in 4 bits (paged_cache.h).
-#include "paged_cache.h"
+#include "cached_attention.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace vgo {
 namespace paged {
 namespace {
 
-struct Attend {
-  Pages pages;
-  const void* q;
-  void* out;
-  int64_t q_stride[3], out_stride[3];
-  const int32_t* lengths;
-  const int32_t* counts;
-  int64_t n_query, rows;
-  int heads, causal;
-  float scale;
-};
-
-// A wave takes one query of one head; its lanes 64 keys at a time for the scores, then two channels each (one
-// of 64) for the values.
+// Joins the pieces of a row: a wave a row, D / 64 channels a lane.  Rows of sequences in one piece are written already.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void attend_kernel(const Attend a) {
-  using L = Layout<D>;
+__global__ __launch_bounds__(256) void merge_kernel(const Attend a) {
   constexpr int kEach = D / 64;
-  __shared__ float q[D];
-  __shared__ float weight[64];
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
-  const int64_t i = row % a.n_query;
-  const int h = static_cast<int>(row / a.n_query % a.heads);
-  const int64_t b = row / a.n_query / a.heads;
-  const int hk = h / (a.heads / a.pages.kv_heads);
-  const int64_t length = min(static_cast<int64_t>(a.lengths[b]), a.pages.width << a.pages.shift);
-  const int64_t count = a.counts ? min(max(static_cast<int64_t>(a.counts[b]), int64_t{0}), a.n_query) : a.n_query;
-  T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[1] + i * a.out_stride[2];
-  const T* from = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[1] + i * a.q_stride[2];
-  for (int e = lane; e < D; e += 64) q[e] = to_f32(from[e]) * a.scale;
-  __syncthreads();
-  int64_t end = a.causal ? min(length, a.lengths[b] - count + i + 1) : length;
-  if (i >= count) end = 0;
-  float top = -INFINITY, total = 0.0f, acc[kEach] = {};
-  for (int64_t j0 = 0; j0 < end; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const int page = j < end ? page_of(a.pages, b, j) : -1;
-    float z = -INFINITY;
-    if (page >= 0) {
-      const uint8_t* block = a.pages.data + block_of<D>(a.pages, page, hk, j);
-      const int slot = static_cast<int>(j) & 31;
-      z = 0.0f;
-      for (int w = 0; w < D / 8; ++w) {
-        const uint32_t word = reinterpret_cast<const uint32_t*>(block + slot * L::kKeyBytes)[w];
-        const float s = scale_of<0>(block[L::kKeyScales + slot * L::kParts + w / 4]);
-        const bf16x2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 1),
-                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 3)};
-        for (int e = 0; e < 8; ++e) z = fmaf(q[8 * w + e], to_f32(p[e / 2][e % 2]), z);
-      }
-      if (a.pages.mass) z += a.pages.mass[(static_cast<int64_t>(page) << a.pages.shift) + (j & ((1 << a.pages.shift) - 1))];
-    }
-    float most = z;
-    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-    const float next = fmaxf(top, most), safe = next == -INFINITY ? 0.0f : next;
-    const float shrink = expf(top - safe), p = expf(z - safe);
-    top = next;
-    total = total * shrink + p;
-    for (int e = 0; e < kEach; ++e) acc[e] *= shrink;
-    __syncthreads();
-    weight[lane] = p;
-    __syncthreads();
-    for (int t = 0; t < 64 && j0 + t < end; ++t) {
-      const int at = page_of(a.pages, b, j0 + t);
-      if (at < 0) continue;
-      const uint8_t* block = a.pages.data + block_of<D>(a.pages, at, hk, j0 + t);
-      const int slot = static_cast<int>(j0 + t) & 31;
-      for (int e = 0; e < kEach; ++e) {
-        const int ch = lane + 64 * e;
-        const uint32_t byte = block[L::kValues + slot / 8 * L::kGroup + ch / 2 * 8 + slot % 8];
-        const float s = scale_of<0>(block[L::kValueScales + slot / 8 * L::kScaleGroup + ch / 32 * 8 + slot % 8]);
-        const bf16x2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(byte, s, 0);
-        acc[e] = fmaf(weight[t], to_f32(v[ch % 2]), acc[e]);
-      }
-    }
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int rows = a.n_query * a.group, lane = lane_id(), kv = a.pages.kv_heads;
+  const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(at % rows));
+  const int64_t rest = at / rows;
+  const int hk = __builtin_amdgcn_readfirstlane(static_cast<int>(rest % kv));
+  const int64_t b = rest / kv;
+  if (b >= a.batch) return;
+  const int tokens = piece_tokens(a), length = length_of(a, b);
+  const int all = pieces_of(length, tokens);
+  if (all == 1) return;
+  int64_t first = 0;
+  for (int64_t o = lane; o < b; o += 64) first += pieces_of(length_of(a, o), tokens);
+  first = wave_sum(first);
+  const int count = count_of(a, b), tile = row / a.tile_rows;
+  const int last = min((tile + 1) * a.tile_rows, count * a.group) - 1;  // (as the tile's work-groups reckon)
+  const int stop = last < tile * a.tile_rows ? 0
+                   : a.causal ? max(0, min(length, a.lengths[b] - count + last / a.group + 1)) : length;
+  const int n = max(1, (stop + tokens - 1) / tokens);
+  const auto place = [&](int piece) {
+    return (((first + piece) * kv + hk) * a.tiles + tile) * a.tile_rows + row % a.tile_rows;
+  };
+  float most = -INFINITY;
+  for (int piece = 0; piece < n; ++piece) most = fmaxf(most, a.ends[place(piece)].x);
+  const float from = most == -INFINITY ? 0.0f : most;
+  float sum = 0.0f, v[kEach] = {};
+  for (int piece = 0; piece < n; ++piece) {
+    const float2 end = a.ends[place(piece)];
+    const float share = __builtin_amdgcn_exp2f(end.x - from);
+    sum = fmaf(end.y, share, sum);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) v[e] = fmaf(a.sums[place(piece) * D + lane + 64 * e], share, v[e]);
   }
-  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-  for (int e = 0; e < kEach; ++e) out[lane + 64 * e] = from_f32<T>(total > 0.0f || total != total ? acc[e] / total : 0.0f);
+  const bool none = row >= count * a.group || most == -INFINITY;
+  T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
+           row / a.group * a.out_stride[2];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) out[lane + 64 * e] = from_f32<T>(none ? 0.0f : v[e] / sum);
+}
+
+// How a call is cut.
+struct Plan {
+  int tile_rows, slots, least;
+  int64_t tiles, pieces;
+  size_t sums, ends;  // bytes of the workspace
+};
+Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query) {
+  Plan p{};
+  const int64_t rows = n_query * (heads / c->kv_heads), capacity = c->table_width * c->page_size;
+  p.tile_rows = few_rows(rows);
+  p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  p.least = 512;
+  const int64_t groups = 2 * device_cus(), beside = c->kv_heads * p.tiles;
+  const int64_t slots = groups / beside - c->batch;
+  // (no more pieces than the tables could hold)
+  p.slots = capacity <= p.least ? 0 : static_cast<int>(std::max<int64_t>(0, std::min(slots, c->batch * ((capacity - 1) / p.least))));
+  p.pieces = c->batch + p.slots;
+  if (p.slots > 0) {
+    const size_t parts = static_cast<size_t>(p.pieces) * beside * p.tile_rows;
+    p.sums = parts * c->head_dim * sizeof(float);
+    p.ends = parts * sizeof(float2);
+  }
+  return p;
 }
 
 int check_attend(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int dtype) {
@@ -95,6 +84,9 @@ int check_attend(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, i
   VGO_REQUIRE(heads % cache->kv_heads == 0, "cached_attn: heads must be a multiple of the key heads");
   return VGO_OK;
 }
+// A grid's threads are counted in 32 bits; work-groups of 512.
+constexpr int64_t kMostGroups = (int64_t{1} << 32) / 512;
+
 bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
   const int64_t size = dtype == VGO_F32 ? 4 : 2;
   if (!p || !aligned(p, 16) || !stride) return false;
@@ -115,6 +107,9 @@ extern "C" int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t h
   if (status != VGO_OK) return status;
   VGO_REQUIRE(bytes, "cached_attn: null pointer");
   *bytes = 0;
+  if (cache->batch == 0 || n_query == 0) return VGO_OK;
+  const Plan p = plan_of(cache, heads, n_query);
+  *bytes = p.sums + p.ends;
   return VGO_OK;
 }
 
@@ -131,23 +126,32 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
   VGO_REQUIRE(lengths, "cached_attn: null lengths");
   VGO_REQUIRE(rows_fit(q, q_stride, dtype) && rows_fit(out, out_stride, dtype),
               "cached_attn: q and out must be 16-byte aligned, with strides of whole 16 bytes");
+  const Plan p = plan_of(cache, heads, n_query);
+  VGO_REQUIRE(p.pieces < kMostGroups / (p.tiles * cache->kv_heads) && cache->batch < kMostGroups * 8 / heads / n_query,
+              "cached_attn: too many rows");  // (the join: four rows a work-group of 256)
+  if (p.sums > 0 && (!workspace || workspace_bytes < p.sums + p.ends || !aligned(workspace, 16)))
+    return fail(VGO_EWORKSPACE, "cached_attn: workspace of " + std::to_string(p.sums + p.ends) + " bytes needed");
   Attend a{};
   a.pages = pages_of(cache);
-  a.q = q, a.out = out, a.lengths = lengths, a.counts = counts, a.n_query = n_query;
+  a.q = q, a.out = out, a.lengths = lengths, a.counts = counts, a.batch = cache->batch;
+  a.sums = static_cast<float*>(workspace), a.ends = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.sums);
   for (int i = 0; i < 3; ++i) a.q_stride[i] = q_stride[i], a.out_stride[i] = out_stride[i];
-  a.heads = static_cast<int>(heads), a.causal = causal, a.scale = scale;
-  VGO_REQUIRE(cache->batch < ((int64_t{1} << 32) / 64) / heads / n_query, "cached_attn: too many rows");
-  a.rows = cache->batch * heads * n_query;
-  const unsigned grid = static_cast<unsigned>(a.rows);
+  a.n_query = static_cast<int32_t>(n_query), a.heads = static_cast<int32_t>(heads);
+  a.group = static_cast<int32_t>(heads / cache->kv_heads);
+  a.tiles = static_cast<int32_t>(p.tiles), a.tile_rows = p.tile_rows, a.slots = p.slots, a.least = p.least;
+  a.causal = causal != 0, a.scale = scale * 1.4426950408889634f;
   const hipStream_t s = as_stream(stream);
+  const int run = launch_few(a, p.pieces, static_cast<int>(cache->head_dim), dtype, s);
+  if (run != VGO_OK || p.slots == 0) return run;
+  const unsigned grid = static_cast<unsigned>((cache->batch * heads * n_query + 3) / 4);
   if (cache->head_dim == 64) {
-    if (dtype == VGO_BF16) attend_kernel<bf16_t, 64><<<grid, 64, 0, s>>>(a);
-    else if (dtype == VGO_F16) attend_kernel<f16_t, 64><<<grid, 64, 0, s>>>(a);
-    else attend_kernel<float, 64><<<grid, 64, 0, s>>>(a);
+    if (dtype == VGO_BF16) merge_kernel<bf16_t, 64><<<grid, 256, 0, s>>>(a);
+    else if (dtype == VGO_F16) merge_kernel<f16_t, 64><<<grid, 256, 0, s>>>(a);
+    else merge_kernel<float, 64><<<grid, 256, 0, s>>>(a);
   } else {
-    if (dtype == VGO_BF16) attend_kernel<bf16_t, 128><<<grid, 64, 0, s>>>(a);
-    else if (dtype == VGO_F16) attend_kernel<f16_t, 128><<<grid, 64, 0, s>>>(a);
-    else attend_kernel<float, 128><<<grid, 64, 0, s>>>(a);
+    if (dtype == VGO_BF16) merge_kernel<bf16_t, 128><<<grid, 256, 0, s>>>(a);
+    else if (dtype == VGO_F16) merge_kernel<f16_t, 128><<<grid, 256, 0, s>>>(a);
+    else merge_kernel<float, 128><<<grid, 256, 0, s>>>(a);
   }
   return check_launch("cached_attn");
 }

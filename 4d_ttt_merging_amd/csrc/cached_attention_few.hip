@@ -1,0 +1,277 @@
+// Attention over the paged cache for few queries (decoding steps): up to 64 rows beside a key head.
+//
+// Bound by the cache's bytes, 17/16 D a token and key head, which are read once; the rest is to keep the vector units
+// out of the way (a conversion makes two numbers of a byte, and a token of 64 channels needs 64 of them).  A wave takes blocks of
+// 32 tokens on its own, the next one's codes on their way meanwhile:
+//   scores^T = K Q^T, two 16 x 16 tiles; row m of tile i holds token 8 (m / 4) + 4 i + m % 4, so that the
+//     lane that gets rows 4 g .. 4 g + 3 of both has tokens 8 g .. 8 g + 7 -- as the next product's operand wants them
+//   out^T += V^T P^T; a lane has converted two channels of eight tokens, operands of two tiles
+// Maxima are kept in common by the wave and moved only where a score exceeds them by 2^8; sums stay in their lanes.
+// Eight waves share a piece of a sequence and join their sums in LDS.
+#include "cached_attention.h"
+
+namespace vgo {
+namespace paged {
+namespace {
+
+constexpr int kWaves = 8;
+constexpr float kLazy = 8.0f;
+
+// What a lane reads of a block of 32 tokens.
+template <int D>
+struct Codes {
+  uint2 k[2][D / 64], v[D / 32], vs[D / 32];
+  uint32_t ks[2];
+};
+
+template <int D>
+__device__ __forceinline__ void read_codes(Codes<D>& c, const uint8_t* block, int lane) {
+  using L = Layout<D>;
+  const int m = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int token = 8 * (m >> 2) + 4 * i + (m & 3);
+    const uint8_t* from = block + token * L::kKeyBytes + g * (D / 8);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) c.k[i][e] = reinterpret_cast<const uint2*>(from)[e];
+    c.ks[i] = block[L::kKeyScales + token * L::kParts + g * L::kParts / 4];
+  }
+#pragma unroll
+  for (int u = 0; u < D / 32; ++u) {
+    c.v[u] = *reinterpret_cast<const uint2*>(block + L::kValues + g * L::kGroup + (16 * u + m) * 8);
+    c.vs[u] = *reinterpret_cast<const uint2*>(block + L::kValueScales + g * L::kScaleGroup + 8 * u);
+  }
+}
+
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
+  using L = Layout<D>;
+  constexpr int kQ = Terms<T>::kQuery, kP = Terms<T>::kWeight;
+  constexpr int kSteps = D / 32;
+  __shared__ float joined[kWaves][16][D + 4];
+  __shared__ float tops[kWaves][16], totals[kWaves][16];
+  const int lane = lane_id(), m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kv = a.pages.kv_heads;
+  const int hk = blockIdx.x % kv;
+  const int rest = blockIdx.x / kv;
+  const int tile = rest % a.tiles;
+  const int64_t x = rest / a.tiles;
+  const Piece piece = piece_of(a, x);
+  if (piece.b < 0) return;
+  const int64_t b = piece.b;
+  const int count = count_of(a, b);
+  const int row0 = tile * a.tile_rows, rows = a.n_query * a.group;
+  // Places of the tile's first and last real query, and the first token that none of its rows sees.
+  const int place0 = a.lengths[b] - count;
+  const int last = min(row0 + a.tile_rows, count * a.group) - 1;
+  const int stop = last < row0 ? 0 : a.causal ? max(0, min(piece.length, place0 + last / a.group + 1)) : piece.length;
+  const int end = min(piece.end, stop);
+  if (!piece.whole && piece.begin > 0 && piece.begin >= stop) return;  // (merge_kernel does not ask for it)
+
+  // Queries: row m of each tile, channels 8 s .. of this lane's D / 4.
+  bf16x8 q[NT][kSteps][kQ];
+  int place[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = row0 + 16 * nt + m, token = row / a.group;
+    const bool real = row < count * a.group;
+    place[nt] = !real ? -1 : a.causal ? place0 + token : INT32_MAX;
+    const T* from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (hk * a.group + row % a.group) * a.q_stride[1] +
+                    token * a.q_stride[2] + g * (D / 4);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      float v[8] = {};
+      if (real) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x4 four = load4(from + 8 * s + 4 * e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bf16_t t[kQ];
+        split<kQ>(v[i], t);
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) q[nt][s][n][i] = t[n];
+      }
+    }
+  }
+  f32x4 acc[NT][D / 16] = {};
+  float top[NT], total[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) top[nt] = -INFINITY, total[nt] = 0.0f;
+
+  const auto base_of = [&](int block) -> const uint8_t* {
+    const int64_t t = static_cast<int64_t>(block) * kBlock;
+    const int page = t < end ? page_of(a.pages, b, t) : -1;
+    return page < 0 ? nullptr : a.pages.data + block_of<D>(a.pages, page, hk, t);
+  };
+  const int first = piece.begin / kBlock, blocks = (end + kBlock - 1) / kBlock;
+  Codes<D> codes, ahead;
+  int block = first + wave;
+  const uint8_t* at = base_of(block);
+  if (at) read_codes(codes, at, lane);
+  const uint8_t* next = base_of(block + kWaves);
+  for (; block < blocks; block += kWaves) {
+    if (next) read_codes(ahead, next, lane);
+    const uint8_t* after = base_of(block + 2 * kWaves);
+    if (at) {
+      const int t0 = block * kBlock;
+      const bool inside = t0 + kBlock <= piece.length;
+      float mass[8];
+      if (a.pages.mass) {
+        const int64_t page = page_of(a.pages, b, t0);
+        const float* from = a.pages.mass + (page << a.pages.shift) + (t0 & ((1 << a.pages.shift) - 1)) + 8 * g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mass[i] = from[i] * 1.4426950408889634f;
+      }
+      bf16x8 keys[2][kSteps];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float scale = scale_of<0>(codes.ks[i]);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+          keys[i][s] = key_operand(s % 2 ? codes.k[i][s / 2].y : codes.k[i][s / 2].x, scale);
+      }
+      bf16x8 weights[NT][kP];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x4 c = {};
+#pragma unroll
+          for (int n = kQ - 1; n >= 0; --n)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[i][s], q[nt][s][n], c, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[4 * i + e] = c[e] * a.scale;
+        }
+        if (a.pages.mass) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] += mass[i];
+        }
+        if (a.causal || !inside) {
+          const int most = min(place[nt], piece.length - 1) - t0 - 8 * g;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] = i <= most ? z[i] : -INFINITY;
+        }
+        float local = z[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
+        if (__any(local > top[nt] + kLazy)) {
+          local = fmaxf(local, __shfl_xor(local, 16));
+          local = half_max(local);
+          const float to = fmaxf(top[nt], local);
+          const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[nt] - to);
+          top[nt] = to;
+          total[nt] *= shrink;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][c][e] *= shrink;
+        }
+        const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = __builtin_amdgcn_exp2f(z[i] - from);
+          total[nt] += p;
+          bf16_t t[kP];
+          split<kP>(p, t);
+#pragma unroll
+          for (int n = 0; n < kP; ++n) weights[nt][n][i] = t[n];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < D / 32; ++u) {
+        bf16x8 even, odd;
+        value_operands(codes.v[u], inside ? codes.vs[u] : kept_scales(codes.vs[u], piece.length - t0 - 8 * g), even, odd);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int n = kP - 1; n >= 0; --n) {
+            acc[nt][2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, weights[nt][n], acc[nt][2 * u], 0, 0, 0);
+            acc[nt][2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, weights[nt][n], acc[nt][2 * u + 1], 0, 0, 0);
+          }
+      }
+    }
+    codes = ahead;
+    at = next, next = after;
+  }
+
+  // The waves' sums, 16 rows at a time.
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    total[nt] += __shfl_xor(total[nt], 16);
+    total[nt] = half_sum(total[nt]);
+    if (nt > 0) __syncthreads();
+    if (g == 0) tops[wave][m] = top[nt], totals[wave][m] = total[nt];
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      const f32x4 e = acc[nt][2 * u], o = acc[nt][2 * u + 1];
+      f32x4* to = reinterpret_cast<f32x4*>(&joined[wave][m][32 * u + 8 * g]);
+      to[0] = f32x4{e[0], o[0], e[1], o[1]};
+      to[1] = f32x4{e[2], o[2], e[3], o[3]};
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * D / 4; i += kWaves * 64) {
+      const int r = i / (D / 4), c = i % (D / 4) * 4;
+      const int row = row0 + 16 * nt + r;
+      if (row >= rows) continue;
+      float most = tops[0][r];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) most = fmaxf(most, tops[w][r]);
+      const float from = most == -INFINITY ? 0.0f : most;
+      float sum = 0.0f;
+      f32x4 v = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float share = __builtin_amdgcn_exp2f(tops[w][r] - from);
+        const f32x4 part = *reinterpret_cast<const f32x4*>(&joined[w][r][c]);
+        sum = fmaf(totals[w][r], share, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
+      }
+      if (piece.whole) {
+        const bool none = row >= count * a.group || most == -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
+        store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
+                   row / a.group * a.out_stride[2] + c, v);
+      } else {
+        const int64_t to = ((x * kv + hk) * a.tiles + tile) * a.tile_rows + 16 * nt + r;
+        store4(a.sums + to * D + c, v);
+        if (c == 0) a.ends[to] = {most, sum};
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+int launch(const Attend& a, int64_t pieces, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(pieces * a.tiles * a.pages.kv_heads);
+  if (a.tile_rows == 16) few_kernel<T, D, 1><<<grid, kWaves * 64, 0, s>>>(a);
+  else few_kernel<T, D, 2><<<grid, kWaves * 64, 0, s>>>(a);
+  return check_launch("cached_attn");
+}
+
+}  // namespace
+
+int few_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
+
+int launch_few(const Attend& a, int64_t pieces, int head_dim, int dtype, hipStream_t s) {
+  if (head_dim == 64) {
+    if (dtype == VGO_BF16) return launch<bf16_t, 64>(a, pieces, s);
+    if (dtype == VGO_F16) return launch<f16_t, 64>(a, pieces, s);
+    return launch<float, 64>(a, pieces, s);
+  }
+  if (dtype == VGO_BF16) return launch<bf16_t, 128>(a, pieces, s);
+  if (dtype == VGO_F16) return launch<f16_t, 128>(a, pieces, s);
+  return launch<float, 128>(a, pieces, s);
+}
+
+}  // namespace paged
+}  // namespace vgo

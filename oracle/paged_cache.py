@@ -113,7 +113,11 @@ def attention(q, pages: Pages, table, lengths, counts=None, *, causal=False, sca
     e_j = u (D + 4) scale sum_d |q_d k_jd| + 4 u (|z_j| + |largest z|), of which the last part are the change to base 2, the
     mass and the distance from the running maximum; p_j by p_j (e_j + 8 u) (exp2 to 4 ulp) and its rounding; sums
     over n keys by (32 + n / 16) u of their magnitudes (32 or fewer products at a time, then one addition per
-    32 keys and per part), in the numerator and in the denominator; and the result by half a step of its type."""
+    32 keys and per part), in the numerator and in the denominator; and the result by half a step of its type.
+    Beside these relative ones, what is below the normal numbers of fp32 and bf16, 2^-126, may be taken as zero: a
+    probability p itself, which loses at most 2^-126, or a bf16 term of it -- the second and third are below p 2^-8 and
+    p 2^-16, so that one is lost only where p < 2^-118 or p < 2^-110, and with it less than p 2^-8 < 2^-126 or
+    p 2^-16 < 2^-126; the sum of the running products likewise, once a key.  Together less than 2^-124 (|v_j| + 1) a key."""
     u, half = 2.0 ** -24, torch.finfo(q.dtype).eps / 2
     p_bits = half if p_bits is None else p_bits
     b, h, n, d = q.shape
@@ -143,14 +147,15 @@ def attention(q, pages: Pages, table, lengths, counts=None, *, causal=False, sca
             p = torch.exp(z - torch.where(top == -math.inf, 0.0, top))
             total = p.sum(1, keepdim=True)
             p = p / torch.where(total == 0, 1.0, total)
-            value = torch.where((p > 0).any(0)[:, None], value, 0.0)
+            value = torch.where(ok.any(0)[:, None] & (z > -math.inf).any(0)[:, None], value, 0.0)
             off = u * (d + 4) * size_z + torch.where(p > 0, 4 * u * (z.abs() + top.abs()), 0.0) + 8 * u
             off = torch.where(p > 0, off, 0.0)
             sums = (32 + seen.numel() / 16) * u
             o = p @ value
             out[i, head, :count] = o
+            tiny = 2.0 ** -124 * (value.abs() + 1.0).sum(0)
             weight = (p * (off + p_bits + sums)) @ value.abs()
-            bound[i, head, :count] = weight + o.abs() * ((p * off).sum(1, keepdim=True) + sums + half) + 2.0 ** -126
+            bound[i, head, :count] = weight + o.abs() * ((p * off).sum(1, keepdim=True) + sums + half) + tiny
             if q.dtype == torch.float16:
                 bound[i, head, :count] += 2.0 ** -25
     return out, bound
