@@ -8,9 +8,9 @@
 // r % group, so that a tile of keys serves them all.
 //
 // Work split over the keys: the host does not know the lengths, so the grid holds `slots` pieces more than sequences, and
-// each work-group cuts the sequences' tokens into pieces of one length (split_of): about slots of
-// them in all, at least one a sequence, whatever the lengths are.  Sequences of one piece are written at once, the
-// others' pieces leave their sums in the workspace for merge_kernel.
+// each work-group cuts the sequences' tokens into pieces of one length, which the grid holds whatever the lengths
+// are.  Tiles of rows that see one piece alone are written at once, the others' pieces leave their sums in the workspace
+// for merge_kernel.
 #pragma once
 
 #include "paged_cache.h"
@@ -29,10 +29,13 @@ struct Attend {
   const int32_t* counts;
   int64_t batch;
   int32_t n_query, heads, group;
+  int32_t first_row, last_row;  // the rows of this launch: from .. to before
   int32_t tiles, tile_rows;   // row tiles of a key head, rows of one
   int32_t slots, least;       // pieces beside one a sequence (0: no splitting), tokens of a piece at least
+  int32_t fold;               // whether all work-groups are there at once
+  int32_t merge_groups;       // work-groups of the join that a sequence has
   int32_t causal;
-  float scale;                // times log2(e)
+  float scale, per_scale;     // times log2(e); 1 / the scale itself
 };
 
 __device__ __forceinline__ int64_t capacity_of(const Attend& a) { return a.pages.width << a.pages.shift; }
@@ -43,40 +46,62 @@ __device__ __forceinline__ int count_of(const Attend& a, int64_t b) {
   return a.counts ? min(max(a.counts[b], 0), a.n_query) : a.n_query;
 }
 
+// (Said to be the wave's, so that what follows from it is scalar: a page looked up by vector loads waits for all that
+// are on their way.)
 __device__ __forceinline__ int64_t wave_sum(int64_t v) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
 }
 
-// Tokens of a piece: a multiple of 64.
-__device__ __forceinline__ int piece_tokens(const Attend& a) {
-  if (a.slots == 0) return INT32_MAX;
-  int64_t sum = 0;
-  for (int64_t b = lane_id(); b < a.batch; b += 64) sum += length_of(a, b);
+__device__ __forceinline__ int pieces_of(int length, int tokens) { return max(1, (length - 1) / tokens + 1); }
+
+// The sequences' pieces, as every work-group reckons them: all lanes of a wave together, the same in each.
+struct Pieces {
+  int mine;    // length of sequence `lane`, of the first 64
+  int tokens;  // of a piece: a multiple of 64
+};
+// The shortest pieces of which no more than `slots` beside one a sequence are needed, or nearly so.
+__device__ __forceinline__ Pieces pieces(const Attend& a) {
+  Pieces p{lane_id() < a.batch ? length_of(a, lane_id()) : 0, INT32_MAX};
+  if (a.slots == 0) return p;
+  int64_t sum = p.mine;
+  for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += length_of(a, b);
   sum = wave_sum(sum);
-  const int64_t each = (sum + a.slots - 1) / a.slots;
-  return static_cast<int>(max((each + 63) / 64 * 64, static_cast<int64_t>(a.least)));
-}
-__device__ __forceinline__ int pieces_of(int length, int tokens) {
-  return tokens == INT32_MAX ? 1 : max(1, (length + tokens - 1) / tokens);
+  const int64_t most = a.slots + a.batch;
+  const auto rounded = [&](int64_t n) {
+    n = max((n + 63) / 64 * 64, static_cast<int64_t>(a.least));
+    return static_cast<int>(min(n, static_cast<int64_t>(INT32_MAX)));
+  };
+  p.tokens = rounded((sum + most - 1) / most);
+  for (int round = 0;; ++round) {
+    int64_t n = lane_id() < a.batch ? pieces_of(p.mine, p.tokens) : 0;
+    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) n += pieces_of(length_of(a, b), p.tokens);
+    n = wave_sum(n);
+    if (n <= most) return p;
+    if (round == 3) break;
+    p.tokens = rounded(p.tokens * n / most + 1);
+  }
+  p.tokens = rounded((sum + a.slots - 1) / a.slots);  // (at most one more a sequence than sum / tokens)
+  return p;
 }
 
 struct Piece {
   int64_t b;           // -1: there is no such piece
   int begin, end;      // its tokens
   int length;          // of the sequence
-  bool whole;          // the only one of its sequence
 };
 
-// Piece x of all sequences' pieces in a row.  All lanes of a wave together; the same in each.
+// Piece x of all sequences' pieces in a row.
 __device__ __forceinline__ Piece piece_of(const Attend& a, int64_t x) {
-  const int tokens = piece_tokens(a);
+  const Pieces all = pieces(a);
   int64_t before = 0;
   for (int64_t b0 = 0; b0 < a.batch; b0 += 64) {
     const int64_t b = b0 + lane_id();
-    const int length = b < a.batch ? length_of(a, b) : 0;
-    const int n = b < a.batch ? pieces_of(length, tokens) : 0;
+    const int length = b0 == 0 ? all.mine : b < a.batch ? length_of(a, b) : 0;
+    const int n = b < a.batch ? pieces_of(length, all.tokens) : 0;
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -86,19 +111,36 @@ __device__ __forceinline__ Piece piece_of(const Attend& a, int64_t x) {
     const uint64_t past = __ballot(x < before + upto);
     if (past != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      const int mine = static_cast<int>(x - before) - (__shfl(upto, at) - __shfl(n, at));
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+      const int mine = of(static_cast<int>(x - before) - (upto - n));
       Piece p;
-      p.b = b0 + __builtin_amdgcn_readfirstlane(at);
-      p.length = __builtin_amdgcn_readfirstlane(__shfl(length, at));
-      const int begin = __builtin_amdgcn_readfirstlane(mine) * (tokens == INT32_MAX ? 0 : tokens);
-      p.begin = begin;
-      p.end = tokens == INT32_MAX ? p.length : min(p.length, begin + min(tokens, INT32_MAX - begin));
-      p.whole = __builtin_amdgcn_readfirstlane(__shfl(n, at)) == 1;
+      p.b = b0 + at;
+      p.length = of(length);
+      p.begin = mine == 0 ? 0 : mine * all.tokens;
+      p.end = min(p.length, p.begin + min(all.tokens, INT32_MAX - p.begin));
       return p;
     }
-    before += __shfl(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  return {-1, 0, 0, 0, true};
+  return {-1, 0, 0, 0};
+}
+
+// Which tile the n-th is: of a causal call the longest first, and, where all run at once, the second half of them from
+// the shortest, so that a CU that got a long one gets a short one (16 heads of 8,192 x 8,192 x 64: FOLDED us).
+__device__ __forceinline__ int tile_at(const Attend& a, int n) {
+  const int half = (a.tiles + 1) / 2;
+  return a.fold && n >= half ? n - half : a.tiles - 1 - n;
+}
+
+// Tokens that any row of the tile at row `row0` sees: from 0 to before this one.  `place0`: where a sequence's first query stands.
+__device__ __forceinline__ int stop_of(const Attend& a, int length, int count, int place0, int row0) {
+  const int last = min(min(row0 + a.tile_rows, a.last_row), count * a.group) - 1;
+  return last < row0 ? 0 : a.causal ? max(0, min(length, place0 + last / a.group + 1)) : length;
+}
+
+// A mass as the kernels take it: a type's lowest value is a number, and with the scales that are allowed it stays one.
+__device__ __forceinline__ float mass_of(float mass) {
+  return mass == -INFINITY ? mass : fminf(fmaxf(mass, -1e30f), 1e30f);
 }
 
 // bf16 terms that a query, and a probability, is split into.
@@ -169,8 +211,17 @@ __device__ __forceinline__ void split(float x, bf16_t (&t)[kTerms]) {
   }
 }
 
+// The two kernels: few rows beside a key head (cached_attention_few.hip), many (cached_attention_many.h, a file a type).
+constexpr int kFewRows = 64;
+int few_tile(int64_t rows);  // rows of a tile
 int launch_few(const Attend& a, int64_t pieces, int head_dim, int dtype, hipStream_t s);
-int few_rows(int64_t rows);  // rows of a tile
+struct ManyShape {
+  int tile_rows, resident;  // rows of a work-group, work-groups that a CU holds
+};
+template <typename T>
+ManyShape many_shape(int head_dim);
+template <typename T>
+int launch_many(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
 
 }  // namespace paged
 }  // namespace vgo

@@ -8,71 +8,123 @@ namespace vgo {
 namespace paged {
 namespace {
 
-// Joins the pieces of a row: a wave a row, D / 64 channels a lane.  Rows of sequences in one piece are written already.
+// Joins the pieces of the rows that have several: D / 4 lanes a row.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(const Attend a) {
-  constexpr int kEach = D / 64;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int rows = a.n_query * a.group, lane = lane_id(), kv = a.pages.kv_heads;
-  const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(at % rows));
-  const int64_t rest = at / rows;
-  const int hk = __builtin_amdgcn_readfirstlane(static_cast<int>(rest % kv));
-  const int64_t b = rest / kv;
-  if (b >= a.batch) return;
-  const int tokens = piece_tokens(a), length = length_of(a, b);
-  const int all = pieces_of(length, tokens);
-  if (all == 1) return;
-  int64_t first = 0;
-  for (int64_t o = lane; o < b; o += 64) first += pieces_of(length_of(a, o), tokens);
+  constexpr int kLanes = D / 4;
+  const int rows = a.last_row - a.first_row, kv = a.pages.kv_heads;
+  const int tiles_of_b = blockIdx.x % a.merge_groups;  // work-groups of a sequence
+  const int64_t b = blockIdx.x / a.merge_groups;
+  const Pieces all = pieces(a);
+  const int tokens = all.tokens, length = b < 64 ? __builtin_amdgcn_readlane(all.mine, static_cast<int>(b)) : length_of(a, b);
+  if (pieces_of(length, tokens) == 1) return;
+  int64_t first = lane_id() < b ? pieces_of(all.mine, tokens) : 0;
+  for (int64_t o = lane_id() + 64; o < b; o += 64) first += pieces_of(length_of(a, o), tokens);
   first = wave_sum(first);
-  const int count = count_of(a, b), tile = row / a.tile_rows;
-  const int last = min((tile + 1) * a.tile_rows, count * a.group) - 1;  // (as the tile's work-groups reckon)
-  const int stop = last < tile * a.tile_rows ? 0
-                   : a.causal ? max(0, min(length, a.lengths[b] - count + last / a.group + 1)) : length;
-  const int n = max(1, (stop + tokens - 1) / tokens);
-  const auto place = [&](int piece) {
-    return (((first + piece) * kv + hk) * a.tiles + tile) * a.tile_rows + row % a.tile_rows;
-  };
+  const int at = tiles_of_b * (256 / kLanes) + threadIdx.x / kLanes, c = threadIdx.x % kLanes * 4;
+  if (at >= rows * kv) return;
+  const int hk = at % kv, of = at / kv, row = a.first_row + of, tile = of / a.tile_rows;
+  const int count = count_of(a, b);
+  const int stop = stop_of(a, length, count, a.lengths[b] - count, a.first_row + tile * a.tile_rows);
+  const int n = (stop + tokens - 1) / tokens;
+  if (n <= 1) return;
+  const int64_t step = static_cast<int64_t>(kv) * a.tiles * a.tile_rows;
+  const int64_t start = first * step + (static_cast<int64_t>(hk) * a.tiles + tile) * a.tile_rows + of % a.tile_rows;
+  // Two passes, of independent loads each: the largest maximum, then the sums by their shares of it.
   float most = -INFINITY;
-  for (int piece = 0; piece < n; ++piece) most = fmaxf(most, a.ends[place(piece)].x);
+#pragma unroll 4
+  for (int piece = 0; piece < n; ++piece) most = fmaxf(most, a.ends[start + piece * step].x);
   const float from = most == -INFINITY ? 0.0f : most;
-  float sum = 0.0f, v[kEach] = {};
+  float sum = 0.0f;
+  f32x4 v = {};
+#pragma unroll 4
   for (int piece = 0; piece < n; ++piece) {
-    const float2 end = a.ends[place(piece)];
+    const int64_t place = start + piece * step;
+    const float2 end = a.ends[place];
+    const f32x4 part = *reinterpret_cast<const f32x4*>(a.sums + place * D + c);
     const float share = __builtin_amdgcn_exp2f(end.x - from);
     sum = fmaf(end.y, share, sum);
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e] = fmaf(a.sums[place(piece) * D + lane + 64 * e], share, v[e]);
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
   }
   const bool none = row >= count * a.group || most == -INFINITY;
-  T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
-           row / a.group * a.out_stride[2];
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) out[lane + 64 * e] = from_f32<T>(none ? 0.0f : v[e] / sum);
+  for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
+  store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
+             row / a.group * a.out_stride[2] + c, v);
 }
 
-// How a call is cut.
-struct Plan {
+template <typename T>
+int merge(const Attend& a, int head_dim, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(a.batch * a.merge_groups);
+  if (head_dim == 64) merge_kernel<T, 64><<<grid, 256, 0, s>>>(a);
+  else merge_kernel<T, 128><<<grid, 256, 0, s>>>(a);
+  return check_launch("cached_attn");
+}
+
+}  // namespace
+
+template <>
+ManyShape many_shape<bf16_t>(int head_dim);
+template <>
+ManyShape many_shape<f16_t>(int head_dim);
+template <>
+ManyShape many_shape<float>(int head_dim);
+template <>
+int launch_many<bf16_t>(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
+template <>
+int launch_many<f16_t>(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
+template <>
+int launch_many<float>(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
+
+namespace {
+
+// How a call's rows are run: up to two launches, the second for the few rows that would be a tile of the first.
+struct Part {
+  bool few;
+  int64_t first_row, last_row;
   int tile_rows, slots, least;
+  bool fold;
   int64_t tiles, pieces;
   size_t sums, ends;  // bytes of the workspace
 };
-Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query) {
-  Plan p{};
-  const int64_t rows = n_query * (heads / c->kv_heads), capacity = c->table_width * c->page_size;
-  p.tile_rows = few_rows(rows);
+struct Plan {
+  int parts;
+  Part part[2];
+  size_t bytes() const { return part[0].sums + part[0].ends + (parts > 1 ? part[1].sums + part[1].ends : 0); }
+};
+Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool few, int causal, const ManyShape& shape) {
+  Part p{};
+  const int64_t rows = last_row - first_row, capacity = c->table_width * c->page_size;
+  p.few = few, p.first_row = first_row, p.last_row = last_row;
+  p.tile_rows = few ? few_tile(rows) : shape.tile_rows;
+  p.least = few ? 512 : 256;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-  p.least = 512;
-  const int64_t groups = 2 * device_cus(), beside = c->kv_heads * p.tiles;
-  const int64_t slots = groups / beside - c->batch;
+  // As many work-groups as the chip holds at once; of causal calls that leave room, whose tiles differ, twice as many.
+  const int64_t held = static_cast<int64_t>(few ? 2 : shape.resident) * device_cus(), beside = c->kv_heads * p.tiles;
+  const bool uneven = causal && !few;
+  const int64_t slots = (uneven && c->batch * beside <= held / 2 ? 2 * held : held) / beside - c->batch;
+  p.fold = uneven && c->batch * beside <= held;
   // (no more pieces than the tables could hold)
   p.slots = capacity <= p.least ? 0 : static_cast<int>(std::max<int64_t>(0, std::min(slots, c->batch * ((capacity - 1) / p.least))));
   p.pieces = c->batch + p.slots;
   if (p.slots > 0) {
     const size_t parts = static_cast<size_t>(p.pieces) * beside * p.tile_rows;
     p.sums = parts * c->head_dim * sizeof(float);
-    p.ends = parts * sizeof(float2);
+    p.ends = (parts * sizeof(float2) + 15) / 16 * 16;
   }
+  return p;
+}
+Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, int causal, int dtype) {
+  Plan p{};
+  const int64_t rows = n_query * (heads / c->kv_heads);
+  const int dim = static_cast<int>(c->head_dim);
+  const ManyShape shape = dtype == VGO_BF16 ? many_shape<bf16_t>(dim) : dtype == VGO_F16 ? many_shape<f16_t>(dim) : many_shape<float>(dim);
+  const int64_t over = rows % shape.tile_rows;
+  // Rows of the large tiles.
+  const int64_t split = rows <= kFewRows ? 0 : over <= kFewRows && rows >= 4 * shape.tile_rows ? rows - over : rows;
+  if (split > 0) p.part[p.parts++] = part_of(c, 0, split, false, causal, shape);
+  if (split < rows) p.part[p.parts++] = part_of(c, split, rows, true, causal, shape);
   return p;
 }
 
@@ -84,8 +136,7 @@ int check_attend(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, i
   VGO_REQUIRE(heads % cache->kv_heads == 0, "cached_attn: heads must be a multiple of the key heads");
   return VGO_OK;
 }
-// A grid's threads are counted in 32 bits; work-groups of 512.
-constexpr int64_t kMostGroups = (int64_t{1} << 32) / 512;
+constexpr int64_t kMostThreads = int64_t{1} << 32;
 
 bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
   const int64_t size = dtype == VGO_F32 ? 4 : 2;
@@ -99,8 +150,8 @@ bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
 }  // namespace paged
 }  // namespace vgo
 
-extern "C" int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int dtype,
-                                         size_t* bytes) {
+extern "C" int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int causal,
+                                         int dtype, size_t* bytes) {
   using namespace vgo;
   using namespace vgo::paged;
   const int status = check_attend(cache, heads, n_query, dtype);
@@ -108,8 +159,8 @@ extern "C" int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t h
   VGO_REQUIRE(bytes, "cached_attn: null pointer");
   *bytes = 0;
   if (cache->batch == 0 || n_query == 0) return VGO_OK;
-  const Plan p = plan_of(cache, heads, n_query);
-  *bytes = p.sums + p.ends;
+  const Plan p = plan_of(cache, heads, n_query, causal, dtype);
+  *bytes = p.bytes();
   return VGO_OK;
 }
 
@@ -121,37 +172,47 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
   using namespace vgo::paged;
   const int status = check_attend(cache, heads, n_query, dtype);
   if (status != VGO_OK) return status;
-  VGO_REQUIRE(scale > 0.0f && scale < INFINITY, "cached_attn: the scale must be positive and finite");
+  VGO_REQUIRE(scale >= 1e-8f && scale <= 1e8f, "cached_attn: the scale must be from 1e-8 to 1e8");
   if (cache->batch == 0 || n_query == 0) return VGO_OK;
   VGO_REQUIRE(lengths, "cached_attn: null lengths");
   VGO_REQUIRE(rows_fit(q, q_stride, dtype) && rows_fit(out, out_stride, dtype),
               "cached_attn: q and out must be 16-byte aligned, with strides of whole 16 bytes");
-  const Plan p = plan_of(cache, heads, n_query);
-  VGO_REQUIRE(p.pieces < kMostGroups / (p.tiles * cache->kv_heads) && cache->batch < kMostGroups * 8 / heads / n_query,
-              "cached_attn: too many rows");  // (the join: four rows a work-group of 256)
-  if (p.sums > 0 && (!workspace || workspace_bytes < p.sums + p.ends || !aligned(workspace, 16)))
-    return fail(VGO_EWORKSPACE, "cached_attn: workspace of " + std::to_string(p.sums + p.ends) + " bytes needed");
+  // (a grid's threads are counted in 32 bits; rows and their places among a launch's in 31)
+  VGO_REQUIRE(cache->batch < kMostThreads / heads / n_query / 32, "cached_attn: too many rows");
+  const Plan p = plan_of(cache, heads, n_query, causal, dtype);
+  for (int i = 0; i < p.parts; ++i)
+    VGO_REQUIRE(p.part[i].pieces < kMostThreads / 512 / (p.part[i].tiles * cache->kv_heads), "cached_attn: too many rows");
+  if (p.bytes() > 0 && (!workspace || workspace_bytes < p.bytes() || !aligned(workspace, 16)))
+    return fail(VGO_EWORKSPACE, "cached_attn: workspace of " + std::to_string(p.bytes()) + " bytes needed");
   Attend a{};
   a.pages = pages_of(cache);
   a.q = q, a.out = out, a.lengths = lengths, a.counts = counts, a.batch = cache->batch;
-  a.sums = static_cast<float*>(workspace), a.ends = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.sums);
   for (int i = 0; i < 3; ++i) a.q_stride[i] = q_stride[i], a.out_stride[i] = out_stride[i];
   a.n_query = static_cast<int32_t>(n_query), a.heads = static_cast<int32_t>(heads);
   a.group = static_cast<int32_t>(heads / cache->kv_heads);
-  a.tiles = static_cast<int32_t>(p.tiles), a.tile_rows = p.tile_rows, a.slots = p.slots, a.least = p.least;
-  a.causal = causal != 0, a.scale = scale * 1.4426950408889634f;
+  a.causal = causal != 0, a.scale = scale * 1.4426950408889634f, a.per_scale = 1.0f / scale;
   const hipStream_t s = as_stream(stream);
-  const int run = launch_few(a, p.pieces, static_cast<int>(cache->head_dim), dtype, s);
-  if (run != VGO_OK || p.slots == 0) return run;
-  const unsigned grid = static_cast<unsigned>((cache->batch * heads * n_query + 3) / 4);
-  if (cache->head_dim == 64) {
-    if (dtype == VGO_BF16) merge_kernel<bf16_t, 64><<<grid, 256, 0, s>>>(a);
-    else if (dtype == VGO_F16) merge_kernel<f16_t, 64><<<grid, 256, 0, s>>>(a);
-    else merge_kernel<float, 64><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (dtype == VGO_BF16) merge_kernel<bf16_t, 128><<<grid, 256, 0, s>>>(a);
-    else if (dtype == VGO_F16) merge_kernel<f16_t, 128><<<grid, 256, 0, s>>>(a);
-    else merge_kernel<float, 128><<<grid, 256, 0, s>>>(a);
+  const int dim = static_cast<int>(cache->head_dim);
+  char* ws = static_cast<char*>(workspace);
+  for (int i = 0; i < p.parts; ++i) {
+    const Part& part = p.part[i];
+    a.first_row = static_cast<int32_t>(part.first_row), a.last_row = static_cast<int32_t>(part.last_row);
+    a.tiles = static_cast<int32_t>(part.tiles), a.tile_rows = part.tile_rows, a.slots = part.slots, a.least = part.least;
+    a.fold = part.fold;
+    a.sums = reinterpret_cast<float*>(ws), a.ends = reinterpret_cast<float2*>(ws + part.sums);
+    ws += part.sums + part.ends;
+    int run = part.few            ? launch_few(a, part.pieces, dim, dtype, s)
+              : dtype == VGO_BF16 ? launch_many<bf16_t>(a, part.pieces, dim, s)
+              : dtype == VGO_F16  ? launch_many<f16_t>(a, part.pieces, dim, s)
+                                  : launch_many<float>(a, part.pieces, dim, s);
+    if (run == VGO_OK && part.slots > 0) {
+      const int64_t each = 256 / (dim / 4);
+      a.merge_groups = static_cast<int32_t>(((part.last_row - part.first_row) * cache->kv_heads + each - 1) / each);
+      run = dtype == VGO_BF16  ? merge<bf16_t>(a, dim, s)
+            : dtype == VGO_F16 ? merge<f16_t>(a, dim, s)
+                               : merge<float>(a, dim, s);
+    }
+    if (run != VGO_OK) return run;
   }
-  return check_launch("cached_attn");
+  return VGO_OK;
 }

@@ -18,14 +18,15 @@ constexpr int kWaves = 8;
 constexpr float kLazy = 8.0f;
 
 // What a lane reads of a block of 32 tokens.
-template <int D>
+template <int D, bool kMass>
 struct Codes {
   uint2 k[2][D / 64], v[D / 32], vs[D / 32];
   uint32_t ks[2];
+  f32x4 mass[kMass ? 2 : 1];
 };
 
-template <int D>
-__device__ __forceinline__ void read_codes(Codes<D>& c, const uint8_t* block, int lane) {
+template <int D, bool kMass>
+__device__ __forceinline__ void read_codes(Codes<D, kMass>& c, const uint8_t* block, const float* mass, int lane) {
   using L = Layout<D>;
   const int m = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -41,9 +42,27 @@ __device__ __forceinline__ void read_codes(Codes<D>& c, const uint8_t* block, in
     c.v[u] = *reinterpret_cast<const uint2*>(block + L::kValues + g * L::kGroup + (16 * u + m) * 8);
     c.vs[u] = *reinterpret_cast<const uint2*>(block + L::kValueScales + g * L::kScaleGroup + 8 * u);
   }
+  if constexpr (kMass) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c.mass[i] = *reinterpret_cast<const f32x4*>(mass + 8 * g + 4 * i);
+  }
 }
 
-template <typename T, int D, int NT>
+// Two numbers as kTerms bf16 terms each, in pairs.
+template <int kTerms>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[kTerms]) {
+#pragma unroll
+  for (int i = 0; i < kTerms; ++i) {
+    const bf16x2 pair = {static_cast<bf16_t>(x), static_cast<bf16_t>(y)};
+    t[i] = __builtin_bit_cast(uint32_t, pair);
+    if (i + 1 < kTerms) {
+      x -= __uint_as_float(t[i] << 16);
+      y -= __uint_as_float(t[i] & 0xffff0000u);
+    }
+  }
+}
+
+template <typename T, int D, int NT, bool kMass>
 __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   using L = Layout<D>;
   constexpr int kQ = Terms<T>::kQuery, kP = Terms<T>::kWeight;
@@ -55,19 +74,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   const int kv = a.pages.kv_heads;
   const int hk = blockIdx.x % kv;
   const int rest = blockIdx.x / kv;
-  const int tile = rest % a.tiles;
+  const int tile = tile_at(a, rest % a.tiles);
   const int64_t x = rest / a.tiles;
   const Piece piece = piece_of(a, x);
   if (piece.b < 0) return;
   const int64_t b = piece.b;
   const int count = count_of(a, b);
-  const int row0 = tile * a.tile_rows, rows = a.n_query * a.group;
-  // Places of the tile's first and last real query, and the first token that none of its rows sees.
-  const int place0 = a.lengths[b] - count;
-  const int last = min(row0 + a.tile_rows, count * a.group) - 1;
-  const int stop = last < row0 ? 0 : a.causal ? max(0, min(piece.length, place0 + last / a.group + 1)) : piece.length;
+  const int row0 = a.first_row + tile * a.tile_rows;
+  const int place0 = a.lengths[b] - count, stop = stop_of(a, piece.length, count, place0, row0);
   const int end = min(piece.end, stop);
-  if (!piece.whole && piece.begin > 0 && piece.begin >= stop) return;  // (merge_kernel does not ask for it)
+  if (piece.begin > 0 && piece.begin >= stop) return;  // (merge_kernel does not ask for it)
+  const bool whole = piece.begin == 0 && stop <= piece.end;
 
   // Queries: row m of each tile, channels 8 s .. of this lane's D / 4.
   bf16x8 q[NT][kSteps][kQ];
@@ -104,102 +121,113 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) top[nt] = -INFINITY, total[nt] = 0.0f;
 
-  const auto base_of = [&](int block) -> const uint8_t* {
+  // A ring of blocks on their way.  Reads are not conditional, so that the compiler knows how many are outstanding: what has
+  // no page, or lies past the end, reads the start of the cache instead and is left out.
+  constexpr int kRing = 3;
+  Codes<D, kMass> ring[kRing];
+  bool there[kRing];
+  const int first = piece.begin / kBlock, blocks = a.pages.pages > 0 ? (end + kBlock - 1) / kBlock : 0;
+  const auto page_at = [&](int block) {
     const int64_t t = static_cast<int64_t>(block) * kBlock;
-    const int page = t < end ? page_of(a.pages, b, t) : -1;
-    return page < 0 ? nullptr : a.pages.data + block_of<D>(a.pages, page, hk, t);
+    return block < blocks ? page_of(a.pages, b, t) : -1;
   };
-  const int first = piece.begin / kBlock, blocks = (end + kBlock - 1) / kBlock;
-  Codes<D> codes, ahead;
-  int block = first + wave;
-  const uint8_t* at = base_of(block);
-  if (at) read_codes(codes, at, lane);
-  const uint8_t* next = base_of(block + kWaves);
-  for (; block < blocks; block += kWaves) {
-    if (next) read_codes(ahead, next, lane);
-    const uint8_t* after = base_of(block + 2 * kWaves);
-    if (at) {
-      const int t0 = block * kBlock;
-      const bool inside = t0 + kBlock <= piece.length;
-      float mass[8];
-      if (a.pages.mass) {
-        const int64_t page = page_of(a.pages, b, t0);
-        const float* from = a.pages.mass + (page << a.pages.shift) + (t0 & ((1 << a.pages.shift) - 1)) + 8 * g;
+  const auto read = [&](int slot, int block, int page) {
+    const int64_t t = static_cast<int64_t>(block) * kBlock;
+    there[slot] = page >= 0;
+    const uint8_t* from = a.pages.data + (page < 0 ? 0 : block_of<D>(a.pages, page, hk, t));
+    const float* mass = !kMass || page < 0 ? a.pages.mass
+                                           : a.pages.mass + (static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1));
+    read_codes(ring[slot], from, mass, lane);
+  };
+  const auto compute = [&](const Codes<D, kMass>& codes, int block) {
+    const int t0 = block * kBlock;
+    const bool inside = t0 + kBlock <= piece.length;
+    bf16x8 keys[2][kSteps];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mass[i] = from[i] * 1.4426950408889634f;
-      }
-      bf16x8 keys[2][kSteps];
+    for (int i = 0; i < 2; ++i) {
+      const float scale = scale_of<0>(codes.ks[i]);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) keys[i][s] = key_operand(s % 2 ? codes.k[i][s / 2].y : codes.k[i][s / 2].x, scale);
+    }
+    Operand weights[NT][kP];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float z[8];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float scale = scale_of<0>(codes.ks[i]);
+        f32x4 c = {};
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-          keys[i][s] = key_operand(s % 2 ? codes.k[i][s / 2].y : codes.k[i][s / 2].x, scale);
+        for (int n = kQ - 1; n >= 0; --n)
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[i][s], q[nt][s][n], c, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[4 * i + e] = c[e];
       }
-      bf16x8 weights[NT][kP];
+      if constexpr (kMass) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float z[8];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f32x4 c = {};
-#pragma unroll
-          for (int n = kQ - 1; n >= 0; --n)
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[i][s], q[nt][s][n], c, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) z[4 * i + e] = c[e] * a.scale;
-        }
-        if (a.pages.mass) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) z[i] += mass[i];
-        }
-        if (a.causal || !inside) {
-          const int most = min(place[nt], piece.length - 1) - t0 - 8 * g;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) z[i] = i <= most ? z[i] : -INFINITY;
-        }
-        float local = z[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
-        if (__any(local > top[nt] + kLazy)) {
-          local = fmaxf(local, __shfl_xor(local, 16));
-          local = half_max(local);
-          const float to = fmaxf(top[nt], local);
-          const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[nt] - to);
-          top[nt] = to;
-          total[nt] *= shrink;
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][c][e] *= shrink;
-        }
-        const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(z[i] - from);
-          total[nt] += p;
-          bf16_t t[kP];
-          split<kP>(p, t);
-#pragma unroll
-          for (int n = 0; n < kP; ++n) weights[nt][n][i] = t[n];
-        }
+        for (int i = 0; i < 8; ++i) z[i] = fmaf(z[i], a.scale, mass_of(codes.mass[i / 4][i % 4]) * 1.4426950408889634f);
       }
+      const float scale = kMass ? 1.0f : a.scale;  // still to be applied
+      if (a.causal || !inside) {
+        const int most = min(place[nt], piece.length - 1) - t0 - 8 * g;
 #pragma unroll
-      for (int u = 0; u < D / 32; ++u) {
-        bf16x8 even, odd;
-        value_operands(codes.v[u], inside ? codes.vs[u] : kept_scales(codes.vs[u], piece.length - t0 - 8 * g), even, odd);
+        for (int i = 0; i < 8; ++i) z[i] = i <= most ? z[i] : -INFINITY;
+      }
+      float local = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+      local *= scale;
+      if (__any(local > top[nt] + kLazy)) {
+        local = fmaxf(local, __shfl_xor(local, 16));
+        local = half_max(local);
+        const float to = fmaxf(top[nt], local);
+        const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[nt] - to);
+        top[nt] = to;
+        total[nt] *= shrink;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-          for (int n = kP - 1; n >= 0; --n) {
-            acc[nt][2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, weights[nt][n], acc[nt][2 * u], 0, 0, 0);
-            acc[nt][2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, weights[nt][n], acc[nt][2 * u + 1], 0, 0, 0);
-          }
+          for (int e = 0; e < 4; ++e) acc[nt][c][e] *= shrink;
+      }
+      const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(z[2 * i], scale, -from));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(z[2 * i + 1], scale, -from));
+        total[nt] += p0 + p1;
+        uint32_t t[kP];
+        split_pair<kP>(p0, p1, t);
+#pragma unroll
+        for (int n = 0; n < kP; ++n) weights[nt][n].w[i] = t[n];
       }
     }
-    codes = ahead;
-    at = next, next = after;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      uint2 scales = codes.vs[u];
+      if (!inside) scales = kept_scales(scales, piece.length - t0 - 8 * g);
+      bf16x8 even, odd;
+      value_operands(codes.v[u], scales, even, odd);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int n = kP - 1; n >= 0; --n) {
+          acc[nt][2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, weights[nt][n].v, acc[nt][2 * u], 0, 0, 0);
+          acc[nt][2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, weights[nt][n].v, acc[nt][2 * u + 1], 0, 0, 0);
+        }
+    }
+  };
+  int block = first + wave;
+  if (block < blocks) {
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) read(i, block + i * kWaves, page_at(block + i * kWaves));
+    int page = page_at(block + (kRing - 1) * kWaves);
+    while (block < blocks) {
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) {
+        read((i + kRing - 1) % kRing, block + (kRing - 1) * kWaves, page);
+        page = page_at(block + kRing * kWaves);
+        if (there[i]) compute(ring[i], block);
+        block += kWaves;
+      }
+    }
   }
 
   // The waves' sums, 16 rows at a time.
@@ -220,7 +248,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     for (int i = threadIdx.x; i < 16 * D / 4; i += kWaves * 64) {
       const int r = i / (D / 4), c = i % (D / 4) * 4;
       const int row = row0 + 16 * nt + r;
-      if (row >= rows) continue;
+      if (row >= a.last_row) continue;
       float most = tops[0][r];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) most = fmaxf(most, tops[w][r]);
@@ -235,7 +263,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
       }
-      if (piece.whole) {
+      if (whole) {
         const bool none = row >= count * a.group || most == -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
@@ -253,14 +281,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 template <typename T, int D>
 int launch(const Attend& a, int64_t pieces, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(pieces * a.tiles * a.pages.kv_heads);
-  if (a.tile_rows == 16) few_kernel<T, D, 1><<<grid, kWaves * 64, 0, s>>>(a);
-  else few_kernel<T, D, 2><<<grid, kWaves * 64, 0, s>>>(a);
+  const auto run = [&](auto mass) {
+    if (a.tile_rows == 16) few_kernel<T, D, 1, decltype(mass)::value><<<grid, kWaves * 64, 0, s>>>(a);
+    else few_kernel<T, D, 2, decltype(mass)::value><<<grid, kWaves * 64, 0, s>>>(a);
+  };
+  if (a.pages.mass) run(std::true_type());
+  else run(std::false_type());
   return check_launch("cached_attn");
 }
 
 }  // namespace
 
-int few_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
+int few_tile(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
 int launch_few(const Attend& a, int64_t pieces, int head_dim, int dtype, hipStream_t s) {
   if (head_dim == 64) {

@@ -42,11 +42,13 @@ struct Pages {
   int shift;  // log2 of the page size
 };
 
-// Page of token t (not negative) of sequence b, or -1 where the table has none.
+// Page of token t (not negative) of sequence b, or -1 where the table has none.  The table is read as constant memory, by
+// the scalar unit where b and t are the wave's.
 __device__ __forceinline__ int page_of(const Pages& p, int64_t b, int64_t t) {
   const int64_t at = t >> p.shift;
   if (at >= p.width) return -1;
-  const int id = p.table[b * p.width + at];
+  typedef const __attribute__((address_space(4))) int32_t* constant;
+  const int id = reinterpret_cast<constant>(reinterpret_cast<uintptr_t>(p.table))[b * p.width + at];
   return id >= 0 && id < p.pages ? id : -1;
 }
 // The block of a page that holds token t, for one key head.

@@ -114,9 +114,9 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
 
     lengths int32 [B]: tokens of each sequence, those of this call's queries included; counts int32 [B] (default N): how many
     of its queries are real; query i stands at place lengths[b] - counts[b] + i, and with `causal` sees no later one.
-    H is a multiple of the cache's Hk (head h reads key head h // (H // Hk)); scale defaults to 1 / sqrt(D).  Returns
+    H is a multiple of the cache's Hk (head h reads key head h // (H // Hk)); scale (1e-8 to 1e8) defaults to 1 / sqrt(D).  Returns
     [B, H, N, D], token-major in memory where q is; zeros for padding and for queries that attend to nothing (a
-    log mass of -inf, or no page, keeps a token out).
+    log mass of -inf, or no page, keeps a token out; finite masses past 1e30 in size count as that).
 
     Tokens past a length may hold anything; others must be finite where any query of their sequence can see them.  Stored
     numbers enter exactly.  Sums are fp32; probabilities are rounded to the type of q where that is bf16 and
@@ -126,7 +126,5 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     (q,) = _autocast(q)
     if scale is None:
         scale = 1.0 / math.sqrt(cache.head_dim)
-    if not 0.0 < scale < math.inf:
-        raise ValueError("the scale must be positive and finite")
     return torch.ops.vgo.cached_attention(q, cache.data, cache.log_mass, page_table, lengths, counts, bool(causal),
                                           float(scale))
