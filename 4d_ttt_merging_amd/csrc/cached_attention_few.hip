@@ -25,26 +25,42 @@ struct Codes {
   f32x4 mass[kMass ? 2 : 1];
 };
 
+// Where in a block (and, for masses, in a page's) a lane reads: 32-bit offsets, so that a read takes its block's address
+// from scalar registers.
+template <int D>
+struct Offsets {
+  uint32_t k[2], ks[2], v, vs, mass;
+  __device__ __forceinline__ Offsets(int lane) {
+    using L = Layout<D>;
+    const uint32_t m = lane & 15, g = lane >> 4;
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t token = 8 * (m >> 2) + 4 * i + (m & 3);
+      k[i] = token * L::kKeyBytes + g * (D / 8);
+      ks[i] = L::kKeyScales + token * L::kParts + g * L::kParts / 4;
+    }
+    v = L::kValues + g * L::kGroup + m * 8;
+    vs = L::kValueScales + g * L::kScaleGroup;
+    mass = 32 * g;
+  }
+};
+
 template <int D, bool kMass>
-__device__ __forceinline__ void read_codes(Codes<D, kMass>& c, const uint8_t* block, const float* mass, int lane) {
-  using L = Layout<D>;
-  const int m = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void read_codes(Codes<D, kMass>& c, const uint8_t* block, const float* mass, const Offsets<D>& o) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int token = 8 * (m >> 2) + 4 * i + (m & 3);
-    const uint8_t* from = block + token * L::kKeyBytes + g * (D / 8);
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) c.k[i][e] = reinterpret_cast<const uint2*>(from)[e];
-    c.ks[i] = block[L::kKeyScales + token * L::kParts + g * L::kParts / 4];
+    for (int e = 0; e < D / 64; ++e) c.k[i][e] = *reinterpret_cast<const uint2*>(block + o.k[i] + 8 * e);
+    c.ks[i] = block[o.ks[i]];
   }
 #pragma unroll
   for (int u = 0; u < D / 32; ++u) {
-    c.v[u] = *reinterpret_cast<const uint2*>(block + L::kValues + g * L::kGroup + (16 * u + m) * 8);
-    c.vs[u] = *reinterpret_cast<const uint2*>(block + L::kValueScales + g * L::kScaleGroup + 8 * u);
+    c.v[u] = *reinterpret_cast<const uint2*>(block + o.v + 128 * u);
+    c.vs[u] = *reinterpret_cast<const uint2*>(block + o.vs + 8 * u);
   }
   if constexpr (kMass) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) c.mass[i] = *reinterpret_cast<const f32x4*>(mass + 8 * g + 4 * i);
+    for (int i = 0; i < 2; ++i)
+      c.mass[i] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(mass) + o.mass + 16 * i);
   }
 }
 
@@ -55,6 +71,7 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[kTerm
   for (int i = 0; i < kTerms; ++i) {
     const bf16x2 pair = {static_cast<bf16_t>(x), static_cast<bf16_t>(y)};
     t[i] = __builtin_bit_cast(uint32_t, pair);
+    asm("" : "+v"(t[i]));  // (else the first of the pair is converted a second time)
     if (i + 1 < kTerms) {
       x -= __uint_as_float(t[i] << 16);
       y -= __uint_as_float(t[i] & 0xffff0000u);
@@ -124,6 +141,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   // A ring of blocks on their way.  Reads are not conditional, so that the compiler knows how many are outstanding: what has
   // no page, or lies past the end, reads the start of the cache instead and is left out.
   constexpr int kRing = 3;
+  const Offsets<D> offsets(lane);
   Codes<D, kMass> ring[kRing];
   bool there[kRing];
   const int first = piece.begin / kBlock, blocks = a.pages.pages > 0 ? (end + kBlock - 1) / kBlock : 0;
@@ -137,7 +155,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     const uint8_t* from = a.pages.data + (page < 0 ? 0 : block_of<D>(a.pages, page, hk, t));
     const float* mass = !kMass || page < 0 ? a.pages.mass
                                            : a.pages.mass + (static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1));
-    read_codes(ring[slot], from, mass, lane);
+    read_codes(ring[slot], from, mass, offsets);
   };
   const auto compute = [&](const Codes<D, kMass>& codes, int block) {
     const int t0 = block * kBlock;
@@ -173,7 +191,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[i] = i <= most ? z[i] : -INFINITY;
       }
-      float local = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+      float local = z[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
       local *= scale;
       if (__any(local > top[nt] + kLazy)) {
         local = fmaxf(local, __shfl_xor(local, 16));

@@ -58,10 +58,21 @@ __device__ __forceinline__ int64_t block_of(const Pages& p, int64_t page, int he
   return ((page * p.kv_heads + head) * blocks + ((t >> 5) & (blocks - 1))) * Layout<D>::kBytes;
 }
 
-// 2^(byte - 127) of byte kAt of a word; 255 becomes infinity, of which the conversion makes NaN.
+// 2^(byte - 127) of byte kAt of a word; 255 becomes infinity, of which the conversion makes NaN.  One instruction, where
+// the shifts and masks of C++ become two for the outer bytes.
 template <int kAt>
 __device__ __forceinline__ float scale_of(uint32_t word) {
-  return __uint_as_float(((word >> (8 * kAt)) & 0xff) << 23);
+  static_assert(kAt >= 0 && kAt < 4, "four bytes");
+  uint32_t r;
+  if constexpr (kAt == 0)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(word));
+  else if constexpr (kAt == 1)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(word));
+  else if constexpr (kAt == 2)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(word));
+  else
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(word));
+  return __uint_as_float(r);
 }
 
 // Checks of the host, shared by the entry points.
