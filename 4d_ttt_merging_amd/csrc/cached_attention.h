@@ -24,6 +24,7 @@ struct Attend {
   void* out;
   float* sums;   // [piece][key head][row tile][rows of a tile] of D sums of values, then as many (maximum, sum) pairs
   float2* ends;
+  int2* firsts;  // [batch]: a sequence's first piece, tokens of a piece
   int64_t q_stride[3], out_stride[3];
   const int32_t* lengths;
   const int32_t* counts;
@@ -33,7 +34,6 @@ struct Attend {
   int32_t tiles, tile_rows;   // row tiles of a key head, rows of one
   int32_t slots, least;       // pieces beside one a sequence (0: no splitting), tokens of a piece at least
   int32_t fold;               // whether all work-groups are there at once
-  int32_t merge_groups;       // work-groups of the join that a sequence has
   int32_t causal;
   float scale, per_scale;     // times log2(e); 1 / the scale itself
 };
@@ -46,14 +46,25 @@ __device__ __forceinline__ int count_of(const Attend& a, int64_t b) {
   return a.counts ? min(max(a.counts[b], 0), a.n_query) : a.n_query;
 }
 
-// (Said to be the wave's, so that what follows from it is scalar: a page looked up by vector loads waits for all that
-// are on their way.)
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-  return static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+// Reductions over a wave stay in the vector unit (a shuffle through LDS takes a hundred cycles, and a step of a short
+// sequence is little else).  Their results are said to be the wave's, so that what follows from them is scalar: a page
+// looked up by vector loads waits for all that are on their way.
+template <int kCtrl, int kRows = 0xF>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xF, false));
+}
+// Sums over the lanes up to each (row_shr 1, 2, 4, 8 within 16 lanes, then their last lanes' to the rows behind).
+__device__ __forceinline__ uint32_t sums_upto(uint32_t v) {
+  v += moved<0x111>(v);
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<0x142, 0xA>(v);
+  v += moved<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+  return __builtin_amdgcn_readlane(static_cast<int>(sums_upto(v)), 63);
 }
 
 __device__ __forceinline__ int pieces_of(int length, int tokens) { return max(1, (length - 1) / tokens + 1); }
@@ -67,23 +78,27 @@ struct Pieces {
 __device__ __forceinline__ Pieces pieces(const Attend& a) {
   Pieces p{lane_id() < a.batch ? length_of(a, lane_id()) : 0, INT32_MAX};
   if (a.slots == 0) return p;
-  int64_t sum = p.mine;
-  for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += length_of(a, b);
-  sum = wave_sum(sum);
-  const int64_t most = a.slots + a.batch;
-  const auto rounded = [&](int64_t n) {
-    n = max((n + 63) / 64 * 64, static_cast<int64_t>(a.least));
-    return static_cast<int>(min(n, static_cast<int64_t>(INT32_MAX)));
+  const auto over_all = [&](auto of) {  // at most 2^26 a lane, so that 64 of them fit
+    int64_t sum = lane_id() < a.batch ? of(p.mine) : 0;
+    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += of(length_of(a, b));
+    return static_cast<int64_t>(wave_sum(static_cast<uint32_t>(min(sum, int64_t{1} << 25))));
   };
+  const int most = a.slots + static_cast<int>(a.batch);
+  const auto rounded = [&](int64_t units) {  // of 64 tokens
+    return static_cast<int>(min(max(units * 64, static_cast<int64_t>(a.least)), static_cast<int64_t>(INT32_MAX)));
+  };
+  const int64_t sum = over_all([](int length) { return (static_cast<int64_t>(length) + 63) / 64; });
+  // (more than the sums hold: a piece a sequence)
+  if (sum >= int64_t{1} << 25) return p;
   p.tokens = rounded((sum + most - 1) / most);
-  for (int round = 0;; ++round) {
-    int64_t n = lane_id() < a.batch ? pieces_of(p.mine, p.tokens) : 0;
-    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) n += pieces_of(length_of(a, b), p.tokens);
-    n = wave_sum(n);
+  for (int round = 0; round < 3; ++round) {
+    const int tokens = p.tokens;
+    const int64_t n = over_all([&](int length) { return static_cast<int64_t>(pieces_of(length, tokens)); });
     if (n <= most) return p;
-    if (round == 3) break;
-    p.tokens = rounded(p.tokens * n / most + 1);
+    p.tokens = rounded(p.tokens / 64 * n / most + 1);
   }
+  const int tokens = p.tokens;
+  if (over_all([&](int length) { return static_cast<int64_t>(pieces_of(length, tokens)); }) <= most) return p;
   p.tokens = rounded((sum + a.slots - 1) / a.slots);  // (at most one more a sequence than sum / tokens)
   return p;
 }
@@ -92,37 +107,37 @@ struct Piece {
   int64_t b;           // -1: there is no such piece
   int begin, end;      // its tokens
   int length;          // of the sequence
+  int tokens;          // of a piece
 };
 
 // Piece x of all sequences' pieces in a row.
-__device__ __forceinline__ Piece piece_of(const Attend& a, int64_t x) {
+__device__ __forceinline__ Piece piece_of(const Attend& a, int x) {
   const Pieces all = pieces(a);
-  int64_t before = 0;
+  int before = 0;
   for (int64_t b0 = 0; b0 < a.batch; b0 += 64) {
     const int64_t b = b0 + lane_id();
     const int length = b0 == 0 ? all.mine : b < a.batch ? length_of(a, b) : 0;
     const int n = b < a.batch ? pieces_of(length, all.tokens) : 0;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int other = __shfl_up(upto, o);
-      if (lane_id() >= o) upto += other;
-    }
+    const int upto = static_cast<int>(sums_upto(static_cast<uint32_t>(n)));
     const uint64_t past = __ballot(x < before + upto);
     if (past != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
-      const int mine = of(static_cast<int>(x - before) - (upto - n));
+      const int mine = x - before - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
       Piece p;
       p.b = b0 + at;
-      p.length = of(length);
+      p.length = __builtin_amdgcn_readlane(length, at);
       p.begin = mine == 0 ? 0 : mine * all.tokens;
       p.end = min(p.length, p.begin + min(all.tokens, INT32_MAX - p.begin));
+      p.tokens = all.tokens;
       return p;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
-  return {-1, 0, 0, 0};
+  return {-1, 0, 0, 0, 0};
+}
+// What merge_kernel asks of a sequence: its first piece and their length, left by that piece.
+__device__ __forceinline__ void leave(const Attend& a, const Piece& piece, int x, bool one) {
+  if (a.slots > 0 && piece.begin == 0 && one) a.firsts[piece.b] = {x, piece.tokens};
 }
 
 // Which tile the n-th is: of a causal call the longest first, and, where all run at once, the second half of them from

@@ -8,46 +8,63 @@ namespace vgo {
 namespace paged {
 namespace {
 
-// Joins the pieces of the rows that have several: D / 4 lanes a row.
+// Joins the pieces of the rows that have several.  A wave takes a row, D / 4 lanes four channels each of every second
+// (fourth) piece: what they read does not depend on what they have read, so that up to 8 (16) pieces take one trip to memory.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(const Attend a) {
-  constexpr int kLanes = D / 4;
+  constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
   const int rows = a.last_row - a.first_row, kv = a.pages.kv_heads;
-  const int tiles_of_b = blockIdx.x % a.merge_groups;  // work-groups of a sequence
-  const int64_t b = blockIdx.x / a.merge_groups;
-  const Pieces all = pieces(a);
-  const int tokens = all.tokens, length = b < 64 ? __builtin_amdgcn_readlane(all.mine, static_cast<int>(b)) : length_of(a, b);
-  if (pieces_of(length, tokens) == 1) return;
-  int64_t first = lane_id() < b ? pieces_of(all.mine, tokens) : 0;
-  for (int64_t o = lane_id() + 64; o < b; o += 64) first += pieces_of(length_of(a, o), tokens);
-  first = wave_sum(first);
-  const int at = tiles_of_b * (256 / kLanes) + threadIdx.x / kLanes, c = threadIdx.x % kLanes * 4;
-  if (at >= rows * kv) return;
-  const int hk = at % kv, of = at / kv, row = a.first_row + of, tile = of / a.tile_rows;
-  const int count = count_of(a, b);
+  const int64_t task = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6));
+  const int hk = static_cast<int>(task % kv), of = static_cast<int>(task / kv % rows);
+  const int64_t b = task / kv / rows;
+  if (b >= a.batch) return;
+  const int2 first = a.firsts[b];
+  const int length = length_of(a, b), count = count_of(a, b);
+  const int row = a.first_row + of, tile = of / a.tile_rows, tokens = first.y;
   const int stop = stop_of(a, length, count, a.lengths[b] - count, a.first_row + tile * a.tile_rows);
-  const int n = (stop + tokens - 1) / tokens;
-  if (n <= 1) return;
+  const int n = (stop - 1) / tokens + 1;
+  if (stop <= 0 || n <= 1) return;
+  const int group = lane_id() / kLanes, c = lane_id() % kLanes * 4;
   const int64_t step = static_cast<int64_t>(kv) * a.tiles * a.tile_rows;
-  const int64_t start = first * step + (static_cast<int64_t>(hk) * a.tiles + tile) * a.tile_rows + of % a.tile_rows;
-  // Two passes, of independent loads each: the largest maximum, then the sums by their shares of it.
-  float most = -INFINITY;
-#pragma unroll 4
-  for (int piece = 0; piece < n; ++piece) most = fmaxf(most, a.ends[start + piece * step].x);
-  const float from = most == -INFINITY ? 0.0f : most;
-  float sum = 0.0f;
+  const int64_t start = first.x * step + (static_cast<int64_t>(hk) * a.tiles + tile) * a.tile_rows + of % a.tile_rows;
+  float top = -INFINITY, sum = 0.0f;
   f32x4 v = {};
-#pragma unroll 4
-  for (int piece = 0; piece < n; ++piece) {
-    const int64_t place = start + piece * step;
-    const float2 end = a.ends[place];
-    const f32x4 part = *reinterpret_cast<const f32x4*>(a.sums + place * D + c);
-    const float share = __builtin_amdgcn_exp2f(end.x - from);
-    sum = fmaf(end.y, share, sum);
+  for (int piece = group; piece < n; piece += 4 * kGroups) {
+    float2 end[4];
+    f32x4 part[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t place = start + min(piece + i * kGroups, n - 1) * step;
+      end[i] = a.ends[place];
+      part[i] = *reinterpret_cast<const f32x4*>(a.sums + place * D + c);
+      if (piece + i * kGroups >= n) end[i] = {-INFINITY, 0.0f};
+    }
+    const float most = fmaxf(fmaxf(top, fmaxf(end[0].x, end[1].x)), fmaxf(end[2].x, end[3].x));
+    const float from = most == -INFINITY ? 0.0f : most;
+    const float shrink = __builtin_amdgcn_exp2f(top - from);
+    top = most, sum *= shrink;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= shrink;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float share = __builtin_amdgcn_exp2f(end[i].x - from);
+      sum = fmaf(end[i].y, share, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(part[i][e], share, v[e]);
+    }
   }
-  const bool none = row >= count * a.group || most == -INFINITY;
+#pragma unroll
+  for (int o = kLanes; o < 64; o <<= 1) {
+    const float other = __shfl_xor(top, o), most = fmaxf(top, other), from = most == -INFINITY ? 0.0f : most;
+    const float mine = __builtin_amdgcn_exp2f(top - from), theirs = __builtin_amdgcn_exp2f(other - from);
+    // (the same products and one sum on both sides: the same bits)
+    sum = sum * mine + __shfl_xor(sum, o) * theirs;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] * mine + __shfl_xor(v[e], o) * theirs;
+    top = most;
+  }
+  if (group > 0) return;
+  const bool none = row >= count * a.group || top == -INFINITY;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
   store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
@@ -56,7 +73,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const Attend a) {
 
 template <typename T>
 int merge(const Attend& a, int head_dim, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(a.batch * a.merge_groups);
+  const unsigned grid = static_cast<unsigned>((a.batch * (a.last_row - a.first_row) * a.pages.kv_heads + 3) / 4);
   if (head_dim == 64) merge_kernel<T, 64><<<grid, 256, 0, s>>>(a);
   else merge_kernel<T, 128><<<grid, 256, 0, s>>>(a);
   return check_launch("cached_attn");
@@ -79,26 +96,34 @@ int launch_many<float>(const Attend& a, int64_t pieces, int head_dim, hipStream_
 
 namespace {
 
+// Tokens of a piece at least, and (few queries) up to how many a sequence stays whole: the join is a launch of 3 us.
+// One query of 16 heads over 4 key heads, us: 1,044 tokens whole 8.2, in pieces of 512 9.8; 2,048 11.1, 10.0; 32,768 in
+// pieces of at least 256, 512, 1,024: 16.1, 12.1, 12.6.  Many: 8 heads of 261 queries in fp32 over 1,044 tokens in
+// pieces of 64, 128, 256: 20.0, 16.3, 19.1.
+constexpr int64_t kLeastFew = 512, kWholeFew = 1536, kLeastMany = 128;
+
 // How a call's rows are run: up to two launches, the second for the few rows that would be a tile of the first.
 struct Part {
   bool few;
   int64_t first_row, last_row;
-  int tile_rows, slots, least;
+  int tile_rows, slots;
+  int64_t least;
   bool fold;
   int64_t tiles, pieces;
-  size_t sums, ends;  // bytes of the workspace
+  size_t sums, ends, firsts;  // bytes of the workspace
+  size_t bytes() const { return sums + ends + firsts; }
 };
 struct Plan {
   int parts;
   Part part[2];
-  size_t bytes() const { return part[0].sums + part[0].ends + (parts > 1 ? part[1].sums + part[1].ends : 0); }
+  size_t bytes() const { return part[0].bytes() + (parts > 1 ? part[1].bytes() : 0); }
 };
 Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool few, int causal, const ManyShape& shape) {
   Part p{};
   const int64_t rows = last_row - first_row, capacity = c->table_width * c->page_size;
   p.few = few, p.first_row = first_row, p.last_row = last_row;
   p.tile_rows = few ? few_tile(rows) : shape.tile_rows;
-  p.least = few ? 512 : 256;
+  p.least = few ? kLeastFew : kLeastMany;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // As many work-groups as the chip holds at once; of causal calls that leave room, whose tiles differ, twice as many.
   const int64_t held = static_cast<int64_t>(few ? 2 : shape.resident) * device_cus(), beside = c->kv_heads * p.tiles;
@@ -106,12 +131,13 @@ Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool
   const int64_t slots = (uneven && c->batch * beside <= held / 2 ? 2 * held : held) / beside - c->batch;
   p.fold = uneven && c->batch * beside <= held;
   // (no more pieces than the tables could hold)
-  p.slots = capacity <= p.least ? 0 : static_cast<int>(std::max<int64_t>(0, std::min(slots, c->batch * ((capacity - 1) / p.least))));
+  p.slots = capacity <= (few ? kWholeFew : kLeastMany) ? 0 : static_cast<int>(std::max<int64_t>(0, std::min(slots, c->batch * ((capacity - 1) / p.least))));
   p.pieces = c->batch + p.slots;
   if (p.slots > 0) {
     const size_t parts = static_cast<size_t>(p.pieces) * beside * p.tile_rows;
     p.sums = parts * c->head_dim * sizeof(float);
     p.ends = (parts * sizeof(float2) + 15) / 16 * 16;
+    p.firsts = (c->batch * sizeof(int2) + 15) / 16 * 16;
   }
   return p;
 }
@@ -197,17 +223,16 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
   for (int i = 0; i < p.parts; ++i) {
     const Part& part = p.part[i];
     a.first_row = static_cast<int32_t>(part.first_row), a.last_row = static_cast<int32_t>(part.last_row);
-    a.tiles = static_cast<int32_t>(part.tiles), a.tile_rows = part.tile_rows, a.slots = part.slots, a.least = part.least;
+    a.tiles = static_cast<int32_t>(part.tiles), a.tile_rows = part.tile_rows, a.slots = part.slots, a.least = static_cast<int32_t>(part.least);
     a.fold = part.fold;
     a.sums = reinterpret_cast<float*>(ws), a.ends = reinterpret_cast<float2*>(ws + part.sums);
-    ws += part.sums + part.ends;
+    a.firsts = reinterpret_cast<int2*>(ws + part.sums + part.ends);
+    ws += part.bytes();
     int run = part.few            ? launch_few(a, part.pieces, dim, dtype, s)
               : dtype == VGO_BF16 ? launch_many<bf16_t>(a, part.pieces, dim, s)
               : dtype == VGO_F16  ? launch_many<f16_t>(a, part.pieces, dim, s)
                                   : launch_many<float>(a, part.pieces, dim, s);
     if (run == VGO_OK && part.slots > 0) {
-      const int64_t each = 256 / (dim / 4);
-      a.merge_groups = static_cast<int32_t>(((part.last_row - part.first_row) * cache->kv_heads + each - 1) / each);
       run = dtype == VGO_BF16  ? merge<bf16_t>(a, dim, s)
             : dtype == VGO_F16 ? merge<f16_t>(a, dim, s)
                                : merge<float>(a, dim, s);

@@ -92,9 +92,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   const int hk = blockIdx.x % kv;
   const int rest = blockIdx.x / kv;
   const int tile = tile_at(a, rest % a.tiles);
-  const int64_t x = rest / a.tiles;
+  const int x = rest / a.tiles;
   const Piece piece = piece_of(a, x);
   if (piece.b < 0) return;
+  leave(a, piece, x, threadIdx.x == 0 && hk == 0 && rest % a.tiles == 0);
   const int64_t b = piece.b;
   const int count = count_of(a, b);
   const int row0 = a.first_row + tile * a.tile_rows;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
         store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
                    row / a.group * a.out_stride[2] + c, v);
       } else {
-        const int64_t to = ((x * kv + hk) * a.tiles + tile) * a.tile_rows + 16 * nt + r;
+        const int64_t to = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + 16 * nt + r;
         store4(a.sums + to * D + c, v);
         if (c == 0) a.ends[to] = {most, sum};
       }

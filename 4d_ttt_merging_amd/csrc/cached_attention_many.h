@@ -63,9 +63,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   const int hk = blockIdx.x % kv;
   const int rest = blockIdx.x / kv;
   const int tile = tile_at(a, rest % a.tiles);
-  const int64_t x = rest / a.tiles;
+  const int x = rest / a.tiles;
   const Piece piece = piece_of(a, x);
   if (piece.b < 0) return;
+  leave(a, piece, x, threadIdx.x == 0 && hk == 0 && rest % a.tiles == 0);
   const int64_t b = piece.b;
   const int count = count_of(a, b);
   const int tile0 = a.first_row + tile * a.tile_rows;
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
     if (row >= min(tile0 + a.tile_rows, a.last_row)) continue;
     const bool none = row >= count * a.group || top[mt] == -INFINITY;
     const float share = whole ? (none ? 0.0f : 1.0f / total[mt]) : 1.0f;
-    const int64_t place_of = ((x * kv + hk) * a.tiles + tile) * a.tile_rows + row - tile0;
+    const int64_t place_of = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + row - tile0;
     T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
              row / a.group * a.out_stride[2];
     float* sums = a.sums + place_of * D;
