@@ -28,6 +28,8 @@ Pages pages_of(const vgo_paged_cache* c) {
 
 namespace {
 
+typedef __attribute__((__vector_size__(16))) uint32_t u32x4;
+
 struct Append {
   Pages pages;
   const void* k;
@@ -47,28 +49,29 @@ struct Append {
   int chunks, per;  // chunks of `per` heads of k, q and v together
 };
 
-// Eight consecutive channels of a row as fp32.
+// Eight consecutive channels of a row, as they are in memory, and as fp32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+struct Raw {
+  u32x4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> raw8(const T* p) {
+  Raw<T> r;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4 v = load4(p + 4 * h);
+  for (size_t i = 0; i < sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void widened(const Raw<T>& r, float (&x)[8]) {
+  typedef __attribute__((__vector_size__(16))) T vec;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[4 * h + i] = v[i];
+  for (int i = 0; i < 8; ++i) {
+    constexpr int kEach = 16 / sizeof(T);
+    x[i] = to_f32(__builtin_bit_cast(vec, r.w[i / kEach])[i % kEach]);
   }
 }
-template <>
-__device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float (&x)[8]) {
-  const bf16x8 v = *reinterpret_cast<const bf16x8*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
-}
-template <>
-__device__ __forceinline__ void load8<f16_t>(const f16_t* p, float (&x)[8]) {
-  const f16x8 v = *reinterpret_cast<const f16x8*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
-}
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) { widened(raw8(p), x); }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
@@ -81,19 +84,6 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(x[i]);
     *reinterpret_cast<vec*>(p) = o;
   }
-}
-
-// fp32 of a 64-bit number, rounded to odd: what is cut off leaves the last bit set, so that a later rounding
-// to fewer bits, or a comparison with a number of fewer bits, comes out as for the 64-bit number itself.
-__device__ __forceinline__ float to_odd(double d) {
-  const float f = static_cast<float>(d);
-  uint32_t bits = __float_as_uint(f);
-  const double back = static_cast<double>(f);
-  if (back != d && d == d) {
-    if (fabs(back) > fabs(d)) bits -= 1;
-    bits |= 1;
-  }
-  return __uint_as_float(bits);
 }
 
 // The scale byte of a block whose largest magnitude has these bits (NaN counts as past infinity).
@@ -109,19 +99,68 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   x = max(x, other(x, std::integral_constant<int, 0xB1>()));  // lane ^ 1
   return max(x, other(x, std::integral_constant<int, 0x4E>()));  // lane ^ 2
 }
-// Codes of eight channels; `byte` gets the scale of the 32 that this lane's quad holds.
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t& byte) {
+// The largest magnitude of 32 channels, eight of this lane and its quad's, as bits.
+__device__ __forceinline__ uint32_t top_of(const float (&x)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  byte = scale_byte(quad_max(top));
-  const float scale = __uint_as_float(byte == 255 ? 0x3f800000u : byte << 23);
+  return quad_max(top);
+}
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale) {
   uint32_t word = 0;
   word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[0], x[1], scale, 0);
   word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[2], x[3], scale, 1);
   word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[4], x[5], scale, 2);
   word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[6], x[7], scale, 3);
   return word;
+}
+__device__ __forceinline__ float factor_of(uint32_t byte) { return __uint_as_float(byte == 255 ? 0x3f800000u : byte << 23); }
+// Codes of eight channels; `byte` gets the scale of the 32 that this lane's quad holds.
+__device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t& byte) {
+  byte = scale_byte(top_of(x));
+  return codes_of(x, factor_of(byte));
+}
+
+// fp32 of a 64-bit number, rounded to odd: what is cut off leaves the last bit set, so that a later rounding
+// to fewer bits, or a comparison with a number of fewer bits, comes out as for the 64-bit number itself.
+__device__ __forceinline__ float to_odd(double d) {
+  const float f = static_cast<float>(d);
+  uint32_t bits = __float_as_uint(f);
+  const double back = static_cast<double>(f);
+  if (back != d && d == d) {
+    if (fabs(back) > fabs(d)) bits -= 1;
+    bits |= 1;
+  }
+  return __uint_as_float(bits);
+}
+
+// Codes of x cos + o sin, exactly those of the 64-bit value: fp32 first, which is off by at most 2^-24 of the
+// product x cos and of the sum each; where some channel of the wave lies so near a border that this may matter (about
+// one of 500 waves), 64 bits.  (64 bits throughout kept the vector unit busy for three times as long as
+// memory takes: 4 ragged prompts of up to 8,232 tokens, 16 heads of 64 channels, 184 us, this AFTER_APPEND.)
+__device__ __forceinline__ uint32_t quantise_rotated(const float (&x)[8], const float (&o)[8], const float (&sin)[8],
+                                                     const float (&cos)[8], bool real, uint32_t& byte) {
+  float y[8], low[8], high[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float part = x[i] * cos[i];
+    y[i] = fmaf(o[i], sin[i], part);
+    const float off = fabsf(part) + fabsf(y[i]);
+    low[i] = fmaf(off, -0x1p-22f, y[i]), high[i] = fmaf(off, 0x1p-22f, y[i]);
+  }
+  const uint32_t top = top_of(y);
+  byte = scale_byte(top);
+  const float scale = factor_of(byte);
+  const uint32_t word = codes_of(low, scale);
+  // The largest one's parts may each be twice as large: 2^-20 of it covers them.  Numbers near the ends of fp32, and
+  // those that are not finite, are left to 64 bits.
+  const uint32_t past = (top & 0x7fffffu) - (0x600000u - 16u);
+  const bool plain = word == codes_of(high, scale) && past > 32u && top > 0x10000000u && top < 0x7e000000u;
+  if (__all(plain || !real)) return word;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    y[i] = to_odd(fma(static_cast<double>(o[i]), static_cast<double>(sin[i]), static_cast<double>(x[i]) * cos[i]));
+  return quantise(y, byte);
 }
 // Bytes of four lanes `kStep` apart as a 4 x 4 matrix, transposed: byte c of lane r goes to byte r of lane c
 // (r counts in steps of kStep).  Its own inverse.
@@ -136,13 +175,14 @@ __device__ __forceinline__ uint32_t transposed_bytes(uint32_t w) {
 }
 
 // A wave takes eight tokens whose positions share position / 8 (so that the values' bytes of a channel pair are one
-// group of the format) and `per` heads; a lane eight channels of a token.
+// group of the format) and `per` heads of k, q and v, one after the other with the next one's channels on their way; a lane
+// eight channels of a token.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void append_kernel(const Append a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;            // of a token
   constexpr int kTokens = 64 / kLanes;     // at a time
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= a.items) return;
   const int lane = lane_id();
   const int chunk = static_cast<int>(item % a.chunks);
@@ -154,15 +194,20 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a) {
   const bool low = c < kLanes / 2;
   const int page = first >= 0 ? page_of(a.pages, b, first) : -1;
   const int kv = a.pages.kv_heads;
+  const bool rotate = a.sin != nullptr;
+  const int begin = chunk * a.per, end = min(begin + a.per, 2 * kv + a.heads);
 #pragma unroll
   for (int pass = 0; pass < 8 / kTokens; ++pass) {
     const int j = pass * kTokens + lane / kLanes;
     const int64_t t = first + j, i = t - start;
     const bool inside = i >= 0 && i < a.n, real = i >= 0 && i < count;
-    const bool stored = real && page >= 0;
+    const int64_t at_row = min(max(i, int64_t{0}), a.n - 1);  // (padding lanes read some row of the call)
+    const int slot = static_cast<int>(t) & 31;
     bool turned = false;
     float sin[8], cos[8];
-    if (a.sin && real) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sin[e] = 0.0f, cos[e] = 1.0f;
+    if (rotate && real) {
       const int64_t row = a.positions ? a.positions[b * a.n + i] : t;
       turned = row >= 0 && row < a.rope_rows;
       if (turned) {
@@ -170,57 +215,73 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a) {
         load8(a.cos + row * D + 8 * c, cos);
       }
     }
-    if (chunk == 0 && a.pages.mass && stored && c == 0)
+    if (chunk == 0 && a.pages.mass && real && page >= 0 && c == 0)
       a.pages.mass[(static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1))] =
           a.log_mass ? a.log_mass[b * a.n + i] : 0.0f;
-    const int end = min((chunk + 1) * a.per, 2 * kv + a.heads);
-    for (int at = chunk * a.per; at < end; ++at) {
+    // The channels of virtual head `at`: keys' heads, the queries', the values'; and those they are rotated with.
+    const int64_t k_row = at_row * a.k_stride[2] + 8 * c, q_row = at_row * a.q_stride[2] + 8 * c, v_row = at_row * a.v_stride[2] + 8 * c;
+    const int across = low ? D / 2 : -D / 2;
+    const auto read = [&](int at, Raw<T>& x, Raw<T>& o) {
+      const T* from;
+      if (at < kv) from = static_cast<const T*>(a.k) + b * a.k_stride[0] + at * a.k_stride[1] + k_row;
+      else if (at < kv + a.heads) from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (at - kv) * a.q_stride[1] + q_row;
+      else from = static_cast<const T*>(a.v) + b * a.v_stride[0] + (at - kv - a.heads) * a.v_stride[1] + v_row;
+      x = raw8(from);
+      if (rotate && at < kv + a.heads) o = raw8(from + across);
+    };
+    const auto use = [&](int at, const Raw<T>& raw, const Raw<T>& raw_other) {
       const bool key = at < kv, value = at >= kv + a.heads;
-      const int head = key ? at : value ? at - kv - a.heads : at - kv;
-      const int64_t* stride = key ? a.k_stride : value ? a.v_stride : a.q_stride;
-      const T* from = static_cast<const T*>(key ? a.k : value ? a.v : a.q) + b * stride[0] + head * stride[1];
-      float x[8] = {};
-      if (real) load8(from + i * stride[2] + 8 * c, x);
-      if (!value && turned) {
-        float other[8];
-        load8(from + i * stride[2] + 8 * (low ? c + kLanes / 2 : c - kLanes / 2), other);
+      float x[8], other[8];
+      widened(raw, x);
+      uint32_t byte = 0, word = 0;
+      if (rotate && !value) {
+        widened(raw_other, other);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // In 64 bits: a code then never depends on how the rotation was rounded.
-          const double y = static_cast<double>(x[e]) * cos[e] + static_cast<double>(low ? -other[e] : other[e]) * sin[e];
-          x[e] = key ? to_odd(y) : static_cast<float>(y);
-        }
+        for (int e = 0; e < 8; ++e) other[e] = !turned ? 0.0f : low ? -other[e] : other[e];  // (not turned: x 1 + 0 0)
       }
       if (!key && !value) {
+        if (rotate) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = fmaf(other[e], sin[e], x[e] * cos[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = real ? x[e] : 0.0f;
         if (inside)
-          store8(static_cast<T*>(a.q_out) + b * a.out_stride[0] + head * a.out_stride[1] + i * a.out_stride[2] + 8 * c, x);
-        continue;
+          store8(static_cast<T*>(a.q_out) + b * a.out_stride[0] + (at - kv) * a.out_stride[1] + i * a.out_stride[2] + 8 * c, x);
+        return;
       }
-      uint32_t byte;
-      uint32_t word = quantise(x, byte);
+      if (rotate && key) word = quantise_rotated(x, other, sin, cos, real, byte);
+      else word = quantise(x, byte);
       if (value) word = transposed_bytes<kLanes>(word);
-      if (page < 0) continue;
-      uint8_t* block = a.pages.data + block_of<D>(a.pages, page, head, first);
-      const int slot = static_cast<int>(t) & 31;
+      if (page < 0) return;
+      uint8_t* block = a.pages.data + block_of<D>(a.pages, page, key ? at : at - kv - a.heads, first);
       if (key) {
         if (real) {
-          *reinterpret_cast<uint32_t*>(block + slot * L::kKeyBytes + 4 * c) = word;
-          if (c % 4 == 0) block[L::kKeyScales + slot * L::kParts + c / 4] = static_cast<uint8_t>(byte);
+          *reinterpret_cast<uint32_t*>(block + static_cast<uint32_t>(slot * L::kKeyBytes + 4 * c)) = word;
+          if (c % 4 == 0) block[static_cast<uint32_t>(L::kKeyScales + slot * L::kParts + c / 4)] = static_cast<uint8_t>(byte);
         }
-      } else {
-        if (real && c % 4 == 0)
-          block[L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8] = static_cast<uint8_t>(byte);
-        // Four tokens of channel pair 4c + j % 4; tokens that are not this call's keep their bytes.
-        const int64_t four = i - j % 4;
-        uint8_t* to = block + L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4);
-        if (four >= 0 && four + 3 < count) {
-          *reinterpret_cast<uint32_t*>(to) = word;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (four + e >= 0 && four + e < count) to[e] = static_cast<uint8_t>(word >> (8 * e));
-        }
+        return;
       }
+      if (real && c % 4 == 0)
+        block[static_cast<uint32_t>(L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8)] = static_cast<uint8_t>(byte);
+      // Four tokens of channel pair 4c + j % 4; tokens that are not this call's keep their bytes.
+      const int64_t four = i - j % 4;
+      uint8_t* to = block + static_cast<uint32_t>(L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4));
+      if (four >= 0 && four + 3 < count) {
+        *reinterpret_cast<uint32_t*>(to) = word;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (four + e >= 0 && four + e < count) to[e] = static_cast<uint8_t>(word >> (8 * e));
+      }
+    };
+    Raw<T> x0{}, o0{}, x1{}, o1{};
+    read(begin, x0, o0);
+    for (int at = begin; at < end; at += 2) {
+      if (at + 1 < end) read(at + 1, x1, o1);
+      use(at, x0, o0);
+      if (at + 2 < end) read(at + 2, x0, o0);
+      if (at + 1 < end) use(at + 1, x1, o1);
     }
   }
 }
@@ -232,51 +293,65 @@ struct Read {
   const int32_t* starts;
   const int32_t* counts;
   int64_t n, items, groups;
+  int chunks, per;  // chunks of `per` heads of keys and values together
 };
 
-// The inverse: eight tokens, one head, keys or values.
+// The inverse: a wave takes eight tokens and `per` heads of keys and values, four heads' codes on their way together.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void read_kernel(const Read a) {
   using L = Layout<D>;
-  constexpr int kLanes = D / 8, kTokens = 64 / kLanes;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  constexpr int kLanes = D / 8, kTokens = 64 / kLanes, kAhead = 4;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= a.items) return;
   const int lane = lane_id(), kv = a.pages.kv_heads;
-  const bool value = item % 2;
-  const int head = static_cast<int>(item / 2 % kv);
-  const int64_t rest = item / 2 / kv, group = rest % a.groups, b = rest / a.groups;
+  const int chunk = static_cast<int>(item % a.chunks);
+  const int64_t rest = item / a.chunks, group = rest % a.groups, b = rest / a.groups;
   const int64_t start = a.starts[b];
   const int64_t count = a.counts ? min(max(static_cast<int64_t>(a.counts[b]), int64_t{0}), a.n) : a.n;
   const int64_t first = (start & ~int64_t{7}) + 8 * group;
   const int c = lane % kLanes;
-  const int page = first >= 0 ? page_of(a.pages, b, first) : -1;
+  const int page = first >= 0 && a.pages.pages > 0 ? page_of(a.pages, b, first) : -1;
+  const int begin = chunk * a.per, end = min(begin + a.per, 2 * kv);
 #pragma unroll
   for (int pass = 0; pass < 8 / kTokens; ++pass) {
     const int j = pass * kTokens + lane / kLanes;
     const int64_t t = first + j, i = t - start;
     const int slot = static_cast<int>(t) & 31;
-    uint32_t word = 0, byte = 0;
-    if (page >= 0) {
-      const uint8_t* block = a.pages.data + block_of<D>(a.pages, page, head, first);
-      if (value) {
-        word = *reinterpret_cast<const uint32_t*>(block + L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4));
-        byte = block[L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8];
-      } else {
-        word = *reinterpret_cast<const uint32_t*>(block + slot * L::kKeyBytes + 4 * c);
-        byte = block[L::kKeyScales + slot * L::kParts + c / 4];
+    const bool inside = i >= 0 && i < a.n, real = inside && i < count;
+    const uint32_t key_at = slot * L::kKeyBytes + 4 * c, key_scale_at = L::kKeyScales + slot * L::kParts + c / 4;
+    const uint32_t value_at = L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4);
+    const uint32_t value_scale_at = L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8;
+    for (int at0 = begin; at0 < end; at0 += kAhead) {
+      uint32_t words[kAhead] = {}, bytes[kAhead] = {};
+      if (page >= 0) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          const int at = min(at0 + e, end - 1);
+          const bool value = at >= kv;
+          const uint8_t* block = a.pages.data + block_of<D>(a.pages, page, value ? at - kv : at, first);
+          words[e] = *reinterpret_cast<const uint32_t*>(block + (value ? value_at : key_at));
+          bytes[e] = block[value ? value_scale_at : key_scale_at];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int at = at0 + e;
+        if (at >= end) break;
+        const bool value = at >= kv;
+        uint32_t word = words[e];
+        if (value) word = transposed_bytes<kLanes>(word);
+        if (!inside) continue;
+        if (!real) word = 0, bytes[e] = 0;  // beyond the sequence's tokens: zeros
+        const float scale = scale_of<0>(bytes[e]);
+        const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
+        const bf16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
+        const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
+        const bf16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
+        const float x[8] = {to_f32(p0[0]), to_f32(p0[1]), to_f32(p1[0]), to_f32(p1[1]),
+                            to_f32(p2[0]), to_f32(p2[1]), to_f32(p3[0]), to_f32(p3[1])};
+        store8(static_cast<T*>(value ? a.v : a.k) + ((b * kv + (value ? at - kv : at)) * a.n + i) * D + 8 * c, x);
       }
     }
-    if (value) word = transposed_bytes<kLanes>(word);
-    if (i < 0 || i >= a.n) continue;
-    if (i >= count) word = 0, byte = 0;  // beyond the sequence's tokens: zeros
-    const float scale = scale_of<0>(byte);
-    const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
-    const bf16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
-    const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
-    const bf16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
-    const float x[8] = {to_f32(p0[0]), to_f32(p0[1]), to_f32(p1[0]), to_f32(p1[1]),
-                        to_f32(p2[0]), to_f32(p2[1]), to_f32(p3[0]), to_f32(p3[1])};
-    store8(static_cast<T*>(value ? a.v : a.k) + ((b * kv + head) * a.n + i) * D + 8 * c, x);
   }
 }
 
@@ -314,6 +389,11 @@ bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
   return true;
 }
 bool known(int dtype) { return dtype == VGO_F32 || dtype == VGO_BF16 || dtype == VGO_F16; }
+// Heads that a wave takes one after the other: more where there are waves enough without (the tables' rows, the page and
+// the addresses are then fetched once for them).
+int heads_of_a_wave(int64_t groups, int heads) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, groups >= (int64_t{1} << 40) ? 8 : groups * heads / 4096)));
+}
 // A grid's threads are counted in 32 bits; four items a work-group of 256.
 constexpr int64_t kMostItems = ((int64_t{1} << 32) / 256 - 1) * 4;
 
@@ -352,7 +432,7 @@ extern "C" int vgo_cache_append(const vgo_paged_cache* cache, const vgo_cache_to
   a.log_mass = t.log_mass, a.rope_rows = t.rope_rows, a.n = t.n_tokens, a.heads = static_cast<int>(t.heads);
   a.groups = (t.n_tokens + 14) / 8;  // (a sequence may start anywhere in its first group)
   const int all = static_cast<int>(2 * cache->kv_heads) + a.heads;
-  a.per = 1;
+  a.per = heads_of_a_wave(cache->batch * a.groups, all);
   a.chunks = (all + a.per - 1) / a.per;
   VGO_REQUIRE(cache->batch <= kMostItems / a.groups / a.chunks, "cache_append: too many tokens");
   a.items = cache->batch * a.groups * a.chunks;
@@ -374,7 +454,10 @@ extern "C" int vgo_cache_read(const vgo_paged_cache* cache, const int32_t* start
   a.pages = pages_of(cache);
   a.k = k, a.v = v, a.starts = starts, a.counts = counts, a.n = n_tokens;
   a.groups = (n_tokens + 14) / 8;
-  VGO_REQUIRE(cache->batch <= kMostItems / a.groups / (2 * cache->kv_heads), "cache_read: too many tokens");
-  a.items = cache->batch * a.groups * 2 * cache->kv_heads;
+  const int all = static_cast<int>(2 * cache->kv_heads);
+  a.per = heads_of_a_wave(cache->batch * a.groups, all);
+  a.chunks = (all + a.per - 1) / a.per;
+  VGO_REQUIRE(cache->batch <= kMostItems / a.groups / a.chunks, "cache_read: too many tokens");
+  a.items = cache->batch * a.groups * a.chunks;
   return by_type<LaunchRead>(a, cache->head_dim, dtype, as_stream(stream));
 }

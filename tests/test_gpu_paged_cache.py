@@ -46,8 +46,12 @@ class Both:
         want = oracle.append(self.pages, k, v, table, starts, counts, q=q, rope=rope, positions=positions, log_mass=log_mass)
         if q is not None:
             got = got.double().cpu()
-            # Rounded once from 64 bits; the smallest normal of the type for what rounds to less.
-            assert ((got - want).abs() <= torch.finfo(q.dtype).eps / 2 * want.abs() + torch.finfo(q.dtype).tiny).all()
+            # One product and one sum in fp32 (2^-24 of each; together less than 2^-23 of the parts' magnitudes, which
+            # rotation by an orthogonal pair bounds by its two channels'), then half a step of the type; the smallest normal
+            # number of the type for what rounds to less.
+            parts = q.double().abs() + q.double().abs().roll(q.shape[-1] // 2, -1)
+            off = torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -23 * parts + torch.finfo(q.dtype).tiny
+            assert ((got - want).abs() <= off).all()
         return got
 
     def check_everything(self):
