@@ -137,7 +137,7 @@ __device__ __forceinline__ float to_odd(double d) {
 // Codes of x cos + o sin, exactly those of the 64-bit value: fp32 first, which is off by at most 2^-24 of the
 // product x cos and of the sum each; where some channel of the wave lies so near a border that this may matter (about
 // one of 500 waves), 64 bits.  (64 bits throughout kept the vector unit busy for three times as long as
-// memory takes: 4 ragged prompts of up to 8,232 tokens, 16 heads of 64 channels, 184 us, this AFTER_APPEND.)
+// memory takes: 4 ragged prompts of up to 8,232 tokens, 16 heads of 64 channels, 184 us, this 79.)
 __device__ __forceinline__ uint32_t quantise_rotated(const float (&x)[8], const float (&o)[8], const float (&sin)[8],
                                                      const float (&cos)[8], bool real, uint32_t& byte) {
   float y[8], low[8], high[8];
@@ -174,19 +174,19 @@ __device__ __forceinline__ uint32_t transposed_bytes(uint32_t w) {
   return (lane & (2 * kStep)) ? __builtin_amdgcn_perm(w, o, 0x07060302) : __builtin_amdgcn_perm(o, w, 0x05040100);
 }
 
-// A wave takes eight tokens whose positions share position / 8 (so that the values' bytes of a channel pair are one
-// group of the format) and `per` heads of k, q and v, one after the other with the next one's channels on their way; a lane
+// A wave takes 512 / D tokens, all or half of those that share position / 8 (whose values of a channel pair are eight bytes
+// of the format), and `per` heads of k, q and v, one after the other with the next one's channels on their way; a lane
 // eight channels of a token.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void append_kernel(const Append a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;            // of a token
-  constexpr int kTokens = 64 / kLanes;     // at a time
+  constexpr int kTokens = 64 / kLanes, kParts = 8 / kTokens;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= a.items) return;
   const int lane = lane_id();
   const int chunk = static_cast<int>(item % a.chunks);
-  const int64_t rest = item / a.chunks, group = rest % a.groups, b = rest / a.groups;
+  const int64_t rest = item / a.chunks, group = rest / kParts % a.groups, b = rest / kParts / a.groups;
   const int64_t start = a.starts[b];
   const int64_t count = a.counts ? min(max(static_cast<int64_t>(a.counts[b]), int64_t{0}), a.n) : a.n;
   const int64_t first = (start & ~int64_t{7}) + 8 * group;
@@ -196,93 +196,91 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a) {
   const int kv = a.pages.kv_heads;
   const bool rotate = a.sin != nullptr;
   const int begin = chunk * a.per, end = min(begin + a.per, 2 * kv + a.heads);
+  const int j = static_cast<int>(rest % kParts) * kTokens + lane / kLanes;
+  const int64_t t = first + j, i = t - start;
+  const bool inside = i >= 0 && i < a.n, real = i >= 0 && i < count;
+  if (!__any(inside)) return;
+  const int64_t at_row = min(max(i, int64_t{0}), a.n - 1);  // (padding lanes read some row of the call)
+  const int slot = static_cast<int>(t) & 31;
+  bool turned = false;
+  float sin[8], cos[8];
 #pragma unroll
-  for (int pass = 0; pass < 8 / kTokens; ++pass) {
-    const int j = pass * kTokens + lane / kLanes;
-    const int64_t t = first + j, i = t - start;
-    const bool inside = i >= 0 && i < a.n, real = i >= 0 && i < count;
-    const int64_t at_row = min(max(i, int64_t{0}), a.n - 1);  // (padding lanes read some row of the call)
-    const int slot = static_cast<int>(t) & 31;
-    bool turned = false;
-    float sin[8], cos[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sin[e] = 0.0f, cos[e] = 1.0f;
-    if (rotate && real) {
-      const int64_t row = a.positions ? a.positions[b * a.n + i] : t;
-      turned = row >= 0 && row < a.rope_rows;
-      if (turned) {
-        load8(a.sin + row * D + 8 * c, sin);
-        load8(a.cos + row * D + 8 * c, cos);
-      }
+  for (int e = 0; e < 8; ++e) sin[e] = 0.0f, cos[e] = 1.0f;
+  if (rotate && real) {
+    const int64_t row = a.positions ? a.positions[b * a.n + i] : t;
+    turned = row >= 0 && row < a.rope_rows;
+    if (turned) {
+      load8(a.sin + row * D + 8 * c, sin);
+      load8(a.cos + row * D + 8 * c, cos);
     }
-    if (chunk == 0 && a.pages.mass && real && page >= 0 && c == 0)
-      a.pages.mass[(static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1))] =
-          a.log_mass ? a.log_mass[b * a.n + i] : 0.0f;
-    // The channels of virtual head `at`: keys' heads, the queries', the values'; and those they are rotated with.
-    const int64_t k_row = at_row * a.k_stride[2] + 8 * c, q_row = at_row * a.q_stride[2] + 8 * c, v_row = at_row * a.v_stride[2] + 8 * c;
-    const int across = low ? D / 2 : -D / 2;
-    const auto read = [&](int at, Raw<T>& x, Raw<T>& o) {
-      const T* from;
-      if (at < kv) from = static_cast<const T*>(a.k) + b * a.k_stride[0] + at * a.k_stride[1] + k_row;
-      else if (at < kv + a.heads) from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (at - kv) * a.q_stride[1] + q_row;
-      else from = static_cast<const T*>(a.v) + b * a.v_stride[0] + (at - kv - a.heads) * a.v_stride[1] + v_row;
-      x = raw8(from);
-      if (rotate && at < kv + a.heads) o = raw8(from + across);
-    };
-    const auto use = [&](int at, const Raw<T>& raw, const Raw<T>& raw_other) {
-      const bool key = at < kv, value = at >= kv + a.heads;
-      float x[8], other[8];
-      widened(raw, x);
-      uint32_t byte = 0, word = 0;
-      if (rotate && !value) {
-        widened(raw_other, other);
+  }
+  if (chunk == 0 && a.pages.mass && real && page >= 0 && c == 0)
+    a.pages.mass[(static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1))] =
+        a.log_mass ? a.log_mass[b * a.n + i] : 0.0f;
+  // The channels of virtual head `at`: keys' heads, the queries', the values'; and those they are rotated with.
+  const int64_t k_row = at_row * a.k_stride[2] + 8 * c, q_row = at_row * a.q_stride[2] + 8 * c, v_row = at_row * a.v_stride[2] + 8 * c;
+  const int across = low ? D / 2 : -D / 2;
+  const auto read = [&](int at, Raw<T>& x, Raw<T>& o) {
+    const T* from;
+    if (at < kv) from = static_cast<const T*>(a.k) + b * a.k_stride[0] + at * a.k_stride[1] + k_row;
+    else if (at < kv + a.heads) from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (at - kv) * a.q_stride[1] + q_row;
+    else from = static_cast<const T*>(a.v) + b * a.v_stride[0] + (at - kv - a.heads) * a.v_stride[1] + v_row;
+    x = raw8(from);
+    if (rotate && at < kv + a.heads) o = raw8(from + across);
+  };
+  const auto use = [&](int at, const Raw<T>& raw, const Raw<T>& raw_other) {
+    const bool key = at < kv, value = at >= kv + a.heads;
+    float x[8], other[8];
+    widened(raw, x);
+    uint32_t byte = 0, word = 0;
+    if (rotate && !value) {
+      widened(raw_other, other);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) other[e] = !turned ? 0.0f : low ? -other[e] : other[e];  // (not turned: x 1 + 0 0)
-      }
-      if (!key && !value) {
-        if (rotate) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = fmaf(other[e], sin[e], x[e] * cos[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = real ? x[e] : 0.0f;
-        if (inside)
-          store8(static_cast<T*>(a.q_out) + b * a.out_stride[0] + (at - kv) * a.out_stride[1] + i * a.out_stride[2] + 8 * c, x);
-        return;
-      }
-      if (rotate && key) word = quantise_rotated(x, other, sin, cos, real, byte);
-      else word = quantise(x, byte);
-      if (value) word = transposed_bytes<kLanes>(word);
-      if (page < 0) return;
-      uint8_t* block = a.pages.data + block_of<D>(a.pages, page, key ? at : at - kv - a.heads, first);
-      if (key) {
-        if (real) {
-          *reinterpret_cast<uint32_t*>(block + static_cast<uint32_t>(slot * L::kKeyBytes + 4 * c)) = word;
-          if (c % 4 == 0) block[static_cast<uint32_t>(L::kKeyScales + slot * L::kParts + c / 4)] = static_cast<uint8_t>(byte);
-        }
-        return;
-      }
-      if (real && c % 4 == 0)
-        block[static_cast<uint32_t>(L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8)] = static_cast<uint8_t>(byte);
-      // Four tokens of channel pair 4c + j % 4; tokens that are not this call's keep their bytes.
-      const int64_t four = i - j % 4;
-      uint8_t* to = block + static_cast<uint32_t>(L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4));
-      if (four >= 0 && four + 3 < count) {
-        *reinterpret_cast<uint32_t*>(to) = word;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (four + e >= 0 && four + e < count) to[e] = static_cast<uint8_t>(word >> (8 * e));
-      }
-    };
-    Raw<T> x0{}, o0{}, x1{}, o1{};
-    read(begin, x0, o0);
-    for (int at = begin; at < end; at += 2) {
-      if (at + 1 < end) read(at + 1, x1, o1);
-      use(at, x0, o0);
-      if (at + 2 < end) read(at + 2, x0, o0);
-      if (at + 1 < end) use(at + 1, x1, o1);
+      for (int e = 0; e < 8; ++e) other[e] = !turned ? 0.0f : low ? -other[e] : other[e];  // (not turned: x 1 + 0 0)
     }
+    if (!key && !value) {
+      if (rotate) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(other[e], sin[e], x[e] * cos[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = real ? x[e] : 0.0f;
+      if (inside)
+        store8(static_cast<T*>(a.q_out) + b * a.out_stride[0] + (at - kv) * a.out_stride[1] + i * a.out_stride[2] + 8 * c, x);
+      return;
+    }
+    if (rotate && key) word = quantise_rotated(x, other, sin, cos, real, byte);
+    else word = quantise(x, byte);
+    if (value) word = transposed_bytes<kLanes>(word);
+    if (page < 0) return;
+    uint8_t* block = a.pages.data + block_of<D>(a.pages, page, key ? at : at - kv - a.heads, first);
+    if (key) {
+      if (real) {
+        *reinterpret_cast<uint32_t*>(block + static_cast<uint32_t>(slot * L::kKeyBytes + 4 * c)) = word;
+        if (c % 4 == 0) block[static_cast<uint32_t>(L::kKeyScales + slot * L::kParts + c / 4)] = static_cast<uint8_t>(byte);
+      }
+      return;
+    }
+    if (real && c % 4 == 0)
+      block[static_cast<uint32_t>(L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8)] = static_cast<uint8_t>(byte);
+    // Four tokens of channel pair 4c + j % 4; tokens that are not this call's keep their bytes.
+    const int64_t four = i - j % 4;
+    uint8_t* to = block + static_cast<uint32_t>(L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4));
+    if (four >= 0 && four + 3 < count) {
+      *reinterpret_cast<uint32_t*>(to) = word;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (four + e >= 0 && four + e < count) to[e] = static_cast<uint8_t>(word >> (8 * e));
+    }
+  };
+  Raw<T> x0{}, o0{}, x1{}, o1{};
+  read(begin, x0, o0);
+  for (int at = begin; at < end; at += 2) {
+    if (at + 1 < end) read(at + 1, x1, o1);
+    use(at, x0, o0);
+    if (at + 2 < end) read(at + 2, x0, o0);
+    if (at + 1 < end) use(at + 1, x1, o1);
   }
 }
 
@@ -300,57 +298,54 @@ struct Read {
 template <typename T, int D>
 __global__ __launch_bounds__(256) void read_kernel(const Read a) {
   using L = Layout<D>;
-  constexpr int kLanes = D / 8, kTokens = 64 / kLanes, kAhead = 4;
+  constexpr int kLanes = D / 8, kTokens = 64 / kLanes, kParts = 8 / kTokens, kAhead = 4;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= a.items) return;
   const int lane = lane_id(), kv = a.pages.kv_heads;
   const int chunk = static_cast<int>(item % a.chunks);
-  const int64_t rest = item / a.chunks, group = rest % a.groups, b = rest / a.groups;
+  const int64_t rest = item / a.chunks, group = rest / kParts % a.groups, b = rest / kParts / a.groups;
   const int64_t start = a.starts[b];
   const int64_t count = a.counts ? min(max(static_cast<int64_t>(a.counts[b]), int64_t{0}), a.n) : a.n;
   const int64_t first = (start & ~int64_t{7}) + 8 * group;
   const int c = lane % kLanes;
   const int page = first >= 0 && a.pages.pages > 0 ? page_of(a.pages, b, first) : -1;
   const int begin = chunk * a.per, end = min(begin + a.per, 2 * kv);
-#pragma unroll
-  for (int pass = 0; pass < 8 / kTokens; ++pass) {
-    const int j = pass * kTokens + lane / kLanes;
-    const int64_t t = first + j, i = t - start;
-    const int slot = static_cast<int>(t) & 31;
-    const bool inside = i >= 0 && i < a.n, real = inside && i < count;
-    const uint32_t key_at = slot * L::kKeyBytes + 4 * c, key_scale_at = L::kKeyScales + slot * L::kParts + c / 4;
-    const uint32_t value_at = L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4);
-    const uint32_t value_scale_at = L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8;
-    for (int at0 = begin; at0 < end; at0 += kAhead) {
-      uint32_t words[kAhead] = {}, bytes[kAhead] = {};
-      if (page >= 0) {
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e) {
-          const int at = min(at0 + e, end - 1);
-          const bool value = at >= kv;
-          const uint8_t* block = a.pages.data + block_of<D>(a.pages, page, value ? at - kv : at, first);
-          words[e] = *reinterpret_cast<const uint32_t*>(block + (value ? value_at : key_at));
-          bytes[e] = block[value ? value_scale_at : key_scale_at];
-        }
-      }
+  const int j = static_cast<int>(rest % kParts) * kTokens + lane / kLanes;
+  const int64_t t = first + j, i = t - start;
+  const int slot = static_cast<int>(t) & 31;
+  const bool inside = i >= 0 && i < a.n, real = inside && i < count;
+  const uint32_t key_at = slot * L::kKeyBytes + 4 * c, key_scale_at = L::kKeyScales + slot * L::kParts + c / 4;
+  const uint32_t value_at = L::kValues + slot / 8 * L::kGroup + (4 * c + j % 4) * 8 + (slot & 4);
+  const uint32_t value_scale_at = L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8;
+  for (int at0 = begin; at0 < end; at0 += kAhead) {
+    uint32_t words[kAhead] = {}, bytes[kAhead] = {};
+    if (page >= 0) {
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
-        const int at = at0 + e;
-        if (at >= end) break;
+        const int at = min(at0 + e, end - 1);
         const bool value = at >= kv;
-        uint32_t word = words[e];
-        if (value) word = transposed_bytes<kLanes>(word);
-        if (!inside) continue;
-        if (!real) word = 0, bytes[e] = 0;  // beyond the sequence's tokens: zeros
-        const float scale = scale_of<0>(bytes[e]);
-        const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
-        const bf16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
-        const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
-        const bf16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
-        const float x[8] = {to_f32(p0[0]), to_f32(p0[1]), to_f32(p1[0]), to_f32(p1[1]),
-                            to_f32(p2[0]), to_f32(p2[1]), to_f32(p3[0]), to_f32(p3[1])};
-        store8(static_cast<T*>(value ? a.v : a.k) + ((b * kv + (value ? at - kv : at)) * a.n + i) * D + 8 * c, x);
+        const uint8_t* block = a.pages.data + block_of<D>(a.pages, page, value ? at - kv : at, first);
+        words[e] = *reinterpret_cast<const uint32_t*>(block + (value ? value_at : key_at));
+        bytes[e] = block[value ? value_scale_at : key_scale_at];
       }
+    }
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      const int at = at0 + e;
+      if (at >= end) break;
+      const bool value = at >= kv;
+      uint32_t word = words[e];
+      if (value) word = transposed_bytes<kLanes>(word);
+      if (!inside) continue;
+      if (!real) word = 0, bytes[e] = 0;  // beyond the sequence's tokens: zeros
+      const float scale = scale_of<0>(bytes[e]);
+      const bf16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
+      const bf16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
+      const bf16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
+      const bf16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
+      const float x[8] = {to_f32(p0[0]), to_f32(p0[1]), to_f32(p1[0]), to_f32(p1[1]),
+                          to_f32(p2[0]), to_f32(p2[1]), to_f32(p3[0]), to_f32(p3[1])};
+      store8(static_cast<T*>(value ? a.v : a.k) + ((b * kv + (value ? at - kv : at)) * a.n + i) * D + 8 * c, x);
     }
   }
 }
@@ -392,7 +387,7 @@ bool known(int dtype) { return dtype == VGO_F32 || dtype == VGO_BF16 || dtype ==
 // Heads that a wave takes one after the other: more where there are waves enough without (the tables' rows, the page and
 // the addresses are then fetched once for them).
 int heads_of_a_wave(int64_t groups, int heads) {
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, groups >= (int64_t{1} << 40) ? 8 : groups * heads / 4096)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, groups >= (int64_t{1} << 40) ? 8 : groups * heads / 2048)));
 }
 // A grid's threads are counted in 32 bits; four items a work-group of 256.
 constexpr int64_t kMostItems = ((int64_t{1} << 32) / 256 - 1) * 4;
@@ -434,8 +429,8 @@ extern "C" int vgo_cache_append(const vgo_paged_cache* cache, const vgo_cache_to
   const int all = static_cast<int>(2 * cache->kv_heads) + a.heads;
   a.per = heads_of_a_wave(cache->batch * a.groups, all);
   a.chunks = (all + a.per - 1) / a.per;
-  VGO_REQUIRE(cache->batch <= kMostItems / a.groups / a.chunks, "cache_append: too many tokens");
-  a.items = cache->batch * a.groups * a.chunks;
+  VGO_REQUIRE(cache->batch <= kMostItems / 2 / a.groups / a.chunks, "cache_append: too many tokens");
+  a.items = cache->batch * a.groups * a.chunks * (cache->head_dim / 64);
   return by_type<LaunchAppend>(a, cache->head_dim, dtype, as_stream(stream));
 }
 
@@ -457,7 +452,7 @@ extern "C" int vgo_cache_read(const vgo_paged_cache* cache, const int32_t* start
   const int all = static_cast<int>(2 * cache->kv_heads);
   a.per = heads_of_a_wave(cache->batch * a.groups, all);
   a.chunks = (all + a.per - 1) / a.per;
-  VGO_REQUIRE(cache->batch <= kMostItems / a.groups / a.chunks, "cache_read: too many tokens");
-  a.items = cache->batch * a.groups * a.chunks;
+  VGO_REQUIRE(cache->batch <= kMostItems / 2 / a.groups / a.chunks, "cache_read: too many tokens");
+  a.items = cache->batch * a.groups * a.chunks * (cache->head_dim / 64);
   return by_type<LaunchRead>(a, cache->head_dim, dtype, as_stream(stream));
 }
