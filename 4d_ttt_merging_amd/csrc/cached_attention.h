@@ -18,6 +18,8 @@
 namespace vgo {
 namespace paged {
 
+typedef __attribute__((__vector_size__(16))) uint32_t u32x4;
+
 struct Attend {
   Pages pages;
   const void* q;
@@ -176,39 +178,34 @@ struct Terms<float> {
 
 union Operand {
   bf16x8 v;
+  u32x4 u;
   uint32_t w[4];
-  bf16x2 p[4];
 };
 
+// Two numbers of byte kAt of a word, as bf16 or f16.
+template <bool kHalf, int kAt>
+__device__ __forceinline__ uint32_t two_of(uint32_t word, float scale) {
+  if constexpr (kHalf) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, kAt));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, kAt));
+}
 // Eight channels of a key: a word of codes, one scale.
-__device__ __forceinline__ bf16x8 key_operand(uint32_t word, float scale) {
-  Operand o;
-  o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
-  o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
-  o.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
-  o.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
-  return o.v;
+template <bool kHalf = false>
+__device__ __forceinline__ u32x4 key_operand(uint32_t word, float scale) {
+  return u32x4{two_of<kHalf, 0>(word, scale), two_of<kHalf, 1>(word, scale), two_of<kHalf, 2>(word, scale),
+               two_of<kHalf, 3>(word, scale)};
 }
 // A channel pair of eight tokens, a scale each: the even channel's operand and the odd one's.
-__device__ __forceinline__ void value_operands(uint2 codes, uint2 scales, bf16x8& even, bf16x8& odd) {
-  const auto at = [](uint32_t word, uint32_t scale, auto i) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale_of<decltype(i)::value>(scale),
-                                                                                 decltype(i)::value));
-  };
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  using I2 = std::integral_constant<int, 2>;
-  using I3 = std::integral_constant<int, 3>;
-  const uint32_t t[8] = {at(codes.x, scales.x, I0()), at(codes.x, scales.x, I1()), at(codes.x, scales.x, I2()),
-                         at(codes.x, scales.x, I3()), at(codes.y, scales.y, I0()), at(codes.y, scales.y, I1()),
-                         at(codes.y, scales.y, I2()), at(codes.y, scales.y, I3())};
-  Operand e, o;
+template <bool kHalf = false>
+__device__ __forceinline__ void value_operands(uint2 codes, uint2 scales, u32x4& even, u32x4& odd) {
+  const uint32_t t[8] = {two_of<kHalf, 0>(codes.x, scale_of<0>(scales.x)), two_of<kHalf, 1>(codes.x, scale_of<1>(scales.x)),
+                         two_of<kHalf, 2>(codes.x, scale_of<2>(scales.x)), two_of<kHalf, 3>(codes.x, scale_of<3>(scales.x)),
+                         two_of<kHalf, 0>(codes.y, scale_of<0>(scales.y)), two_of<kHalf, 1>(codes.y, scale_of<1>(scales.y)),
+                         two_of<kHalf, 2>(codes.y, scale_of<2>(scales.y)), two_of<kHalf, 3>(codes.y, scale_of<3>(scales.y))};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    e.w[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x05040100);
-    o.w[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x07060302);
+    even[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x05040100);
+    odd[i] = __builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x07060302);
   }
-  even = e.v, odd = o.v;
 }
 // Scale bytes of eight tokens with those from `valid` on as zero: what lies past a length may be anything, and a scale of
 // 255 would make a probability of zero NaN.
@@ -216,12 +213,12 @@ __device__ __forceinline__ uint2 kept_scales(uint2 s, int valid) {
   const uint64_t keep = valid >= 8 ? ~uint64_t{0} : valid <= 0 ? 0 : (uint64_t{1} << (8 * valid)) - 1;
   return {s.x & static_cast<uint32_t>(keep), s.y & static_cast<uint32_t>(keep >> 32)};
 }
-// x as kTerms bf16 terms, the first ones rounded to nearest: exact but for what the last one leaves.
-template <int kTerms>
-__device__ __forceinline__ void split(float x, bf16_t (&t)[kTerms]) {
+// x as kTerms terms, the first ones rounded to nearest: exact but for what the last one leaves.
+template <int kTerms, typename N>
+__device__ __forceinline__ void split(float x, N (&t)[kTerms]) {
 #pragma unroll
   for (int i = 0; i < kTerms; ++i) {
-    t[i] = static_cast<bf16_t>(x);
+    t[i] = static_cast<N>(x);
     x -= static_cast<float>(t[i]);
   }
 }
@@ -234,7 +231,7 @@ struct ManyShape {
   int tile_rows, resident;  // rows of a work-group, work-groups that a CU holds
 };
 template <typename T>
-ManyShape many_shape(int head_dim);
+ManyShape many_shape(int head_dim, bool causal);
 template <typename T>
 int launch_many(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
 

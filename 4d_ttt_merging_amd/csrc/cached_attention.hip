@@ -82,11 +82,11 @@ int merge(const Attend& a, int head_dim, hipStream_t s) {
 }  // namespace
 
 template <>
-ManyShape many_shape<bf16_t>(int head_dim);
+ManyShape many_shape<bf16_t>(int head_dim, bool causal);
 template <>
-ManyShape many_shape<f16_t>(int head_dim);
+ManyShape many_shape<f16_t>(int head_dim, bool causal);
 template <>
-ManyShape many_shape<float>(int head_dim);
+ManyShape many_shape<float>(int head_dim, bool causal);
 template <>
 int launch_many<bf16_t>(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
 template <>
@@ -145,7 +145,9 @@ Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, int causa
   Plan p{};
   const int64_t rows = n_query * (heads / c->kv_heads);
   const int dim = static_cast<int>(c->head_dim);
-  const ManyShape shape = dtype == VGO_BF16 ? many_shape<bf16_t>(dim) : dtype == VGO_F16 ? many_shape<f16_t>(dim) : many_shape<float>(dim);
+  const ManyShape shape = dtype == VGO_BF16  ? many_shape<bf16_t>(dim, causal)
+                          : dtype == VGO_F16 ? many_shape<f16_t>(dim, causal)
+                                             : many_shape<float>(dim, causal);
   const int64_t over = rows % shape.tile_rows;
   // Rows of the large tiles.
   const int64_t split = rows <= kFewRows ? 0 : over <= kFewRows && rows >= 4 * shape.tile_rows ? rows - over : rows;

@@ -9,9 +9,8 @@ int launch_many<float>(const Attend& a, int64_t pieces, int head_dim, hipStream_
   return head_dim == 64 ? run_many<float, 64>(a, pieces, s) : run_many<float, 128>(a, pieces, s);
 }
 template <>
-ManyShape many_shape<float>(int head_dim) {
-  return head_dim == 64 ? ManyShape{32 * Many<float, 64>::kTiles * Many<float, 64>::kWaves, 4 * Many<float, 64>::kResident / Many<float, 64>::kWaves}
-                        : ManyShape{32 * Many<float, 128>::kTiles * Many<float, 128>::kWaves, 4 * Many<float, 128>::kResident / Many<float, 128>::kWaves};
+ManyShape many_shape<float>(int head_dim, bool causal) {
+  return head_dim == 64 ? shape_of<float, 64>(causal) : shape_of<float, 128>(causal);
 }
 
 }  // namespace paged

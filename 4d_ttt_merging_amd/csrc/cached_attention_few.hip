@@ -166,7 +166,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     for (int i = 0; i < 2; ++i) {
       const float scale = scale_of<0>(codes.ks[i]);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) keys[i][s] = key_operand(s % 2 ? codes.k[i][s / 2].y : codes.k[i][s / 2].x, scale);
+      for (int s = 0; s < kSteps; ++s)
+        keys[i][s] = __builtin_bit_cast(bf16x8, key_operand(s % 2 ? codes.k[i][s / 2].y : codes.k[i][s / 2].x, scale));
     }
     Operand weights[NT][kP];
 #pragma unroll
@@ -224,8 +225,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     for (int u = 0; u < D / 32; ++u) {
       uint2 scales = codes.vs[u];
       if (!inside) scales = kept_scales(scales, piece.length - t0 - 8 * g);
-      bf16x8 even, odd;
-      value_operands(codes.v[u], scales, even, odd);
+      u32x4 two[2];
+      value_operands(codes.v[u], scales, two[0], two[1]);
+      const bf16x8 even = __builtin_bit_cast(bf16x8, two[0]), odd = __builtin_bit_cast(bf16x8, two[1]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -1,13 +1,18 @@
 // Attention over the paged cache for many queries (chunks and prompts).
 //
-// kWaves waves of 32 MT rows each share 64 tokens at a time: the codes come into registers two tiles ahead, are
+// kWaves waves of 32 rows each share 64 tokens at a time: the codes come into registers two tiles ahead, are
 // converted once for all waves into operands of the 32 x 32 matrix instructions and written to LDS in the order in which
 // their lanes read them (16 bytes a lane, no bank conflicts), double-buffered, one barrier a tile:
 //   scores^T = K Q^T; row m of a block of 32 tokens holds token 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so
 //     that a lane's sixteen scores are two operands of the next product as they stand
 //   out^T += V^T P^T, a lane having converted two channels of eight tokens, operands of two tiles
 // One reference maximum a row, moved only where a score passes it by 2^8.
+//
+// f16: where a piece's scales let keys and values be f16 numbers, and they nearly always do, the products are f16 ones
+// (F16_NATIVE).  Else, and in fp32, bf16 terms (cached_attention.h).
 #pragma once
+
+#include <type_traits>
 
 #include "cached_attention.h"
 
@@ -32,30 +37,75 @@ __device__ __forceinline__ float pair_sum(bf16x2 x, float sum) {
   return __builtin_amdgcn_fdot2_f32_bf16(x, one, sum, false);
 }
 
-// How a type and width are run: waves of a work-group, 32-row tiles of a wave, waves that a SIMD is to hold.
-template <typename T, int D>
+// How a type and width are run: waves of a work-group, waves that a SIMD is to hold.  More waves share what is converted
+// and read from LDS; fewer leave less idle where a causal tile ends.  16 heads, us with 4 waves (2 a SIMD), 8 (2), 8 (4):
+//   bf16  64 channels, 8,192 x 8,192   392 384 327    causal  193 211 205
+//   f16   64                           398 383 352            198 210 247
+//   bf16 128                           567 536 1,628 (registers spilled);  f16, 4,096 x 8,192  331 301 1,121
+//   fp32  64, 2,048 x 2,048             87  82 136;   128  122 114 577;   8 heads of 261 x 1,044, 64  18 21 33
+template <typename T, int D, bool kCausal>
 struct Many {
-  static constexpr int kWaves = 4, kTiles = 1, kResident = 2;
+  static constexpr int kWaves = D == 128 ? 8 : 4, kResident = 2;
+};
+template <bool kCausal>
+struct Many<bf16_t, 64, kCausal> {
+  static constexpr int kWaves = 8, kResident = 4;
 };
 template <>
-struct Many<bf16_t, 64> {
-  static constexpr int kWaves = 8, kTiles = 1, kResident = 4;
-};
-template <>
-struct Many<bf16_t, 128> {
-  static constexpr int kWaves = 8, kTiles = 1, kResident = 2;
+struct Many<f16_t, 64, false> {
+  static constexpr int kWaves = 8, kResident = 4;
 };
 
-template <typename T, int D, int kWaves, int MT, int kResident>
+// The operands of a product in its type.
+template <bool kHalf>
+struct Number {
+  using type = bf16_t;
+  using vec = bf16x8;
+  static __device__ __forceinline__ f32x16 product(vec a, vec b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Number<true> {
+  using type = f16_t;
+  using vec = f16x8;
+  static __device__ __forceinline__ f32x16 product(vec a, vec b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+// Whether tokens [begin, end) are f16 numbers: keys exactly (scales from 2^-23, whose halves are f16's smallest numbers, to 2^13;
+// or below 2^-63, where zero is as good), values to f16's smallest number (to 2^13), as far as their sums are
+// rounded in any case.  All threads of a work-group together.
+template <int D, int kThreads>
+__device__ __forceinline__ bool all_half(const Attend& a, int64_t b, int hk, int begin, int end) {
+  using L = Layout<D>;
+  constexpr int kWords = 2 * D / 16;  // of 16 bytes, keys' scales first
+  bool fit = true;
+  const int blocks = (end - begin + kBlock - 1) / kBlock;
+  for (int i = threadIdx.x; i < blocks * kWords; i += kThreads) {
+    const int t0 = begin + i / kWords * kBlock, at = i % kWords;
+    const int page = page_of(a.pages, b, t0);
+    if (page < 0) continue;
+    const i32x4 word = *reinterpret_cast<const i32x4*>(a.pages.data + block_of<D>(a.pages, page, hk, t0) + L::kKeyScales + 16 * at);
+    const bool key = at < kWords / 2;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int byte = 16 * at + e;
+      const int token = key ? byte / L::kParts : (byte - D) / L::kScaleGroup * 8 + byte % 8;
+      const uint32_t scale = (static_cast<uint32_t>(word[e / 4]) >> (e % 4 * 8)) & 0xff;
+      const bool fine = scale <= 140 && (!key || scale >= 104 || scale <= 64);
+      fit &= fine || t0 + token >= end;
+    }
+  }
+  return __syncthreads_and(fit);
+}
+
+template <typename T, int D, int kWaves, int kResident>
 __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Attend a) {
   using L = Layout<D>;
-  constexpr int kQ = ManyTerms<T>::kQuery, kP = ManyTerms<T>::kWeight;
   constexpr int kSteps = D / 16;        // products over a row's channels
   constexpr int kOut = D / 32;          // tiles of 32 channels
   constexpr bool kApart = kWaves == 8;  // half the waves convert keys, half values
-  // [buffer][block of 32 tokens][step][lane], [buffer][block][tile][step of 16 tokens][lane]
-  __shared__ bf16x8 keys[2][2][kSteps][64];
-  __shared__ bf16x8 values[2][2][kOut][2][64];
+  // [buffer][block of 32 tokens][step][lane], [buffer][block][tile][step of 16 tokens][lane]: operands of 16 bytes
+  __shared__ u32x4 keys[2][2][kSteps][64];
+  __shared__ u32x4 values[2][2][kOut][2][64];
   __shared__ uint2 bias[2][64];  // three bf16 terms of what is added to a token's scores, before the scale
   const int lane = lane_id(), m = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -75,36 +125,11 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   if (piece.begin > 0 && piece.begin >= stop) return;  // (merge_kernel does not ask for it)
   const bool whole = piece.begin == 0 && stop <= piece.end;
 
-  const int row0 = tile0 + wave * 32 * MT;
-  bf16x8 q[MT][kSteps][kQ];
-  int place[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int row = row0 + 32 * mt + m, token = row / a.group;
-    const bool real = row < count * a.group;
-    place[mt] = !real ? -1 : a.causal ? place0 + token : INT32_MAX;
-    const T* from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (hk * a.group + row % a.group) * a.q_stride[1] +
-                    token * a.q_stride[2] + 8 * h;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      float v[8] = {};
-      if (real) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const f32x4 four = load4(from + 16 * s + 4 * e);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        bf16_t t[kQ];
-        split<kQ>(v[i], t);
-#pragma unroll
-        for (int n = 0; n < kQ; ++n) q[mt][s][n][i] = t[n];
-      }
-    }
-  }
+  const int row0 = tile0 + wave * 32, row = row0 + m;
+  const int place = row >= count * a.group ? -1 : a.causal ? place0 + row / a.group : INT32_MAX;
+  // Channels 16 s + 8 h .. of the lane's row (zeros where there is no query).
+  const T* query = static_cast<const T*>(a.q) + b * a.q_stride[0] + (hk * a.group + row % a.group) * a.q_stride[1] +
+                   row / a.group * a.q_stride[2] + 8 * h;
   // The first place of the wave's rows: tiles up to it need no causal mask.
   const int least = a.causal ? place0 + row0 / a.group : INT32_MAX;
   const bool idle = row0 >= count * a.group;
@@ -163,16 +188,17 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       for (int e = 0; e < D / 64; ++e) value_scales[e] = kept_scales(value_scales[e], kept - 8 * group);
     }
   };
-  const auto convert = [&](int buffer) {
+  const auto convert = [&](int buffer, auto half) {
+    constexpr bool kHalf = decltype(half)::value;
     if (does_keys) {
       const float scale = scale_of<0>(key_scale);
-      bf16x8* to = &keys[buffer][block][0][0] + key_row;
+      u32x4* to = &keys[buffer][block][0][0] + key_row;
 #pragma unroll
       for (int e = 0; e < D / 64; ++e) {
         // chunk c of 8 channels: step c / 2, lanes' half c % 2
         const int c = part * (D / 32) + 2 * e;
-        to[c / 2 * 64] = key_operand(key_codes[e].x, scale);
-        to[c / 2 * 64 + 32] = key_operand(key_codes[e].y, scale);
+        to[c / 2 * 64] = key_operand<kHalf>(key_codes[e].x, scale);
+        to[c / 2 * 64 + 32] = key_operand<kHalf>(key_codes[e].y, scale);
       }
       if (part == 0 && (gap_read || a.pages.mass)) {
         const float raw = mass_of(key_mass) * a.per_scale;
@@ -186,172 +212,193 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
     if (does_values) {
 #pragma unroll
       for (int e = 0; e < D / 64; ++e) {
-        bf16x8 even, odd;
-        value_operands(value_codes[e], value_scales[e], even, odd);
+        u32x4 even, odd;
+        value_operands<kHalf>(value_codes[e], value_scales[e], even, odd);
         values[buffer][block][2 * e][group >> 1][(group & 1) * 32 + pair] = even;
         values[buffer][block][2 * e + 1][group >> 1][(group & 1) * 32 + pair] = odd;
       }
     }
   };
 
-  f32x16 acc[MT][kOut] = {};
-  float top[MT], total[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) top[mt] = -INFINITY, total[mt] = 0.0f;
+  f32x16 acc[kOut] = {};
+  float top = -INFINITY, total = 0.0f;
   const int tiles = (end - piece.begin + 63) / 64;  // (none where end is before begin)
-  bool gap = false;
-  if (tiles > 0) {
-    find(0);
-    read(0);
-    find(1);
-    convert(0);
-    gap = gap_read;
-    if (tiles > 1) read(1);
-    find(2);
-  }
-  for (int n = 0; n < tiles; ++n) {
-    const int buffer = n & 1;
-    __syncthreads();
-    const bool uneven = gap || a.pages.mass != nullptr;
-    if (n + 1 < tiles) {
-      convert(buffer ^ 1);
+
+  const auto run = [&](auto half) {
+    constexpr bool kHalf = decltype(half)::value;
+    using N = Number<kHalf>;
+    using vec = typename N::vec;
+    constexpr int kQ = kHalf ? 1 : ManyTerms<T>::kQuery, kP = kHalf ? 1 : ManyTerms<T>::kWeight;
+    // f16 probabilities are taken times 2^7, up to 2^15, which leaves them all their bits down to 2^-21.
+    constexpr float kLift = kHalf ? 7.0f : 0.0f;
+    vec q[kSteps][kQ];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      float v[8] = {};
+      if (row < count * a.group) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x4 four = load4(query + 16 * s + 4 * e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        typename N::type t[kQ];
+        split<kQ>(v[i], t);
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) q[s][n][i] = t[n];
+      }
+    }
+    bool gap = false;
+    if (tiles > 0) {
+      find(0);
+      read(0);
+      find(1);
+      convert(0, half);
       gap = gap_read;
+      if (tiles > 1) read(1);
+      find(2);
     }
-    if (n + 2 < tiles) read(n + 2);
-    find(n + 3);
-    const int t0 = piece.begin + 64 * n;
-    if (idle || (a.causal && t0 > place0 + (row0 + 32 * MT - 1) / a.group)) continue;
-    f32x16 z[MT][2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) z[mt][k] = f32x16{};
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const bf16x8 key_part = keys[buffer][k][s][lane];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int t = kQ - 1; t >= 0; --t)
-            z[mt][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_part, q[mt][s][t], z[mt][k], 0, 0, 0);
+    for (int n = 0; n < tiles; ++n) {
+      const int buffer = n & 1;
+      __syncthreads();
+      const bool uneven = gap || a.pages.mass != nullptr;
+      if (n + 1 < tiles) {
+        convert(buffer ^ 1, half);
+        gap = gap_read;
       }
-    }
-    const bool diagonal = t0 + 63 > least;
-    if (uneven) {
-      // What is added to a token's scores, and what has no place: one more step of the product, by ones.
+      if (n + 2 < tiles) read(n + 2);
+      find(n + 3);
+      const int t0 = piece.begin + 64 * n;
+      if (idle || (a.causal && t0 > place0 + (row0 + 31) / a.group)) continue;
+      f32x16 z[2] = {};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint2 t = bias[buffer][32 * k + m];
-        Operand o, one;
-        o.w[0] = h == 0 ? t.x : 0, o.w[1] = h == 0 ? t.y : 0, o.w[2] = o.w[3] = 0;
-        one.w[0] = h == 0 ? 0x3f803f80u : 0, one.w[1] = h == 0 ? 0x00003f80u : 0, one.w[2] = one.w[3] = 0;
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) z[mt][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(o.v, one.v, z[mt][k], 0, 0, 0);
+        for (int s = 0; s < kSteps; ++s) {
+          const vec key_part = __builtin_bit_cast(vec, keys[buffer][k][s][lane]);
+#pragma unroll
+          for (int t = kQ - 1; t >= 0; --t) z[k] = N::product(key_part, q[s][t], z[k]);
+        }
+      if (uneven) {
+        // What is added to a token's scores, and what has no place: one more step of the product, by ones.
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint2 t = bias[buffer][32 * k + m];
+          Operand o, one;
+          o.w[0] = h == 0 ? t.x : 0, o.w[1] = h == 0 ? t.y : 0, o.w[2] = o.w[3] = 0;
+          one.w[0] = h == 0 ? 0x3f803f80u : 0, one.w[1] = h == 0 ? 0x00003f80u : 0, one.w[2] = one.w[3] = 0;
+          z[k] = Number<false>::product(o.v, one.v, z[k]);
+        }
       }
-    }
-    if (diagonal) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int most = place[mt] - t0 - 8 * h;
+      if (t0 + 63 > least) {
+        const int most = place - t0 - 8 * h;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (32 * k + 16 * (i >> 3) + (i & 7) > most) z[mt][k][i] = -INFINITY;
+            if (32 * k + 16 * (i >> 3) + (i & 7) > most) z[k][i] = -INFINITY;
       }
-    }
-    bf16x8 weights[MT][2][2][kP];
+      float local = z[0][0];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float local = z[mt][0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) local = fmaxf(local, z[mt][i >> 4][i & 15]);
+      for (int i = 1; i < 32; ++i) local = fmaxf(local, z[i >> 4][i & 15]);
       local *= a.scale;
-      if (__any(local > top[mt] + kLazyMany)) {
+      if (__any(local > top + kLazyMany)) {
         local = half_max(local);
-        const float to = fmaxf(top[mt], local);
-        const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[mt] - to);
-        top[mt] = to;
-        total[mt] *= shrink;
+        const float to = fmaxf(top, local);
+        const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+        top = to;
+        total *= shrink;
 #pragma unroll
         for (int c = 0; c < kOut; ++c)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[mt][c][e] *= shrink;
+          for (int e = 0; e < 16; ++e) acc[c][e] *= shrink;
       }
-      const float from = top[mt] == -INFINITY ? 0.0f : top[mt];
+      const float from = top == -INFINITY ? 0.0f : top - kLift;
+      vec weights[2][2][kP];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(z[mt][k][i], a.scale, -from));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(z[mt][k][i + 1], a.scale, -from));
-          if constexpr (kP == 1) {
-            // The sum of the rounded probabilities, as the product takes them.
-            const bf16x2 pair = {static_cast<bf16_t>(p0), static_cast<bf16_t>(p1)};
-            total[mt] = pair_sum(pair, total[mt]);
-            weights[mt][k][i >> 3][0][i & 7] = pair[0], weights[mt][k][i >> 3][0][(i & 7) + 1] = pair[1];
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(z[k][i], a.scale, -from));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(z[k][i + 1], a.scale, -from));
+          typename N::type t0[kP], t1[kP];
+          split<kP>(p0, t0), split<kP>(p1, t1);
+          if constexpr (kP == 1 && !kHalf) {
+            total = pair_sum(bf16x2{t0[0], t1[0]}, total);  // of the rounded ones, as the product takes them
           } else {
-            total[mt] += p0 + p1;
-            bf16_t t0[kP], t1[kP];
-            split<kP>(p0, t0), split<kP>(p1, t1);
-#pragma unroll
-            for (int w = 0; w < kP; ++w) weights[mt][k][i >> 3][w][i & 7] = t0[w], weights[mt][k][i >> 3][w][(i & 7) + 1] = t1[w];
+            total += p0 + p1;
           }
+#pragma unroll
+          for (int w = 0; w < kP; ++w) weights[k][i >> 3][w][i & 7] = t0[w], weights[k][i >> 3][w][(i & 7) + 1] = t1[w];
         }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int c = 0; c < kOut; ++c)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const vec value = __builtin_bit_cast(vec, values[buffer][k][c][t][lane]);
+#pragma unroll
+            for (int w = kP - 1; w >= 0; --w) acc[c] = N::product(value, weights[k][t][w], acc[c]);
+          }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int c = 0; c < kOut; ++c)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bf16x8 value = values[buffer][k][c][t][lane];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int w = kP - 1; w >= 0; --w)
-              acc[mt][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value, weights[mt][k][t][w], acc[mt][c], 0, 0, 0);
-        }
+    top -= kLift;
+  };
+  if constexpr (std::is_same_v<T, f16_t>) {
+    if (all_half<D, kWaves * 64>(a, b, hk, piece.begin, end)) run(std::true_type());
+    else run(std::false_type());
+  } else {
+    run(std::false_type());
   }
 
   // A lane has, for its row, channels 64 c + 16 j + 8 h .. + 7 of tiles 2 c and 2 c + 1.
+  total = half_sum(total);
+  if (row >= min(tile0 + a.tile_rows, a.last_row)) return;
+  const bool none = row >= count * a.group || top == -INFINITY;
+  const float share = whole ? (none ? 0.0f : 1.0f / total) : 1.0f;
+  const int64_t place_of = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + row - tile0;
+  T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
+           row / a.group * a.out_stride[2];
+  float* sums = a.sums + place_of * D;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int row = row0 + 32 * mt + m;
-    total[mt] = half_sum(total[mt]);
-    if (row >= min(tile0 + a.tile_rows, a.last_row)) continue;
-    const bool none = row >= count * a.group || top[mt] == -INFINITY;
-    const float share = whole ? (none ? 0.0f : 1.0f / total[mt]) : 1.0f;
-    const int64_t place_of = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + row - tile0;
-    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
-             row / a.group * a.out_stride[2];
-    float* sums = a.sums + place_of * D;
+  for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c)
+    for (int j = 0; j < 4; ++j) {
+      const int channel = 64 * c + 16 * j + 8 * h;
+      f32x4 v[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int channel = 64 * c + 16 * j + 8 * h;
-        f32x4 v[2];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i >> 2][i & 3] = none && whole ? 0.0f : acc[mt][2 * c + (i & 1)][4 * j + i / 2] * share;
-        if (whole) {
-          store4(out + channel, v[0]);
-          store4(out + channel + 4, v[1]);
-        } else {
-          store4(sums + channel, v[0]);
-          store4(sums + channel + 4, v[1]);
-        }
+      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = none && whole ? 0.0f : acc[2 * c + (i & 1)][4 * j + i / 2] * share;
+      if (whole) {
+        store4(out + channel, v[0]);
+        store4(out + channel + 4, v[1]);
+      } else {
+        store4(sums + channel, v[0]);
+        store4(sums + channel + 4, v[1]);
       }
-    if (!whole && h == 0) a.ends[place_of] = {top[mt], total[mt]};
-  }
+    }
+  if (!whole && h == 0) a.ends[place_of] = {top, total};
 }
 
+template <typename M>
+ManyShape shape_of() {
+  return {32 * M::kWaves, 4 * M::kResident / M::kWaves};
+}
+template <typename T, int D>
+ManyShape shape_of(bool causal) {
+  return causal ? shape_of<Many<T, D, true>>() : shape_of<Many<T, D, false>>();
+}
 template <typename T, int D>
 int run_many(const Attend& a, int64_t pieces, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(pieces * a.tiles * a.pages.kv_heads);
-  using M = Many<T, D>;
-  many_kernel<T, D, M::kWaves, M::kTiles, M::kResident><<<grid, M::kWaves * 64, 0, s>>>(a);
+  const auto run = [&](auto causal) {
+    using M = Many<T, D, decltype(causal)::value>;
+    many_kernel<T, D, M::kWaves, M::kResident><<<grid, M::kWaves * 64, 0, s>>>(a);
+  };
+  if (a.causal) run(std::true_type());
+  else run(std::false_type());
   return check_launch("cached_attn");
 }
 

@@ -117,7 +117,10 @@ def attention(q, pages: Pages, table, lengths, counts=None, *, causal=False, sca
     Beside these relative ones, what is below the normal numbers of fp32 and bf16, 2^-126, may be taken as zero: a
     probability p itself, which loses at most 2^-126, or a bf16 term of it -- the second and third are below p 2^-8 and
     p 2^-16, so that one is lost only where p < 2^-118 or p < 2^-110, and with it less than p 2^-8 < 2^-126 or
-    p 2^-16 < 2^-126; the sum of the running products likewise, once a key.  Together less than 2^-124 (|v_j| + 1) a key."""
+    p 2^-16 < 2^-126; the sum of the running products likewise, once a key.  Together less than 2^-124 (|v_j| + 1) a key.
+    f16: a probability of 2^-21 of the reference or less may be taken to a multiple of 2^-31 of it (the reference is up to
+    2^8 times the largest's below it, never above): off by 2^-32 |v_j| a key; a value below 2^-23 to a multiple of 2^-24 (off by 2^-25);
+    the result, where it is less than f16's smallest normal number, to a multiple of 2^-24."""
     u, half = 2.0 ** -24, torch.finfo(q.dtype).eps / 2
     p_bits = half if p_bits is None else p_bits
     b, h, n, d = q.shape
@@ -157,5 +160,5 @@ def attention(q, pages: Pages, table, lengths, counts=None, *, causal=False, sca
             weight = (p * (off + p_bits + sums)) @ value.abs()
             bound[i, head, :count] = weight + o.abs() * ((p * off).sum(1, keepdim=True) + sums + half) + tiny
             if q.dtype == torch.float16:
-                bound[i, head, :count] += 2.0 ** -25
+                bound[i, head, :count] += 2.0 ** -32 * value.abs().sum(0) + 2.0 ** -24
     return out, bound

@@ -277,3 +277,40 @@ def test_results_are_the_same_bits(vgo, device):
         first = call()
         for _ in range(4):
             assert torch.equal(first, call())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("what", ["small", "zeros", "keys too small", "keys too large", "values too large", "past the length"])
+def test_scales_beyond_f16(vgo, device, what, causal, dim):
+    """Keys and values that f16 holds, and those it does not (f16 queries, many of them: the products' type goes by it)."""
+    table, pages = layout(1, 260, 64, 28)
+    both = Both(vgo, device, pages, 1, 64, dim)
+    both.fill(29)
+    g = torch.Generator().manual_seed(30)
+    scale = {"small": 2.0 ** -20, "zeros": 0.0, "keys too small": 2.0 ** -23, "keys too large": 2.0 ** 16}.get(what, 1.0)
+    k, v = torch.randn(1, 1, 3, dim, generator=g) * scale, torch.randn(1, 1, 3, dim, generator=g)
+    q = torch.randn(1, 2, 140, dim, generator=g).half() * (1.0 if scale <= 1 else 2.0 ** -14)
+    if what == "values too large":
+        v[:, :, 1] *= 2.0 ** 16
+        v[:, :, 1, ::2] = 0.0
+        k[:, :, 1], q = -8.0, q.abs() + 1.0  # (an improbable key: what comes out is finite in f16)
+    both.append(k, v, table, int32([258 if what == "past the length" else 77]))
+    if what == "past the length":
+        bad = torch.full((1, 1, 2, dim), math.nan)
+        both.append(bad, bad, table, int32([258]))
+    both.attend(q, table, int32([258 if what == "past the length" else 260]), causal=causal)
+
+
+def test_f16_probabilities_keep_their_bits(vgo, device):
+    """One key far above 250 equal ones, whose probabilities are 2^-18 of it each."""
+    table, pages = layout(1, 256, 64, 31)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    k = torch.zeros(1, 1, 256, 64)
+    k[0, 0, 100, 0] = 6.0
+    v = torch.randn(1, 1, 256, 64, generator=torch.Generator().manual_seed(32))
+    v[0, 0, 100] = 0.0
+    both.append(k, v, table, int32([0]))
+    q = torch.zeros(1, 1, 130, 64).half()
+    q[..., 0] = 18 * math.log(2.0) / 6.0
+    both.attend(q, table, int32([256]), scale=1.0)
