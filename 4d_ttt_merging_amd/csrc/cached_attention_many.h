@@ -37,23 +37,34 @@ __device__ __forceinline__ float pair_sum(bf16x2 x, float sum) {
   return __builtin_amdgcn_fdot2_f32_bf16(x, one, sum, false);
 }
 
-// How a type and width are run: waves of a work-group, waves that a SIMD is to hold.  More waves share what is converted
-// and read from LDS; fewer leave less idle where a causal tile ends.  16 heads, us with 4 waves (2 a SIMD), 8 (2), 8 (4):
-//   bf16  64 channels, 8,192 x 8,192   392 384 327    causal  193 211 205
-//   f16   64                           398 383 352            198 210 247
-//   bf16 128                           567 536 1,628 (registers spilled);  f16, 4,096 x 8,192  331 301 1,121
-//   fp32  64, 2,048 x 2,048             87  82 136;   128  122 114 577;   8 heads of 261 x 1,044, 64  18 21 33
+// How a type and width are run: waves of a work-group, waves that a SIMD is to hold, whether operands are read from LDS in
+// groups ahead of their products (one by one, as the compiler has it to save registers, each product waits out a read).  More
+// waves share what is converted and read from LDS; fewer leave less idle where a causal tile ends.  16 heads, us with
+// 4 waves (2 a SIMD, 3, 3 grouped), 8 (2, 2 grouped, 4, 4 grouped):
+//   bf16  64 channels, 8,192 x 8,192   382 381 375   385 376 321 340     causal  194 195 184   212 206 204 231
+//   f16   64                           399 409 416   381 386 364 379             199 205 202   206 211 248 254
+//   bf16 128 (else 4: 2, 2 grouped)    572 588       535 534 (4 a SIMD: registers spilled, 1,624 and more)
+//   f16  128, 4,096 x 8,192            324 328       290 282;   fp32, 2,048 x 2,048  121 225  112 205;  64 channels  84 84  80 81
+//   fp32  64, 8 heads of 261 x 1,044    18  17        20  21
 template <typename T, int D, bool kCausal>
 struct Many {
   static constexpr int kWaves = D == 128 ? 8 : 4, kResident = 2;
+  static constexpr bool kGrouped = D == 128 && !std::is_same_v<T, float>;
 };
-template <bool kCausal>
-struct Many<bf16_t, 64, kCausal> {
+template <>
+struct Many<bf16_t, 64, false> {
   static constexpr int kWaves = 8, kResident = 4;
+  static constexpr bool kGrouped = false;
+};
+template <>
+struct Many<bf16_t, 64, true> {
+  static constexpr int kWaves = 4, kResident = 3;
+  static constexpr bool kGrouped = true;
 };
 template <>
 struct Many<f16_t, 64, false> {
   static constexpr int kWaves = 8, kResident = 4;
+  static constexpr bool kGrouped = false;
 };
 
 // The operands of a product in its type.
@@ -97,7 +108,7 @@ __device__ __forceinline__ bool all_half(const Attend& a, int64_t b, int hk, int
   return __syncthreads_and(fit);
 }
 
-template <typename T, int D, int kWaves, int kResident>
+template <typename T, int D, int kWaves, int kResident, bool kGrouped>
 __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Attend a) {
   using L = Layout<D>;
   constexpr int kSteps = D / 16;        // products over a row's channels
@@ -251,6 +262,8 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
         for (int n = 0; n < kQ; ++n) q[s][n][i] = t[n];
       }
     }
+    // (Else the first product of every tile waits for whatever is outstanding, in case it is these.)
+    wait_vmem<0>();
     bool gap = false;
     if (tiles > 0) {
       find(0);
@@ -274,14 +287,19 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       const int t0 = piece.begin + 64 * n;
       if (idle || (a.causal && t0 > place0 + (row0 + 31) / a.group)) continue;
       f32x16 z[2] = {};
+      vec key_parts[2][kSteps];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) key_parts[k][s] = __builtin_bit_cast(vec, keys[buffer][k][s][lane]);
+        if constexpr (kGrouped) __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const vec key_part = __builtin_bit_cast(vec, keys[buffer][k][s][lane]);
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int t = kQ - 1; t >= 0; --t) z[k] = N::product(key_part, q[s][t], z[k]);
-        }
+          for (int t = kQ - 1; t >= 0; --t) z[k] = N::product(key_parts[k][s], q[s][t], z[k]);
       if (uneven) {
         // What is added to a token's scores, and what has no place: one more step of the product, by ones.
 #pragma unroll
@@ -334,16 +352,24 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
 #pragma unroll
           for (int w = 0; w < kP; ++w) weights[k][i >> 3][w][i & 7] = t0[w], weights[k][i >> 3][w][(i & 7) + 1] = t1[w];
         }
+      vec value_parts[2][kOut][2];
+      if constexpr (kGrouped) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int c = 0; c < kOut; ++c)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const vec value = __builtin_bit_cast(vec, values[buffer][k][c][t][lane]);
+          for (int t = 0; t < 2; ++t) value_parts[k][c][t] = __builtin_bit_cast(vec, values[buffer][k][c][t][lane]);
+        if constexpr (kGrouped) __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
-            for (int w = kP - 1; w >= 0; --w) acc[c] = N::product(value, weights[k][t][w], acc[c]);
-          }
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < kOut; ++c)
+#pragma unroll
+            for (int w = kP - 1; w >= 0; --w) acc[c] = N::product(value_parts[k][c][t], weights[k][t][w], acc[c]);
     }
     top -= kLift;
   };
@@ -395,7 +421,7 @@ int run_many(const Attend& a, int64_t pieces, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(pieces * a.tiles * a.pages.kv_heads);
   const auto run = [&](auto causal) {
     using M = Many<T, D, decltype(causal)::value>;
-    many_kernel<T, D, M::kWaves, M::kResident><<<grid, M::kWaves * 64, 0, s>>>(a);
+    many_kernel<T, D, M::kWaves, M::kResident, M::kGrouped><<<grid, M::kWaves * 64, 0, s>>>(a);
   };
   if (a.causal) run(std::true_type());
   else run(std::false_type());
