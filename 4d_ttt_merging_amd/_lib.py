@@ -225,7 +225,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.POINTER(PagedCacheStruct), _c_p, _c_p, _c_i64, _c_p, _c_p, _c_int, _c_p,
     ]),
     "vgo_cached_attn_workspace": (_c_int, [
-        ctypes.POINTER(PagedCacheStruct), _c_i64, _c_i64, _c_int, _c_int, ctypes.POINTER(_c_size),
+        ctypes.POINTER(PagedCacheStruct), _c_i64, _c_i64, _c_int, _c_int, _c_int, ctypes.POINTER(_c_size),
     ]),
     "vgo_cached_attn_fwd": (_c_int, [
         ctypes.POINTER(PagedCacheStruct), _c_p, _i64x3, _c_i64, _c_i64, _c_p, _c_p, _c_int, _c_f32, _c_p, _i64x3,

@@ -10,7 +10,7 @@
 // Work split over the keys: the host does not know the lengths, so the grid holds `slots` pieces more than sequences, and
 // each work-group cuts the sequences' tokens into pieces of one length, which the grid holds whatever the lengths
 // are.  Tiles of rows that see one piece alone are written at once, the others' pieces leave their sums in the workspace
-// for merge_kernel.
+// for a join.
 #pragma once
 
 #include "paged_cache.h"
@@ -35,7 +35,7 @@ struct Attend {
   int32_t first_row, last_row;  // the rows of this launch: from .. to before
   int32_t tiles, tile_rows;   // row tiles of a key head, rows of one
   int32_t slots, least;       // pieces beside one a sequence (0: no splitting), tokens of a piece at least
-  int32_t fold;               // whether all work-groups are there at once
+  int32_t held;               // work-groups that the chip holds at once
   int32_t causal;
   float scale, per_scale;     // times log2(e); 1 / the scale itself
 };
@@ -76,32 +76,52 @@ struct Pieces {
   int mine;    // length of sequence `lane`, of the first 64
   int tokens;  // of a piece: a multiple of 64
 };
-// The shortest pieces of which no more than `slots` beside one a sequence are needed, or nearly so.
+// Row tiles of a sequence that have queries (one at least).
+__device__ __forceinline__ int busy_tiles(const Attend& a, int64_t b) {
+  const int rows = min(count_of(a, b) * a.group, a.last_row) - a.first_row;
+  return max(1, (rows + a.tile_rows - 1) / a.tile_rows);
+}
+// The shortest pieces of which no more than `slots` beside one a sequence are needed, or nearly so, and (kMany), since
+// sequences differ in queries too, whose work-groups that have queries fill the chip about once, or twice where a single
+// round would leave it ragged (2 x 2,058 queries at most over 16,464 tokens of 128 channels, both ragged: one round 282 us, so 242).
+template <bool kMany>
 __device__ __forceinline__ Pieces pieces(const Attend& a) {
-  Pieces p{lane_id() < a.batch ? length_of(a, lane_id()) : 0, INT32_MAX};
+  const bool here = lane_id() < a.batch;
+  Pieces p{here ? length_of(a, lane_id()) : 0, INT32_MAX};
   if (a.slots == 0) return p;
-  const auto over_all = [&](auto of) {  // at most 2^26 a lane, so that 64 of them fit
-    int64_t sum = lane_id() < a.batch ? of(p.mine) : 0;
-    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += of(length_of(a, b));
+  const int weight = kMany && here ? busy_tiles(a, lane_id()) : 1;
+  const auto over_all = [&](auto of) {  // at most 2^25 a lane, so that 64 of them fit
+    int64_t sum = here ? of(p.mine, weight) : 0;
+    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += of(length_of(a, b), kMany ? busy_tiles(a, b) : 1);
     return static_cast<int64_t>(wave_sum(static_cast<uint32_t>(min(sum, int64_t{1} << 25))));
   };
   const int most = a.slots + static_cast<int>(a.batch);
   const auto rounded = [&](int64_t units) {  // of 64 tokens
     return static_cast<int>(min(max(units * 64, static_cast<int64_t>(a.least)), static_cast<int64_t>(INT32_MAX)));
   };
-  const int64_t sum = over_all([](int length) { return (static_cast<int64_t>(length) + 63) / 64; });
+  int64_t target = most;
+  if constexpr (kMany) {
+    const int64_t busy = over_all([&](int, int w) { return static_cast<int64_t>(w) * a.pages.kv_heads; });
+    if (10 * busy >= 9 * static_cast<int64_t>(a.held)) return p;
+    target = 100 * (a.held / busy * busy) >= 85 * static_cast<int64_t>(a.held) ? a.held : 2 * a.held;
+  }
+  const int each = kMany ? a.pages.kv_heads : 1;
+  const int64_t sum = over_all([&](int length, int w) { return (static_cast<int64_t>(length) + 63) / 64 * w * each; });
   // (more than the sums hold: a piece a sequence)
   if (sum >= int64_t{1} << 25) return p;
-  p.tokens = rounded((sum + most - 1) / most);
-  for (int round = 0; round < 3; ++round) {
+  p.tokens = rounded((sum + target - 1) / target);
+  for (int round = 0; round < 4; ++round) {
     const int tokens = p.tokens;
-    const int64_t n = over_all([&](int length) { return static_cast<int64_t>(pieces_of(length, tokens)); });
-    if (n <= most) return p;
-    p.tokens = rounded(p.tokens / 64 * n / most + 1);
+    const int64_t n = over_all([&](int length, int) { return static_cast<int64_t>(pieces_of(length, tokens)); });
+    int64_t groups = n;
+    if constexpr (kMany) groups = over_all([&](int length, int w) { return static_cast<int64_t>(pieces_of(length, tokens)) * w * each; });
+    if (n <= most && (groups <= target || round == 3)) return p;
+    const int64_t by_n = p.tokens / 64 * n / most + 1, by_groups = p.tokens / 64 * groups / target + 1;
+    p.tokens = rounded(max(n > most ? by_n : 0, by_groups));
   }
-  const int tokens = p.tokens;
-  if (over_all([&](int length) { return static_cast<int64_t>(pieces_of(length, tokens)); }) <= most) return p;
-  p.tokens = rounded((sum + a.slots - 1) / a.slots);  // (at most one more a sequence than sum / tokens)
+  // (at most one more a sequence than all the tokens / tokens)
+  const int64_t all = kMany ? over_all([](int length, int) { return (static_cast<int64_t>(length) + 63) / 64; }) : sum;
+  p.tokens = rounded((all + a.slots - 1) / a.slots);
   return p;
 }
 
@@ -113,8 +133,9 @@ struct Piece {
 };
 
 // Piece x of all sequences' pieces in a row.
+template <bool kMany>
 __device__ __forceinline__ Piece piece_of(const Attend& a, int x) {
-  const Pieces all = pieces(a);
+  const Pieces all = pieces<kMany>(a);
   int before = 0;
   for (int64_t b0 = 0; b0 < a.batch; b0 += 64) {
     const int64_t b = b0 + lane_id();
@@ -137,16 +158,9 @@ __device__ __forceinline__ Piece piece_of(const Attend& a, int x) {
   }
   return {-1, 0, 0, 0, 0};
 }
-// What merge_kernel asks of a sequence: its first piece and their length, left by that piece.
+// What the join asks of a sequence: its first piece and their length, left by that piece.
 __device__ __forceinline__ void leave(const Attend& a, const Piece& piece, int x, bool one) {
   if (a.slots > 0 && piece.begin == 0 && one) a.firsts[piece.b] = {x, piece.tokens};
-}
-
-// Which tile the n-th is: of a causal call the longest first, and, where all run at once, the second half of them from
-// the shortest, so that a CU that got a long one gets a short one (16 heads of 8,192 x 8,192 x 64: FOLDED us).
-__device__ __forceinline__ int tile_at(const Attend& a, int n) {
-  const int half = (a.tiles + 1) / 2;
-  return a.fold && n >= half ? n - half : a.tiles - 1 - n;
 }
 
 // Tokens that any row of the tile at row `row0` sees: from 0 to before this one.  `place0`: where a sequence's first query stands.

@@ -8,74 +8,97 @@ namespace vgo {
 namespace paged {
 namespace {
 
-// Joins the pieces of the rows that have several.  A wave takes a row, D / 4 lanes four channels each of every second
-// (fourth) piece: what they read does not depend on what they have read, so that up to 8 (16) pieces take one trip to memory.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void merge_kernel(const Attend a) {
-  constexpr int kLanes = D / 4, kGroups = 64 / kLanes;
-  const int rows = a.last_row - a.first_row, kv = a.pages.kv_heads;
-  const int64_t task = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6));
-  const int hk = static_cast<int>(task % kv), of = static_cast<int>(task / kv % rows);
-  const int64_t b = task / kv / rows;
-  if (b >= a.batch) return;
-  const int2 first = a.firsts[b];
-  const int length = length_of(a, b), count = count_of(a, b);
-  const int row = a.first_row + of, tile = of / a.tile_rows, tokens = first.y;
-  const int stop = stop_of(a, length, count, a.lengths[b] - count, a.first_row + tile * a.tile_rows);
-  const int n = (stop - 1) / tokens + 1;
-  if (stop <= 0 || n <= 1) return;
-  const int group = lane_id() / kLanes, c = lane_id() % kLanes * 4;
-  const int64_t step = static_cast<int64_t>(kv) * a.tiles * a.tile_rows;
-  const int64_t start = first.x * step + (static_cast<int64_t>(hk) * a.tiles + tile) * a.tile_rows + of % a.tile_rows;
+// The sums of a row's parts, as one.
+struct Joined {
   float top = -INFINITY, sum = 0.0f;
   f32x4 v = {};
-  for (int piece = group; piece < n; piece += 4 * kGroups) {
+};
+// Parts part, part + stride, ... of n, from place `start` on by `step`: what is read does not depend on what has been read, so
+// that four parts take one trip to memory.
+template <int D>
+__device__ __forceinline__ void join(const Attend& a, Joined& j, int part, int stride, int n, int64_t start, int64_t step, int c) {
+  for (; part < n; part += 4 * stride) {
     float2 end[4];
-    f32x4 part[4];
+    f32x4 values[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t place = start + min(piece + i * kGroups, n - 1) * step;
+      const int64_t place = start + min(part + i * stride, n - 1) * step;
       end[i] = a.ends[place];
-      part[i] = *reinterpret_cast<const f32x4*>(a.sums + place * D + c);
-      if (piece + i * kGroups >= n) end[i] = {-INFINITY, 0.0f};
+      values[i] = *reinterpret_cast<const f32x4*>(a.sums + place * D + c);
+      if (part + i * stride >= n) end[i] = {-INFINITY, 0.0f};
     }
-    const float most = fmaxf(fmaxf(top, fmaxf(end[0].x, end[1].x)), fmaxf(end[2].x, end[3].x));
+    const float most = fmaxf(fmaxf(j.top, fmaxf(end[0].x, end[1].x)), fmaxf(end[2].x, end[3].x));
     const float from = most == -INFINITY ? 0.0f : most;
-    const float shrink = __builtin_amdgcn_exp2f(top - from);
-    top = most, sum *= shrink;
+    const float shrink = __builtin_amdgcn_exp2f(j.top - from);
+    j.top = most, j.sum *= shrink;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= shrink;
+    for (int e = 0; e < 4; ++e) j.v[e] *= shrink;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float share = __builtin_amdgcn_exp2f(end[i].x - from);
-      sum = fmaf(end[i].y, share, sum);
+      j.sum = fmaf(end[i].y, share, j.sum);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(part[i][e], share, v[e]);
+      for (int e = 0; e < 4; ++e) j.v[e] = fmaf(values[i][e], share, j.v[e]);
     }
   }
-#pragma unroll
-  for (int o = kLanes; o < 64; o <<= 1) {
-    const float other = __shfl_xor(top, o), most = fmaxf(top, other), from = most == -INFINITY ? 0.0f : most;
-    const float mine = __builtin_amdgcn_exp2f(top - from), theirs = __builtin_amdgcn_exp2f(other - from);
-    // (the same products and one sum on both sides: the same bits)
-    sum = sum * mine + __shfl_xor(sum, o) * theirs;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = v[e] * mine + __shfl_xor(v[e], o) * theirs;
-    top = most;
-  }
-  if (group > 0) return;
-  const bool none = row >= count * a.group || top == -INFINITY;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
-  store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
-             row / a.group * a.out_stride[2] + c, v);
 }
 
+// Joins the pieces of `kRows` rows of a tile, where there are several.  D / 4 lanes take four channels of a row each; a
+// wave's others, if kApart (few rows), every second or fourth piece of the same row, else the next rows.
+template <typename T, int D, int kRows, bool kApart>
+__global__ __launch_bounds__(256) void join_kernel(const Attend a) {
+  constexpr int kLanes = D / 4, kGroups = kApart ? 64 / kLanes : 1, kAtOnce = 256 / kLanes / kGroups;
+  const int rows = a.last_row - a.first_row, kv = a.pages.kv_heads, chunks = (rows + kRows - 1) / kRows;
+  const int of0 = static_cast<int>(blockIdx.x % chunks) * kRows, hk = static_cast<int>(blockIdx.x / chunks % kv);
+  const int64_t b = blockIdx.x / chunks / kv;
+  const int2 piece = a.firsts[b];
+  const int count = count_of(a, b), tile = of0 / a.tile_rows;
+  const int stop = stop_of(a, length_of(a, b), count, a.lengths[b] - count, a.first_row + tile * a.tile_rows);
+  const int n = stop <= 0 ? 1 : (stop - 1) / piece.y + 1;
+  if (n <= 1) return;
+  const int64_t step = static_cast<int64_t>(kv) * a.tiles * a.tile_rows;
+  const int64_t start = piece.x * step + (static_cast<int64_t>(hk) * a.tiles + tile) * a.tile_rows - tile * a.tile_rows;
+  const int c = threadIdx.x % kLanes * 4, group = kApart ? lane_id() / kLanes : 0;
+  for (int r = kApart ? threadIdx.x / 64 : threadIdx.x / kLanes; r < kRows && of0 + r < rows; r += kAtOnce) {
+    Joined j;
+    join<D>(a, j, group, kGroups, n, start + of0 + r, step, c);
+#pragma unroll
+    for (int o = kLanes; o < kLanes * kGroups; o <<= 1) {
+      const float other = __shfl_xor(j.top, o), most = fmaxf(j.top, other), from = most == -INFINITY ? 0.0f : most;
+      const float mine = __builtin_amdgcn_exp2f(j.top - from), theirs = __builtin_amdgcn_exp2f(other - from);
+      // (the same products and one sum on both sides: the same bits)
+      j.sum = j.sum * mine + __shfl_xor(j.sum, o) * theirs;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) j.v[e] = j.v[e] * mine + __shfl_xor(j.v[e], o) * theirs;
+      j.top = most;
+    }
+    const int row = a.first_row + of0 + r;
+    const bool none = row >= count * a.group || j.top == -INFINITY;
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : j.v[e] / j.sum;
+    if (group == 0)
+      store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
+                 row / a.group * a.out_stride[2] + c, v);
+  }
+}
+
+// Rows of a work-group: four, a wave each, where there are few; else 32, so that calls of which no row has several pieces
+// are soon through with them (64 rows of 8 key heads over 16 pieces 42 us with the one, 52 with the other; 3 x 16,464 rows in one
+// piece each 196, 154).
+template <typename T, int D>
+void join_pieces(const Attend& a, hipStream_t s) {
+  const int64_t rows = a.last_row - a.first_row, all = a.batch * a.pages.kv_heads;
+  const bool few = rows * all <= 16384;
+  const int64_t each = few ? 4 : 32;
+  const unsigned grid = static_cast<unsigned>(all * ((rows + each - 1) / each));
+  if (few) join_kernel<T, D, 4, true><<<grid, 256, 0, s>>>(a);
+  else join_kernel<T, D, 32, false><<<grid, 256, 0, s>>>(a);
+}
 template <typename T>
-int merge(const Attend& a, int head_dim, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>((a.batch * (a.last_row - a.first_row) * a.pages.kv_heads + 3) / 4);
-  if (head_dim == 64) merge_kernel<T, 64><<<grid, 256, 0, s>>>(a);
-  else merge_kernel<T, 128><<<grid, 256, 0, s>>>(a);
+int join_pieces(const Attend& a, int head_dim, hipStream_t s) {
+  if (head_dim == 64) join_pieces<T, 64>(a, s);
+  else join_pieces<T, 128>(a, s);
   return check_launch("cached_attn");
 }
 
@@ -108,7 +131,7 @@ struct Part {
   int64_t first_row, last_row;
   int tile_rows, slots;
   int64_t least;
-  bool fold;
+  int held;
   int64_t tiles, pieces;
   size_t sums, ends, firsts;  // bytes of the workspace
   size_t bytes() const { return sums + ends + firsts; }
@@ -118,18 +141,21 @@ struct Plan {
   Part part[2];
   size_t bytes() const { return part[0].bytes() + (parts > 1 ? part[1].bytes() : 0); }
 };
-Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool few, int causal, const ManyShape& shape) {
+Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool few, bool ragged, const ManyShape& shape) {
   Part p{};
   const int64_t rows = last_row - first_row, capacity = c->table_width * c->page_size;
   p.few = few, p.first_row = first_row, p.last_row = last_row;
   p.tile_rows = few ? few_tile(rows) : shape.tile_rows;
   p.least = few ? kLeastFew : kLeastMany;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-  // As many work-groups as the chip holds at once; of causal calls that leave room, whose tiles differ, twice as many.
+  // Few queries: as many work-groups as the chip holds at once.  Many, of which some sequences may have fewer than others: more,
+  // which those that have queries then share (a grid of four times as many is through with its idle ones in 8 us);
+  // none beside one a tile where all are busy and fill it.
   const int64_t held = static_cast<int64_t>(few ? 2 : shape.resident) * device_cus(), beside = c->kv_heads * p.tiles;
-  const bool uneven = causal && !few;
-  const int64_t slots = (uneven && c->batch * beside <= held / 2 ? 2 * held : held) / beside - c->batch;
-  p.fold = uneven && c->batch * beside <= held;
+  const bool full = !few && !ragged && 10 * c->batch * beside >= 9 * held;
+  const int64_t rounds = few || (p.tiles == 1 && c->batch * beside <= held / 4) ? 1 : p.tiles < 8 ? 2 : 4;
+  const int64_t slots = full ? 0 : rounds * held / beside - c->batch;
+  p.held = static_cast<int>(held);
   // (no more pieces than the tables could hold)
   p.slots = capacity <= (few ? kWholeFew : kLeastMany) ? 0 : static_cast<int>(std::max<int64_t>(0, std::min(slots, c->batch * ((capacity - 1) / p.least))));
   p.pieces = c->batch + p.slots;
@@ -141,7 +167,7 @@ Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool
   }
   return p;
 }
-Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, int causal, int dtype) {
+Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, bool causal, bool ragged, int dtype) {
   Plan p{};
   const int64_t rows = n_query * (heads / c->kv_heads);
   const int dim = static_cast<int>(c->head_dim);
@@ -151,8 +177,8 @@ Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, int causa
   const int64_t over = rows % shape.tile_rows;
   // Rows of the large tiles.
   const int64_t split = rows <= kFewRows ? 0 : over <= kFewRows && rows >= 4 * shape.tile_rows ? rows - over : rows;
-  if (split > 0) p.part[p.parts++] = part_of(c, 0, split, false, causal, shape);
-  if (split < rows) p.part[p.parts++] = part_of(c, split, rows, true, causal, shape);
+  if (split > 0) p.part[p.parts++] = part_of(c, 0, split, false, ragged, shape);
+  if (split < rows) p.part[p.parts++] = part_of(c, split, rows, true, ragged, shape);
   return p;
 }
 
@@ -179,7 +205,7 @@ bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
 }  // namespace vgo
 
 extern "C" int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int causal,
-                                         int dtype, size_t* bytes) {
+                                         int ragged, int dtype, size_t* bytes) {
   using namespace vgo;
   using namespace vgo::paged;
   const int status = check_attend(cache, heads, n_query, dtype);
@@ -187,7 +213,7 @@ extern "C" int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t h
   VGO_REQUIRE(bytes, "cached_attn: null pointer");
   *bytes = 0;
   if (cache->batch == 0 || n_query == 0) return VGO_OK;
-  const Plan p = plan_of(cache, heads, n_query, causal, dtype);
+  const Plan p = plan_of(cache, heads, n_query, causal != 0, ragged != 0, dtype);
   *bytes = p.bytes();
   return VGO_OK;
 }
@@ -207,7 +233,7 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
               "cached_attn: q and out must be 16-byte aligned, with strides of whole 16 bytes");
   // (a grid's threads are counted in 32 bits; rows and their places among a launch's in 31)
   VGO_REQUIRE(cache->batch < kMostThreads / heads / n_query / 32, "cached_attn: too many rows");
-  const Plan p = plan_of(cache, heads, n_query, causal, dtype);
+  const Plan p = plan_of(cache, heads, n_query, causal != 0, counts != nullptr, dtype);
   for (int i = 0; i < p.parts; ++i)
     VGO_REQUIRE(p.part[i].pieces < kMostThreads / 512 / (p.part[i].tiles * cache->kv_heads), "cached_attn: too many rows");
   if (p.bytes() > 0 && (!workspace || workspace_bytes < p.bytes() || !aligned(workspace, 16)))
@@ -226,7 +252,7 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
     const Part& part = p.part[i];
     a.first_row = static_cast<int32_t>(part.first_row), a.last_row = static_cast<int32_t>(part.last_row);
     a.tiles = static_cast<int32_t>(part.tiles), a.tile_rows = part.tile_rows, a.slots = part.slots, a.least = static_cast<int32_t>(part.least);
-    a.fold = part.fold;
+    a.held = part.held;
     a.sums = reinterpret_cast<float*>(ws), a.ends = reinterpret_cast<float2*>(ws + part.sums);
     a.firsts = reinterpret_cast<int2*>(ws + part.sums + part.ends);
     ws += part.bytes();
@@ -235,9 +261,9 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
               : dtype == VGO_F16  ? launch_many<f16_t>(a, part.pieces, dim, s)
                                   : launch_many<float>(a, part.pieces, dim, s);
     if (run == VGO_OK && part.slots > 0) {
-      run = dtype == VGO_BF16  ? merge<bf16_t>(a, dim, s)
-            : dtype == VGO_F16 ? merge<f16_t>(a, dim, s)
-                               : merge<float>(a, dim, s);
+      run = dtype == VGO_BF16  ? join_pieces<bf16_t>(a, dim, s)
+            : dtype == VGO_F16 ? join_pieces<f16_t>(a, dim, s)
+                               : join_pieces<float>(a, dim, s);
     }
     if (run != VGO_OK) return run;
   }

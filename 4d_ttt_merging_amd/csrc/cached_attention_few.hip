@@ -91,9 +91,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   const int kv = a.pages.kv_heads;
   const int hk = blockIdx.x % kv;
   const int rest = blockIdx.x / kv;
-  const int tile = tile_at(a, rest % a.tiles);
+  const int tile = rest % a.tiles;
   const int x = rest / a.tiles;
-  const Piece piece = piece_of(a, x);
+  const Piece piece = piece_of<false>(a, x);
   if (piece.b < 0) return;
   leave(a, piece, x, threadIdx.x == 0 && hk == 0 && rest % a.tiles == 0);
   const int64_t b = piece.b;
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   const int row0 = a.first_row + tile * a.tile_rows;
   const int place0 = a.lengths[b] - count, stop = stop_of(a, piece.length, count, place0, row0);
   const int end = min(piece.end, stop);
-  if (piece.begin > 0 && piece.begin >= stop) return;  // (merge_kernel does not ask for it)
+  if (piece.begin > 0 && piece.begin >= stop) return;  // (the join does not ask for it)
   const bool whole = piece.begin == 0 && stop <= piece.end;
 
   // Queries: row m of each tile, channels 8 s .. of this lane's D / 4.

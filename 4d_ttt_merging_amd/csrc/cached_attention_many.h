@@ -123,9 +123,9 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   const int kv = a.pages.kv_heads;
   const int hk = blockIdx.x % kv;
   const int rest = blockIdx.x / kv;
-  const int tile = tile_at(a, rest % a.tiles);
+  const int tile = a.tiles - 1 - rest % a.tiles;  // (of a causal call the longest first)
   const int x = rest / a.tiles;
-  const Piece piece = piece_of(a, x);
+  const Piece piece = piece_of<true>(a, x);
   if (piece.b < 0) return;
   leave(a, piece, x, threadIdx.x == 0 && hk == 0 && rest % a.tiles == 0);
   const int64_t b = piece.b;
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   const int tile0 = a.first_row + tile * a.tile_rows;
   const int place0 = a.lengths[b] - count, stop = stop_of(a, piece.length, count, place0, tile0);
   const int end = min(piece.end, stop);
-  if (piece.begin > 0 && piece.begin >= stop) return;  // (merge_kernel does not ask for it)
+  if (piece.begin > 0 && piece.begin >= stop) return;  // (the join does not ask for it)
   const bool whole = piece.begin == 0 && stop <= piece.end;
 
   const int row0 = tile0 + wave * 32, row = row0 + m;
@@ -408,13 +408,20 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   if (!whole && h == 0) a.ends[place_of] = {top, total};
 }
 
-template <typename M>
+// (What a CU holds, asked once: registers may leave room for more than the bound asked of the compiler.)
+template <typename T, int D, typename M>
 ManyShape shape_of() {
-  return {32 * M::kWaves, 4 * M::kResident / M::kWaves};
+  static const int resident = [] {
+    int n = 0;
+    const bool known = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, many_kernel<T, D, M::kWaves, M::kResident, M::kGrouped>,
+                                                                    M::kWaves * 64, 0) == hipSuccess;
+    return known && n > 0 ? n : 4 * M::kResident / M::kWaves;
+  }();
+  return {32 * M::kWaves, resident};
 }
 template <typename T, int D>
 ManyShape shape_of(bool causal) {
-  return causal ? shape_of<Many<T, D, true>>() : shape_of<Many<T, D, false>>();
+  return causal ? shape_of<T, D, Many<T, D, true>>() : shape_of<T, D, Many<T, D, false>>();
 }
 template <typename T, int D>
 int run_many(const Attend& a, int64_t pieces, hipStream_t s) {

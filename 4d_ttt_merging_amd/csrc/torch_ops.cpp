@@ -469,7 +469,7 @@ Tensor cached_attention(const Tensor& q0, const Tensor& data, const OptTensor& p
   const Tensor lengths = whole(lengths0, {c.p.batch}, q0, name, "lengths");
   const Tensor counts = whole(counts0, {c.p.batch}, q0, name, "counts");
   size_t need = 0;
-  check(vgo_cached_attn_workspace(&c.p, q.size(1), q.size(2), causal, dtype, &need));
+  check(vgo_cached_attn_workspace(&c.p, q.size(1), q.size(2), causal, counts.defined(), dtype, &need));
   const Tensor ws = need > 0 ? scratch(need, q) : Tensor();
   int64_t q_stride[3], out_stride[3];
   set_strides(q_stride, q), set_strides(out_stride, out);

@@ -717,10 +717,10 @@ int vgo_cache_read(const vgo_paged_cache* cache, const int32_t* starts, const in
  * Queries from counts[b] on, and those that attend to nothing, give zeros.  q / out [batch, heads, n_query, head_dim],
  * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)), strides as in vgo_cache_tokens.
  * Tokens past a sequence's length are not read.  Workspace (16-byte aligned, any contents): the states of work split over the keys; its size
- * is for the device that is current.
+ * is for the device that is current, `ragged` saying whether counts are given.
  */
-int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int causal, int dtype,
-                              size_t* bytes);
+int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int causal, int ragged,
+                              int dtype, size_t* bytes);
 int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, const int64_t q_stride[3], int64_t heads,
                         int64_t n_query, const int32_t* lengths, const int32_t* counts, int causal, float scale,
                         void* out, const int64_t out_stride[3], int dtype, void* workspace, size_t workspace_bytes,

@@ -55,7 +55,7 @@ def test_bad_caches_are_refused(over):
     lib_mod = import_package("_lib")
     lib = lib_mod.load()
     cache, size = struct(lib_mod, **over), ctypes.c_size_t()
-    assert lib.vgo_cached_attn_workspace(ctypes.byref(cache), 2, 1, 0, 1, ctypes.byref(size)) == lib_mod.VGO_EINVAL
+    assert lib.vgo_cached_attn_workspace(ctypes.byref(cache), 2, 1, 0, 0, 1, ctypes.byref(size)) == lib_mod.VGO_EINVAL
     assert lib.vgo_cache_append(ctypes.byref(cache), ctypes.byref(lib_mod.CacheTokens()), 1, None) == lib_mod.VGO_EINVAL
     assert lib.vgo_cache_read(ctypes.byref(cache), 16, None, 1, 16, 16, 1, None) == lib_mod.VGO_EINVAL
 
