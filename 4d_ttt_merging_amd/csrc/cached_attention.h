@@ -169,6 +169,11 @@ __device__ __forceinline__ int stop_of(const Attend& a, int length, int count, i
   return last < row0 ? 0 : a.causal ? max(0, min(length, place0 + last / a.group + 1)) : length;
 }
 
+// Exponents are z scale - reference in one instruction, whose product is not rounded while the reference's was: they are off by
+// its rounding, the same for all of a row, which normalising takes out.  From references of this size on, where that could
+// pass what an exponential holds (a row of a type's lowest values, say), the difference is taken before the scale.
+constexpr float kFar = 0x1p20f;
+
 // A mass as the kernels take it: a type's lowest value is a number, and with the scales that are allowed it stays one.
 __device__ __forceinline__ float mass_of(float mass) {
   return mass == -INFINITY ? mass : fminf(fmaxf(mass, -1e30f), 1e30f);

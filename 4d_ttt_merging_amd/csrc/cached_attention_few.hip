@@ -135,9 +135,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     }
   }
   f32x4 acc[NT][D / 16] = {};
-  float top[NT], total[NT];
+  float raw[NT], top[NT], total[NT];  // the reference maximum, before and after the scale
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) top[nt] = -INFINITY, total[nt] = 0.0f;
+  for (int nt = 0; nt < NT; ++nt) raw[nt] = top[nt] = -INFINITY, total[nt] = 0.0f;
 
   // A ring of blocks on their way.  Reads are not conditional, so that the compiler knows how many are outstanding: what has
   // no page, or lies past the end, reads the start of the cache instead and is left out.
@@ -196,11 +196,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
       float local = z[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
-      local *= scale;
-      if (__any(local > top[nt] + kLazy)) {
+      if (__any(local * scale > top[nt] + kLazy)) {
         local = fmaxf(local, __shfl_xor(local, 16));
         local = half_max(local);
-        const float to = fmaxf(top[nt], local);
+        raw[nt] = fmaxf(raw[nt], local);
+        const float to = raw[nt] * scale;
         const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[nt] - to);
         top[nt] = to;
         total[nt] *= shrink;
@@ -209,7 +209,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[nt][c][e] *= shrink;
       }
-      const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+      float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+      if (__any(fabsf(from) > kFar)) {  // (see kFar)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] -= raw[nt] == -INFINITY ? 0.0f : raw[nt];
+        from = 0.0f;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(z[2 * i], scale, -from));

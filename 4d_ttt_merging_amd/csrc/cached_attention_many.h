@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   };
 
   f32x16 acc[kOut] = {};
-  float top = -INFINITY, total = 0.0f;
+  float raw = -INFINITY, top = -INFINITY, total = 0.0f;  // the reference maximum, before and after the scale
   const int tiles = (end - piece.begin + 63) / 64;  // (none where end is before begin)
 
   const auto run = [&](auto half) {
@@ -322,10 +322,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       float local = z[0][0];
 #pragma unroll
       for (int i = 1; i < 32; ++i) local = fmaxf(local, z[i >> 4][i & 15]);
-      local *= a.scale;
-      if (__any(local > top + kLazyMany)) {
+      if (__any(local * a.scale > top + kLazyMany)) {
         local = half_max(local);
-        const float to = fmaxf(top, local);
+        raw = fmaxf(raw, local);
+        const float to = raw * a.scale;
         const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
         top = to;
         total *= shrink;
@@ -334,7 +334,14 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[c][e] *= shrink;
       }
-      const float from = top == -INFINITY ? 0.0f : top - kLift;
+      float from = top == -INFINITY ? 0.0f : top - kLift;
+      if (__any(fabsf(from) > kFar)) {  // (see kFar)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[k][i] -= raw == -INFINITY ? 0.0f : raw;
+        from = -kLift;
+      }
       vec weights[2][2][kP];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -415,6 +422,7 @@ ManyShape shape_of() {
     int n = 0;
     const bool known = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, many_kernel<T, D, M::kWaves, M::kResident, M::kGrouped>,
                                                                     M::kWaves * 64, 0) == hipSuccess;
+    if (!known) (void)hipGetLastError();  // (no device: nothing is launched either)
     return known && n > 0 ? n : 4 * M::kResident / M::kWaves;
   }();
   return {32 * M::kWaves, resident};

@@ -144,7 +144,8 @@ def attention(q, pages: Pages, table, lengths, counts=None, *, causal=False, sca
             z = scale * (x @ key.T)
             size_z = scale * (x.abs() @ key.abs().T)
             if masses:
-                z = z + pages.mass[page, slot]
+                mass = pages.mass[page, slot]
+                z = z + torch.where(mass == -math.inf, mass, mass.clamp(-1e30, 1e30))
             z = torch.where(ok, z, -math.inf)
             top = z.amax(1, keepdim=True)
             p = torch.exp(z - torch.where(top == -math.inf, 0.0, top))

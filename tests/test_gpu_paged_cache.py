@@ -314,3 +314,33 @@ def test_f16_probabilities_keep_their_bits(vgo, device):
     q = torch.zeros(1, 1, 130, 64).half()
     q[..., 0] = 18 * math.log(2.0) / 6.0
     both.attend(q, table, int32([256]), scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 40, 140])
+@pytest.mark.parametrize("lowest", [torch.finfo(F32).min, -1e9, -1e4])
+def test_masses_of_the_lowest_value_are_numbers(vgo, device, n, dtype, lowest):
+    """A sequence that has nothing else, one that has one other key, one whose first 64 keys are such."""
+    table = int32([[0, 1, 2], [3, 4, 5], [6, 7, 8]])
+    both = Both(vgo, device, 9, 2, 64, 64, masses=True)
+    both.fill(33)
+    for mass in (both.pages.mass, both.cache.log_mass):
+        mass[:6] = lowest
+        mass[4, 9] = 0.5
+        mass[6] = lowest
+    q = torch.randn(3, 4, n, 64, generator=torch.Generator().manual_seed(34)).to(dtype)
+    both.attend(q, table, int32([180, 192, 150]))
+    both.attend(q, table, int32([180, 192, 150]), causal=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 40, 140])
+def test_scores_of_any_size_stay_finite(vgo, device, n, dtype):
+    """Scores of 1e10, of which fp32 knows no more than hundreds: finite, and within the range of the values."""
+    table, pages = layout(1, 300, 64, 35)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    both.fill(36, gain=2.0 ** 13)
+    q = (torch.randn(1, 2, n, 64, generator=torch.Generator().manual_seed(37)) * 2.0 ** 14).to(dtype)
+    out = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([300])), scale=10.0).double().cpu()
+    out = out[torch.isfinite(q).all(-1)]  # (2^16 is past f16: the scores of such a query are not finite by definition)
+    assert torch.isfinite(out).all() and out.abs().max() <= both.pages.v.abs().max() * (1 + 2.0 ** -7)
