@@ -22,7 +22,8 @@ Frame and register blocks (no plan) in bf16/f16 run the same attention kernel
 behind vgo_qkv_epilogue (LayerNorm64 + RoPE); other dtypes and layouts take
 the reference's torch op sequence.  With `attn_bias` (keyword arguments of
 `masked_attention`) an unmerged block attends under masks and position biases, in
-inference and in training.
+inference and in training; with `cached` it stores its keys and values in a paged cache and
+attends over what the cache holds, in inference.
 The reference's experimental hooks that import the absent module
 `sampled_update_operator` (attention.py:267-299) and the source-query
 correction branch (attention.py:304-312, 376-385) are not part of this path
@@ -40,6 +41,7 @@ from torch import Tensor, nn
 from . import _kernels, profiling
 from .masked_attention import masked_attention
 from .mass_bias_attention import _attention_into, _attention_pair_into
+from .paged_cache import cache_append, cached_attention
 from .token_merging import TokenPlan
 
 
@@ -198,12 +200,18 @@ class SelfAttention(nn.Module):
             if getattr(self, name, None) is not None:
                 raise NotImplementedError(f"{name} is outside the merged global-attention path")
 
-    def forward(self, x: Tensor, attn_bias=None, rope: Tensor = None, token_plan=None) -> Tensor:
+    def forward(self, x: Tensor, attn_bias=None, rope: Tensor = None, token_plan=None, cached=None) -> Tensor:
         if token_plan is not None and self.training:
             raise RuntimeError("token compaction is inference-only")
         self._check_hooks()
         if attn_bias is not None and token_plan is not None:
             raise ValueError("attn_bias does not go with a token plan")
+        if cached is not None:
+            if self.training:
+                raise RuntimeError("a cache of keys and values is inference-only")
+            if attn_bias is not None or token_plan is not None:
+                raise ValueError("a cache goes with neither attn_bias nor a token plan")
+            return self.proj_drop(self.proj(self._attend_cached(self.qkv(x), rope, **cached)))
         if token_plan is None:
             qkv = self.qkv(x)
             return self.proj_drop(self.proj(self.compute_attention(qkv=qkv, attn_bias=attn_bias,
@@ -300,6 +308,38 @@ class SelfAttention(nn.Module):
         out = torch.empty((B, N, H, 64), device=qkv.device, dtype=dtype)
         _attention_into(q, k, v, None, out.permute(0, 2, 1, 3))
         return out.view(B, N, C)
+
+    def _attend_cached(self, qkv: Tensor, rope, *, cache, page_table: Tensor, lengths: Tensor,
+                       counts: Tensor | None = None, positions: Tensor | None = None, log_mass: Tensor | None = None,
+                       causal: bool = False) -> Tensor:
+        """Attention of packed qkv over a cache that gets its keys and values first (`cached` of `forward`).
+
+        lengths [B]: tokens of each sequence with this call's, of which counts [B] (default N) are new, the last ones;
+        the others as in `cache_append` and `cached_attention`.  Keys are stored after LayerNorm and RoPE;
+        `positions` default to the block's own: the tables' rows in order, for the tokens behind those that they leave."""
+        B, N, _ = qkv.shape
+        C, H = self.qkv.in_features, self.num_heads
+        D = C // H
+        starts = lengths - (N if counts is None else counts.clamp(0, N))
+        if rope is not None and positions is None:
+            prefix = N - rope[0].shape[-2]
+            if prefix < 0:
+                raise ValueError(f"{N} tokens need positions, with RoPE tables of {rope[0].shape[-2]} rows")
+            positions = torch.arange(-prefix, N - prefix, dtype=torch.int32, device=qkv.device).expand(B, N)
+        dtype = self._attention_dtype(qkv)
+        if self._fusable(qkv, C, H):
+            qn, kn = self._norm_params()
+            q, k, v = _kernels.qkv_epilogue(
+                qkv.reshape(B * N, 3 * C), H, tokens_in=N, q_norm=None if qn is None else qn[:2],
+                k_norm=None if kn is None else kn[:2], eps=qn[2] if qn is not None else 1e-5, out_dtype=dtype)
+        else:
+            q, k, v = (t.transpose(1, 2) for t in torch.unbind(qkv.reshape(B, N, 3, H, D), 2))
+            if self.use_qk_norm:
+                q, k = self.q_norm(q), self.k_norm(k)
+            q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+        q = cache_append(cache, k, v, page_table, starts, counts, q=q, rope=rope, positions=positions, log_mass=log_mass)
+        x = cached_attention(q, cache, page_table, lengths, counts, causal=causal)
+        return x.transpose(1, 2).reshape(B, N, C)
 
     def _merged_fused(self, qkv: Tensor, plan, B: int, N: int, C: int, H: int) -> Tensor:
         """Merged global attention straight from the packed projection.
@@ -480,13 +520,17 @@ class SelfAttentionBlock(nn.Module):
         self.ls2 = LayerScale(dim, init_values=init_values, device=device) if init_values else nn.Identity()
         self.sample_drop_ratio = drop_path
 
-    def forward(self, x: Tensor, rope=None, attn_bias=None) -> Tensor:
+    def forward(self, x: Tensor, rope=None, attn_bias=None, cached=None) -> Tensor:
         """Forward of block.py:89-129 (no stochastic depth).  `attn_bias`: keyword arguments of
         `masked_attention` for the block's attention (not in the reference); trainable with it, under
-        autocast too."""
+        autocast too.  `cached`: a dict of a `PagedCache` (cache) with its page_table and the sequences' lengths, and
+        of counts, positions, log_mass and causal where they differ from the defaults: the block's keys and
+        values are appended and its queries attend over all that is stored (not in the reference; inference)."""
         masked = {} if attn_bias is None else {"attn_bias": attn_bias}
+        if cached is not None:
+            masked["cached"] = cached
         if self._fused_rows(x):
-            arguments = self._native_dense(x, rope) if attn_bias is None else None
+            arguments = self._native_dense(x, rope) if not masked else None
             if arguments is not None:
                 return torch.ops.vgo.dense_block(x, *arguments)
             return self._fused_tail(x, self.attn(self._norm1_input(x), rope=rope, **masked))

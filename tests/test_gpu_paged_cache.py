@@ -344,3 +344,38 @@ def test_scores_of_any_size_stay_finite(vgo, device, n, dtype):
     out = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([300])), scale=10.0).double().cpu()
     out = out[torch.isfinite(q).all(-1)]  # (2^16 is past f16: the scores of such a query are not finite by definition)
     assert torch.isfinite(out).all() and out.abs().max() <= both.pages.v.abs().max() * (1 + 2.0 ** -7)
+
+
+# (sequences, heads, key heads, queries, tokens, channels): kept tokens enough for several pieces, joined afterwards.
+LONG = [(1, 2, 1, 1, 5000, 64), (3, 16, 1, 1, 2100, 128), (2, 3, 1, 7, 3333, 64), (1, 5, 5, 1, 4097, 64), (1, 4, 2, 31, 2500, 128),
+        (2, 2, 1, 33, 3000, 64), (1, 3, 1, 86, 1111, 128), (1, 1, 1, 1029, 1500, 64), (1, 1, 1, 1100, 1500, 128),
+        (2, 6, 2, 350, 700, 64), (1, 1, 1, 130, 4500, 64)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", LONG)
+def test_long_sequences(vgo, device, shape, causal, dtype):
+    b, h, hk, n, length, d = shape
+    table, pages = layout(b, length, 128, 5)
+    both = Both(vgo, device, pages, hk, 128, d, masses=n % 2 == 1)
+    both.fill(6)
+    q = torch.randn(b, h, n, d, generator=torch.Generator().manual_seed(7)).to(dtype)
+    both.attend(q, table, int32([length - 701 * i if i else length for i in range(b)]), causal=causal)
+
+
+@pytest.mark.parametrize("n", [1, 3, 40, 90])
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_sequences_of_very_different_lengths(vgo, device, n, causal):
+    """More sequences than a wave has lanes, three of them far longer than the others; pages in common."""
+    g = torch.Generator().manual_seed(8)
+    lengths = torch.randint(0, 200, (150,), generator=g).int()
+    lengths[[3, 77, 149]] = int32([2500, 1400, 3000])
+    counts = torch.randint(0, n + 1, (150,), generator=g).int()
+    both = Both(vgo, device, 60, 1, 64, 64)
+    both.fill(9)
+    table = torch.randint(0, 60, (150, 47), generator=g).int()
+    q = torch.randn(150, 2, n, 64, generator=g)
+    both.attend(q, table, lengths, counts, causal=causal)
+    both.attend(q, table, lengths.flip(0), counts, causal=causal)
+    both.attend(q, table, lengths, causal=causal)
