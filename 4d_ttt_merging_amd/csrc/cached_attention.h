@@ -31,7 +31,7 @@ struct Attend {
   const int32_t* lengths;
   const int32_t* counts;
   int64_t batch;
-  int32_t n_query, heads, group;
+  int32_t n_query, group;
   int32_t first_row, last_row;  // the rows of this launch: from .. to before
   int32_t tiles, tile_rows;   // row tiles of a key head, rows of one
   int32_t slots, least;       // pieces beside one a sequence (0: no splitting), tokens of a piece at least
@@ -46,6 +46,11 @@ __device__ __forceinline__ int length_of(const Attend& a, int64_t b) {
 }
 __device__ __forceinline__ int count_of(const Attend& a, int64_t b) {
   return a.counts ? min(max(a.counts[b], 0), a.n_query) : a.n_query;
+}
+
+// Where a sequence's first query stands.  (Past every table: seen from there all is earlier, and sums of places fit 32 bits.)
+__device__ __forceinline__ int first_place(const Attend& a, int64_t b, int count) {
+  return min(max(a.lengths[b], 0), 1 << 30) - count;
 }
 
 // Reductions over a wave stay in the vector unit (a shuffle through LDS takes a hundred cycles, and a step of a short
@@ -163,7 +168,7 @@ __device__ __forceinline__ void leave(const Attend& a, const Piece& piece, int x
   if (a.slots > 0 && piece.begin == 0 && one) a.firsts[piece.b] = {x, piece.tokens};
 }
 
-// Tokens that any row of the tile at row `row0` sees: from 0 to before this one.  `place0`: where a sequence's first query stands.
+// Tokens that any row of the tile at row `row0` sees: from 0 to before this one.
 __device__ __forceinline__ int stop_of(const Attend& a, int length, int count, int place0, int row0) {
   const int last = min(min(row0 + a.tile_rows, a.last_row), count * a.group) - 1;
   return last < row0 ? 0 : a.causal ? max(0, min(length, place0 + last / a.group + 1)) : length;
@@ -179,7 +184,7 @@ __device__ __forceinline__ float mass_of(float mass) {
   return mass == -INFINITY ? mass : fminf(fmaxf(mass, -1e30f), 1e30f);
 }
 
-// bf16 terms that a query, and a probability, is split into.
+// bf16 terms that a query, and a probability, is split into (many bf16 queries: one each, see ManyTerms).
 template <typename T>
 struct Terms;
 template <>

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Attend a) {
   const int64_t b = blockIdx.x / chunks / kv;
   const int2 piece = a.firsts[b];
   const int count = count_of(a, b), tile = of0 / a.tile_rows;
-  const int stop = stop_of(a, length_of(a, b), count, a.lengths[b] - count, a.first_row + tile * a.tile_rows);
+  const int stop = stop_of(a, length_of(a, b), count, first_place(a, b, count), a.first_row + tile * a.tile_rows);
   const int n = stop <= 0 ? 1 : (stop - 1) / piece.y + 1;
   if (n <= 1) return;
   const int64_t step = static_cast<int64_t>(kv) * a.tiles * a.tile_rows;
@@ -242,7 +242,7 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
   a.pages = pages_of(cache);
   a.q = q, a.out = out, a.lengths = lengths, a.counts = counts, a.batch = cache->batch;
   for (int i = 0; i < 3; ++i) a.q_stride[i] = q_stride[i], a.out_stride[i] = out_stride[i];
-  a.n_query = static_cast<int32_t>(n_query), a.heads = static_cast<int32_t>(heads);
+  a.n_query = static_cast<int32_t>(n_query);
   a.group = static_cast<int32_t>(heads / cache->kv_heads);
   a.causal = causal != 0, a.scale = scale * 1.4426950408889634f, a.per_scale = 1.0f / scale;
   const hipStream_t s = as_stream(stream);

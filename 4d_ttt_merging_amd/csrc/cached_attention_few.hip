@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   const int64_t b = piece.b;
   const int count = count_of(a, b);
   const int row0 = a.first_row + tile * a.tile_rows;
-  const int place0 = a.lengths[b] - count, stop = stop_of(a, piece.length, count, place0, row0);
+  const int place0 = first_place(a, b, count), stop = stop_of(a, piece.length, count, place0, row0);
   const int end = min(piece.end, stop);
   if (piece.begin > 0 && piece.begin >= stop) return;  // (the join does not ask for it)
   const bool whole = piece.begin == 0 && stop <= piece.end;

@@ -12,7 +12,7 @@ int check_cache(const vgo_paged_cache* c) {
   VGO_REQUIRE(c->page_size >= kMinPage && c->page_size <= kMaxPage && (c->page_size & (c->page_size - 1)) == 0,
               "paged cache: the page size must be a power of two from 32 to 1,024");
   VGO_REQUIRE(c->pages >= 0 && c->pages <= INT32_MAX && c->kv_heads >= 1 && c->kv_heads <= 65535 && c->batch >= 0 &&
-                  c->batch <= INT32_MAX && c->table_width >= 0 && c->table_width <= INT32_MAX / c->page_size,
+                  c->batch <= INT32_MAX && c->table_width >= 0 && c->table_width <= (int64_t{1} << 30) / c->page_size,
               "paged cache: size out of range");
   VGO_REQUIRE(c->pages == 0 || (c->data && aligned(c->data, 16)), "paged cache: the data must be 16-byte aligned");
   VGO_REQUIRE(c->batch == 0 || c->table_width == 0 || c->page_table, "paged cache: null page table");

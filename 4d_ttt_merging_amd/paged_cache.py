@@ -85,7 +85,7 @@ def cache_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table
       positions  int32 [B, N]: the tables' row of a token; default its place.  Tokens with no such row (a frame's
                  special tokens: -1) are not rotated
       log_mass   floating [B, N]: added to every score of the token, for caches with masses; default zeros
-    The rotation is taken in 64 bits, so a code is the nearest to the exact value.  Tokens past the page table, or
+    A rotated key's codes are the nearest to the exact values; q is rotated in fp32.  Tokens past the page table, or
     whose entry is not a page of the cache (-1, say), are left out.  Two tokens of one call must not have
     the same place in the cache.  Under bf16 or f16 autocast fp32 operands are cast first."""
     _ready(cache.data, cache.log_mass, k, v, q, page_table, starts, counts, positions, log_mass, *(rope or ()))
@@ -118,10 +118,11 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     [B, H, N, D], token-major in memory where q is; zeros for padding and for queries that attend to nothing (a
     log mass of -inf, or no page, keeps a token out; finite masses past 1e30 in size count as that).
 
-    Tokens past a length may hold anything; others must be finite where any query of their sequence can see them.  Stored
-    numbers enter exactly.  Sums are fp32; probabilities are rounded to the type of q where that is bf16 and
-    queries are many, else taken to twice its bits.  Results are the same bits every time.  Under bf16 or f16
-    autocast fp32 q is cast first."""
+    Tokens past a length, or past the table (2**30 tokens a sequence at most), are not there and may hold anything; others
+    must be finite where any query of their sequence can see them.  Stored numbers enter exactly (in f16, with many
+    queries, values below 2**-23 to its smallest number, 2**-24).  Sums are fp32; probabilities are rounded to a 16-bit
+    type of q where queries are many (more than 64 rows beside a key head), else taken to twice its bits, and to
+    24 bits in fp32.  Results are the same bits every time.  Under bf16 or f16 autocast fp32 q is cast first."""
     _ready(q, cache.data, cache.log_mass, page_table, lengths, counts)
     (q,) = _autocast(q)
     if scale is None:

@@ -669,7 +669,7 @@ int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64_t heads, c
  * page_size: a power of two, 32 to 1,024; head_dim 64 or 128.
  * page_table: int32 [batch, table_width]; token t of sequence b lies in page page_table[b, t / page_size].  Tokens past
  * the table, or whose page is not one of the cache's, are not there: appending leaves them out, reading gives zeros,
- * no query attends to them.  A sequence has at most INT32_MAX tokens.
+ * no query attends to them.  A table holds at most 2^30 tokens of a sequence.
  */
 typedef struct vgo_paged_cache {
   void* data;
@@ -685,7 +685,8 @@ typedef struct vgo_paged_cache {
  * clamped to 0 .. n_tokens) are padding and are not stored.
  * rope_sin / rope_cos fp32 [rope_rows, head_dim] or NULL: k is stored, and q is written to q_out, as
  *   x cos + (-x[D/2 ..], x[.. D/2]) sin   with row positions[b, i] (int32 [batch, n_tokens]; NULL: starts[b] + i) of
- * the tables, taken in 64 bits and rounded once; tokens whose row the tables do not have are not rotated.  q_out's padding is zeros.
+ * the tables (a key's code is the nearest to the exact value; q in fp32, rounded to its type); tokens whose row the
+ * tables do not have are not rotated.  q_out's padding is zeros.
  * log_mass fp32 [batch, n_tokens]; NULL: zeros, where the cache holds masses.
  * Tokens of one call must not share a place (sequences that share a page may do so only for tokens that are there).
  */
@@ -716,8 +717,10 @@ int vgo_cache_read(const vgo_paged_cache* cache, const int32_t* starts, const in
  *   out_i = sum_j softmax_j(scale * q_i.k_j + log_mass[j]) v_j   over j < lengths[b], and, if causal, j <= its place.
  * Queries from counts[b] on, and those that attend to nothing, give zeros.  q / out [batch, heads, n_query, head_dim],
  * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)), strides as in vgo_cache_tokens.
- * Tokens past a sequence's length are not read.  Workspace (16-byte aligned, any contents): the states of work split over the keys; its size
- * is for the device that is current, `ragged` saying whether counts are given.
+ * scale: 1e-8 to 1e8.  Finite masses past 1e30 in size count as that; -inf keeps a token out.
+ * Tokens past a sequence's length, or past the table, are not there and may hold anything.  Workspace (16-byte aligned, any
+ * contents): the states of work split over the keys; its size is for the device that is current, `ragged` saying
+ * whether counts are given.
  */
 int vgo_cached_attn_workspace(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int causal, int ragged,
                               int dtype, size_t* bytes);

@@ -220,7 +220,8 @@ def test_refusals(vgo, device):
                 dict(positions=torch.zeros(2, 5, dtype=torch.int32, device=device)), dict(log_mass=torch.zeros(2, 5, device=device)),
                 dict(rope=(rope[0], rope[1][:5])), dict(rope=(rope[0][:, :32], rope[1][:, :32])),
                 dict(rope=rope, positions=torch.zeros(2, 4, dtype=torch.int32, device=device)), dict(k=k.double(), v=v.double()),
-                dict(cache=cache._replace(data=cache.data.transpose(0, 1)))):
+                dict(cache=cache._replace(data=cache.data.transpose(0, 1))),
+                dict(table=torch.zeros(2, (1 << 24) + 1, dtype=torch.int32, device=device))):
         with pytest.raises((ValueError, RuntimeError)):
             append(**bad)
     for bad in (dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[0]), dict(q=q.double()), dict(table=table[:1]), dict(lengths=starts[:1]),

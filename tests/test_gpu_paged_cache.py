@@ -379,3 +379,17 @@ def test_many_sequences_of_very_different_lengths(vgo, device, n, causal):
     both.attend(q, table, lengths, counts, causal=causal)
     both.attend(q, table, lengths.flip(0), counts, causal=causal)
     both.attend(q, table, lengths, causal=causal)
+
+
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_lengths_beyond_any_table(vgo, device, n):
+    """Queries that stand past the table see all of it, those of a negative length nothing."""
+    table, pages = layout(2, 700, 64, 5)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    both.fill(6)
+    q = torch.randn(2, 2, n, 64, generator=torch.Generator().manual_seed(7))
+    held = 64 * table.shape[1]
+    want = both.attend(q, table, int32([held + n, 0]), causal=True)
+    for ends in ([2 ** 31 - 1, -2 ** 31], [2 ** 31 - 32, -5], [2 ** 30, -1]):
+        assert torch.equal(want, both.to(q).new_zeros(()) + vgo.cached_attention(both.to(q), both.cache, both.to(table),
+                                                                                both.to(int32(ends)), causal=True))
