@@ -137,10 +137,14 @@ struct Piece {
   int tokens;          // of a piece
 };
 
+// Pieces of all sequences together.
+__device__ __forceinline__ int pieces_in_all(const Attend& a, const Pieces& all) {
+  int n = lane_id() < a.batch ? pieces_of(all.mine, all.tokens) : 0;
+  for (int64_t b = lane_id() + 64; b < a.batch; b += 64) n += pieces_of(length_of(a, b), all.tokens);
+  return static_cast<int>(wave_sum(static_cast<uint32_t>(n)));
+}
 // Piece x of all sequences' pieces in a row.
-template <bool kMany>
-__device__ __forceinline__ Piece piece_of(const Attend& a, int x) {
-  const Pieces all = pieces<kMany>(a);
+__device__ __forceinline__ Piece piece_of(const Attend& a, const Pieces& all, int x) {
   int before = 0;
   for (int64_t b0 = 0; b0 < a.batch; b0 += 64) {
     const int64_t b = b0 + lane_id();

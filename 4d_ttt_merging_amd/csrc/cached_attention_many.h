@@ -123,11 +123,19 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   const int kv = a.pages.kv_heads;
   const int hk = blockIdx.x % kv;
   const int rest = blockIdx.x / kv;
-  const int tile = a.tiles - 1 - rest % a.tiles;  // (of a causal call the longest first)
-  const int x = rest / a.tiles;
-  const Piece piece = piece_of<true>(a, x);
+  // The tiles of a piece one after the other, so that they find its tokens in the cache, and the longest of a causal call first.
+  // Where sequences are whole, the longest of all sequences first (3 causal prompts of up to 4,116 tokens, f16, 16 heads of 64
+  // channels: 129 us, so 112; cut ones in this order 265, 290: 2 x 2,058 queries over 16,464).
+  const Pieces all = pieces<true>(a);
+  int tile = a.tiles - 1 - rest % a.tiles, x = rest / a.tiles;
+  if (a.causal && all.tokens == INT32_MAX) {
+    const int n = pieces_in_all(a, all);
+    tile = a.tiles - 1 - rest / n, x = rest % n;
+    if (tile < 0) return;
+  }
+  const Piece piece = piece_of(a, all, x);
   if (piece.b < 0) return;
-  leave(a, piece, x, threadIdx.x == 0 && hk == 0 && rest % a.tiles == 0);
+  leave(a, piece, x, threadIdx.x == 0 && hk == 0 && tile == 0);
   const int64_t b = piece.b;
   const int count = count_of(a, b);
   const int tile0 = a.first_row + tile * a.tile_rows;
