@@ -13,6 +13,8 @@
 // for a join.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_cache.h"
 
 namespace vgo {
@@ -74,6 +76,21 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
   return __builtin_amdgcn_readlane(static_cast<int>(sums_upto(v)), 63);
 }
 
+__device__ __forceinline__ int wave_max(int v) {
+  // (a lane without another sees zero there, or its own)
+  const auto step = [&](auto at, auto rows) {
+    v = max(v, static_cast<int>(__builtin_amdgcn_update_dpp(v, v, decltype(at)::value, decltype(rows)::value, 0xF, false)));
+  };
+  using All = std::integral_constant<int, 0xF>;
+  step(std::integral_constant<int, 0x111>(), All());
+  step(std::integral_constant<int, 0x112>(), All());
+  step(std::integral_constant<int, 0x114>(), All());
+  step(std::integral_constant<int, 0x118>(), All());
+  step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xA>());
+  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xC>());
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 __device__ __forceinline__ int pieces_of(int length, int tokens) { return max(1, (length - 1) / tokens + 1); }
 
 // The sequences' pieces, as every work-group reckons them: all lanes of a wave together, the same in each.
@@ -84,52 +101,77 @@ struct Pieces {
 // Row tiles of a sequence that have queries (one at least).
 __device__ __forceinline__ int busy_tiles(const Attend& a, int64_t b) {
   const int rows = min(count_of(a, b) * a.group, a.last_row) - a.first_row;
-  return max(1, (rows + a.tile_rows - 1) / a.tile_rows);
+  return max(1, (rows + a.tile_rows - 1) >> __builtin_ctz(a.tile_rows));
 }
-// The shortest pieces of which no more than `slots` beside one a sequence are needed, or nearly so, and (kMany), since
-// sequences differ in queries too, whose work-groups that have queries fill the chip about once, or twice where a single
-// round would leave it ragged (2 x 2,058 queries at most over 16,464 tokens of 128 channels, both ragged: one round 282 us, so 242).
-template <bool kMany>
-__device__ __forceinline__ Pieces pieces(const Attend& a) {
+// Few queries: the shortest pieces of which no more than `slots` beside one a sequence are needed, or nearly so.
+__device__ __forceinline__ Pieces few_pieces(const Attend& a) {
   const bool here = lane_id() < a.batch;
   Pieces p{here ? length_of(a, lane_id()) : 0, INT32_MAX};
   if (a.slots == 0) return p;
-  const int weight = kMany && here ? busy_tiles(a, lane_id()) : 1;
   const auto over_all = [&](auto of) {  // at most 2^25 a lane, so that 64 of them fit
-    int64_t sum = here ? of(p.mine, weight) : 0;
-    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += of(length_of(a, b), kMany ? busy_tiles(a, b) : 1);
+    int64_t sum = here ? of(p.mine) : 0;
+    for (int64_t b = lane_id() + 64; b < a.batch; b += 64) sum += of(length_of(a, b));
     return static_cast<int64_t>(wave_sum(static_cast<uint32_t>(min(sum, int64_t{1} << 25))));
   };
   const int most = a.slots + static_cast<int>(a.batch);
   const auto rounded = [&](int64_t units) {  // of 64 tokens
     return static_cast<int>(min(max(units * 64, static_cast<int64_t>(a.least)), static_cast<int64_t>(INT32_MAX)));
   };
-  int64_t target = most;
-  if constexpr (kMany) {
-    const int64_t busy = over_all([&](int, int w) { return static_cast<int64_t>(w) * a.pages.kv_heads; });
-    if (10 * busy >= 9 * static_cast<int64_t>(a.held)) return p;
-    target = 100 * (a.held / busy * busy) >= 85 * static_cast<int64_t>(a.held) ? a.held : 2 * a.held;
-  }
-  const int each = kMany ? a.pages.kv_heads : 1;
-  const int64_t sum = over_all([&](int length, int w) { return (static_cast<int64_t>(length) + 63) / 64 * w * each; });
+  const int64_t sum = over_all([](int length) { return (static_cast<int64_t>(length) + 63) / 64; });
   // (more than the sums hold: a piece a sequence)
   if (sum >= int64_t{1} << 25) return p;
-  p.tokens = rounded((sum + target - 1) / target);
+  p.tokens = rounded((sum + most - 1) / most);
   for (int round = 0; round < 4; ++round) {
     const int tokens = p.tokens;
-    const int64_t n = over_all([&](int length, int) { return static_cast<int64_t>(pieces_of(length, tokens)); });
-    int64_t groups = n;
-    if constexpr (kMany) groups = over_all([&](int length, int w) { return static_cast<int64_t>(pieces_of(length, tokens)) * w * each; });
-    if (n <= most && (groups <= target || round == 3)) return p;
-    const int64_t by_n = p.tokens / 64 * n / most + 1, by_groups = p.tokens / 64 * groups / target + 1;
-    p.tokens = rounded(max(n > most ? by_n : 0, by_groups));
+    const int64_t n = over_all([&](int length) { return static_cast<int64_t>(pieces_of(length, tokens)); });
+    if (n <= most) return p;
+    p.tokens = rounded(p.tokens / 64 * n / most + 1);
   }
   // (at most one more a sequence than all the tokens / tokens)
-  const int64_t all = kMany ? over_all([](int length, int) { return (static_cast<int64_t>(length) + 63) / 64; }) : sum;
-  p.tokens = rounded((all + a.slots - 1) / a.slots);
+  p.tokens = rounded((sum + a.slots - 1) / a.slots);
   return p;
 }
 
+// x / y of numbers from 0 to 2^30, if less than 2^20 (more is then nearly right).
+__device__ __forceinline__ int quotient(int x, int y) {
+  const int q = static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y)));
+  const int64_t left = x - static_cast<int64_t>(q) * y;
+  return left < 0 ? q - 1 : left >= y ? q + 1 : q;
+}
+
+// Many queries: the length of pieces that costs least, in tokens of a tile: rounds of work-groups that have queries, each a
+// piece and what it begins and ends with; and what they leave to the join, for as many as the chip holds.  A lane looks at one
+// length, a part of the longest sequence.  (The sequences differ in queries and lengths, and a ragged last round idles most
+// of the chip: one or two full rounds by the sums alone took, of calls with 2 or 3 ragged causal sequences, 4% longer in bf16 and 9% in fp32.
+// kRound, kJoin of 64 to 512, 300 to 1,200: within 2% up to 192, 450.)
+constexpr float kRound = 192.0f, kJoin = 300.0f;
+__device__ __forceinline__ Pieces many_pieces(const Attend& a) {
+  const int lane = lane_id();
+  Pieces p{lane < a.batch ? length_of(a, lane) : 0, INT32_MAX};
+  if (a.slots == 0) return p;
+  int busy = 0, longest = 0;
+  for (int64_t b = lane; b < a.batch; b += 64) busy += busy_tiles(a, b), longest = max(longest, length_of(a, b));
+  busy = static_cast<int>(wave_sum(static_cast<uint32_t>(busy))) * a.pages.kv_heads;
+  longest = wave_max(longest);
+  if (10 * static_cast<int64_t>(busy) >= 9 * static_cast<int64_t>(a.held)) return p;
+  // 1 .. 32 of the longest, then eight a doubling.
+  const int parts = lane < 32 ? lane + 1 : static_cast<int>(32.0f * __builtin_amdgcn_exp2f((lane - 31) * 0.125f));
+  const int tokens = max((quotient(longest, parts) + 64) & ~63, a.least);
+  int64_t n = 0, groups = 0;
+  for (int b = 0; b < a.batch; ++b) {
+    const int one = quotient(max(0, length_of(a, b) - 1), tokens) + 1;
+    n += one, groups += static_cast<int64_t>(one) * busy_tiles(a, b);
+  }
+  const int all = static_cast<int>(min(groups * a.pages.kv_heads, int64_t{1} << 29));  // (the grid holds fewer than 2^23)
+  const int rounds = quotient(all + a.held - 1, a.held);
+  const float join = tokens < longest ? kJoin * static_cast<float>(all) / static_cast<float>(a.held) : 0.0f;
+  const float cost = n > a.slots + a.batch ? INFINITY : static_cast<float>(rounds) * (static_cast<float>(tokens) + kRound) + join;
+  const int order = -static_cast<int>(__float_as_uint(cost));
+  const uint64_t best = __ballot(order == wave_max(order));
+  const int taken = __builtin_amdgcn_readlane(tokens, __ffsll(static_cast<unsigned long long>(best)) - 1);
+  if (taken < longest) p.tokens = taken;
+  return p;
+}
 struct Piece {
   int64_t b;           // -1: there is no such piece
   int begin, end;      // its tokens

@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   const int rest = blockIdx.x / kv;
   const int tile = rest % a.tiles;
   const int x = rest / a.tiles;
-  const Piece piece = piece_of(a, pieces<false>(a), x);
+  const Piece piece = piece_of(a, few_pieces(a), x);
   if (piece.b < 0) return;
   leave(a, piece, x, threadIdx.x == 0 && hk == 0 && rest % a.tiles == 0);
   const int64_t b = piece.b;

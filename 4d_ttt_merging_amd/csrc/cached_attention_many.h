@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   // The tiles of a piece one after the other, so that they find its tokens in the cache, and the longest of a causal call first.
   // Where sequences are whole, the longest of all sequences first (3 causal prompts of up to 4,116 tokens, f16, 16 heads of 64
   // channels: 129 us, so 112; cut ones in this order 265, 290: 2 x 2,058 queries over 16,464).
-  const Pieces all = pieces<true>(a);
+  const Pieces all = many_pieces(a);
   int tile = a.tiles - 1 - rest % a.tiles, x = rest / a.tiles;
   if (a.causal && all.tokens == INT32_MAX) {
     const int n = pieces_in_all(a, all);
