@@ -150,9 +150,10 @@ Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // Few queries: as many work-groups as the chip holds at once.  Many, of which some sequences may have fewer than others: more,
   // which those that have queries then share (a grid of four times as many is through with its idle ones in 8 us);
-  // none beside one a tile where all are busy and fill it.
+  // none beside one a tile where all are busy and leave little of their last round idle, or rounds are many.
   const int64_t held = static_cast<int64_t>(few ? 2 : shape.resident) * device_cus(), beside = c->kv_heads * p.tiles;
-  const bool full = !few && !ragged && 10 * c->batch * beside >= 9 * held;
+  const int64_t busy = c->batch * beside, last = (busy + held - 1) / held * held;
+  const bool full = !few && (busy >= 8 * held || (!ragged && 20 * busy >= 17 * last));
   const int64_t rounds = few || (p.tiles == 1 && c->batch * beside <= held / 4) ? 1 : p.tiles < 8 ? 2 : 4;
   const int64_t slots = full ? 0 : rounds * held / beside - c->batch;
   p.held = static_cast<int>(held);

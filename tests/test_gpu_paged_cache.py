@@ -349,7 +349,7 @@ def test_scores_of_any_size_stay_finite(vgo, device, n, dtype):
 # (sequences, heads, key heads, queries, tokens, channels): kept tokens enough for several pieces, joined afterwards.
 LONG = [(1, 2, 1, 1, 5000, 64), (3, 16, 1, 1, 2100, 128), (2, 3, 1, 7, 3333, 64), (1, 5, 5, 1, 4097, 64), (1, 4, 2, 31, 2500, 128),
         (2, 2, 1, 33, 3000, 64), (1, 3, 1, 86, 1111, 128), (1, 1, 1, 1029, 1500, 64), (1, 1, 1, 1100, 1500, 128),
-        (2, 6, 2, 350, 700, 64), (1, 1, 1, 130, 4500, 64)]
+        (2, 6, 2, 350, 700, 64), (1, 1, 1, 130, 4500, 64), (1, 9, 9, 4200, 300, 128)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
