@@ -71,6 +71,18 @@ __device__ __forceinline__ void widened(const Raw<T>& r, float (&x)[8]) {
   }
 }
 
+// The channels of lane ^ kLanes, 4 or 8, by the LDS unit's crossbar.
+template <int kLanes, typename T>
+__device__ __forceinline__ Raw<T> across(const Raw<T>& r) {
+  Raw<T> o;
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o.w[i][e] = static_cast<uint32_t>(__builtin_amdgcn_ds_swizzle(static_cast<int>(r.w[i][e]), kLanes << 10 | 0x1f));
+  return o;
+}
+
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) { widened(raw8(p), x); }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
@@ -178,7 +190,7 @@ __device__ __forceinline__ uint32_t transposed_bytes(uint32_t w) {
 // of the format), and `per` heads of k, q and v, one after the other with the next one's channels on their way; a lane
 // eight channels of a token.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void append_kernel(const Append a) {
+__global__ __launch_bounds__(256, 5) void append_kernel(const Append a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;            // of a token
   constexpr int kTokens = 64 / kLanes, kParts = 8 / kTokens;
@@ -200,6 +212,12 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a) {
   const int64_t t = first + j, i = t - start;
   const bool inside = i >= 0 && i < a.n, real = i >= 0 && i < count;
   if (!__any(inside)) return;
+  if (!__any(real)) {  // padding alone: nothing to read
+    const float zeros[8] = {};
+    for (int h = max(begin - kv, 0); h < min(end - kv, a.heads); ++h)
+      if (inside) store8(static_cast<T*>(a.q_out) + b * a.out_stride[0] + h * a.out_stride[1] + i * a.out_stride[2] + 8 * c, zeros);
+    return;
+  }
   const int64_t at_row = min(max(i, int64_t{0}), a.n - 1);  // (padding lanes read some row of the call)
   const int slot = static_cast<int>(t) & 31;
   bool turned = false;
@@ -217,24 +235,22 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a) {
   if (chunk == 0 && a.pages.mass && real && page >= 0 && c == 0)
     a.pages.mass[(static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1))] =
         a.log_mass ? a.log_mass[b * a.n + i] : 0.0f;
-  // The channels of virtual head `at`: keys' heads, the queries', the values'; and those they are rotated with.
+  // The channels of virtual head `at`: keys' heads, the queries', the values'.
   const int64_t k_row = at_row * a.k_stride[2] + 8 * c, q_row = at_row * a.q_stride[2] + 8 * c, v_row = at_row * a.v_stride[2] + 8 * c;
-  const int across = low ? D / 2 : -D / 2;
-  const auto read = [&](int at, Raw<T>& x, Raw<T>& o) {
+  const auto read = [&](int at, Raw<T>& x) {
     const T* from;
     if (at < kv) from = static_cast<const T*>(a.k) + b * a.k_stride[0] + at * a.k_stride[1] + k_row;
     else if (at < kv + a.heads) from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (at - kv) * a.q_stride[1] + q_row;
     else from = static_cast<const T*>(a.v) + b * a.v_stride[0] + (at - kv - a.heads) * a.v_stride[1] + v_row;
     x = raw8(from);
-    if (rotate && at < kv + a.heads) o = raw8(from + across);
   };
-  const auto use = [&](int at, const Raw<T>& raw, const Raw<T>& raw_other) {
+  const auto use = [&](int at, const Raw<T>& raw) {
     const bool key = at < kv, value = at >= kv + a.heads;
     float x[8], other[8];
     widened(raw, x);
     uint32_t byte = 0, word = 0;
     if (rotate && !value) {
-      widened(raw_other, other);
+      widened(across<kLanes / 2>(raw), other);
 #pragma unroll
       for (int e = 0; e < 8; ++e) other[e] = !turned ? 0.0f : low ? -other[e] : other[e];  // (not turned: x 1 + 0 0)
     }
@@ -274,13 +290,13 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a) {
         if (four + e >= 0 && four + e < count) to[e] = static_cast<uint8_t>(word >> (8 * e));
     }
   };
-  Raw<T> x0{}, o0{}, x1{}, o1{};
-  read(begin, x0, o0);
+  Raw<T> x0{}, x1{};
+  read(begin, x0);
   for (int at = begin; at < end; at += 2) {
-    if (at + 1 < end) read(at + 1, x1, o1);
-    use(at, x0, o0);
-    if (at + 2 < end) read(at + 2, x0, o0);
-    if (at + 1 < end) use(at + 1, x1, o1);
+    if (at + 1 < end) read(at + 1, x1);
+    use(at, x0);
+    if (at + 2 < end) read(at + 2, x0);
+    if (at + 1 < end) use(at + 1, x1);
   }
 }
 
@@ -319,7 +335,7 @@ __global__ __launch_bounds__(256) void read_kernel(const Read a) {
   const uint32_t value_scale_at = L::kValueScales + slot / 8 * L::kScaleGroup + c / 4 * 8 + slot % 8;
   for (int at0 = begin; at0 < end; at0 += kAhead) {
     uint32_t words[kAhead] = {}, bytes[kAhead] = {};
-    if (page >= 0) {
+    if (page >= 0 && __any(real)) {
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
         const int at = min(at0 + e, end - 1);
