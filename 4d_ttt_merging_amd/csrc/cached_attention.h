@@ -308,7 +308,7 @@ struct ManyShape {
   int tile_rows, resident;  // rows of a work-group, work-groups that a CU holds
 };
 template <typename T>
-ManyShape many_shape(int head_dim, bool causal);
+ManyShape many_shape(int head_dim, bool causal, int64_t group);
 template <typename T>
 int launch_many(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
 

@@ -105,11 +105,11 @@ int join_pieces(const Attend& a, int head_dim, hipStream_t s) {
 }  // namespace
 
 template <>
-ManyShape many_shape<bf16_t>(int head_dim, bool causal);
+ManyShape many_shape<bf16_t>(int head_dim, bool causal, int64_t group);
 template <>
-ManyShape many_shape<f16_t>(int head_dim, bool causal);
+ManyShape many_shape<f16_t>(int head_dim, bool causal, int64_t group);
 template <>
-ManyShape many_shape<float>(int head_dim, bool causal);
+ManyShape many_shape<float>(int head_dim, bool causal, int64_t group);
 template <>
 int launch_many<bf16_t>(const Attend& a, int64_t pieces, int head_dim, hipStream_t s);
 template <>
@@ -172,9 +172,9 @@ Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, bool caus
   Plan p{};
   const int64_t rows = n_query * (heads / c->kv_heads);
   const int dim = static_cast<int>(c->head_dim);
-  const ManyShape shape = dtype == VGO_BF16  ? many_shape<bf16_t>(dim, causal)
-                          : dtype == VGO_F16 ? many_shape<f16_t>(dim, causal)
-                                             : many_shape<float>(dim, causal);
+  const ManyShape shape = dtype == VGO_BF16  ? many_shape<bf16_t>(dim, causal, heads / c->kv_heads)
+                          : dtype == VGO_F16 ? many_shape<f16_t>(dim, causal, heads / c->kv_heads)
+                                             : many_shape<float>(dim, causal, heads / c->kv_heads);
   const int64_t over = rows % shape.tile_rows;
   // Rows of the large tiles.
   const int64_t split = rows <= kFewRows ? 0 : over <= kFewRows && rows >= 4 * shape.tile_rows ? rows - over : rows;

@@ -9,8 +9,8 @@ int launch_many<bf16_t>(const Attend& a, int64_t pieces, int head_dim, hipStream
   return head_dim == 64 ? run_many<bf16_t, 64>(a, pieces, s) : run_many<bf16_t, 128>(a, pieces, s);
 }
 template <>
-ManyShape many_shape<bf16_t>(int head_dim, bool causal) {
-  return head_dim == 64 ? shape_of<bf16_t, 64>(causal) : shape_of<bf16_t, 128>(causal);
+ManyShape many_shape<bf16_t>(int head_dim, bool causal, int64_t group) {
+  return head_dim == 64 ? shape_of<bf16_t, 64>(causal, group) : shape_of<bf16_t, 128>(causal, group);
 }
 
 }  // namespace paged

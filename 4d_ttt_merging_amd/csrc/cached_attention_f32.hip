@@ -9,8 +9,8 @@ int launch_many<float>(const Attend& a, int64_t pieces, int head_dim, hipStream_
   return head_dim == 64 ? run_many<float, 64>(a, pieces, s) : run_many<float, 128>(a, pieces, s);
 }
 template <>
-ManyShape many_shape<float>(int head_dim, bool causal) {
-  return head_dim == 64 ? shape_of<float, 64>(causal) : shape_of<float, 128>(causal);
+ManyShape many_shape<float>(int head_dim, bool causal, int64_t group) {
+  return head_dim == 64 ? shape_of<float, 64>(causal, group) : shape_of<float, 128>(causal, group);
 }
 
 }  // namespace paged

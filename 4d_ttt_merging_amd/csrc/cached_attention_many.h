@@ -2,7 +2,7 @@
 //
 // kWaves waves of 32 rows each share 64 tokens at a time: the codes come into registers two tiles ahead, are
 // converted once for all waves into operands of the 32 x 32 matrix instructions and written to LDS in the order in which
-// their lanes read them (16 bytes a lane, no bank conflicts), double-buffered, one barrier a tile:
+// their lanes read them (16 bytes a lane), double-buffered, one barrier a tile:
 //   scores^T = K Q^T; row m of a block of 32 tokens holds token 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so
 //     that a lane's sixteen scores are two operands of the next product as they stand
 //   out^T += V^T P^T, a lane having converted two channels of eight tokens, operands of two tiles
@@ -10,7 +10,7 @@
 //
 // Bound by matrix and vector instructions in turn: a wave's products wait for its conversions and softmax, which other waves'
 // products cover in part (64 channels: MFMA busy 0.38 of the time, VALU 0.63; 128: 0.38, 0.41).  bf16, 16 heads of 8,192 x 8,192:
-// 64 channels 317 us, 867 TFLOP/s; 128 535, 1,028; a product of 8,192^3 reaches 1,141.
+// 64 channels 322 us, 853 TFLOP/s; 128 505, 1,089; a product of 8,192^3 reaches 1,141.
 //
 // f16: where a piece's scales let keys and values be f16 numbers, and they nearly always do, the products are f16 ones
 // (16 heads, 8,192 x 8,192, 64 channels: two bf16 terms of q and of p 592 us, so 361).  Else, and in fp32, bf16 terms.
@@ -41,35 +41,23 @@ __device__ __forceinline__ float pair_sum(bf16x2 x, float sum) {
   return __builtin_amdgcn_fdot2_f32_bf16(x, one, sum, false);
 }
 
-// How a type and width are run: waves of a work-group, waves that a SIMD is to hold, whether operands are read from LDS in
-// groups ahead of their products (one by one, as the compiler has it to save registers, each product waits out a read).  More
-// waves share what is converted and read from LDS; fewer leave less idle where a causal tile ends.  16 heads, us with
-// 4 waves (2 a SIMD, 3, 3 grouped), 8 (2, 2 grouped, 4, 4 grouped):
-//   bf16  64 channels, 8,192 x 8,192   382 381 375   385 376 321 340     causal  194 195 184   212 206 204 231
-//   f16   64                           399 409 416   381 386 364 379             199 205 202   206 211 248 254
-//   bf16 128 (else 4: 2, 2 grouped)    572 588       535 534 (4 a SIMD: registers spilled, 1,624 and more)
-//   f16  128, 4,096 x 8,192            324 328       290 282;   fp32, 2,048 x 2,048  121 225  112 205;  64 channels  84 84  80 81
-//   fp32  64, 8 heads of 261 x 1,044    18  17        20  21
-template <typename T, int D, bool kCausal>
+// How a type and width are run: waves of a work-group, waves that a SIMD is to hold.  More waves share what is converted and
+// read from LDS; fewer (kSharp) leave less idle where a causal tile ends: with few heads beside a key head its rows are many
+// tokens.  16 heads, us with 4 waves (2 a SIMD), 4 (3), 8 (2), 8 (4):
+//   64 channels, 8,192 x 8,192         bf16  379 376 381 330   f16  390 390 383 356     causal  193 192 206 206   204 203 212 248
+//   3 causal prompts over 4 key heads  bf16  153 153 175 141   f16  154 154 155 163     (4,096; up to 4,116)
+//   128 channels, over 8,192           bf16  586     533       f16  325     290         (8,192; 4,096)
+//   128, causal, 4,096                 bf16  123     128       f16  130     135
+//   fp32  2,048 x 2,048, 64 and 128 channels  71, 108  70, 106;   8 heads of 261 x 1,044  17  20
+template <typename T, int D, bool kSharp>
 struct Many {
-  static constexpr int kWaves = D == 128 ? 8 : 4, kResident = 2;
-  static constexpr bool kGrouped = D == 128 && !std::is_same_v<T, float>;
+  static constexpr bool kFull = std::is_same_v<T, float>;
+  static constexpr int kWaves = kSharp || (D == 64 && kFull) ? 4 : 8, kResident = kSharp || D == 128 || kFull ? 2 : 4;
 };
-template <>
-struct Many<bf16_t, 64, false> {
-  static constexpr int kWaves = 8, kResident = 4;
-  static constexpr bool kGrouped = false;
-};
-template <>
-struct Many<bf16_t, 64, true> {
-  static constexpr int kWaves = 4, kResident = 3;
-  static constexpr bool kGrouped = true;
-};
-template <>
-struct Many<f16_t, 64, false> {
-  static constexpr int kWaves = 8, kResident = 4;
-  static constexpr bool kGrouped = false;
-};
+template <typename T, int D>
+constexpr bool sharp(bool causal, int64_t group) {
+  return causal && (group < 4 || (D == 64 && std::is_same_v<T, f16_t>));
+}
 
 // The operands of a product in its type.
 template <bool kHalf>
@@ -112,7 +100,7 @@ __device__ __forceinline__ bool all_half(const Attend& a, int64_t b, int hk, int
   return __syncthreads_and(fit);
 }
 
-template <typename T, int D, int kWaves, int kResident, bool kGrouped>
+template <typename T, int D, int kWaves, int kResident>
 __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Attend a) {
   using L = Layout<D>;
   constexpr int kSteps = D / 16;        // products over a row's channels
@@ -170,30 +158,38 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   uint2 key_codes[D / 64] = {}, value_codes[D / 64] = {}, value_scales[D / 64] = {};
   uint32_t key_scale = 0;
   float key_mass = 0.0f;
-  // The page of this wave's block of a tile, known a tile before it is read.
+  // The page of this wave's block of a tile, looked up a tile before it is read and looked at then.  (Tokens before `end` are
+  // within the table.)
+  typedef const __attribute__((address_space(4))) int32_t* constant;
+  const constant table = reinterpret_cast<constant>(reinterpret_cast<uintptr_t>(a.pages.table + b * a.pages.width));
+  const int shift = a.pages.shift, pages = static_cast<int>(a.pages.pages), in_page = (1 << shift) - 1;
+  const uint32_t page_blocks = static_cast<uint32_t>(kv) << (shift - 5);
+  const uint8_t* head_data = a.pages.data + static_cast<int64_t>(hk << (shift - 5)) * L::kBytes;
+  const float* masses = a.pages.mass;
+  int first_found = -1, second_found = -1;
   int page = -1;
   bool gap_read = false;  // whether the tile has tokens that have no page, or lie past the end
-  bool gap_found = false;
   const auto find = [&](int n) {
     const int t0 = piece.begin + 64 * n;
-    const int first = t0 < end ? page_of(a.pages, b, t0) : -1;
-    const int second = t0 + 32 < end ? a.pages.shift > 5 ? first : page_of(a.pages, b, t0 + 32) : -1;
-    page = __builtin_amdgcn_readfirstlane(block == 0 ? first : second);
-    gap_found = first < 0 || second < 0 || t0 + 64 > piece.length;
+    if (t0 >= end) return;
+    first_found = table[t0 >> shift];
+    second_found = shift == 5 && t0 + 32 < end ? table[(t0 >> 5) + 1] : first_found;
   };
   // Reads the wave's block of tile n.  Without a page nothing is read: scales of zero keep what is left finite, and the
   // bias keeps it out.
   const auto read = [&](int n) {
     const int t0 = piece.begin + 64 * n + 32 * block;
-    gap_read = gap_found;
+    const bool first = static_cast<uint32_t>(first_found) < static_cast<uint32_t>(pages);
+    const bool second = static_cast<uint32_t>(second_found) < static_cast<uint32_t>(pages) && t0 - 32 * block + 32 < end;
+    page = block == 0 ? (first ? first_found : -1) : second ? second_found : -1;
+    gap_read = !first || !second || t0 - 32 * block + 64 > piece.length;
     if (page >= 0) {
-      const uint8_t* base = a.pages.data + block_of<D>(a.pages, page, hk, t0);
+      const uint8_t* base = head_data + (static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_blocks + ((t0 & in_page) >> 5)) * L::kBytes;
       if (does_keys) {
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) key_codes[e] = reinterpret_cast<const uint2*>(base + key_from)[e];
         key_scale = base[key_scale_from];
-        if (part == 0 && a.pages.mass)
-          key_mass = a.pages.mass[(static_cast<int64_t>(page) << a.pages.shift) + (t0 & ((1 << a.pages.shift) - 1)) + key];
+        if (part == 0 && masses) key_mass = masses[(static_cast<int64_t>(page) << shift) + (t0 & in_page) + key];
       }
       if (does_values) {
 #pragma unroll
@@ -206,7 +202,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
     if (gap_read) {
       const int kept = page < 0 ? 0 : piece.length - t0;
       if (key >= kept) key_scale = 0;
-      key_mass = key >= kept ? -INFINITY : a.pages.mass ? key_mass : 0.0f;
+      key_mass = key >= kept ? -INFINITY : masses ? key_mass : 0.0f;
 #pragma unroll
       for (int e = 0; e < D / 64; ++e) value_scales[e] = kept_scales(value_scales[e], kept - 8 * group);
     }
@@ -223,7 +219,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
         to[c / 2 * 64] = key_operand<kHalf>(key_codes[e].x, scale);
         to[c / 2 * 64 + 32] = key_operand<kHalf>(key_codes[e].y, scale);
       }
-      if (part == 0 && (gap_read || a.pages.mass)) {
+      if (part == 0 && (gap_read || masses)) {
         const float raw = mass_of(key_mass) * a.per_scale;
         bf16_t t[3];
         split<3>(raw, t);
@@ -289,7 +285,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
     for (int n = 0; n < tiles; ++n) {
       const int buffer = n & 1;
       __syncthreads();
-      const bool uneven = gap || a.pages.mass != nullptr;
+      const bool uneven = gap || masses != nullptr;
       if (n + 1 < tiles) {
         convert(buffer ^ 1, half);
         gap = gap_read;
@@ -304,7 +300,6 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) key_parts[k][s] = __builtin_bit_cast(vec, keys[buffer][k][s][lane]);
-        if constexpr (kGrouped) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -324,12 +319,18 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
         }
       }
       if (t0 + 63 > least) {
+        // Bits of the tokens that are seen, a word for 32 (comparisons would keep 64 scalar registers).
         const int most = place - t0 - 8 * h;
+        const uint64_t seen = most < 0 ? 0 : most >= 63 ? ~uint64_t{0} : (uint64_t{2} << most) - 1;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+          const int word = static_cast<int>(seen >> (32 * k));
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * k + 16 * (i >> 3) + (i & 7) > most) z[k][i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(word, 16 * (i >> 3) + (i & 7), 1));
+            z[k][i] = __uint_as_float((__float_as_uint(z[k][i]) & keep) | (0xff800000u & ~keep));
+          }
+        }
       }
       float local = z[0][0];
 #pragma unroll
@@ -372,14 +373,12 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
           for (int w = 0; w < kP; ++w) weights[k][i >> 3][w][i & 7] = t0[w], weights[k][i >> 3][w][(i & 7) + 1] = t1[w];
         }
       vec value_parts[2][kOut][2];
-      if constexpr (kGrouped) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int c = 0; c < kOut; ++c)
 #pragma unroll
           for (int t = 0; t < 2; ++t) value_parts[k][c][t] = __builtin_bit_cast(vec, values[buffer][k][c][t][lane]);
-        if constexpr (kGrouped) __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -432,25 +431,25 @@ template <typename T, int D, typename M>
 ManyShape shape_of() {
   static const int resident = [] {
     int n = 0;
-    const bool known = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, many_kernel<T, D, M::kWaves, M::kResident, M::kGrouped>,
-                                                                    M::kWaves * 64, 0) == hipSuccess;
+    const bool known = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, many_kernel<T, D, M::kWaves, M::kResident>, M::kWaves * 64,
+                                                                    0) == hipSuccess;
     if (!known) (void)hipGetLastError();  // (no device: nothing is launched either)
     return known && n > 0 ? n : 4 * M::kResident / M::kWaves;
   }();
   return {32 * M::kWaves, resident};
 }
 template <typename T, int D>
-ManyShape shape_of(bool causal) {
-  return causal ? shape_of<T, D, Many<T, D, true>>() : shape_of<T, D, Many<T, D, false>>();
+ManyShape shape_of(bool causal, int64_t group) {
+  return sharp<T, D>(causal, group) ? shape_of<T, D, Many<T, D, true>>() : shape_of<T, D, Many<T, D, false>>();
 }
 template <typename T, int D>
 int run_many(const Attend& a, int64_t pieces, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(pieces * a.tiles * a.pages.kv_heads);
-  const auto run = [&](auto causal) {
-    using M = Many<T, D, decltype(causal)::value>;
-    many_kernel<T, D, M::kWaves, M::kResident, M::kGrouped><<<grid, M::kWaves * 64, 0, s>>>(a);
+  const auto run = [&](auto shape) {
+    using M = Many<T, D, decltype(shape)::value>;
+    many_kernel<T, D, M::kWaves, M::kResident><<<grid, M::kWaves * 64, 0, s>>>(a);
   };
-  if (a.causal) run(std::true_type());
+  if (sharp<T, D>(a.causal, a.group)) run(std::true_type());
   else run(std::false_type());
   return check_launch("cached_attn");
 }
