@@ -147,16 +147,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   Codes<D, kMass> ring[kRing];
   bool there[kRing];
   const int first = piece.begin / kBlock, blocks = a.pages.pages > 0 ? (end + kBlock - 1) / kBlock : 0;
-  const auto page_at = [&](int block) {
-    const int64_t t = static_cast<int64_t>(block) * kBlock;
-    return block < blocks ? page_of(a.pages, b, t) : -1;
-  };
+  // (Looked up a step before it is looked at.  Tokens before `end` are within the table.)
+  typedef const __attribute__((address_space(4))) int32_t* constant;
+  const constant table = reinterpret_cast<constant>(reinterpret_cast<uintptr_t>(a.pages.table + b * a.pages.width));
+  const int shift = a.pages.shift - 5, in_page = (1 << shift) - 1;  // in blocks
+  const uint32_t pages = static_cast<uint32_t>(a.pages.pages), page_blocks = static_cast<uint32_t>(kv) << shift;
+  const uint8_t* head_data = a.pages.data + static_cast<int64_t>(hk << shift) * L::kBytes;
+  const auto page_at = [&](int block) { return block < blocks ? table[block >> shift] : -1; };
   const auto read = [&](int slot, int block, int page) {
-    const int64_t t = static_cast<int64_t>(block) * kBlock;
-    there[slot] = page >= 0;
-    const uint8_t* from = a.pages.data + (page < 0 ? 0 : block_of<D>(a.pages, page, hk, t));
-    const float* mass = !kMass || page < 0 ? a.pages.mass
-                                           : a.pages.mass + (static_cast<int64_t>(page) << a.pages.shift) + (t & ((1 << a.pages.shift) - 1));
+    there[slot] = static_cast<uint32_t>(page) < pages;
+    const uint8_t* from = a.pages.data;
+    const float* mass = a.pages.mass;
+    if (there[slot]) {
+      from = head_data + (static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_blocks + (block & in_page)) * L::kBytes;
+      if (kMass) mass += ((static_cast<int64_t>(page) << shift) + (block & in_page)) * kBlock;
+    }
     read_codes(ring[slot], from, mass, offsets);
   };
   const auto compute = [&](const Codes<D, kMass>& codes, int block) {
