@@ -301,8 +301,7 @@ __device__ __forceinline__ void split(float x, N (&t)[kTerms]) {
 }
 
 // The two kernels: few rows beside a key head (cached_attention_few.hip), many (cached_attention_many.h, a file a type).
-constexpr int kFewRows = 64;
-int few_tile(int64_t rows);  // rows of a tile
+constexpr int kFewRows = 64, kFewTile = 16;
 int launch_few(const Attend& a, int64_t pieces, int head_dim, int dtype, hipStream_t s);
 struct ManyShape {
   int tile_rows, resident;  // rows of a work-group, work-groups that a CU holds

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Attend a) {
 
 // Rows of a work-group: four, a wave each, where there are few; else 32, so that calls of which no row has several pieces
 // are soon through with them (64 rows of 8 key heads over 16 pieces 42 us with the one, 52 with the other; 3 x 16,464 rows in one
-// piece each 196, 154).
+// piece each 196, 154).  Neither passes the end of a tile: of tiles of 16 a launch with pieces has fewer than 8,192 rows.
 template <typename T, int D>
 void join_pieces(const Attend& a, hipStream_t s) {
   const int64_t rows = a.last_row - a.first_row, all = a.batch * a.pages.kv_heads;
@@ -145,7 +145,7 @@ Part part_of(const vgo_paged_cache* c, int64_t first_row, int64_t last_row, bool
   Part p{};
   const int64_t rows = last_row - first_row, capacity = c->table_width * c->page_size;
   p.few = few, p.first_row = first_row, p.last_row = last_row;
-  p.tile_rows = few ? few_tile(rows) : shape.tile_rows;
+  p.tile_rows = few ? kFewTile : shape.tile_rows;
   p.least = few ? kLeastFew : kLeastMany;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // Few queries: as many work-groups as the chip holds at once.  Many, of which some sequences may have fewer than others: more,

@@ -8,7 +8,9 @@
 //     lane that gets rows 4 g .. 4 g + 3 of both has tokens 8 g .. 8 g + 7 -- as the next product's operand wants them
 //   out^T += V^T P^T; a lane has converted two channels of eight tokens, operands of two tiles
 // Maxima are kept in common by the wave and moved only where a score exceeds them by 2^8; sums stay in their lanes.
-// Eight waves share a piece of a sequence and join their sums in LDS.
+// Eight waves share a piece of a sequence and join their sums in LDS.  Rows go by 16, whose further tiles find the codes in the
+// caches; 32 at a time spill registers with 128 channels (32 rows of 8 x 16,384 tokens with masses, us: f16 91, so 45; fp32 139,
+// 50; bf16 52, 43) and are as fast as this with 64 (bf16 30, 32 with masses; 64 rows without 38, 36).
 #include "cached_attention.h"
 
 namespace vgo {
@@ -80,7 +82,7 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[kTerm
   }
 }
 
-template <typename T, int D, int NT, bool kMass>
+template <typename T, int D, bool kMass>
 __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   using L = Layout<D>;
   constexpr int kQ = Terms<T>::kQuery, kP = Terms<T>::kWeight;
@@ -105,40 +107,34 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
   if (piece.begin > 0 && piece.begin >= stop) return;  // (the join does not ask for it)
   const bool whole = piece.begin == 0 && stop <= piece.end;
 
-  // Queries: row m of each tile, channels 8 s .. of this lane's D / 4.
-  bf16x8 q[NT][kSteps][kQ];
-  int place[NT];
+  // Queries: row m of the tile, channels 8 s .. of this lane's D / 4.
+  bf16x8 q[kSteps][kQ];
+  const int mine = row0 + m, token = mine / a.group;
+  const bool real = mine < count * a.group;
+  const int place = !real ? -1 : a.causal ? place0 + token : INT32_MAX;
+  const T* query = static_cast<const T*>(a.q) + b * a.q_stride[0] + (hk * a.group + mine % a.group) * a.q_stride[1] +
+                   token * a.q_stride[2] + g * (D / 4);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = row0 + 16 * nt + m, token = row / a.group;
-    const bool real = row < count * a.group;
-    place[nt] = !real ? -1 : a.causal ? place0 + token : INT32_MAX;
-    const T* from = static_cast<const T*>(a.q) + b * a.q_stride[0] + (hk * a.group + row % a.group) * a.q_stride[1] +
-                    token * a.q_stride[2] + g * (D / 4);
+  for (int s = 0; s < kSteps; ++s) {
+    float v[8] = {};
+    if (real) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      float v[8] = {};
-      if (real) {
+      for (int e = 0; e < 2; ++e) {
+        const f32x4 four = load4(query + 8 * s + 4 * e);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const f32x4 four = load4(from + 8 * s + 4 * e);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        bf16_t t[kQ];
-        split<kQ>(v[i], t);
-#pragma unroll
-        for (int n = 0; n < kQ; ++n) q[nt][s][n][i] = t[n];
+        for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
       }
     }
-  }
-  f32x4 acc[NT][D / 16] = {};
-  float raw[NT], top[NT], total[NT];  // the reference maximum, before and after the scale
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) raw[nt] = top[nt] = -INFINITY, total[nt] = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+      bf16_t t[kQ];
+      split<kQ>(v[i], t);
+#pragma unroll
+      for (int n = 0; n < kQ; ++n) q[s][n][i] = t[n];
+    }
+  }
+  f32x4 acc[D / 16] = {};
+  float raw = -INFINITY, top = -INFINITY, total = 0.0f;  // the reference maximum, before and after the scale
 
   // A ring of blocks on their way.  Reads are not conditional, so that the compiler knows how many are outstanding: what has
   // no page, or lies past the end, reads the start of the cache instead and is left out.
@@ -175,62 +171,59 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
       for (int s = 0; s < kSteps; ++s)
         keys[i][s] = __builtin_bit_cast(bf16x8, key_operand(s % 2 ? codes.k[i][s / 2].y : codes.k[i][s / 2].x, scale));
     }
-    Operand weights[NT][kP];
+    Operand weights[kP];
+    float z[8];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float z[8];
+    for (int i = 0; i < 2; ++i) {
+      f32x4 c = {};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        f32x4 c = {};
+      for (int n = kQ - 1; n >= 0; --n)
 #pragma unroll
-        for (int n = kQ - 1; n >= 0; --n)
+        for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[i][s], q[s][n], c, 0, 0, 0);
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[i][s], q[nt][s][n], c, 0, 0, 0);
+      for (int e = 0; e < 4; ++e) z[4 * i + e] = c[e];
+    }
+    if constexpr (kMass) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[4 * i + e] = c[e];
-      }
-      if constexpr (kMass) {
+      for (int i = 0; i < 8; ++i) z[i] = fmaf(z[i], a.scale, mass_of(codes.mass[i / 4][i % 4]) * 1.4426950408889634f);
+    }
+    const float scale = kMass ? 1.0f : a.scale;  // still to be applied
+    if (a.causal || !inside) {
+      const int most = min(place, piece.length - 1) - t0 - 8 * g;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = fmaf(z[i], a.scale, mass_of(codes.mass[i / 4][i % 4]) * 1.4426950408889634f);
-      }
-      const float scale = kMass ? 1.0f : a.scale;  // still to be applied
-      if (a.causal || !inside) {
-        const int most = min(place[nt], piece.length - 1) - t0 - 8 * g;
+      for (int i = 0; i < 8; ++i) z[i] = i <= most ? z[i] : -INFINITY;
+    }
+    float local = z[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = i <= most ? z[i] : -INFINITY;
-      }
-      float local = z[0];
+    for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
+    if (__any(local * scale > top + kLazy)) {
+      local = fmaxf(local, __shfl_xor(local, 16));
+      local = half_max(local);
+      raw = fmaxf(raw, local);
+      const float to = raw * scale;
+      const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      total *= shrink;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
-      if (__any(local * scale > top[nt] + kLazy)) {
-        local = fmaxf(local, __shfl_xor(local, 16));
-        local = half_max(local);
-        raw[nt] = fmaxf(raw[nt], local);
-        const float to = raw[nt] * scale;
-        const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[nt] - to);
-        top[nt] = to;
-        total[nt] *= shrink;
+      for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c)
+        for (int e = 0; e < 4; ++e) acc[c][e] *= shrink;
+    }
+    float from = top == -INFINITY ? 0.0f : top;
+    if (__any(fabsf(from) > kFar)) {  // (see kFar)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][c][e] *= shrink;
-      }
-      float from = top[nt] == -INFINITY ? 0.0f : top[nt];
-      if (__any(fabsf(from) > kFar)) {  // (see kFar)
+      for (int i = 0; i < 8; ++i) z[i] -= raw == -INFINITY ? 0.0f : raw;
+      from = 0.0f;
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] -= raw[nt] == -INFINITY ? 0.0f : raw[nt];
-        from = 0.0f;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(z[2 * i], scale, -from));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(z[2 * i + 1], scale, -from));
+      total += p0 + p1;
+      uint32_t t[kP];
+      split_pair<kP>(p0, p1, t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(z[2 * i], scale, -from));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(z[2 * i + 1], scale, -from));
-        total[nt] += p0 + p1;
-        uint32_t t[kP];
-        split_pair<kP>(p0, p1, t);
-#pragma unroll
-        for (int n = 0; n < kP; ++n) weights[nt][n].w[i] = t[n];
-      }
+      for (int n = 0; n < kP; ++n) weights[n].w[i] = t[n];
     }
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) {
@@ -240,12 +233,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
       value_operands(codes.v[u], scales, two[0], two[1]);
       const bf16x8 even = __builtin_bit_cast(bf16x8, two[0]), odd = __builtin_bit_cast(bf16x8, two[1]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int n = kP - 1; n >= 0; --n) {
-          acc[nt][2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, weights[nt][n].v, acc[nt][2 * u], 0, 0, 0);
-          acc[nt][2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, weights[nt][n].v, acc[nt][2 * u + 1], 0, 0, 0);
-        }
+      for (int n = kP - 1; n >= 0; --n) {
+        acc[2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, weights[n].v, acc[2 * u], 0, 0, 0);
+        acc[2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, weights[n].v, acc[2 * u + 1], 0, 0, 0);
+      }
     }
   };
   int block = first + wave;
@@ -264,50 +255,46 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     }
   }
 
-  // The waves' sums, 16 rows at a time.
+  // The waves' sums.
+  total += __shfl_xor(total, 16);
+  total = half_sum(total);
+  if (g == 0) tops[wave][m] = top, totals[wave][m] = total;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    total[nt] += __shfl_xor(total[nt], 16);
-    total[nt] = half_sum(total[nt]);
-    if (nt > 0) __syncthreads();
-    if (g == 0) tops[wave][m] = top[nt], totals[wave][m] = total[nt];
+  for (int u = 0; u < D / 32; ++u) {
+    const f32x4 e = acc[2 * u], o = acc[2 * u + 1];
+    f32x4* to = reinterpret_cast<f32x4*>(&joined[wave][m][32 * u + 8 * g]);
+    to[0] = f32x4{e[0], o[0], e[1], o[1]};
+    to[1] = f32x4{e[2], o[2], e[3], o[3]};
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * D / 4; i += kWaves * 64) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    const int row = row0 + r;
+    if (row >= a.last_row) continue;
+    float most = tops[0][r];
 #pragma unroll
-    for (int u = 0; u < D / 32; ++u) {
-      const f32x4 e = acc[nt][2 * u], o = acc[nt][2 * u + 1];
-      f32x4* to = reinterpret_cast<f32x4*>(&joined[wave][m][32 * u + 8 * g]);
-      to[0] = f32x4{e[0], o[0], e[1], o[1]};
-      to[1] = f32x4{e[2], o[2], e[3], o[3]};
+    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, tops[w][r]);
+    const float from = most == -INFINITY ? 0.0f : most;
+    float sum = 0.0f;
+    f32x4 v = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float share = __builtin_amdgcn_exp2f(tops[w][r] - from);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(&joined[w][r][c]);
+      sum = fmaf(totals[w][r], share, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * D / 4; i += kWaves * 64) {
-      const int r = i / (D / 4), c = i % (D / 4) * 4;
-      const int row = row0 + 16 * nt + r;
-      if (row >= a.last_row) continue;
-      float most = tops[0][r];
+    if (whole) {
+      const bool none = row >= count * a.group || most == -INFINITY;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) most = fmaxf(most, tops[w][r]);
-      const float from = most == -INFINITY ? 0.0f : most;
-      float sum = 0.0f;
-      f32x4 v = {};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float share = __builtin_amdgcn_exp2f(tops[w][r] - from);
-        const f32x4 part = *reinterpret_cast<const f32x4*>(&joined[w][r][c]);
-        sum = fmaf(totals[w][r], share, sum);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
-      }
-      if (whole) {
-        const bool none = row >= count * a.group || most == -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
-        store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
-                   row / a.group * a.out_stride[2] + c, v);
-      } else {
-        const int64_t to = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + 16 * nt + r;
-        store4(a.sums + to * D + c, v);
-        if (c == 0) a.ends[to] = {most, sum};
-      }
+      for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
+      store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +
+                 row / a.group * a.out_stride[2] + c, v);
+    } else {
+      const int64_t to = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + r;
+      store4(a.sums + to * D + c, v);
+      if (c == 0) a.ends[to] = {most, sum};
     }
   }
 }
@@ -315,18 +302,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 template <typename T, int D>
 int launch(const Attend& a, int64_t pieces, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(pieces * a.tiles * a.pages.kv_heads);
-  const auto run = [&](auto mass) {
-    if (a.tile_rows == 16) few_kernel<T, D, 1, decltype(mass)::value><<<grid, kWaves * 64, 0, s>>>(a);
-    else few_kernel<T, D, 2, decltype(mass)::value><<<grid, kWaves * 64, 0, s>>>(a);
-  };
-  if (a.pages.mass) run(std::true_type());
-  else run(std::false_type());
+  if (a.pages.mass) few_kernel<T, D, true><<<grid, kWaves * 64, 0, s>>>(a);
+  else few_kernel<T, D, false><<<grid, kWaves * 64, 0, s>>>(a);
   return check_launch("cached_attn");
 }
 
 }  // namespace
-
-int few_tile(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
 int launch_few(const Attend& a, int64_t pieces, int head_dim, int dtype, hipStream_t s) {
   if (head_dim == 64) {
