@@ -149,7 +149,7 @@ __device__ __forceinline__ float to_odd(double d) {
 // Codes of x cos + o sin, exactly those of the 64-bit value: fp32 first, which is off by at most 2^-24 of the
 // product x cos and of the sum each; where some channel of the wave lies so near a border that this may matter (about
 // one of 500 waves), 64 bits.  (64 bits throughout kept the vector unit busy for three times as long as
-// memory takes: 4 ragged prompts of up to 8,232 tokens, 16 heads of 64 channels, 184 us, this 79.)
+// memory takes: 4 ragged prompts of up to 8,232 tokens, 16 heads of 64 channels, 184 us, this 67.)
 __device__ __forceinline__ uint32_t quantise_rotated(const float (&x)[8], const float (&o)[8], const float (&sin)[8],
                                                      const float (&cos)[8], bool real, uint32_t& byte) {
   float y[8], low[8], high[8];
