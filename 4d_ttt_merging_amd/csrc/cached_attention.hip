@@ -83,17 +83,18 @@ __global__ __launch_bounds__(256) void join_kernel(const Attend a) {
   }
 }
 
-// Rows of a work-group: four, a wave each, where there are few; else 32, so that calls of which no row has several pieces
-// are soon through with them (64 rows of 8 key heads over 16 pieces 42 us with the one, 52 with the other; 3 x 16,464 rows in one
-// piece each 196, 154).  Neither passes the end of a tile: of tiles of 16 a launch with pieces has fewer than 8,192 rows.
+// Rows of a work-group: four, a wave each, where there are few; else 128, so that calls of which no row has several pieces
+// are soon through with them (64 rows of 8 key heads over 16 pieces 42 us with the one, 52 with 32; 3 causal prompts, whole:
+// 16,464 rows each 196 by 4, 154 by 32, some 9,000 rows each 73 by 32, 70 by 128; two cut chunks of 8,232 rows alike by 32 and
+// 128).  Neither passes the end of a tile: of tiles of 16 a launch with pieces has fewer than 8,192 rows.
 template <typename T, int D>
 void join_pieces(const Attend& a, hipStream_t s) {
   const int64_t rows = a.last_row - a.first_row, all = a.batch * a.pages.kv_heads;
   const bool few = rows * all <= 16384;
-  const int64_t each = few ? 4 : 32;
+  const int64_t each = few ? 4 : 128;
   const unsigned grid = static_cast<unsigned>(all * ((rows + each - 1) / each));
   if (few) join_kernel<T, D, 4, true><<<grid, 256, 0, s>>>(a);
-  else join_kernel<T, D, 32, false><<<grid, 256, 0, s>>>(a);
+  else join_kernel<T, D, 128, false><<<grid, 256, 0, s>>>(a);
 }
 template <typename T>
 int join_pieces(const Attend& a, int head_dim, hipStream_t s) {
