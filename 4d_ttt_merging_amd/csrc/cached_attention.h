@@ -140,8 +140,8 @@ __device__ __forceinline__ int quotient(int x, int y) {
 }
 
 // Many queries: the length of pieces that costs least, in tokens of a tile: rounds of work-groups that have queries, each a
-// piece and what it begins and ends with; and what they leave to the join, for as many as the chip holds.  A lane looks at one
-// length, a part of the longest sequence.  (The sequences differ in queries and lengths, and a ragged last round idles most
+// piece and what it begins and ends with; and what they leave to the join, for as many as the chip holds.  Lengths are
+// parts of the longest sequence.  (The sequences differ in queries and lengths, and a ragged last round idles most
 // of the chip: one or two full rounds by the sums alone took, of calls with 2 or 3 ragged causal sequences, 4% longer in bf16 and
 // 9% in fp32; 2 x 2,300 queries over 16,464 tokens of 128 channels, 288 work-groups of which 256 fit, whole 901 us, so 649.
 // kRound, kJoin of 64 to 512, 300 to 1,200: within 2% up to 192, 450.)
@@ -161,24 +161,46 @@ __device__ __forceinline__ Pieces many_pieces(const Attend& a) {
   steep = static_cast<int>(wave_sum(static_cast<uint32_t>(steep))) * a.pages.kv_heads;
   longest = wave_max(longest);
   if (2 * static_cast<int64_t>(steep) > busy && 10 * static_cast<int64_t>(busy) >= 9 * static_cast<int64_t>(a.held)) return p;
-  // 1 .. 32 of the longest, then eight a doubling.
-  const int parts = lane < 32 ? lane + 1 : static_cast<int>(32.0f * __builtin_amdgcn_exp2f((lane - 31) * 0.125f));
-  const int tokens = max((quotient(longest, parts) + 64) & ~63, a.least);
-  int64_t n = 0, groups = 0;
-  for (int b = 0; b < a.batch; ++b) {
-    const int one = quotient(max(0, length_of(a, b) - 1), tokens) + 1;
-    n += one, groups += static_cast<int64_t>(one) * busy_tiles(a, b);
+  const int64_t most = a.slots + a.batch;
+  const auto cost = [&](int tokens, int64_t n, int64_t tiles) {
+    const int groups = static_cast<int>(min(tiles * a.pages.kv_heads, int64_t{1} << 29));  // (the grid holds fewer than 2^23)
+    const int rounds = quotient(groups + a.held - 1, a.held);
+    const float join = tokens < longest ? kJoin * static_cast<float>(groups) / static_cast<float>(a.held) : 0.0f;
+    return n > most ? INFINITY : static_cast<float>(rounds) * (static_cast<float>(tokens) + kRound) + join;
+  };
+  const auto part = [&](int parts) { return max((quotient(longest, parts) + 64) & ~63, a.least); };
+  int taken = longest;
+  if (a.batch <= 64) {
+    // A lane looks at one: 1 .. 32 parts, then eight a doubling.
+    const int tokens = part(lane < 32 ? lane + 1 : static_cast<int>(32.0f * __builtin_amdgcn_exp2f((lane - 31) * 0.125f)));
+    const int mine = lane < a.batch ? busy_tiles(a, lane) : 0;
+    int n = 0, tiles = 0;
+    for (int b = 0; b < a.batch; ++b) {
+      const int one = quotient(max(0, __builtin_amdgcn_readlane(p.mine, b) - 1), tokens) + 1;
+      n += one, tiles += one * __builtin_amdgcn_readlane(mine, b);
+    }
+    const int order = -static_cast<int>(__float_as_uint(cost(tokens, n, tiles)));
+    const uint64_t best = __ballot(order == wave_max(order));
+    taken = __builtin_amdgcn_readlane(tokens, __ffsll(static_cast<unsigned long long>(best)) - 1);
+  } else {
+    // One after the other, a lane a sequence: 1 .. 4 parts, then two a doubling.  (500 sequences of up to 80 queries over
+    // 1,000 tokens, a lane a length 250 us, so 120.)
+    float least_cost = INFINITY;
+    for (int c = 0; c < 16; ++c) {
+      const int tokens = part(c < 4 ? c + 1 : (c & 1 ? 4 : 3) << ((c - 2) / 2));
+      int n = 0, tiles = 0;
+      for (int64_t b = lane; b < a.batch; b += 64) {
+        const int one = quotient(max(0, length_of(a, b) - 1), tokens) + 1;
+        n += one, tiles += one * busy_tiles(a, b);
+      }
+      const float mine = cost(tokens, wave_sum(static_cast<uint32_t>(n)), wave_sum(static_cast<uint32_t>(tiles)));
+      if (mine < least_cost) least_cost = mine, taken = tokens;
+    }
   }
-  const int all = static_cast<int>(min(groups * a.pages.kv_heads, int64_t{1} << 29));  // (the grid holds fewer than 2^23)
-  const int rounds = quotient(all + a.held - 1, a.held);
-  const float join = tokens < longest ? kJoin * static_cast<float>(all) / static_cast<float>(a.held) : 0.0f;
-  const float cost = n > a.slots + a.batch ? INFINITY : static_cast<float>(rounds) * (static_cast<float>(tokens) + kRound) + join;
-  const int order = -static_cast<int>(__float_as_uint(cost));
-  const uint64_t best = __ballot(order == wave_max(order));
-  const int taken = __builtin_amdgcn_readlane(tokens, __ffsll(static_cast<unsigned long long>(best)) - 1);
   if (taken < longest) p.tokens = taken;
   return p;
 }
+
 struct Piece {
   int64_t b;           // -1: there is no such piece
   int begin, end;      // its tokens
