@@ -289,3 +289,36 @@ def test_another_device_or_a_current_one(vgo, device, n):
         vgo.cached_attention(new[0], cache, table, starts.cpu())
     with pytest.raises(RuntimeError):
         vgo.cache_append(cache, new[1], new[2], table.cpu(), starts)
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_a_block_with_gradients_enabled_and_captured(vgo, device, autocast):
+    """Forward with gradients enabled gives what it gives without, and has no backward; a captured block's step replays."""
+    torch.manual_seed(0)
+    block = vgo.SelfAttentionBlock(128, 2, qkv_bias=True, use_qk_norm=True, init_values=0.5).to(device).eval()
+    rope = import_package("layers").rope_sincos(4, 5, 64, device=device)
+    table, lengths = int32([[1, 0], [2, 3]], device), int32([30, 25], device)
+    x = torch.randn(2, 25, 128, device=device)
+    caches = [vgo.PagedCache.empty(4, 2, 64, page_size=32, device=device) for _ in range(2)]
+    steps = [dict(cache=c, page_table=table, lengths=lengths, causal=True) for c in caches]
+    with torch.autocast("cuda", dtype=BF16, enabled=autocast):
+        with torch.no_grad():
+            want = block(x, rope, cached=steps[0])
+        out = block(x, rope, cached=steps[1])
+    assert (out - want).abs().max() <= (2.0 ** -4 if autocast else 2.0 ** -16) * want.abs().max()  # (other launches round elsewhere)
+    with pytest.raises(RuntimeError):
+        out.sum().backward()
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16, enabled=autocast, cache_enabled=False), torch.cuda.stream(stream):
+        block(x, rope, cached=steps[0])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            got = block(x, rope, cached=steps[0])
+    for turn in range(3):
+        x.copy_(torch.randn_like(x))
+        lengths.copy_(int32([30 + turn, 40 - turn], device))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad(), torch.autocast("cuda", dtype=BF16, enabled=autocast, cache_enabled=False):
+            assert torch.equal(got, block(x, rope, cached=steps[0]))
