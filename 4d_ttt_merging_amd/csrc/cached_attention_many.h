@@ -2,7 +2,7 @@
 //
 // kWaves waves of 32 rows each share 64 tokens at a time: the codes come into registers two tiles ahead, are
 // converted once for all waves into operands of the 32 x 32 matrix instructions and written to LDS in the order in which
-// their lanes read them (16 bytes a lane), double-buffered, one barrier a tile:
+// their lanes read them (16 bytes a lane), double-buffered, one barrier a tile or two:
 //   scores^T = K Q^T; row m of a block of 32 tokens holds token 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so
 //     that a lane's sixteen scores are two operands of the next product as they stand
 //   out^T += V^T P^T, a lane having converted two channels of eight tokens, operands of two tiles
@@ -106,10 +106,13 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   constexpr int kSteps = D / 16;        // products over a row's channels
   constexpr int kOut = D / 32;          // tiles of 32 channels
   constexpr bool kApart = kWaves == 8;  // half the waves convert keys, half values
-  // [buffer][block of 32 tokens][step][lane], [buffer][block][tile][step of 16 tokens][lane]: operands of 16 bytes
-  __shared__ u32x4 keys[2][2][kSteps][64];
-  __shared__ u32x4 values[2][2][kOut][2][64];
-  __shared__ uint2 bias[2][64];  // three bf16 terms of what is added to a token's scores, before the scale
+  // Tiles from one barrier to the next, as many as of which twice fit LDS beside other work-groups (2 x 2,058 ragged queries over 16,464
+  // tokens of 128 channels: bf16 228 us with one, 219 with two, f16 249, 241; fp32 110, 112; 64 channels within 2%).
+  constexpr int kSpan = kApart && !std::is_same_v<T, float> ? 2 : 1, kSlots = 2 * kSpan;
+  // [slot][block of 32 tokens][step][lane], [slot][block][tile][step of 16 tokens][lane]: operands of 16 bytes
+  __shared__ u32x4 keys[kSlots][2][kSteps][64];
+  __shared__ u32x4 values[kSlots][2][kOut][2][64];
+  __shared__ uint2 bias[kSlots][64];  // three bf16 terms of what is added to a token's scores, before the scale
   const int lane = lane_id(), m = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kv = a.pages.kv_heads;
@@ -207,11 +210,11 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       for (int e = 0; e < D / 64; ++e) value_scales[e] = kept_scales(value_scales[e], kept - 8 * group);
     }
   };
-  const auto convert = [&](int buffer, auto half) {
+  const auto convert = [&](int slot, auto half) {
     constexpr bool kHalf = decltype(half)::value;
     if (does_keys) {
       const float scale = scale_of<0>(key_scale);
-      u32x4* to = &keys[buffer][block][0][0] + key_row;
+      u32x4* to = &keys[slot][block][0][0] + key_row;
 #pragma unroll
       for (int e = 0; e < D / 64; ++e) {
         // chunk c of 8 channels: step c / 2, lanes' half c % 2
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
         split<3>(raw, t);
         if (raw == -INFINITY) t[1] = t[2] = static_cast<bf16_t>(0.0f);
         const bf16x2 first = {t[0], t[1]}, second = {t[2], static_cast<bf16_t>(0.0f)};
-        bias[buffer][32 * block + key_row] = {__builtin_bit_cast(uint32_t, first), __builtin_bit_cast(uint32_t, second)};
+        bias[slot][32 * block + key_row] = {__builtin_bit_cast(uint32_t, first), __builtin_bit_cast(uint32_t, second)};
       }
     }
     if (does_values) {
@@ -233,8 +236,8 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       for (int e = 0; e < D / 64; ++e) {
         u32x4 even, odd;
         value_operands<kHalf>(value_codes[e], value_scales[e], even, odd);
-        values[buffer][block][2 * e][group >> 1][(group & 1) * 32 + pair] = even;
-        values[buffer][block][2 * e + 1][group >> 1][(group & 1) * 32 + pair] = odd;
+        values[slot][block][2 * e][group >> 1][(group & 1) * 32 + pair] = even;
+        values[slot][block][2 * e + 1][group >> 1][(group & 1) * 32 + pair] = odd;
       }
     }
   };
@@ -272,26 +275,32 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
     }
     // (Else the first product of every tile waits for whatever is outstanding, in case it is these.)
     wait_vmem<0>();
-    bool gap = false;
+    bool gaps[kSpan] = {};  // of tiles n, ..
     if (tiles > 0) {
       find(0);
-      read(0);
-      find(1);
-      convert(0, half);
-      gap = gap_read;
-      if (tiles > 1) read(1);
-      find(2);
+#pragma unroll
+      for (int i = 0; i < kSpan; ++i)
+        if (i < tiles) {
+          read(i);
+          find(i + 1);
+          convert(i, half);
+          gaps[i] = gap_read;
+        }
+      if (tiles > kSpan) read(kSpan);
+      find(kSpan + 1);
     }
     for (int n = 0; n < tiles; ++n) {
-      const int buffer = n & 1;
-      __syncthreads();
-      const bool uneven = gap || masses != nullptr;
-      if (n + 1 < tiles) {
-        convert(buffer ^ 1, half);
-        gap = gap_read;
+      const int slot = n % kSlots;
+      if (n % kSpan == 0) __syncthreads();
+      const bool uneven = gaps[0] || masses != nullptr;
+#pragma unroll
+      for (int i = 0; i + 1 < kSpan; ++i) gaps[i] = gaps[i + 1];
+      if (n + kSpan < tiles) {
+        convert((n + kSpan) % kSlots, half);
+        gaps[kSpan - 1] = gap_read;
       }
-      if (n + 2 < tiles) read(n + 2);
-      find(n + 3);
+      if (n + kSpan + 1 < tiles) read(n + kSpan + 1);
+      find(n + kSpan + 2);
       const int t0 = piece.begin + 64 * n;
       if (idle || (a.causal && t0 > place0 + (row0 + 31) / a.group)) continue;
       f32x16 z[2] = {};
@@ -299,7 +308,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) key_parts[k][s] = __builtin_bit_cast(vec, keys[buffer][k][s][lane]);
+        for (int s = 0; s < kSteps; ++s) key_parts[k][s] = __builtin_bit_cast(vec, keys[slot][k][s][lane]);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -311,7 +320,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
         // What is added to a token's scores, and what has no place: one more step of the product, by ones.
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint2 t = bias[buffer][32 * k + m];
+          const uint2 t = bias[slot][32 * k + m];
           Operand o, one;
           o.w[0] = h == 0 ? t.x : 0, o.w[1] = h == 0 ? t.y : 0, o.w[2] = o.w[3] = 0;
           one.w[0] = h == 0 ? 0x3f803f80u : 0, one.w[1] = h == 0 ? 0x00003f80u : 0, one.w[2] = one.w[3] = 0;
@@ -378,7 +387,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
 #pragma unroll
         for (int c = 0; c < kOut; ++c)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) value_parts[k][c][t] = __builtin_bit_cast(vec, values[buffer][k][c][t][lane]);
+          for (int t = 0; t < 2; ++t) value_parts[k][c][t] = __builtin_bit_cast(vec, values[slot][k][c][t][lane]);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
