@@ -9,8 +9,8 @@
 // One reference maximum a row, moved only where a score passes it by 2^8.
 //
 // Bound by matrix and vector instructions in turn: a wave's products wait for its conversions and softmax, which other waves'
-// products cover in part (64 channels: MFMA busy 0.40 of the time, VALU 0.60; 128: 0.41, 0.40).  bf16, 16 heads of 8,192 x 8,192:
-// 64 channels 322 to 331 us, 830 to 853 TFLOP/s; 128 505 to 528, 1,041 to 1,089; a product of 8,192^3 reaches 1,141.
+// products cover in part (64 channels: MFMA busy 0.41 of the time, VALU 0.62; 128: 0.43, 0.43).  bf16, 16 heads of 8,192 x 8,192:
+// 64 channels 321 us, 855 TFLOP/s; 128 503, 1,093; a product of 8,192^3 reaches 1,141.
 //
 // f16: where a piece's scales let keys and values be f16 numbers, and they nearly always do, the products are f16 ones
 // (16 heads, 8,192 x 8,192, 64 channels: two bf16 terms of q and of p 592 us, so 361).  Else, and in fp32, bf16 terms.
