@@ -75,7 +75,8 @@ struct Number<true> {
 
 // Whether tokens [begin, end) are f16 numbers: keys exactly (scales from 2^-23, whose halves are f16's smallest numbers, to 2^13;
 // or below 2^-63, where zero is as good), values to f16's smallest number (to 2^13), as far as their sums are
-// rounded in any case.  All threads of a work-group together.
+// rounded in any case.  `end` is where what is converted ends: a probability of zero times a value that has become an
+// infinity is NaN.  All threads of a work-group together.
 template <int D, int kThreads>
 __device__ __forceinline__ bool all_half(const Attend& a, int64_t b, int hk, int begin, int end) {
   using L = Layout<D>;
@@ -401,7 +402,9 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
     top -= kLift;
   };
   if constexpr (std::is_same_v<T, f16_t>) {
-    if (all_half<D, kWaves * 64>(a, b, hk, piece.begin, end)) run(std::true_type());
+    // (Blocks are converted whole, the last one past what a causal tile sees.)
+    const int converted = min((end + kBlock - 1) & -kBlock, piece.length);
+    if (all_half<D, kWaves * 64>(a, b, hk, piece.begin, converted)) run(std::true_type());
     else run(std::false_type());
   } else {
     run(std::false_type());

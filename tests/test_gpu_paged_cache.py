@@ -393,3 +393,19 @@ def test_lengths_beyond_any_table(vgo, device, n):
     for ends in ([2 ** 31 - 1, -2 ** 31], [2 ** 31 - 32, -5], [2 ** 30, -1]):
         assert torch.equal(want, both.to(q).new_zeros(()) + vgo.cached_attention(both.to(q), both.cache, both.to(table),
                                                                                 both.to(int32(ends)), causal=True))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,place", [(1, 140), (1, 265), (3, 50), (4, 40), (4, 70)])
+def test_a_later_value_beyond_f16_leaves_earlier_rows_alone(vgo, device, dim, group, place):
+    """One value that f16 does not hold, of a new token in the block of 32 in which a tile of 128 or 256 causal rows ends,
+    behind the last one that the tile's rows see."""
+    table, pages = layout(1, 305, 64, 40)
+    both = Both(vgo, device, pages, 1, 64, dim)
+    both.fill(41)
+    k, v = torch.full((1, 1, 1, dim), -8.0), torch.zeros(1, 1, 1, dim)
+    v[..., 1::2] = 6 * 2.0 ** 14
+    both.append(k, v, table, int32([place]))
+    # (an improbable key: what later rows make of it is finite in f16)
+    q = torch.randn(1, group, 300, dim, generator=torch.Generator().manual_seed(42)).abs().half() + 1.0
+    both.attend(q, table, int32([305]), causal=True)
