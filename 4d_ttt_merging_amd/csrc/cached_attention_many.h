@@ -74,7 +74,7 @@ struct Number<true> {
 };
 
 // Whether tokens [begin, end) are f16 numbers: keys exactly (scales from 2^-23, whose halves are f16's smallest numbers, to 2^13;
-// or below 2^-63, where zero is as good), values to f16's smallest number (to 2^13), as far as their sums are
+// or below 2^-87, where zero is as good: scores of them are below 2^-34 at the largest scale), values to f16's smallest number (to 2^13), as far as their sums are
 // rounded in any case.  `end` is where what is converted ends: a probability of zero times a value that has become an
 // infinity is NaN.  All threads of a work-group together.
 template <int D, int kThreads>
@@ -94,7 +94,7 @@ __device__ __forceinline__ bool all_half(const Attend& a, int64_t b, int hk, int
       const int byte = 16 * at + e;
       const int token = key ? byte / L::kParts : (byte - D) / L::kScaleGroup * 8 + byte % 8;
       const uint32_t scale = (static_cast<uint32_t>(word[e / 4]) >> (e % 4 * 8)) & 0xff;
-      const bool fine = scale <= 140 && (!key || scale >= 104 || scale <= 64);
+      const bool fine = scale <= 140 && (!key || scale >= 104 || scale <= 40);
       fit &= fine || t0 + token >= end;
     }
   }

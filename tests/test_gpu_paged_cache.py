@@ -409,3 +409,15 @@ def test_a_later_value_beyond_f16_leaves_earlier_rows_alone(vgo, device, dim, gr
     # (an improbable key: what later rows make of it is finite in f16)
     q = torch.randn(1, group, 300, dim, generator=torch.Generator().manual_seed(42)).abs().half() + 1.0
     both.attend(q, table, int32([305]), causal=True)
+
+
+def test_tiny_keys_under_a_large_scale_in_f16(vgo, device):
+    """Keys of 2^-62, scores of which the largest scale makes thousandths: two keys of one size and two signs, values of two signs."""
+    table, pages = layout(1, 64, 64, 56)
+    both = Both(vgo, device, pages, 1, 64, 128)
+    k, v = torch.full((1, 1, 2, 128), 6 * 2.0 ** -63), torch.ones(1, 1, 2, 128)
+    k[:, :, 1] *= -1
+    v[:, :, 1] *= -1
+    both.append(k, v, table, int32([0]))
+    for n in (1, 140):
+        both.attend(torch.full((1, 1, n, 128), 65504.0).half(), table, int32([2]), scale=1e8)
