@@ -147,27 +147,31 @@ __device__ __forceinline__ float to_odd(double d) {
 }
 
 // Codes of x cos + o sin, exactly those of the 64-bit value: fp32 first, which is off by at most 2^-24 of the
-// product x cos and of the sum each; where some channel of the wave lies so near a border that this may matter (about
-// one of 500 waves), 64 bits.  (64 bits throughout kept the vector unit busy for three times as long as
+// product x cos and of the sum each; where the codes, or the scale, at the two ends of four times that differ in some
+// channel of the wave (about one of 500 waves), 64 bits.  The ends, and not the largest magnitude, say whether the
+// scale is certain: a channel's partner is in another block, so that all of a block may cancel to far less than its parts.
+// (64 bits throughout kept the vector unit busy for three times as long as
 // memory takes: 4 ragged prompts of up to 8,232 tokens, 16 heads of 64 channels, 184 us, this 67.)
 __device__ __forceinline__ uint32_t quantise_rotated(const float (&x)[8], const float (&o)[8], const float (&sin)[8],
                                                      const float (&cos)[8], bool real, uint32_t& byte) {
   float y[8], low[8], high[8];
+  float least = 0.0f, most = 0.0f;  // what the largest magnitude is at least, and at most; NaN in any channel is kept
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float part = x[i] * cos[i];
     y[i] = fmaf(o[i], sin[i], part);
     const float off = fabsf(part) + fabsf(y[i]);
     low[i] = fmaf(off, -0x1p-22f, y[i]), high[i] = fmaf(off, 0x1p-22f, y[i]);
+    least = __builtin_elementwise_maximum(__builtin_elementwise_maximum(least, low[i]), -high[i]);
+    most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most, high[i]), -low[i]);
   }
-  const uint32_t top = top_of(y);
+  const uint32_t top = quad_max(__float_as_uint(most) & 0x7fffffffu);
   byte = scale_byte(top);
   const float scale = factor_of(byte);
   const uint32_t word = codes_of(low, scale);
-  // The largest one's parts may each be twice as large: 2^-20 of it covers them.  Numbers near the ends of fp32, and
-  // those that are not finite, are left to 64 bits.
-  const uint32_t past = (top & 0x7fffffu) - (0x600000u - 16u);
-  const bool plain = word == codes_of(high, scale) && past > 32u && top > 0x10000000u && top < 0x7e000000u;
+  // Numbers near the ends of fp32, and those that are not finite, are left to 64 bits.
+  const bool plain = word == codes_of(high, scale) && byte == scale_byte(quad_max(__float_as_uint(least) & 0x7fffffffu)) &&
+                     top > 0x10000000u && top < 0x7e000000u;
   if (__all(plain || !real)) return word;
 #pragma unroll
   for (int i = 0; i < 8; ++i)

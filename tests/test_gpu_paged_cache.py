@@ -421,3 +421,31 @@ def test_tiny_keys_under_a_large_scale_in_f16(vgo, device):
     both.append(k, v, table, int32([0]))
     for n in (1, 140):
         both.attend(torch.full((1, 1, n, 128), 65504.0).half(), table, int32([2]), scale=1e8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_blocks_that_cancel(vgo, device, dtype, dim):
+    """Rotated blocks of one channel whose two parts, some 600 each, leave a little more than 7 or 3.5, where the scale doubles: in
+    fp32 the parts' roundings alone (2^-15 each) leave less."""
+    n, heads, half = 160, 2, dim // 2
+    g = torch.Generator().manual_seed(43)
+    pool = 1 << 18
+    sin, o = torch.rand(pool, generator=g) * 0.5 + 0.3, (torch.rand(pool, generator=g) * 900 + 300).to(dtype).float()
+    y = torch.tensor([7.0, 3.5])[torch.arange(pool) % 2]
+    x = ((y + o * sin) / 0.6).to(dtype).float()
+    cos = ((y.double() * (1 + 2.0 ** -18) + o.double() * sin.double()) / x.double()).float()
+    exact = x.double() * cos.double() - o.double() * sin.double()
+    in_fp32 = ((x * cos).double() - o.double() * sin.double()).float()
+    chosen = ((exact > y) & (in_fp32 < y * (1 - 2.0 ** -19))).nonzero().flatten()[:n * heads * half // 32].view(half // 32, heads, n)
+    assert chosen.numel() == n * heads * half // 32
+    k, tables_of = torch.zeros(1, heads, n, dim), (torch.zeros(n, dim), torch.ones(n, dim))
+    for block in range(half // 32):
+        for head in range(heads):
+            at, of = 32 * block + 5 * head + 3, chosen[block, head]
+            k[0, head, :, at], k[0, head, :, at + half] = x[of], o[of]
+            tables_of[0][:, at], tables_of[1][:, at] = sin[of], cos[of]
+    both = Both(vgo, device, 6, heads, 32, dim)
+    both.append(k.to(dtype), k.to(dtype), torch.arange(6, dtype=torch.int32)[None], int32([3]), rope=tables_of,
+                positions=torch.arange(n, dtype=torch.int32)[None])
+    both.check_everything()
