@@ -259,6 +259,13 @@ __device__ __forceinline__ float mass_of(float mass) {
   return mass == -INFINITY ? mass : fminf(fmaxf(mass, -1e30f), 1e30f);
 }
 
+// A channel of a query, infinities as NaN: such a query's scores are infinite or NaN, all of them, and NaN is what its row is.
+__device__ __forceinline__ float channel_of(float x) { return fmaf(x, 0.0f, x); }
+
+// Whether a row attends to nothing: no score has moved its maximum, and it has no sum either.  (Scores of NaN do not move the
+// maximum, but they are in the sum.)
+__device__ __forceinline__ bool sees_nothing(float top, float sum) { return top == -INFINITY && sum == 0.0f; }
+
 // bf16 terms that a query, and a probability, is split into (many bf16 queries: one each, see ManyTerms).
 template <typename T>
 struct Terms;

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Attend a) {
       j.top = most;
     }
     const int row = a.first_row + of0 + r;
-    const bool none = row >= count * a.group || j.top == -INFINITY;
+    const bool none = row >= count * a.group || sees_nothing(j.top, j.sum);
     f32x4 v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : j.v[e] / j.sum;

@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
       for (int e = 0; e < 2; ++e) {
         const f32x4 four = load4(query + 8 * s + 4 * e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
+        for (int i = 0; i < 4; ++i) v[4 * e + i] = channel_of(four[i]);
       }
     }
 #pragma unroll
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
       for (int e = 0; e < 4; ++e) v[e] = fmaf(part[e], share, v[e]);
     }
     if (whole) {
-      const bool none = row >= count * a.group || most == -INFINITY;
+      const bool none = row >= count * a.group || sees_nothing(most, sum);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : v[e] / sum;
       store4(static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
         for (int e = 0; e < 2; ++e) {
           const f32x4 four = load4(query + 16 * s + 4 * e);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * e + i] = four[i];
+          for (int i = 0; i < 4; ++i) v[4 * e + i] = channel_of(four[i]);
         }
       }
 #pragma unroll
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   // A lane has, for its row, channels 64 c + 16 j + 8 h .. + 7 of tiles 2 c and 2 c + 1.
   total = half_sum(total);
   if (row >= min(tile0 + a.tile_rows, a.last_row)) return;
-  const bool none = row >= count * a.group || top == -INFINITY;
+  const bool none = row >= count * a.group || sees_nothing(top, total);
   const float share = whole ? (none ? 0.0f : 1.0f / total) : 1.0f;
   const int64_t place_of = ((static_cast<int64_t>(x) * kv + hk) * a.tiles + tile) * a.tile_rows + row - tile0;
   T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + (hk * a.group + row % a.group) * a.out_stride[1] +

@@ -116,7 +116,8 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     of its queries are real; query i stands at place lengths[b] - counts[b] + i, and with `causal` sees no later one.
     H is a multiple of the cache's Hk (head h reads key head h // (H // Hk)); scale (1e-8 to 1e8) defaults to 1 / sqrt(D).  Returns
     [B, H, N, D], token-major in memory where q is; zeros for padding and for queries that attend to nothing (a
-    log mass of -inf, or no page, keeps a token out; finite masses past 1e30 in size count as that).
+    log mass of -inf, or no page, keeps a token out; finite masses past 1e30 in size count as that).  A query with a channel that
+    is not finite comes out as NaN, unless it attends to nothing.
 
     Tokens past a length, or past the table (2**30 tokens a sequence at most), are not there and may hold anything; others
     must be finite where any query of their sequence can see them.  Stored numbers enter exactly (in f16, with many

@@ -449,3 +449,42 @@ def test_append_blocks_that_cancel(vgo, device, dtype, dim):
     both.append(k.to(dtype), k.to(dtype), torch.arange(6, dtype=torch.int32)[None], int32([3]), rope=tables_of,
                 positions=torch.arange(n, dtype=torch.int32)[None])
     both.check_everything()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 40, 140])
+@pytest.mark.parametrize("length", [70, 5000])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_queries_that_are_not_finite_come_out_as_nan(vgo, device, bad, length, n, dtype):
+    """One channel of one query: its row is NaN, its neighbours are as they were, and a row that sees nothing is zeros still.
+    (Whole sequences, and those cut into pieces.)"""
+    table, pages = layout(1, length, 64, 44)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    both.fill(45)
+    q = torch.randn(1, 2, n, 64, generator=torch.Generator().manual_seed(46)).to(dtype)
+    want, bound = oracle.attention(q, both.pages, table, int32([length]))
+    row = n // 3
+    q[0, 1, row, 13] = bad
+    got = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([length]))).double().cpu()
+    assert torch.isnan(got[0, 1, row]).all()
+    got[0, 1, row], want[0, 1, row] = 0.0, 0.0
+    assert ((got - want).abs() <= bound).all()
+    none = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([min(row, length)])),
+                                causal=True).cpu()  # (the first n - row queries stand before the first token)
+    before = n - min(row, length)
+    if row < before:
+        assert not none[:, :, :before].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 140])
+def test_an_infinite_query_whose_scores_are_all_minus_infinity(vgo, device, n, dtype):
+    table, pages = layout(1, 70, 64, 44)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    both.fill(45)
+    k = torch.full((1, 1, 70, 64), -1.0)
+    both.append(k, k, table, int32([0]))
+    q = torch.ones(1, 1, n, 64, dtype=dtype)
+    q[0, 0, 0, 0] = math.inf
+    got = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([70]))).cpu()
+    assert torch.isnan(got[0, 0, 0]).all() and ((got[0, 0, 1:].double() + 1).abs() <= 2.0 ** -8).all()  # (others: the values' -1)
