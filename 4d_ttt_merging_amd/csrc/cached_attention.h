@@ -40,6 +40,7 @@ struct Attend {
   int32_t held;               // work-groups that the chip holds at once
   int32_t causal;
   float scale, per_scale;     // times log2(e); 1 / the scale itself
+  float lazy;                 // kLazy / scale
 };
 
 __device__ __forceinline__ int64_t capacity_of(const Attend& a) { return a.pages.width << a.pages.shift; }
@@ -249,10 +250,20 @@ __device__ __forceinline__ int stop_of(const Attend& a, int length, int count, i
   return last < row0 ? 0 : a.causal ? max(0, min(length, place0 + last / a.group + 1)) : length;
 }
 
+// A row's reference maximum moves where a score passes it by more than this, in powers of two.
+constexpr float kLazy = 8.0f;
+
 // Exponents are z scale - reference in one instruction, whose product is not rounded while the reference's was: they are off by
 // its rounding, the same for all of a row, which normalising takes out.  From references of this size on, where that could
-// pass what an exponential holds (a row of a type's lowest values, say), the difference is taken before the scale.
+// pass what an exponential holds (a row of a type's lowest values, say), the difference is taken before the scale.  Whether a
+// reference moves always goes by the difference before the scale: of neighbouring fp32 scores past 2^27 the products
+// with it may be one number, and the larger one's exponential past every number.
 constexpr float kFar = 0x1p20f;
+// What sums are multiplied by where a row's reference moves.
+__device__ __forceinline__ float shrink_of(float from, float to, float scale) {
+  const float top = to * scale;
+  return top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fabsf(top) > kFar ? (from - to) * scale : from * scale - top);
+}
 
 // A mass as the kernels take it: a type's lowest value is a number, and with the scales that are allowed it stays one.
 __device__ __forceinline__ float mass_of(float mass) {

@@ -246,7 +246,7 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
   for (int i = 0; i < 3; ++i) a.q_stride[i] = q_stride[i], a.out_stride[i] = out_stride[i];
   a.n_query = static_cast<int32_t>(n_query);
   a.group = static_cast<int32_t>(heads / cache->kv_heads);
-  a.causal = causal != 0, a.scale = scale * 1.4426950408889634f, a.per_scale = 1.0f / scale;
+  a.causal = causal != 0, a.scale = scale * 1.4426950408889634f, a.per_scale = 1.0f / scale, a.lazy = kLazy / a.scale;
   const hipStream_t s = as_stream(stream);
   const int dim = static_cast<int>(cache->head_dim);
   char* ws = static_cast<char*>(workspace);

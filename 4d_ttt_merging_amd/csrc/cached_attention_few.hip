@@ -18,7 +18,6 @@ namespace paged {
 namespace {
 
 constexpr int kWaves = 8;
-constexpr float kLazy = 8.0f;
 
 // What a lane reads of a block of 32 tokens.
 template <int D, bool kMass>
@@ -196,13 +195,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     float local = z[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) local = fmaxf(local, z[i]);
-    if (__any(local * scale > top + kLazy)) {
+    if (__any(local - raw > (kMass ? kLazy : a.lazy))) {
       local = fmaxf(local, __shfl_xor(local, 16));
       local = half_max(local);
-      raw = fmaxf(raw, local);
-      const float to = raw * scale;
-      const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-      top = to;
+      const float shrink = shrink_of(raw, fmaxf(raw, local), scale);
+      raw = fmaxf(raw, local), top = raw * scale;
       total *= shrink;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c)

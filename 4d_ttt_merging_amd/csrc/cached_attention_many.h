@@ -6,7 +6,8 @@
 //   scores^T = K Q^T; row m of a block of 32 tokens holds token 16 (m / 16) + 8 (m / 4 % 2) + 4 (m / 8 % 2) + m % 4, so
 //     that a lane's sixteen scores are two operands of the next product as they stand
 //   out^T += V^T P^T, a lane having converted two channels of eight tokens, operands of two tiles
-// One reference maximum a row, moved only where a score passes it by 2^8.
+// One reference maximum a row, moved only where a score passes it by 2^8.  (Told to the compiler as seldom: 2% of calls with 128
+// channels.)
 //
 // Bound by matrix and vector instructions in turn: a wave's products wait for its conversions and softmax, which other waves'
 // products cover in part (64 channels: MFMA busy 0.41 of the time, VALU 0.62; 128: 0.43, 0.43).  bf16, 16 heads of 8,192 x 8,192:
@@ -23,8 +24,6 @@
 namespace vgo {
 namespace paged {
 namespace {
-
-constexpr float kLazyMany = 8.0f;
 
 template <typename T>
 struct ManyTerms {
@@ -345,12 +344,10 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
       float local = z[0][0];
 #pragma unroll
       for (int i = 1; i < 32; ++i) local = fmaxf(local, z[i >> 4][i & 15]);
-      if (__any(local * a.scale > top + kLazyMany)) {
+      if (__builtin_expect(__any(local - raw > a.lazy), 0)) {
         local = half_max(local);
-        raw = fmaxf(raw, local);
-        const float to = raw * a.scale;
-        const float shrink = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-        top = to;
+        const float shrink = shrink_of(raw, fmaxf(raw, local), a.scale);
+        raw = fmaxf(raw, local), top = raw * a.scale;
         total *= shrink;
 #pragma unroll
         for (int c = 0; c < kOut; ++c)
@@ -358,7 +355,7 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
           for (int e = 0; e < 16; ++e) acc[c][e] *= shrink;
       }
       float from = top == -INFINITY ? 0.0f : top - kLift;
-      if (__any(fabsf(from) > kFar)) {  // (see kFar)
+      if (__builtin_expect(__any(fabsf(from) > kFar), 0)) {  // (see kFar)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll

@@ -488,3 +488,26 @@ def test_an_infinite_query_whose_scores_are_all_minus_infinity(vgo, device, n, d
     q[0, 0, 0, 0] = math.inf
     got = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([70]))).cpu()
     assert torch.isnan(got[0, 0, 0]).all() and ((got[0, 0, 1:].double() + 1).abs() <= 2.0 ** -8).all()  # (others: the values' -1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 40, 140])
+@pytest.mark.parametrize("masses", [False, True])
+@pytest.mark.parametrize("far", [14, 20])
+@pytest.mark.parametrize("first", [185, 189, -184, -188])
+def test_neighbouring_scores_far_from_zero_stay_finite(vgo, device, first, far, masses, n, dtype):
+    """Scores that are adjacent fp32 numbers past 2^27 or 2^33, 16 or 1,024 apart, the larger one later, and one number with the
+    scale.  (Keys of 2^14 are f16 numbers, those of 2^20 are not.)"""
+    scale = torch.tensor(1.4426950408889634, dtype=F32)
+    low = torch.tensor(first * 2.0 ** (far + 6), dtype=F32)
+    assert low * scale == (low + 2.0 ** (far - 10)) * scale != low + 2.0 ** (far - 10) != low
+    table, pages = layout(1, 320, 64, 47)
+    both = Both(vgo, device, pages, 1, 64, 64, masses=masses)
+    k, v = torch.zeros(1, 1, 320, 64), torch.randn(1, 1, 320, 64, generator=torch.Generator().manual_seed(48))
+    k[..., 0] = 2.0 ** far
+    k[0, 0, 100 if n > 64 else 300, 32] = 2.0 ** (far - 10)
+    both.append(k, v, table, int32([0]))
+    q = torch.zeros(1, 1, n, 64)
+    q[..., 0], q[..., 32] = first * 64.0, 1.0
+    out = vgo.cached_attention(both.to(q.to(dtype)), both.cache, both.to(table), both.to(int32([320])), scale=1.0).double().cpu()
+    assert torch.isfinite(out).all() and out.abs().max() <= both.pages.v.abs().max() * (1 + 2.0 ** -7)
