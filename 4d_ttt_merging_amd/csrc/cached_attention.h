@@ -266,8 +266,9 @@ __device__ __forceinline__ float shrink_of(float from, float to, float scale) {
 }
 
 // A mass as the kernels take it: a type's lowest value is a number, and with the scales that are allowed it stays one.
+constexpr float kMostMass = 1e30f;
 __device__ __forceinline__ float mass_of(float mass) {
-  return mass == -INFINITY ? mass : fminf(fmaxf(mass, -1e30f), 1e30f);
+  return mass == -INFINITY ? mass : fminf(fmaxf(mass, -kMostMass), kMostMass);
 }
 
 // A channel of a query, infinities as NaN: such a query's scores are infinite or NaN, all of them, and NaN is what its row is.
@@ -329,6 +330,11 @@ __device__ __forceinline__ void value_operands(uint2 codes, uint2 scales, u32x4&
 __device__ __forceinline__ uint2 kept_scales(uint2 s, int valid) {
   const uint64_t keep = valid >= 8 ? ~uint64_t{0} : valid <= 0 ? 0 : (uint64_t{1} << (8 * valid)) - 1;
   return {s.x & static_cast<uint32_t>(keep), s.y & static_cast<uint32_t>(keep >> 32)};
+}
+// Those with the bits of `out`, one a token, as zero: what a mass of -infinity keeps out may be anything, too.
+__device__ __forceinline__ uint2 scales_without(uint2 s, uint32_t out) {
+  const auto bytes = [](uint32_t four) { return (((four & 15) * 0x00204081u) & 0x01010101u) * 0xffu; };
+  return {s.x & ~bytes(out), s.y & ~bytes(out >> 4)};
 }
 // x as kTerms terms, the first ones rounded to nearest: exact but for what the last one leaves.
 template <int kTerms, typename N>

@@ -182,9 +182,28 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[4 * i + e] = c[e];
     }
-    if constexpr (kMass) {
+    uint2 value_scales[D / 32];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = fmaf(z[i], a.scale, mass_of(codes.mass[i / 4][i % 4]) * 1.4426950408889634f);
+    for (int u = 0; u < D / 32; ++u) value_scales[u] = codes.vs[u];
+    if constexpr (kMass) {
+      const auto mass = [&](int i) { return codes.mass[i / 4][i % 4]; };
+      float largest = 0.0f;  // (NaN in any is kept)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) largest = __builtin_elementwise_maximum(largest, fabsf(mass(i)));
+      if (!__any(!(largest <= kMostMass))) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = fmaf(z[i], a.scale, mass(i) * 1.4426950408889634f);
+      } else {
+        uint32_t out = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool gone = mass(i) == -INFINITY;
+          z[i] = gone ? -INFINITY : fmaf(z[i], a.scale, mass_of(mass(i)) * 1.4426950408889634f);
+          out |= gone ? 1u << i : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) value_scales[u] = scales_without(value_scales[u], out);
+      }
     }
     const float scale = kMass ? 1.0f : a.scale;  // still to be applied
     if (a.causal || !inside) {
@@ -224,7 +243,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void few_kernel(const Attend a) {
     }
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) {
-      uint2 scales = codes.vs[u];
+      uint2 scales = value_scales[u];
       if (!inside) scales = kept_scales(scales, piece.length - t0 - 8 * g);
       u32x4 two[2];
       value_operands(codes.v[u], scales, two[0], two[1]);

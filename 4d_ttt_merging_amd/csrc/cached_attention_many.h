@@ -192,8 +192,8 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) key_codes[e] = reinterpret_cast<const uint2*>(base + key_from)[e];
         key_scale = base[key_scale_from];
-        if (part == 0 && masses) key_mass = masses[(static_cast<int64_t>(page) << shift) + (t0 & in_page) + key];
       }
+      if (masses) key_mass = masses[(static_cast<int64_t>(page) << shift) + (t0 & in_page) + key];
       if (does_values) {
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) {
@@ -212,6 +212,15 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   };
   const auto convert = [&](int slot, auto half) {
     constexpr bool kHalf = decltype(half)::value;
+    if (masses) {
+      // Tokens that their masses keep out, a bit each: as zeros, of which no product is NaN.
+      const uint32_t out = static_cast<uint32_t>(__ballot(key_mass == -INFINITY));
+      if (out != 0) {
+        if (key_mass == -INFINITY) key_scale = 0;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) value_scales[e] = scales_without(value_scales[e], out >> (8 * group));
+      }
+    }
     if (does_keys) {
       const float scale = scale_of<0>(key_scale);
       u32x4* to = &keys[slot][block][0][0] + key_row;

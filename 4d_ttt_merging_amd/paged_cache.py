@@ -119,8 +119,8 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     log mass of -inf, or no page, keeps a token out; finite masses past 1e30 in size count as that).  A query with a channel that
     is not finite comes out as NaN, unless it attends to nothing.
 
-    Tokens past a length, or past the table (2**30 tokens a sequence at most), are not there and may hold anything; others
-    must be finite where any query of their sequence can see them.  Stored numbers enter exactly (in f16, with many
+    Tokens past a length, or past the table (2**30 tokens a sequence at most), are not there and may hold anything, and so may
+    those that a mass of -inf keeps out; others must be finite where any query of their sequence can see them.  Stored numbers enter exactly (in f16, with many
     queries, values below 2**-23 to its smallest number, 2**-24).  Sums are fp32; probabilities are rounded to a 16-bit
     type of q where queries are many (more than 64 rows beside a key head), else taken to twice its bits, and to
     24 bits in fp32.  Results are the same bits every time.  Under bf16 or f16 autocast fp32 q is cast first."""

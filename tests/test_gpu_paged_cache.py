@@ -511,3 +511,21 @@ def test_neighbouring_scores_far_from_zero_stay_finite(vgo, device, first, far, 
     q[..., 0], q[..., 32] = first * 64.0, 1.0
     out = vgo.cached_attention(both.to(q.to(dtype)), both.cache, both.to(table), both.to(int32([320])), scale=1.0).double().cpu()
     assert torch.isfinite(out).all() and out.abs().max() <= both.pages.v.abs().max() * (1 + 2.0 ** -7)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 40, 140])
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_mass_of_minus_infinity_keeps_out_whatever_is_stored(vgo, device, causal, n, dtype):
+    """Blocks of NaN at tokens that no query sees: one in a tile, a whole tile, every second one of a page, the last one."""
+    table, pages = layout(2, 260, 64, 50)
+    both = Both(vgo, device, pages, 2, 64, 64, masses=True)
+    both.fill(51)
+    bad = torch.full((1, 2, 1, 64), math.nan)
+    bad[..., 32:] = 1.0  # (a block that is a number beside it)
+    for t in [0, 45, *range(64, 128), *range(128, 192, 2), 259]:
+        page, slot = int(table[0, t // 64]), t % 64
+        both.append(bad, bad, int32([[page]]), int32([slot]), log_mass=torch.full((1, 1), -math.inf))
+        both.pages.k[page, :, slot] = both.pages.v[page, :, slot] = 0.0
+    q = torch.randn(2, 4, n, 64, generator=torch.Generator().manual_seed(52)).to(dtype)
+    both.attend(q, table, int32([260, 230]), causal=causal)
