@@ -265,10 +265,11 @@ __device__ __forceinline__ float shrink_of(float from, float to, float scale) {
   return top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fabsf(top) > kFar ? (from - to) * scale : from * scale - top);
 }
 
-// A mass as the kernels take it: a type's lowest value is a number, and with the scales that are allowed it stays one.
+// A mass as the kernels take it: a type's lowest value is a number, and with the scales that are allowed it stays one.  (NaN is
+// neither below nor above.)
 constexpr float kMostMass = 1e30f;
 __device__ __forceinline__ float mass_of(float mass) {
-  return mass == -INFINITY ? mass : fminf(fmaxf(mass, -kMostMass), kMostMass);
+  return mass < -kMostMass ? (mass == -INFINITY ? mass : -kMostMass) : mass > kMostMass ? kMostMass : mass;
 }
 
 // A channel of a query, infinities as NaN: such a query's scores are infinite or NaN, all of them, and NaN is what its row is.

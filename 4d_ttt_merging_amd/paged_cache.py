@@ -116,14 +116,14 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     of its queries are real; query i stands at place lengths[b] - counts[b] + i, and with `causal` sees no later one.
     H is a multiple of the cache's Hk (head h reads key head h // (H // Hk)); scale (1e-8 to 1e8) defaults to 1 / sqrt(D).  Returns
     [B, H, N, D], token-major in memory where q is; zeros for padding and for queries that attend to nothing (a
-    log mass of -inf, or no page, keeps a token out; finite masses past 1e30 in size count as that).  A query with a channel that
-    is not finite comes out as NaN, unless it attends to nothing.
+    log mass of -inf, or no page, keeps a token out; masses past 1e30 in size count as that, but for -inf).  A query with a channel
+    that is not finite, or that sees a mass of NaN, comes out as NaN, unless it attends to nothing.
 
     Tokens past a length, or past the table (2**30 tokens a sequence at most), are not there and may hold anything, and so may
-    those that a mass of -inf keeps out; others must be finite where any query of their sequence can see them.  Stored numbers enter exactly (in f16, with many
-    queries, values below 2**-23 to its smallest number, 2**-24).  Sums are fp32; probabilities are rounded to a 16-bit
-    type of q where queries are many (more than 64 rows beside a key head), else taken to twice its bits, and to
-    24 bits in fp32.  Results are the same bits every time.  Under bf16 or f16 autocast fp32 q is cast first."""
+    those that a mass of -inf keeps out; others must be finite where any query of their sequence can see them.  Stored numbers
+    enter exactly (in f16, with many queries, values below 2**-23 to its smallest number, 2**-24).  Sums are fp32; probabilities
+    are rounded to a 16-bit type of q where queries are many (more than 64 rows beside a key head), else taken to twice its
+    bits, and to 24 bits in fp32.  Results are the same bits every time.  Under bf16 or f16 autocast fp32 q is cast first."""
     _ready(q, cache.data, cache.log_mass, page_table, lengths, counts)
     (q,) = _autocast(q)
     if scale is None:

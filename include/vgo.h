@@ -715,10 +715,11 @@ int vgo_cache_read(const vgo_paged_cache* cache, const int32_t* starts, const in
 /*
  * Attention over the cache: query i of sequence b stands at place lengths[b] - counts[b] + i (counts NULL: n_query) and
  *   out_i = sum_j softmax_j(scale * q_i.k_j + log_mass[j]) v_j   over j < lengths[b], and, if causal, j <= its place.
- * Queries from counts[b] on, and those that attend to nothing, give zeros; others with a channel that is not finite NaN.  q / out [batch, heads, n_query, head_dim],
- * heads a multiple of kv_heads (head h reads key head h / (heads / kv_heads)), strides as in vgo_cache_tokens.
- * scale: 1e-8 to 1e8.  Finite masses past 1e30 in size count as that; -inf keeps a token out,
- * whatever it holds.  Tokens past a sequence's length, or past the table, are not there and may hold anything.  Workspace (16-byte aligned, any
+ * Queries from counts[b] on, and those that attend to nothing, give zeros; others with a channel that is not finite, or that
+ * see a mass of NaN, give NaN.  q / out [batch, heads, n_query, head_dim], heads a multiple of kv_heads (head h reads key head
+ * h / (heads / kv_heads)), strides as in vgo_cache_tokens.
+ * scale: 1e-8 to 1e8.  Masses past 1e30 in size count as that, but -inf keeps a token out, whatever it holds.
+ * Tokens past a sequence's length, or past the table, are not there and may hold anything.  Workspace (16-byte aligned, any
  * contents): the states of work split over the keys; its size is for the device that is current, `ragged` saying
  * whether counts are given.
  */

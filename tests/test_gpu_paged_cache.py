@@ -529,3 +529,21 @@ def test_a_mass_of_minus_infinity_keeps_out_whatever_is_stored(vgo, device, caus
         both.pages.k[page, :, slot] = both.pages.v[page, :, slot] = 0.0
     q = torch.randn(2, 4, n, 64, generator=torch.Generator().manual_seed(52)).to(dtype)
     both.attend(q, table, int32([260, 230]), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 40, 140])
+def test_a_mass_of_nan_shows(vgo, device, n, dtype):
+    """Queries that see the token are NaN; those before it, and the other sequence's, are as they were."""
+    table, pages = layout(2, 260, 64, 53)
+    both = Both(vgo, device, pages, 1, 64, 64, masses=True)
+    both.fill(54)
+    lengths, t = int32([260, 230]), 260 - n // 2 - 1
+    q = torch.randn(2, 2, n, 64, generator=torch.Generator().manual_seed(55)).to(dtype)
+    want, bound = oracle.attention(q, both.pages, table, lengths, causal=True, masses=True)
+    both.cache.log_mass[int(table[0, t // 64]), t % 64] = math.nan
+    got = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(lengths), causal=True).double().cpu()
+    sees = torch.arange(260 - n, 260) >= t
+    assert torch.isnan(got[0, :, sees]).all()
+    got[0, :, sees], want[0, :, sees] = 0.0, 0.0
+    assert ((got - want).abs() <= bound).all()
