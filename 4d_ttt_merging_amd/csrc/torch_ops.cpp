@@ -12,7 +12,7 @@
 // synchronises.  Autograd: outputs of a path operator whose inputs
 // require grad have a backward that raises (the path is inference only), those
 // of a planner's operator do not require grad, and tangents are dropped; the masked
-// attention and the position bias have gradients.
+// attention and the position bias have gradients, and they and the paged cache refuse tangents.
 // No operator has a batching rule (see register_batched).
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
@@ -361,7 +361,7 @@ struct CacheProblem {
   vgo_paged_cache p{};
   Tensor data, mass, table;
 
-  // `dim`: channels a head of the tensor beside it.
+  // `beside`: the tensor whose device all others share.
   CacheProblem(const Tensor& data0, const OptTensor& mass0, const Tensor& table0, const Tensor& beside, const char* name) {
     require_gpu({&data0, opt(mass0), &table0, &beside});
     TORCH_CHECK(data0.device() == beside.device() && table0.device() == beside.device() &&
@@ -1027,7 +1027,8 @@ constexpr const char* kPlanInto[] = {"similarity_topk", "rope_table"};
 
 // Operators with a derivative, and those of their derivatives (path operators: no second one).
 constexpr const char* kGradients[] = {"masked_attention_grad", "position_bias_grad"};
-// The paged cache: path operators, and the one that writes (path, with a written argument).
+// The paged cache: as path operators, and the one that writes, but tangents are refused: dropped, they would be a derivative of
+// zero.
 constexpr const char* kCache[] = {"cache_read", "cached_attention"};
 constexpr const char* kCacheInto[] = {"cache_append"};
 
@@ -1041,11 +1042,18 @@ void each_tensor(const c10::IValue& value, Visit visit) {
 }
 
 // Autograd key.  History: where an input requires grad (and grad mode is on) floating outputs do too,
-// with a backward that raises; written tensors are left as they are.
-template <bool kHistory>
+// with a backward that raises; written tensors are left as they are.  Forward: tangents of any input may pass by; else they
+// are refused.
+template <bool kHistory, bool kForward = true>
 void autograd(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   const size_t arguments = op.schema().arguments().size(), returns = op.schema().returns().size();
   torch::autograd::edge_list inputs;
+  if (!kForward && c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    for (const c10::IValue& value : torch::jit::last(*stack, arguments))
+      each_tensor(value, [&](const Tensor& t) {
+        TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), op.operator_name().name, ": no forward-mode derivative");
+      });
+  }
   if constexpr (kHistory) {
     if (at::GradMode::is_enabled()) {
       bool tangent = false;
@@ -1254,8 +1262,8 @@ void register_autograd(torch::Library& m) {
   for (const char* name : kPlan) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<false>>());
   for (const char* name : kPlanInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<false>>());
   for (const char* name : kGradients) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
-  for (const char* name : kCache) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
-  for (const char* name : kCacheInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true>>());
+  for (const char* name : kCache) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true, false>>());
+  for (const char* name : kCacheInto) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&autograd<true, false>>());
   m.impl("masked_attention", masked_attention_autograd);
   m.impl("position_bias", position_bias_autograd);
 }

@@ -322,3 +322,25 @@ def test_a_block_with_gradients_enabled_and_captured(vgo, device, autocast):
         torch.cuda.synchronize()
         with torch.no_grad(), torch.autocast("cuda", dtype=BF16, enabled=autocast, cache_enabled=False):
             assert torch.equal(got, block(x, rope, cached=steps[0]))
+
+
+def test_tangents_are_refused(vgo, device):
+    """A tangent dropped would be a derivative of zero."""
+    cache, table, starts, (q, k, v) = scene(vgo, device, n=5, masses=True)
+    mass, rope = torch.zeros(2, 5, device=device), tables(900, 64, device)
+    forward = torch.autograd.forward_ad
+    before = cache.data.clone()
+    with forward.dual_level():
+        dual = lambda t: forward.make_dual(t, torch.ones_like(t))
+        for call in (lambda: vgo.cached_attention(dual(q), cache, table, starts),
+                     lambda: vgo.cache_append(cache, dual(k), v, table, starts), lambda: vgo.cache_append(cache, k, dual(v), table, starts),
+                     lambda: vgo.cache_append(cache, k, v, table, starts, q=dual(q)),
+                     lambda: vgo.cache_append(cache, k, v, table, starts, rope=(dual(rope[0]), rope[1])),
+                     lambda: vgo.cache_append(cache, k, v, table, starts, log_mass=dual(mass))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        want = vgo.cached_attention(q, cache, table, starts)  # (without tangents as ever)
+    assert torch.equal(before, cache.data) and torch.equal(want, vgo.cached_attention(q, cache, table, starts))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: vgo.cached_attention(t, cache, table, starts), (q,), (torch.ones_like(q),))
