@@ -19,6 +19,9 @@ namespace {
 
 constexpr int kWaves = 8;
 
+// Four floats anywhere: masses are aligned as floats are (one load of 16 bytes all the same).
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
 // What a lane reads of a block of 32 tokens.
 template <int D, bool kMass>
 struct Codes {
@@ -62,7 +65,7 @@ __device__ __forceinline__ void read_codes(Codes<D, kMass>& c, const uint8_t* bl
   if constexpr (kMass) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      c.mass[i] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const uint8_t*>(mass) + o.mass + 16 * i);
+      c.mass[i] = *reinterpret_cast<const f32x4_any*>(reinterpret_cast<const uint8_t*>(mass) + o.mass + 16 * i);
   }
 }
 

@@ -15,6 +15,7 @@ int check_cache(const vgo_paged_cache* c) {
                   c->batch <= INT32_MAX && c->table_width >= 0 && c->table_width <= (int64_t{1} << 30) / c->page_size,
               "paged cache: size out of range");
   VGO_REQUIRE(c->pages == 0 || (c->data && aligned(c->data, 16)), "paged cache: the data must be 16-byte aligned");
+  VGO_REQUIRE(aligned(c->log_mass, 4), "paged cache: the masses must be aligned as floats are");
   VGO_REQUIRE(c->batch == 0 || c->table_width == 0 || c->page_table, "paged cache: null page table");
   return VGO_OK;
 }

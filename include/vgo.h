@@ -665,7 +665,7 @@ int vgo_position_bias_grad(const void* grad, int64_t n_buckets, int64_t heads, c
  *   keys' codes [32][head_dim / 2] (byte c: channel 2c in its low half, 2c + 1 in its high half), values' codes
  *   [4][head_dim / 2][8] (tokens 8g .. 8g + 7 of a channel pair side by side), keys' scales [32][head_dim / 32],
  *   values' scales [4][head_dim / 32][8].
- * log_mass: fp32 [pages, page_size], added to every score of a token; NULL: the cache holds none.
+ * log_mass: fp32 [pages, page_size], 4-byte aligned, added to every score of a token; NULL: the cache holds none.
  * page_size: a power of two, 32 to 1,024; head_dim 64 or 128.
  * page_table: int32 [batch, table_width]; token t of sequence b lies in page page_table[b, t / page_size].  Tokens past
  * the table, or whose page is not one of the cache's, are not there: appending leaves them out, reading gives zeros,

@@ -344,3 +344,18 @@ def test_tangents_are_refused(vgo, device):
     assert torch.equal(before, cache.data) and torch.equal(want, vgo.cached_attention(q, cache, table, starts))
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: vgo.cached_attention(t, cache, table, starts), (q,), (torch.ones_like(q),))
+
+
+@pytest.mark.parametrize("n", [1, 40, 140])
+def test_masses_at_any_float(vgo, device, n):
+    """Masses that begin 4, 8 or 12 bytes past a multiple of 16: the same bits."""
+    cache, table, starts, (q, k, v) = scene(vgo, device, n=n, masses=True)
+    cache.log_mass.copy_(torch.randn(cache.log_mass.shape, generator=torch.Generator().manual_seed(3)))
+    want = vgo.cached_attention(q, cache, table, starts)
+    for at in (1, 2, 3):
+        wide = torch.zeros(cache.log_mass.numel() + 4, device=device)
+        view = wide[at:at + cache.log_mass.numel()].view(cache.log_mass.shape)
+        view.copy_(cache.log_mass)
+        assert torch.equal(want, vgo.cached_attention(q, cache._replace(log_mass=view), table, starts))
+        vgo.cache_append(cache._replace(log_mass=view), k, v, table, starts, log_mass=torch.ones(2, n, device=device))
+        assert (view != cache.log_mass).sum() == 2 * n and not wide[:at].any() and not wide[at + view.numel():].any()

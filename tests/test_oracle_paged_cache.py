@@ -127,3 +127,13 @@ def test_host_tensors_and_shapes_are_refused():
         arguments = {**dict(pages=1, kv_heads=1, head_dim=64, device="cpu"), **over}
         with pytest.raises(ValueError):
             vgo.PagedCache.empty(**arguments)
+
+
+@pytest.mark.parametrize("at", [17, 18])
+def test_masses_that_are_no_floats_are_refused(at):
+    """(Any float's address will do: the kernels' wide loads of masses ask for no more.)"""
+    lib_mod = import_package("_lib")
+    lib, size = lib_mod.load(), ctypes.c_size_t()
+    status = lambda cache: lib.vgo_cached_attn_workspace(ctypes.byref(cache), 2, 1, 0, 0, 1, ctypes.byref(size))
+    assert status(struct(lib_mod, log_mass=at)) == lib_mod.VGO_EINVAL
+    assert status(struct(lib_mod, log_mass=20)) == lib_mod.VGO_OK
