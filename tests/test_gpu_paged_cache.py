@@ -547,3 +547,33 @@ def test_a_mass_of_nan_shows(vgo, device, n, dtype):
     assert torch.isnan(got[0, :, sees]).all()
     got[0, :, sees], want[0, :, sees] = 0.0, 0.0
     assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n", [1, 40])
+def test_few_queries_take_probabilities_to_two_terms(vgo, device, n, dtype):
+    """Two keys whose values nearly cancel: what is left shows how far a probability was rounded.  A probability is the sum of two
+    bf16 numbers, off by half a step, 2^-8, of half a step at most: 2^-16."""
+    table, pages = layout(1, 64, 64, 57)
+    both = Both(vgo, device, pages, 1, 64, 64)
+    k, v = torch.zeros(1, 1, 2, 64), torch.ones(1, 1, 2, 64)
+    k[0, 0, 0, 0], v[0, 0, 1] = 1.0, -2.0
+    both.append(k, v, table, int32([0]))
+    q = torch.zeros(1, 1, n, 64)
+    q[..., 0] = 0.6796875 + torch.arange(n) * 2.0 ** -8  # (about log 2: the first key twice as probable)
+    q = q.to(dtype)
+    want, bound = oracle.attention(q, both.pages, table, int32([2]), scale=1.0, p_bits=2.0 ** -16)
+    got = vgo.cached_attention(both.to(q), both.cache, both.to(table), both.to(int32([2])), scale=1.0).double().cpu()
+    assert ((got - want).abs() <= bound).all()
+
+
+def test_read_in_f16_rounds_to_nearest(vgo, device):
+    """Numbers that f16 holds, those below its normal and its smallest ones, and those past it."""
+    both = Both(vgo, device, 4, 2, 64, 64)
+    for page, gain in enumerate((1.0, 2.0 ** -16, 2.0 ** -24, 2.0 ** 15)):
+        x = torch.randn(1, 2, 64, 64, generator=torch.Generator().manual_seed(58 + page)) * gain
+        both.append(x, x.flip(2), int32([[page]]), int32([0]))
+    table, zero = both.to(int32([[0, 1, 2, 3]])), both.to(int32([0]))
+    whole, half = (vgo.cache_read(both.cache, table, zero, 256, dtype=t) for t in (F32, F16))
+    for x, y in zip(whole, half):
+        assert y.dtype == F16 and torch.equal(x.cpu().to(F16), y.cpu()) and torch.isinf(y).any()

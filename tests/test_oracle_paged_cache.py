@@ -137,3 +137,20 @@ def test_masses_that_are_no_floats_are_refused(at):
     status = lambda cache: lib.vgo_cached_attn_workspace(ctypes.byref(cache), 2, 1, 0, 0, 1, ctypes.byref(size))
     assert status(struct(lib_mod, log_mass=at)) == lib_mod.VGO_EINVAL
     assert status(struct(lib_mod, log_mass=20)) == lib_mod.VGO_OK
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_bounds_tell_two_terms_of_a_probability_from_one(dtype):
+    """The two keys of the GPU's test of few queries: one bf16 number a probability is past the bound of two, two are not."""
+    pages = oracle.Pages(1, 1, 64, 64)
+    pages.k[0, 0, 0, 0], pages.v[0, 0, 0], pages.v[0, 0, 1] = 1.0, 1.0, -2.0
+    q = torch.zeros(1, 1, 40, 64)
+    q[..., 0] = 0.6796875 + torch.arange(40) * 2.0 ** -8
+    q = q.to(dtype)
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.tensor([2], dtype=torch.int32)
+    want, bound = oracle.attention(q, pages, table, lengths, scale=1.0, p_bits=2.0 ** -16)
+    p = torch.stack([torch.ones(40, dtype=torch.float64), torch.exp(-q[0, 0, :, 0].double())])
+    one = p.bfloat16().double()
+    two = one + (p - one).bfloat16().double()
+    off = lambda t: ((t[0] - 2 * t[1]) / p.sum(0) - want[0, 0, :, 0]).abs() - bound[0, 0, :, 0]
+    assert off(two).max() <= 0 and off(one)[0] > 0 and (off(one) > 0).sum() > 30  # (some are bf16 numbers, nearly)
