@@ -184,15 +184,17 @@ Plan plan_of(const vgo_paged_cache* c, int64_t heads, int64_t n_query, bool caus
   return p;
 }
 
+constexpr int64_t kMostThreads = int64_t{1} << 32;
 int check_attend(const vgo_paged_cache* cache, int64_t heads, int64_t n_query, int dtype) {
   const int status = check_cache(cache);
   if (status != VGO_OK) return status;
   VGO_REQUIRE(dtype == VGO_F32 || dtype == VGO_BF16 || dtype == VGO_F16, "cached_attn: unsupported dtype");
   VGO_REQUIRE(n_query >= 0 && n_query <= INT32_MAX && heads >= 1 && heads <= 65535, "cached_attn: size out of range");
   VGO_REQUIRE(heads % cache->kv_heads == 0, "cached_attn: heads must be a multiple of the key heads");
+  // (a grid's threads are counted in 32 bits; rows and their places among a launch's in 31)
+  VGO_REQUIRE(cache->batch == 0 || n_query == 0 || cache->batch < kMostThreads / heads / n_query / 32, "cached_attn: too many rows");
   return VGO_OK;
 }
-constexpr int64_t kMostThreads = int64_t{1} << 32;
 
 bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
   const int64_t size = dtype == VGO_F32 ? 4 : 2;
@@ -233,8 +235,6 @@ extern "C" int vgo_cached_attn_fwd(const vgo_paged_cache* cache, const void* q, 
   VGO_REQUIRE(lengths, "cached_attn: null lengths");
   VGO_REQUIRE(rows_fit(q, q_stride, dtype) && rows_fit(out, out_stride, dtype),
               "cached_attn: q and out must be 16-byte aligned, with strides of whole 16 bytes");
-  // (a grid's threads are counted in 32 bits; rows and their places among a launch's in 31)
-  VGO_REQUIRE(cache->batch < kMostThreads / heads / n_query / 32, "cached_attn: too many rows");
   const Plan p = plan_of(cache, heads, n_query, causal != 0, counts != nullptr, dtype);
   for (int i = 0; i < p.parts; ++i)
     VGO_REQUIRE(p.part[i].pieces < kMostThreads / 512 / (p.part[i].tiles * cache->kv_heads), "cached_attn: too many rows");

@@ -154,3 +154,14 @@ def test_bounds_tell_two_terms_of_a_probability_from_one(dtype):
     two = one + (p - one).bfloat16().double()
     off = lambda t: ((t[0] - 2 * t[1]) / p.sum(0) - want[0, 0, :, 0]).abs() - bound[0, 0, :, 0]
     assert off(two).max() <= 0 and off(one)[0] > 0 and (off(one) > 0).sum() > 30  # (some are bf16 numbers, nearly)
+
+
+@pytest.mark.parametrize("over", [dict(n_query=1 << 30, heads=64), dict(batch=1 << 30, n_query=1 << 30, heads=65534, kv_heads=32767),
+                                  dict(batch=(1 << 31) - 1, n_query=(1 << 31) - 1, heads=65535, kv_heads=65535)])
+def test_a_workspace_is_asked_for_what_can_be_run(over):
+    """The sizes that the attention itself refuses are refused here, too, before they overflow 64 bits."""
+    lib_mod = import_package("_lib")
+    v = {**dict(batch=1, kv_heads=2, heads=2, n_query=1), **over}
+    cache, size = struct(lib_mod, batch=v["batch"], kv_heads=v["kv_heads"]), ctypes.c_size_t(7)
+    status = lib_mod.load().vgo_cached_attn_workspace(ctypes.byref(cache), v["heads"], v["n_query"], 0, 0, 1, ctypes.byref(size))
+    assert status == lib_mod.VGO_EINVAL
