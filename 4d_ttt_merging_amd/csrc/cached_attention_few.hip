@@ -2,7 +2,8 @@
 //
 // Bound by the cache's bytes, 17/16 D a token and key head, which are read once, and, with 64 channels, nearly as much by the
 // vector units (a conversion makes two numbers of a byte, and a token of 64 channels needs 64 of them): one query of 16 heads
-// over 4 key heads, 32 sequences of 32,768 tokens, 64 channels 66 us, 4.3 TB/s; 128 114, 5.0; a copy reaches 5.1.  A wave takes
+// over 4 key heads, 32 sequences of 32,768 tokens, codes from memory, with the join: 64 channels 66 us, 4.3 TB/s
+// (f16 67, fp32 78); 128 114, 5.0 (115, 126); a copy reaches 5.1.  A wave takes
 // blocks of 32 tokens on its own, the next two's codes on their way meanwhile:
 //   scores^T = K Q^T, two 16 x 16 tiles; row m of tile i holds token 8 (m / 4) + 4 i + m % 4, so that the
 //     lane that gets rows 4 g .. 4 g + 3 of both has tokens 8 g .. 8 g + 7 -- as the next product's operand wants them

@@ -10,11 +10,12 @@
 // channels.)
 //
 // Bound by matrix and vector instructions in turn: a wave's products wait for its conversions and softmax, which other waves'
-// products cover in part (64 channels: MFMA busy 0.41 of the time, VALU 0.62; 128: 0.43, 0.43).  bf16, 16 heads of 8,192 x 8,192:
-// 64 channels 321 us, 855 TFLOP/s; 128 503, 1,093; a product of 8,192^3 reaches 1,141.
+// products cover in part (64 channels: MFMA busy 0.40 of the time, VALU 0.62; 128: 0.43, 0.43).  bf16, 16 heads of 8,192 x 8,192:
+// 64 channels 301 us, 913 TFLOP/s; 128 494, 1,112; a product of 8,192^3 reaches 1,141.
 //
 // f16: where a piece's scales let keys and values be f16 numbers, and they nearly always do, the products are f16 ones
-// (16 heads, 8,192 x 8,192, 64 channels: two bf16 terms of q and of p 592 us, so 361).  Else, and in fp32, bf16 terms.
+// (16 heads, 8,192 x 8,192, 64 channels: two bf16 terms of q and of p 529 us, so 334; 4,096 x 8,192, 128 channels: 419, 282).
+// Else, and in fp32, bf16 terms.
 #pragma once
 
 #include <type_traits>
@@ -42,12 +43,13 @@ __device__ __forceinline__ float pair_sum(bf16x2 x, float sum) {
 
 // How a type and width are run: waves of a work-group, waves that a SIMD is to hold.  More waves share what is converted and
 // read from LDS; fewer (kSharp) leave less idle where a causal tile ends: with few heads beside a key head its rows are many
-// tokens.  16 heads, us with 4 waves (2 a SIMD), 4 (3), 8 (2), 8 (4):
-//   64 channels, 8,192 x 8,192         bf16  379 376 381 330   f16  390 390 383 356     causal  193 192 206 206   204 203 212 248
-//   3 causal prompts over 4 key heads  bf16  153 153 175 141   f16  154 154 155 163     (4,096; up to 4,116)
-//   128 channels, over 8,192           bf16  586     533       f16  325     290         (8,192; 4,096)
-//   128, causal, 4,096                 bf16  123     128       f16  130     135
-//   fp32  2,048 x 2,048, 64 and 128 channels  71, 108  70, 106;   8 heads of 261 x 1,044  17  20
+// tokens.  16 heads, us (in a graph) with 4 waves (2 a SIMD), 4 (3), 8 (2), 8 (4):
+//   64 channels, 8,192 x 8,192         bf16  359 359 351 301   f16  386 386 364 334     causal  185 185 191 199   196 196 199 228
+//   3 causal prompts over 4 key heads  bf16  148 148 164 135   f16  159 159 172 153     (of 4,096)
+//                                            127 127 137 127         139 139 145 143     (of up to 4,116)
+//   128 channels, over 8,192           bf16  560     496       f16  320     282         (8,192; 4,096)
+//   128, causal, 4,096                 bf16  119     118       f16  127     128
+//   fp32  2,048 x 2,048, 64 and 128 channels  72, 112  71, 109;   8 heads of 261 x 1,044  17  20
 template <typename T, int D, bool kSharp>
 struct Many {
   static constexpr bool kFull = std::is_same_v<T, float>;
@@ -73,9 +75,9 @@ struct Number<true> {
 };
 
 // Whether tokens [begin, end) are f16 numbers: keys exactly (scales from 2^-23, whose halves are f16's smallest numbers, to 2^13;
-// or below 2^-87, where zero is as good: scores of them are below 2^-34 at the largest scale), values to f16's smallest number (to 2^13), as far as their sums are
-// rounded in any case.  `end` is where what is converted ends: a probability of zero times a value that has become an
-// infinity is NaN.  All threads of a work-group together.
+// or below 2^-87, where zero is as good: scores of them are below 2^-34 at the largest scale), values to f16's smallest number
+// (to 2^13), as far as their sums are rounded in any case.  `end` is where what is converted ends: a probability of zero
+// times a value that has become an infinity is NaN.  All threads of a work-group together.
 template <int D, int kThreads>
 __device__ __forceinline__ bool all_half(const Attend& a, int64_t b, int hk, int begin, int end) {
   using L = Layout<D>;
@@ -106,8 +108,8 @@ __global__ __launch_bounds__(kWaves * 64, kResident) void many_kernel(const Atte
   constexpr int kSteps = D / 16;        // products over a row's channels
   constexpr int kOut = D / 32;          // tiles of 32 channels
   constexpr bool kApart = kWaves == 8;  // half the waves convert keys, half values
-  // Tiles from one barrier to the next, as many as of which twice fit LDS beside other work-groups (2 x 2,058 ragged queries over 16,464
-  // tokens of 128 channels: bf16 228 us with one, 219 with two, f16 249, 241; fp32 110, 112; 64 channels within 2%).
+  // Tiles from one barrier to the next, as many as of which twice fit LDS beside other work-groups (2 x 2,058 ragged causal queries
+  // over 16,464 tokens of 128 channels: bf16 230 us with one, 218 with two, f16 242, 236, fp32 444, 451; 64 channels within 2%).
   constexpr int kSpan = kApart && !std::is_same_v<T, float> ? 2 : 1, kSlots = 2 * kSpan;
   // [slot][block of 32 tokens][step][lane], [slot][block][tile][step of 16 tokens][lane]: operands of 16 bytes
   __shared__ u32x4 keys[kSlots][2][kSteps][64];

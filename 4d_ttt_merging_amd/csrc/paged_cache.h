@@ -77,6 +77,7 @@ __device__ __forceinline__ float scale_of(uint32_t word) {
 
 // Checks of the host, shared by the entry points.
 int check_cache(const vgo_paged_cache* c);
+bool rows_fit(const void* p, const int64_t stride[3], int dtype);  // rows that are read and written by 16 bytes
 Pages pages_of(const vgo_paged_cache* c);
 
 }  // namespace paged

@@ -20,6 +20,14 @@ int check_cache(const vgo_paged_cache* c) {
   return VGO_OK;
 }
 
+bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
+  const int64_t size = dtype == VGO_F32 ? 4 : 2;
+  if (!p || !aligned(p, 16) || !stride) return false;
+  for (int i = 0; i < 3; ++i)
+    if (stride[i] < 0 || stride[i] * size % 16 != 0) return false;
+  return true;
+}
+
 Pages pages_of(const vgo_paged_cache* c) {
   int shift = 5;
   while ((int64_t{1} << shift) < c->page_size) ++shift;
@@ -397,13 +405,6 @@ struct LaunchRead {
   }
 };
 
-bool rows_fit(const void* p, const int64_t stride[3], int dtype) {
-  const int64_t size = dtype == VGO_F32 ? 4 : 2;
-  if (!p || !aligned(p, 16) || !stride) return false;
-  for (int i = 0; i < 3; ++i)
-    if (stride[i] < 0 || stride[i] * size % 16 != 0) return false;
-  return true;
-}
 bool known(int dtype) { return dtype == VGO_F32 || dtype == VGO_BF16 || dtype == VGO_F16; }
 // Heads that a wave takes one after the other: more where there are waves enough without (the tables' rows, the page and
 // the addresses are then fetched once for them).

@@ -122,8 +122,10 @@ def cached_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tenso
     Tokens past a length, or past the table (2**30 tokens a sequence at most), are not there and may hold anything, and so may
     those that a mass of -inf keeps out; others must be finite where any query of their sequence can see them.  Stored numbers
     enter exactly (in f16, with many queries, values below 2**-23 to its smallest number, 2**-24).  Sums are fp32; probabilities
-    are rounded to a 16-bit type of q where queries are many (more than 64 rows beside a key head), else taken to twice its
-    bits, and to 24 bits in fp32.  Results are the same bits every time.  Under bf16 or f16 autocast fp32 q is cast first."""
+    are rounded to a 16-bit type of q where queries are many (more than 64 rows beside a key head, a row being a query of one
+    of the key head's heads), else taken to twice its bits (as may be the last 64 of many rows), and to 24 bits in fp32.
+    Results are the same bits every time for the same call; which queries stand beside one may change its last bits.  Products
+    and sums must lie within fp32's range.  Under bf16 or f16 autocast fp32 q is cast first."""
     _ready(q, cache.data, cache.log_mass, page_table, lengths, counts)
     (q,) = _autocast(q)
     if scale is None:
